@@ -94,7 +94,12 @@ extern "C" {
     X(SGEMM_GELU, "g2k_sgemm_gelu") X(SGEMM_RESID, "g2k_sgemm_resid")         \
     X(SGEMM_QKV, "g2k_sgemm_qkv") X(SGEMM_PARTIAL, "g2k_sgemm_partial")       \
     X(SPLITK_EPI, "g2k_splitk_epi")                                           \
-    X(LN_FOLD_F32, "g2k_ln_fold_f32") X(LN_FOLD_F16, "g2k_ln_fold_f16")
+    X(LN_FOLD_F32, "g2k_ln_fold_f32") X(LN_FOLD_F16, "g2k_ln_fold_f16")       \
+    X(Q4_PACK_F32, "g2k_q4_pack_f32") X(Q4_PACK_F16, "g2k_q4_pack_f16")       \
+    X(Q4_READ, "g2k_q4_read") X(Q4_MATVEC, "g2k_q4_matvec")                   \
+    X(KV8_APPEND, "g2k_kv8_append") X(KV8_READ, "g2k_kv8_read")               \
+    X(KV8_ATTN, "g2k_kv8_attn")                                               \
+    X(LOGITS, "g2k_logits") X(LOGITS_PICK, "g2k_logits_pick")
 
 #define G2_ENUM_ENTRY(id, name) G2F_##id,
 enum { G2_KERNEL_LIST(G2_ENUM_ENTRY) G2F_COUNT };
@@ -169,6 +174,12 @@ int g2i_attn_out_groups(const float *scores, const float *v_cache, const float *
  * else partials, then merge. */
 int g2i_attn_one_launch(const float *q, const float *k_cache, const float *v_cache, const float *out, int T, int D, int S);
 int g2i_attn_launch(g2_attn1q_args *a, unsigned chunks);
+
+/* Whether np bytes at p and nq bytes at q share any. */
+static inline int g2i_overlap(const void *p, size_t np, const void *q, size_t nq)
+{
+    return (uintptr_t)p < (uintptr_t)q + nq && (uintptr_t)q < (uintptr_t)p + np;
+}
 
 /* host helpers (g2_host.c) */
 void g2i_f32_to_f16(uint16_t *dst, const float *src, size_t n);

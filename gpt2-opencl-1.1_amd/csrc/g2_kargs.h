@@ -375,4 +375,80 @@ typedef struct {
     int *err;
 } g2_attnp_args;
 
+/* 4-bit weights (g2_lowbit_plan.h).  quantize: W (fp32 or fp16, [N,K] or with
+ * in_out [K,N]) to codes and scales; dequantize: codes and scales to W (fp32). */
+typedef struct {
+    const void *W;
+    uint8_t *codes;
+    uint16_t *scales;
+    float *out;
+    int N, K, group, in_out;
+} g2_q4_args;
+
+/* y[m,n] = act(sum_k W[n,k] x[m,k] + bias[n] + res[m,n]) over 4-bit weights */
+typedef struct {
+    const float *x;
+    const uint8_t *codes;
+    const uint16_t *scales;
+    const float *bias;
+    const float *res;
+    float *y;
+    int M, N, K, group, gelu;
+} g2_q4mv_args;
+
+/* Append: rows qkv[S][T][3 D] (keys at column D, values at 2 D; D = 64 NH) of
+ * sequence s go to positions p0 .. p0 + count - 1, p0 = pos ? pos[s] : start,
+ * count = count ? min(count[s], T) : T, as far as they lie in 0 .. max_seq - 1. */
+typedef struct {
+    const float *qkv;
+    int8_t *codes;
+    float *scales;
+    float *last;
+    const int *pos;
+    const int *count;
+    int start, T, S, NH, max_seq, blocks;
+} g2_kv8_append_args;
+
+/* Read: positions start .. start + T - 1 of every sequence to k, v [S][T][D],
+ * those below its length (len ? min(len[s], T_kv) : T_kv) only. */
+typedef struct {
+    const int8_t *codes;
+    const float *scales;
+    const float *last;
+    float *k;
+    float *v;
+    const int *len;
+    int T_kv, start, T, S, NH, blocks;
+} g2_kv8_read_args;
+
+/* Single-query attention of S sequences over the 8-bit cache. */
+typedef struct {
+    const float *q;
+    const int8_t *codes;
+    const float *scales;
+    const float *last;
+    float *out;
+    float *part;
+    const int *len;
+    int q_stride, out_stride, T_kv, S, NH, blocks, splits, span;
+    float scale;
+} g2_kv8_attn_args;
+
+/* Rules on logits (g2_logit_rules): rows x parts work-groups, each a slice of
+ * `slice` ids; part: the best (value, id) of each slice, [rows][parts]. */
+typedef struct {
+    const float *logits;
+    float *out;
+    int *pick;
+    float *part;
+    const int *ctx;
+    const int *ctx_len;
+    const int *bias_id;
+    const float *bias;
+    const uint32_t *mask;
+    int max_ctx, n_bias, mask_stride, forbid;
+    int rows, V, slice, parts;
+    float repetition, frequency, presence;
+} g2_logits_args;
+
 #endif /* G2_KARGS_H */

@@ -24,6 +24,7 @@
 #include "g2_step_plan.h"
 #include "g2_gemm_plan.h"
 #include "g2_attn_plan.h"
+#include "g2_lowbit_plan.h"
 
 #define G2K extern "C" __global__ __launch_bounds__(256)
 
@@ -2187,6 +2188,9 @@ G2K void g2k_ln_fold_f16(const g2_lnfold_args a) { ln_fold_impl<_Float16>(a); }
 /* Fused decode kernels (packed matvecs, single-query attention). */
 #include "g2_matmul.hip"
 #include "g2_decode.hip"
+
+/* 4-bit weights, the 8-bit K/V cache, rules on logits. */
+#include "g2_lowbit.hip"
 
 /* The persistent decode step (one cooperative launch per token). */
 #include "g2_step.hip"

@@ -327,10 +327,7 @@ int g2_sync(void)
 
 static unsigned cdiv(long a, long b) { return (unsigned)((a + b - 1) / b); }
 static int aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
-static int overlap(const void *p, size_t np, const void *q, size_t nq)
-{
-    return (uintptr_t)p < (uintptr_t)q + nq && (uintptr_t)q < (uintptr_t)p + np;
-}
+#define overlap g2i_overlap
 
 /* The launches that write and read a scratch buffer are enqueued without another
  * thread's between them; the stream then keeps their order. */

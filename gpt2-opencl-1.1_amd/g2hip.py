@@ -61,6 +61,13 @@ def preset(name):
     return make_config(L, E, H)
 
 
+class LogitRules(C.Structure):
+    """g2_logit_rules; logit_rules() fills one."""
+    _fields_ = [("ctx", C.c_void_p), ("ctx_len", C.c_void_p), ("max_ctx", C.c_int), ("repetition", C.c_float),
+                ("frequency", C.c_float), ("presence", C.c_float), ("bias_id", C.c_void_p), ("bias", C.c_void_p),
+                ("n_bias", C.c_int), ("mask", C.c_void_p), ("mask_stride", C.c_int), ("forbid", C.c_int)]
+
+
 _vp = C.c_void_p
 _i = C.c_int
 _f = C.c_float
@@ -93,6 +100,11 @@ for _n, _a in {
     "g2_attn_1q": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f],
     "g2_attn_1q_noalloc": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f],
     "g2_matvec_rows": [_vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i],
+    "g2_quantize_q4": [_vp, _i, _i, _vp, _vp, _i, _i, _i], "g2_dequantize_q4": [_vp, _vp, _vp, _i, _i, _i, _i],
+    "g2_matvec_q4": [_vp] * 6 + [_i] * 5,
+    "g2_kv8_append": [_vp] * 4 + [_i] * 5, "g2_kv8_read": [_vp] * 4 + [_i] * 6,
+    "g2_attn_kv8": [_vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _f, _vp],
+    "g2_apply_logit_rules": [_vp, _vp, _vp, _i, _i, C.POINTER(LogitRules), _vp],
     "g2_model_uses_graph": [_vp], "g2_read_kv": [_vp, _i, _vp, _vp],
     "g2_config_load": [C.c_char_p, C.POINTER(Config)], "g2_config_parse": [C.c_char_p, C.POINTER(Config)],
     "g2_model_load": [C.c_char_p, _i, _i, C.POINTER(_vp)],
@@ -112,6 +124,11 @@ _sig("g2_convert_f16", None, _vp, _vp, _sz)
 _sig("g2_model_weight_bytes", _sz, _vp)
 _sig("g2_model_step_kernel", C.c_char_p, _vp)
 _sig("g2_stream", _vp)
+_sig("g2_q4_code_bytes", _sz, _i, _i)
+_sig("g2_q4_scale_bytes", _sz, _i, _i, _i)
+_sig("g2_kv8_bytes", _sz, _i, _i, _i)
+_sig("g2_kv8_work_bytes", _sz, _i, _i)
+_sig("g2_logits_work_bytes", _sz, _i)
 
 
 def last_error():
@@ -275,6 +292,71 @@ def attn_out_1q(scores, v_cache, out, T_kv, D, DH, out_base):
 def attn_1q(qkv, k_cache, v_cache, out, q_base, T_kv, D, NH, max_seq, out_base, scale):
     check(_lib.g2_attn_1q(_p(qkv), _p(k_cache), _p(v_cache), _p(out), q_base, T_kv, D, NH,
                           max_seq, out_base, scale))
+
+
+# ---------------------------------------------------------------- decode in fewer bits
+
+def q4_bytes(N, K, group):
+    """(bytes of the codes, bytes of the scales) of 4-bit weights [N, K]; 0 where the sizes are not supported."""
+    return _lib.g2_q4_code_bytes(N, K), _lib.g2_q4_scale_bytes(N, K, group)
+
+
+def quantize_q4(W, w_dtype, in_out, codes, scales, N, K, group):
+    """Lays out W ([N, K], or [K, N] with in_out) in 4 bits with a scale for each row and group of columns."""
+    check(_lib.g2_quantize_q4(_p(W), w_dtype, int(in_out), _p(codes), _p(scales), N, K, group))
+
+
+def dequantize_q4(codes, scales, W, in_out, N, K, group):
+    """The fp32 values that 4-bit weights stand for."""
+    check(_lib.g2_dequantize_q4(_p(codes), _p(scales), _p(W), int(in_out), N, K, group))
+
+
+def matvec_q4(x, codes, scales, bias, residual, y, M, N, K, group, apply_gelu=0):
+    """y[M, N] = act(x[M, K] W^T + bias + residual) over 4-bit weights."""
+    check(_lib.g2_matvec_q4(_p(x), _p(codes), _p(scales), _p(bias), _p(residual), _p(y), M, N, K, group, int(apply_gelu)))
+
+
+def kv8_bytes(n_seq, n_head, max_seq):
+    """Bytes of an 8-bit K/V cache (0 where the sizes are not supported)."""
+    return _lib.g2_kv8_bytes(n_seq, n_head, max_seq)
+
+
+def kv8_work_bytes(n_seq, n_head):
+    """Bytes of attn_kv8's workspace."""
+    return _lib.g2_kv8_work_bytes(n_seq, n_head)
+
+
+def kv8_append(qkv, cache, pos, count, start, n_seq, T, n_head, max_seq):
+    """Appends rows of q/k/v to the cache at pos (device array, or None: at start)."""
+    check(_lib.g2_kv8_append(_p(qkv), _p(cache), _p(pos), _p(count), start, n_seq, T, n_head, max_seq))
+
+
+def kv8_read(cache, k, v, lens, T_kv, start, T, n_seq, n_head, max_seq):
+    """Keys and values at positions start .. start + T - 1 that lie below a sequence's length, fp32."""
+    check(_lib.g2_kv8_read(_p(cache), _p(k), _p(v), _p(lens), T_kv, start, T, n_seq, n_head, max_seq))
+
+
+def attn_kv8(q, q_stride, cache, out, out_stride, lens, T_kv, n_seq, n_head, max_seq, scale, work):
+    """Attention of one query row per sequence over the 8-bit cache."""
+    check(_lib.g2_attn_kv8(_p(q), q_stride, _p(cache), _p(out), out_stride, _p(lens), T_kv, n_seq, n_head, max_seq,
+                           scale, _p(work)))
+
+
+def logits_work_bytes(rows):
+    """Bytes of apply_logit_rules' workspace (needed where a pick is wanted)."""
+    return _lib.g2_logits_work_bytes(rows)
+
+
+def logit_rules(ctx=None, ctx_len=None, max_ctx=0, repetition=1.0, frequency=0.0, presence=0.0, bias_id=None, bias=None,
+                n_bias=0, mask=None, mask_stride=0, forbid=-1):
+    """A g2_logit_rules: penalties for the context's ids, a list of biases, a mask of allowed ids, a forbidden id."""
+    return LogitRules(_p(ctx), _p(ctx_len), max_ctx, repetition, frequency, presence, _p(bias_id), _p(bias), n_bias, _p(mask),
+                      mask_stride, forbid)
+
+
+def apply_logit_rules(logits, out, pick, rows, V, rules, work):
+    """out = logits under the rules, pick = each row's greatest id; either may be None."""
+    check(_lib.g2_apply_logit_rules(_p(logits), _p(out), _p(pick), rows, V, C.byref(rules), _p(work)))
 
 
 # ---------------------------------------------------------------- host-only

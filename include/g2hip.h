@@ -168,6 +168,112 @@ int g2_attn_1q_noalloc(const float *qkv, const float *k_cache, const float *v_ca
 int g2_matvec_rows(const float *x, const void *W, int w_dtype, const float *bias,
                    const float *residual, float *y, int N, int K, int apply_gelu);
 
+/* ---- decode in fewer bits (no counterpart in the reference) ---------------
+ * 4-bit weights, an 8-bit K/V cache and rules on logits: a decode step that
+ * reads 4.1 to 4.5 bits a weight and 8 bits a cached value, and chooses its
+ * token without the host.  Same conventions as the operators above; none of
+ * these calls uses a buffer of the library, so a graph that recorded them
+ * shares nothing but its operands.  Each checks its arguments (also before
+ * g2_init) and refuses outputs that overlap its inputs, except where a line
+ * below allows it.  Device arrays of lengths, positions and ids are checked by
+ * the kernels: what they say outside the stated range is cut off or left out.
+ */
+
+/* 4-bit weights W[N,K] (output-major, as g2_matvec_rows): E2M1 values 0, 0.5,
+ * 1, 1.5, 2, 3, 4, 6 and their negatives times a bf16 scale for each row and
+ * `group` (32, 64 or 128) columns, group 32 being the most exact and 4.5 bits
+ * a weight, group 128 4.125.  Any N, K >= 1 up to 2^24.  Bytes of the two
+ * buffers (0 if the sizes are not supported); both 16-byte aligned.  Their
+ * layout is that of the matrix instructions' operand:
+ *   codes: tiles of 16 rows [ceil(N/16)]; in a tile its columns 32 at a time
+ *     (256 bytes each), in chunks of four, the last with r <= 4 of them; in a
+ *     chunk [place 4][row 16][r][4 bytes], the bytes holding the columns
+ *     32 j + 8 place + 0..7 of the chunk, an even column in the low half;
+ *   scales: [ceil(N/16)][ceil(K/128)][row 16][128/group].
+ * Padding rows and columns have code 0, groups behind K scale 0. */
+size_t g2_q4_code_bytes(int N, int K);
+size_t g2_q4_scale_bytes(int N, int K, int group);
+/* Lays out W of w_dtype G2_F32 or G2_F16, [N,K] or, with in_out, [K,N] (the
+ * checkpoint's Conv1D order): scale = bf16(max |w| / 6) of the group, code =
+ * the value nearest to w / scale (fp32), ties to the even code.  A group with
+ * an infinity, a NaN or a magnitude above 2^96 gets a NaN scale and reads
+ * back as NaN. */
+int g2_quantize_q4(const void *W, int w_dtype, int in_out, uint8_t *codes,
+                   uint16_t *scales, int N, int K, int group);
+/* The values that codes and scales stand for, fp32, [N,K] or [K,N]. */
+int g2_dequantize_q4(const uint8_t *codes, const uint16_t *scales, float *W,
+                     int in_out, int N, int K, int group);
+/* y[M,N] = act(x[M,K] W^T + bias[n] + residual[m,n]) for M activation rows
+ * (one token of M sequences, or M tokens), fp32 accuracy in x and in the sums;
+ * bias and residual may be NULL, residual == y is legal; 8 rows share one
+ * reading of the weights. */
+int g2_matvec_q4(const float *x, const uint8_t *codes, const uint16_t *scales,
+                 const float *bias, const float *residual, float *y,
+                 int M, int N, int K, int group, int apply_gelu);
+
+/* 8-bit K/V cache of n_seq sequences, n_head heads of 64 dims (D = 64 n_head),
+ * max_seq positions: blocks of 16 positions of a head hold int8 codes and one
+ * fp32 scale (max |x| / 127) for keys and one for values; the positions of a
+ * sequence's last, incomplete block stand in fp32 until it is full, so what a
+ * cache holds does not depend on how its positions were appended.  A block
+ * with an infinity or NaN reads back as NaN.  One buffer, 16-byte aligned, no
+ * initial state: g2_kv8_bytes of it (0 if the sizes are not supported), with
+ * blocks = ceil(max_seq / 16):
+ *   codes  int8 [n_seq][n_head][blocks][K, V][16][64]
+ *   scales fp32 [n_seq][n_head][blocks][K, V], padded to 256 bytes
+ *   last   fp32 [n_seq][n_head][K, V][16][64]
+ * A sequence may be cut back to a length in its last block or to whole blocks
+ * and appended to from there. */
+size_t g2_kv8_bytes(int n_seq, int n_head, int max_seq);
+/* g2_split_kv for this cache: rows qkv[n_seq][T][3 D] (keys at column D, values
+ * at 2 D) go to positions p .. p + c - 1 of their sequence; p = pos[s], or
+ * start where pos is NULL; c = count[s] at most T, or T where count is NULL
+ * (rows behind the count are not read).  Positions outside 0..max_seq-1 are
+ * left out, a sequence whose p is outside altogether. */
+int g2_kv8_append(const float *qkv, void *cache, const int *pos, const int *count,
+                  int start, int n_seq, int T, int n_head, int max_seq);
+/* The values at positions start .. start + T - 1 of every sequence, k and v
+ * [n_seq][T][D] fp32; a sequence's length is len[s] at most T_kv, or T_kv where
+ * len is NULL, and rows at or behind it are left as they were. */
+int g2_kv8_read(const void *cache, float *k, float *v, const int *len, int T_kv,
+                int start, int T, int n_seq, int n_head, int max_seq);
+/* Bytes of g2_attn_kv8's workspace (0 if the sizes are not supported). */
+size_t g2_kv8_work_bytes(int n_seq, int n_head);
+/* Attention of one query row per sequence over its cached positions (the
+ * fused g2_attn_1q over this cache): row s of q begins at q + s * q_stride (a
+ * qkv row serves: its queries are the first D), row s of out at out + s *
+ * out_stride, strides in floats.  Lengths as in g2_kv8_read; a length of 0
+ * gives zeros.  The cache must hold what g2_kv8_append left at these lengths.
+ * work: g2_kv8_work_bytes, 4-byte aligned, for this call alone while it runs. */
+int g2_attn_kv8(const float *q, int q_stride, const void *cache, float *out,
+                int out_stride, const int *len, int T_kv, int n_seq, int n_head,
+                int max_seq, float scale, float *work);
+
+/* What may become of a row of logits before its token is chosen (pointers are
+ * device arrays; NULL or 0 where a rule is not wanted). */
+typedef struct {
+    const int *ctx;         /* [rows][max_ctx] ids so far (outside 0..V-1: ignored)      */
+    const int *ctx_len;     /* [rows] how many of them count; NULL: max_ctx              */
+    int max_ctx;
+    float repetition;       /* ids of the context: l > 0 ? l / r : l * r; 1 or 0: none   */
+    float frequency;        /* then minus this for each time an id occurs                */
+    float presence;         /* then minus this                                           */
+    const int *bias_id;     /* [n_bias] ids whose logit gets bias added after that       */
+    const float *bias;      /*   (an id that is there twice: its later entry)            */
+    int n_bias;
+    const uint32_t *mask;   /* bit v % 32 of word v / 32: whether id v is allowed, else  */
+    int mask_stride;        /*   -infinity; words from row to row, 0: one mask for all   */
+    int forbid;             /* an id that is never allowed, -1: none                     */
+} g2_logit_rules;
+/* Bytes of g2_apply_logit_rules' workspace (used where pick is wanted). */
+size_t g2_logits_work_bytes(int rows);
+/* out[rows,V] = logits under the rules (NULL: not wanted; out == logits is
+ * legal) and pick[r] = the id of the greatest (NULL: not wanted): the lowest
+ * of equal ones, NaN never, -1 where nothing is above -infinity.  The device
+ * form of g2_sample_greedy.  1 <= V <= 262144. */
+int g2_apply_logit_rules(const float *logits, float *out, int *pick, int rows,
+                         int V, const g2_logit_rules *rules, void *work);
+
 /* ---- configuration, weights, model (main.c:272-331, 1137-1512, 1739-1904) -- */
 
 typedef struct {
