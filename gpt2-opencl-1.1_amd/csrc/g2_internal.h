@@ -31,6 +31,18 @@ extern "C" {
     X(ROWS_##E##_F32_256X8, "g2k_rows_" s "_f32_s256x8")                      \
     X(ROWS_##E##_F16_256X8, "g2k_rows_" s "_f16_s256x8")
 
+/* 4-bit products of 1 or up to 8 activation rows (MT), groups of 32, 64 and
+ * 128 (g2_lowbit.hip): KW waves to a work-group, which takes TR tiles, or as
+ * many as come to it with NC chunks of activations in a wave's registers. */
+#define G2_Q4MV_LIST(X, MT, KW, TR)                                           \
+    X(Q4_MV##MT##_##KW##_##TR##_32, "g2k_q4_mv" #MT "_" #KW "_" #TR "_32")    \
+    X(Q4_MV##MT##_##KW##_##TR##_64, "g2k_q4_mv" #MT "_" #KW "_" #TR "_64")    \
+    X(Q4_MV##MT##_##KW##_##TR##_128, "g2k_q4_mv" #MT "_" #KW "_" #TR "_128")
+#define G2_Q4MVH_LIST(X, MT, KW, NC)                                          \
+    X(Q4_MVH##MT##_##KW##_##NC##_32, "g2k_q4_mvh" #MT "_" #KW "_" #NC "_32")  \
+    X(Q4_MVH##MT##_##KW##_##NC##_64, "g2k_q4_mvh" #MT "_" #KW "_" #NC "_64")  \
+    X(Q4_MVH##MT##_##KW##_##NC##_128, "g2k_q4_mvh" #MT "_" #KW "_" #NC "_128")
+
 /* Kernel table: index -> symbol name in the gfx950 code object. */
 #define G2_KERNEL_LIST(X)                                                     \
     X(MVSK4_F32, "g2k_mvsk_f32_4") X(MVSK4_F16, "g2k_mvsk_f16_4")       \
@@ -96,10 +108,20 @@ extern "C" {
     X(SPLITK_EPI, "g2k_splitk_epi")                                           \
     X(LN_FOLD_F32, "g2k_ln_fold_f32") X(LN_FOLD_F16, "g2k_ln_fold_f16")       \
     X(Q4_PACK_F32, "g2k_q4_pack_f32") X(Q4_PACK_F16, "g2k_q4_pack_f16")       \
-    X(Q4_READ, "g2k_q4_read") X(Q4_MATVEC, "g2k_q4_matvec")                   \
+    X(Q4_PACK_T_F32, "g2k_q4_pack_t_f32")                                     \
+    X(Q4_PACK_T_F16, "g2k_q4_pack_t_f16")                                     \
+    X(Q4_READ, "g2k_q4_read") X(Q4_READ_T, "g2k_q4_read_t")                   \
+    G2_Q4MV_LIST(X, 1, 8, 1) G2_Q4MV_LIST(X, 1, 16, 1)                        \
+    G2_Q4MV_LIST(X, 8, 8, 1) G2_Q4MV_LIST(X, 8, 16, 1)                        \
+    G2_Q4MV_LIST(X, 8, 8, 2) G2_Q4MV_LIST(X, 8, 8, 4)                         \
+    G2_Q4MVH_LIST(X, 1, 8, 1) G2_Q4MVH_LIST(X, 1, 8, 2)                       \
+    G2_Q4MVH_LIST(X, 8, 8, 1) G2_Q4MVH_LIST(X, 8, 8, 2)                       \
+    G2_Q4MVH_LIST(X, 8, 16, 2)                                                \
     X(KV8_APPEND, "g2k_kv8_append") X(KV8_READ, "g2k_kv8_read")               \
-    X(KV8_ATTN, "g2k_kv8_attn")                                               \
-    X(LOGITS, "g2k_logits") X(LOGITS_PICK, "g2k_logits_pick")
+    X(KV8_ATTN1, "g2k_kv8_attn1") X(KV8_ATTN4, "g2k_kv8_attn4")               \
+    X(KV8_ATTN8, "g2k_kv8_attn8") X(KV8_JOIN, "g2k_kv8_join")                 \
+    X(LOGITS, "g2k_logits") X(LOGITS_WIDE, "g2k_logits_wide")                 \
+    X(LOGITS_PICK, "g2k_logits_pick")
 
 #define G2_ENUM_ENTRY(id, name) G2F_##id,
 enum { G2_KERNEL_LIST(G2_ENUM_ENTRY) G2F_COUNT };
@@ -174,6 +196,13 @@ int g2i_attn_out_groups(const float *scores, const float *v_cache, const float *
  * else partials, then merge. */
 int g2i_attn_one_launch(const float *q, const float *k_cache, const float *v_cache, const float *out, int T, int D, int S);
 int g2i_attn_launch(g2_attn1q_args *a, unsigned chunks);
+
+/* g2_matvec_q4's kernel (its form for groups of 32), waves to a work-group and
+ * work-groups to 8 activation rows. */
+int g2i_q4_form(int M, int N, int K, int *waves, unsigned *wgs);
+
+/* g2_attn_kv8's parts of a head, blocks to a part and waves to a work-group. */
+int g2i_kv8_form(long heads, int T_kv, int *span, int *waves);
 
 /* Whether np bytes at p and nq bytes at q share any. */
 static inline int g2i_overlap(const void *p, size_t np, const void *q, size_t nq)

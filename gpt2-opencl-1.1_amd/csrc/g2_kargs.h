@@ -435,7 +435,7 @@ typedef struct {
 } g2_kv8_attn_args;
 
 /* Rules on logits (g2_logit_rules): rows x parts work-groups, each a slice of
- * `slice` ids; part: the best (value, id) of each slice, [rows][parts]. */
+ * the ids; part: the best (value, id) of each slice, [rows][parts]. */
 typedef struct {
     const float *logits;
     float *out;
@@ -447,7 +447,7 @@ typedef struct {
     const float *bias;
     const uint32_t *mask;
     int max_ctx, n_bias, mask_stride, forbid;
-    int rows, V, slice, parts;
+    int rows, V, parts;
     float repetition, frequency, presence;
 } g2_logits_args;
 

@@ -14,6 +14,7 @@
 #define MAX_DIM (1 << 24)      /* N, K: products of two stay far inside 64 bits */
 #define MAX_SEQ (1 << 24)      /* positions of a cache */
 #define MAX_HEADS 1024
+#define MAX_VOCAB (1 << 18)
 
 static int aligned(const void *p, size_t a) { return (uintptr_t)p % a == 0; }
 static unsigned cdiv(long a, long b) { return (unsigned)((a + b - 1) / b); }
@@ -49,6 +50,15 @@ static int q4_check(const char *fn, const void *codes, const void *scales, int N
     return G2_OK;
 }
 
+/* Work-groups that lay out or read back: 64 rows of 128 columns of [K,N], two
+ * times 16 of [N,K]; the kernels stride over what is more. */
+static unsigned q4_groups(int N, int K, int in_out)
+{
+    const long chunks = g2l_chunks(K), tiles = g2l_tiles(N);
+    const long n = in_out ? (tiles + 3) / 4 * chunks : (tiles * chunks + 1) / 2;
+    return n < 1 << 20 ? (unsigned)n : 1u << 20;
+}
+
 int g2_quantize_q4(const void *W, int w_dtype, int in_out, uint8_t *codes, uint16_t *scales, int N, int K, int group)
 {
     int rc = q4_check("g2_quantize_q4", codes, scales, N, K, group);
@@ -61,8 +71,8 @@ int g2_quantize_q4(const void *W, int w_dtype, int in_out, uint8_t *codes, uint1
         return g2i_err(G2_E_ARG, "g2_quantize_q4: overlapping buffers");
     if ((rc = ready())) return rc;
     g2_q4_args a = { W, codes, scales, NULL, N, K, group, in_out ? 1 : 0 };
-    const long items = g2l_tiles(N) * 16 * g2l_chunks(K) * (128 / group);
-    return g2i_launch(w_dtype == G2_F16 ? G2F_Q4_PACK_F16 : G2F_Q4_PACK_F32, strided(items), 1, 256, &a);
+    if (in_out) return g2i_launch(w_dtype == G2_F16 ? G2F_Q4_PACK_T_F16 : G2F_Q4_PACK_T_F32, q4_groups(N, K, 1), 1, 256, &a);
+    return g2i_launch(w_dtype == G2_F16 ? G2F_Q4_PACK_F16 : G2F_Q4_PACK_F32, q4_groups(N, K, 0), 1, 256, &a);
 }
 
 int g2_dequantize_q4(const uint8_t *codes, const uint16_t *scales, float *W, int in_out, int N, int K, int group)
@@ -75,7 +85,49 @@ int g2_dequantize_q4(const uint8_t *codes, const uint16_t *scales, float *W, int
         return g2i_err(G2_E_ARG, "g2_dequantize_q4: overlapping buffers");
     if ((rc = ready())) return rc;
     g2_q4_args a = { NULL, (uint8_t *)codes, (uint16_t *)scales, W, N, K, group, in_out ? 1 : 0 };
-    return g2i_launch(G2F_Q4_READ, strided((long)N * K), 1, 256, &a);
+    return g2i_launch(in_out ? G2F_Q4_READ_T : G2F_Q4_READ, q4_groups(N, K, in_out), 1, 256, &a);
+}
+
+/* The kernel of a product.  Two forms: the loop (a work-group of 8 or 16 waves
+ * takes TR tiles of 16 rows, each wave every 8th or 16th chunk of 128 columns)
+ * and the held form (fewer work-groups, which keep their chunks' activations
+ * and take tiles in turn).  us in a replayed graph, matrices that no cache
+ * holds, groups of 32 (of 128 where two figures stand):
+ *  - one row: the loop over single tiles; 16 waves for the few tiles of long
+ *    columns (1600 x 6400 5.1, with 8 waves 5.5; 1600 x 1600 3.4 both); the
+ *    held form from 2048 tiles on, where splitting the activations anew for
+ *    each tile costs most (50257 x 1600 11.0 and 9.9, loop 13.9 and 13.0, of 2
+ *    tiles 13.5 and 11.2; 50257 x 768 7.4, 8.3; but 16000 x 1600 6.1, 5.5);
+ *  - up to 8 rows, whose activations take longer to split: 16 waves up to 128
+ *    tiles (1600 x 1600 4.4, 4.7; 1600 x 6400 8.2, 9.4); 2 tiles from 256, 4
+ *    from 512 on (6400 x 1600 6.2, 5.7, 6.6 for 1, 2, 4; 10000 x 6400 22, 18,
+ *    15); held from 2048 tiles (50257 x 1600 14.9, loop 18.8), with 16 waves
+ *    and K to 4096 from 512 (12000 x 4000 10.0, loop 11.5).
+ * Work-groups of the held form: as many as the registers leave resident. */
+int g2i_q4_form(int M, int N, int K, int *waves, unsigned *wgs)
+{
+    const long tiles = g2l_tiles(N), chunks = g2l_chunks(K);
+    long most = 0;
+    int fid, tr = 1;
+    *waves = 8;
+    if (tiles >= 2048 && chunks <= 16) {
+        most = M == 1 || chunks <= 8 ? 768 : 512;
+        fid = M == 1 ? (chunks <= 8 ? G2F_Q4_MVH1_8_1_32 : G2F_Q4_MVH1_8_2_32)
+                     : (chunks <= 8 ? G2F_Q4_MVH8_8_1_32 : G2F_Q4_MVH8_8_2_32);
+    } else if (M > 1 && tiles >= 512 && chunks > 16 && chunks <= 32) {
+        most = 256;
+        *waves = 16;
+        fid = G2F_Q4_MVH8_16_2_32;
+    } else if (tiles <= 128 && chunks > (M == 1 ? 16 : 8)) {
+        *waves = 16;
+        fid = M == 1 ? G2F_Q4_MV1_16_1_32 : G2F_Q4_MV8_16_1_32;
+    } else if (M == 1) fid = G2F_Q4_MV1_8_1_32;
+    else {
+        tr = tiles < 256 ? 1 : tiles < 512 ? 2 : 4;
+        fid = tr == 1 ? G2F_Q4_MV8_8_1_32 : tr == 2 ? G2F_Q4_MV8_8_2_32 : G2F_Q4_MV8_8_4_32;
+    }
+    *wgs = (unsigned)(most ? (tiles < most ? tiles : most) : (tiles + tr - 1) / tr);
+    return fid;
 }
 
 int g2_matvec_q4(const float *x, const uint8_t *codes, const uint16_t *scales, const float *bias, const float *residual,
@@ -93,8 +145,10 @@ int g2_matvec_q4(const float *x, const uint8_t *codes, const uint16_t *scales, c
         return g2i_err(G2_E_ARG, "g2_matvec_q4: the output overlaps an input");
     if ((rc = ready())) return rc;
     g2_q4mv_args a = { x, codes, scales, bias, residual, y, M, N, K, group, apply_gelu ? 1 : 0 };
-    if (!fits((long)N * 256)) return g2i_err(G2_E_LIMIT, "g2_matvec_q4: N=%d too large", N);
-    return g2i_launch(G2F_Q4_MATVEC, (unsigned)N, (unsigned)M, 256, &a);
+    int waves;
+    unsigned wgs;
+    const int fid = g2i_q4_form(M, N, K, &waves, &wgs);
+    return g2i_launch(fid + (group == 32 ? 0 : group == 64 ? 1 : 2), wgs, cdiv(M, 8), 64u * (unsigned)waves, &a);
 }
 
 /* ------------------------------------------------------------- 8-bit cache */
@@ -162,7 +216,31 @@ int g2_kv8_read(const void *cache, float *k, float *v, const int *len, int T_kv,
     const char *c = cache;
     g2_kv8_read_args a = { (const int8_t *)c, (const float *)(c + g2l_kv_scales(n_seq, n_head, nb)),
                            (const float *)(c + g2l_kv_last(n_seq, n_head, nb)), k, v, len, T_kv, start, T, n_seq, n_head, (int)nb };
-    return g2i_launch(G2F_KV8_READ, strided((long)(n / 2)), 1, 256, &a);
+    return g2i_launch(G2F_KV8_READ, strided((long)(n / 16)), 1, 256, &a);
+}
+
+/* Parts of a head's positions, blocks to a part and waves to a work-group.  us
+ * in a replayed graph, caches that no cache holds:
+ *  - one launch up to 1024 positions, and for 256 heads and more of any length;
+ *    beyond, parts of 256 positions and more, as many as 512 work-groups (16
+ *    heads x 2000 9.0 whole, 7.4 in parts; 16 x 4000 10.4 in 3 parts, 7.9 in
+ *    15; 25 x 1024 6.4 and 7.1; 256 x 4000 27.0 and 28.3);
+ *  - a wave takes 64 positions at a time: one wave up to 64 (12 heads 3.3, four
+ *    waves 3.7), for many heads up to 128 (1600 heads 8.7, 9.9), four up to 512
+ *    (200 heads x 512 5.7, eight 6.0), eight beyond (25 x 1024 6.4, four 6.7,
+ *    sixteen 6.7). */
+int g2i_kv8_form(long heads, int T_kv, int *span, int *waves)
+{
+    const long blocks = g2l_blocks(T_kv) > 0 ? g2l_blocks(T_kv) : 1;
+    long splits = 1;
+    if (blocks > 64 && heads < 256) {
+        splits = blocks / 16 < 512 / heads ? blocks / 16 : 512 / heads;
+        if (splits > G2L_SPLITS) splits = G2L_SPLITS;
+    }
+    *span = (int)((blocks + splits - 1) / splits);
+    splits = (blocks + *span - 1) / *span;
+    *waves = *span <= 4 || (*span <= 8 && heads * splits >= 512) ? 1 : *span <= 32 ? 4 : 8;
+    return (int)splits;
 }
 
 int g2_attn_kv8(const float *q, int q_stride, const void *cache, float *out, int out_stride, const int *len, int T_kv,
@@ -193,7 +271,13 @@ int g2_attn_kv8(const float *q, int q_stride, const void *cache, float *out, int
     a.q_stride = n_seq > 1 ? q_stride : 0; a.out_stride = n_seq > 1 ? out_stride : 0;
     a.T_kv = T_kv; a.S = n_seq; a.NH = n_head; a.blocks = (int)nb;
     a.scale = scale;
-    return g2i_launch(G2F_KV8_ATTN, (unsigned)(n_seq * n_head), 1, 64, &a);
+    const long heads = (long)n_seq * n_head;
+    int waves;
+    a.splits = g2i_kv8_form(heads, T_kv, &a.span, &waves);
+    rc = g2i_launch(waves == 1 ? G2F_KV8_ATTN1 : waves == 4 ? G2F_KV8_ATTN4 : G2F_KV8_ATTN8, (unsigned)(heads * a.splits), 1,
+                    64u * (unsigned)waves, &a);
+    if (!rc && a.splits > 1) rc = g2i_launch(G2F_KV8_JOIN, (unsigned)heads, 1, 256, &a);
+    return rc;
 }
 
 /* --------------------------------------------------------- rules on logits */
@@ -207,8 +291,8 @@ int g2_apply_logit_rules(const float *logits, float *out, int *pick, int rows, i
 {
     if (!logits || !rules || (!out && !pick)) return g2i_err(G2_E_ARG, "g2_apply_logit_rules: NULL buffer");
     if (rows < 1 || V < 1) return g2i_err(G2_E_ARG, "g2_apply_logit_rules: rows and V must be positive");
-    if (!logits_rows(rows) || V > G2L_PARTS * G2L_SLICE)
-        return g2i_err(G2_E_LIMIT, "g2_apply_logit_rules: %d rows of %d: at most %d of %d", rows, V, 1 << 16, G2L_PARTS * G2L_SLICE);
+    if (!logits_rows(rows) || V > MAX_VOCAB)
+        return g2i_err(G2_E_LIMIT, "g2_apply_logit_rules: %d rows of %d: at most %d of %d", rows, V, 1 << 16, MAX_VOCAB);
     const g2_logit_rules *r = rules;
     if (r->max_ctx < 0 || r->n_bias < 0 || (r->max_ctx && !r->ctx) || (r->n_bias && (!r->bias_id || !r->bias)))
         return g2i_err(G2_E_ARG, "g2_apply_logit_rules: bad context or bias list");
@@ -240,9 +324,9 @@ int g2_apply_logit_rules(const float *logits, float *out, int *pick, int rows, i
     a.mask = r->mask; a.mask_stride = r->mask_stride; a.forbid = r->forbid;
     a.rows = rows; a.V = V;
     a.repetition = r->repetition > 0.f ? r->repetition : 1.f; a.frequency = r->frequency; a.presence = r->presence;
-    a.slice = V > 1024 * G2L_PARTS ? (int)cdiv(V, G2L_PARTS) : 1024;
-    a.parts = (int)cdiv(V, a.slice);
-    rc = g2i_launch(G2F_LOGITS, (unsigned)(rows * a.parts), 1, 256, &a);
+    const int wide = cdiv(V, G2L_SLICE) > G2L_PARTS || (long)rows * cdiv(V, G2L_SLICE) > 512;
+    a.parts = (int)cdiv(V, wide ? G2L_SLICE_WIDE : G2L_SLICE);
+    rc = g2i_launch(wide ? G2F_LOGITS_WIDE : G2F_LOGITS, (unsigned)(rows * a.parts), 1, wide ? 1024 : 256, &a);
     if (!rc && pick) rc = g2i_launch(G2F_LOGITS_PICK, (unsigned)rows, 1, 64, &a);
     return rc;
 }

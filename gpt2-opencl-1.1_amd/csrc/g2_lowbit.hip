@@ -35,86 +35,622 @@ __device__ __forceinline__ uint16_t q4_scale(unsigned amax)
     return f_bf16(__uint_as_float(amax) / 6.0f);
 }
 
-__device__ __forceinline__ unsigned q4_code(float w, float s)
+/* The codes of eight weights over a scale.  The conversion rounds a value to
+ * the nearest code, ties to even and at most 6, as the definition does; it is
+ * given the quotient correctly rounded: w / s from the reciprocal and one step
+ * on the remainder, exact where neither leaves the normal range (the division
+ * itself elsewhere).  A code of -0 becomes 0; a group's scale of 0 or NaN has
+ * codes 0. */
+__device__ __forceinline__ unsigned q4_codes(const float w[8], float s)
 {
-    const float q = w / s, a = fabsf(q);
-    const unsigned c = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.0f);
-    return s > 0.f && c ? c | (q < 0.f ? 8u : 0u) : 0u;
+    unsigned c = 0;
+    if (s > 0x1p-100f && s < 0x1p+100f) {
+        const float r = 1.0f / s;
+        float q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float q0 = w[i] * r;
+            q[i] = fmaf(fmaf(-q0, s, w[i]), r, q0);
+        }
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, q[0], q[1], 1.0f, 0);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, q[2], q[3], 1.0f, 1);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, q[4], q[5], 1.0f, 2);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, q[6], q[7], 1.0f, 3);
+    } else if (s > 0.f) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const unsigned b = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, w[i] / s, w[i + 1] / s, 1.0f, 0);
+            c |= (b & 255) << 4 * i;
+        }
+    }
+    const unsigned mag = c & 0x77777777u;
+    return c & (0x77777777u | ((mag + 0x77777777u) & 0x88888888u));
 }
 
-__device__ __forceinline__ float q4_value(unsigned code)
+/* The largest magnitude (as bits) among the lanes of a group: four lanes have
+ * the 32 columns of a step, 16 a chunk. */
+template <int CTRL> __device__ __forceinline__ unsigned dpp_umax(unsigned v)
 {
-    const unsigned e = (code >> 1) & 3, m = code & 1;
-    const float v = e ? (float)((2 + m) << e) * 0.25f : 0.5f * (float)m;
-    return code & 8 ? -v : v;
+    const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+    return o > v ? o : v;
+}
+__device__ __forceinline__ unsigned q4_group_max(unsigned amax, int group)
+{
+    amax = dpp_umax<0xB1>(amax);                   /* quad: lanes 1 0 3 2 */
+    amax = dpp_umax<0x4E>(amax);                   /* 2 3 0 1 */
+    if (group > 32) amax = dpp_umax<0x141>(amax);  /* half rows of 8, mirrored */
+    if (group > 64) amax = dpp_umax<0x140>(amax);  /* rows of 16, mirrored */
+    return amax;
 }
 
-/* One thread per row and group. */
+/* Eight weights of a row from column k on, 0 behind the matrix. */
+template <typename WT> struct q4_raw { WT v[8]; };
+template <typename WT>
+__device__ __forceinline__ q4_raw<WT> q4_load8(const WT *W, long n, long k, long N, long K)
+{
+    typedef WT w8 __attribute__((ext_vector_type(8), aligned(sizeof(WT))));
+    q4_raw<WT> r;
+    if (n < N && k + 8 <= K) {
+        const w8 v = *(const w8 *)(W + n * K + k);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.v[i] = v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.v[i] = n < N && k + i < K ? W[n * K + k + i] : (WT)0.f;
+    }
+    return r;
+}
+
+/* Scale and codes of a lane's eight weights to their places: row r of tile t,
+ * step j and place p of chunk c. */
+template <typename WT>
+__device__ __forceinline__ void q4_pack8(const g2_q4_args &a, const q4_raw<WT> &raw, long t, long c, int r, int j, int p)
+{
+    float w[8];
+    unsigned amax = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        w[i] = (float)raw.v[i];
+        const unsigned u = __float_as_uint(w[i]) & 0x7FFFFFFF;
+        amax = u > amax ? u : amax;
+    }
+    const uint16_t sb = q4_scale(q4_group_max(amax, a.group));
+    const int steps = g2l_chunk_steps(a.K, c), per = a.group / 32;
+    if (j < steps) *(unsigned *)(a.codes + g2l_code_at(a.K, t, c, 16 * p + r) + 4 * j) = q4_codes(w, bf16_f(sb));
+    if (p == 0 && j % per == 0) a.scales[g2l_scale_at(a.K, a.group, t, c, r, j / per)] = sb;
+}
+
+/* W [N,K]: a work-group takes chunks of 16 rows x 128 columns, two at a time:
+ * thread = row, step, place, eight consecutive columns.  Bounded by HBM. */
 template <typename WT>
 __device__ void q4_pack_impl(const g2_q4_args &a)
 {
     const WT *W = (const WT *)a.W;
-    const int gpc = 128 / a.group;
-    const long groups = g2l_chunks(a.K) * gpc, rows = g2l_tiles(a.N) * 16;
-    for (long i = blockIdx.x * 256l + threadIdx.x; i < rows * groups; i += gridDim.x * 256l) {
-        const long n = i / groups, g = i % groups, t = n / 16;
-        const int r = (int)(n % 16);
-        const long k0 = g * a.group, k1 = k0 + a.group < 32 * g2l_steps(a.K) ? k0 + a.group : 32 * g2l_steps(a.K);
-        const size_t sn = a.in_out ? 1 : (size_t)a.K, sk = a.in_out ? (size_t)a.N : 1;
-        unsigned amax = 0;
-        for (long k = k0; k < k1; ++k)
-            if (n < a.N && k < a.K) {
-                const unsigned u = __float_as_uint(ldw<WT>(W, n * sn + k * sk)) & 0x7FFFFFFF;
-                amax = u > amax ? u : amax;
-            }
-        const uint16_t sb = q4_scale(amax);
-        const float s = bf16_f(sb);
-        a.scales[g2l_scale_at(a.K, a.group, t, g / gpc, r, (int)(g % gpc))] = sb;
-        for (long k = k0; k < k1; k += 2) {
-            unsigned b = 0;
-            for (int h = 0; h < 2; ++h)
-                if (n < a.N && k + h < a.K) b |= q4_code(ldw<WT>(W, n * sn + (k + h) * sk), s) << 4 * h;
-            const long c = k / 128;
-            const int j = (int)(k % 128 / 32), place = (int)(k % 32 / 8);
-            a.codes[g2l_code_at(a.K, t, c, 16 * place + r) + 4 * j + k % 8 / 2] = (uint8_t)b;
+    const int tid = threadIdx.x, r = tid >> 4, j = tid >> 2 & 3, p = tid & 3;
+    const long chunks = g2l_chunks(a.K), items = g2l_tiles(a.N) * chunks;
+    for (long i = blockIdx.x * 2l; i < items; i += gridDim.x * 2l) {
+        q4_raw<WT> w[2];
+        long t[2], c[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            t[u] = (i + u) / chunks;
+            c[u] = (i + u) % chunks;
+            w[u] = q4_load8<WT>(W, t[u] * 16 + r, c[u] * 128 + 32 * j + 8 * p, a.N, a.K);
         }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (i + u < items) q4_pack8<WT>(a, w[u], t[u], c[u], r, j, p);
     }
 }
 G2K void g2k_q4_pack_f32(const g2_q4_args a) { q4_pack_impl<float>(a); }
 G2K void g2k_q4_pack_f16(const g2_q4_args a) { q4_pack_impl<_Float16>(a); }
 
-__device__ __forceinline__ float q4_at(const uint8_t *codes, const uint16_t *scales, long K, int group, long n, long k)
+/* W [K,N]: 64 rows x 128 columns at a time through LDS (64 neighbouring
+ * values of a column are one run in memory). */
+#define Q4_TROW 65
+template <typename WT>
+__device__ void q4_pack_t_impl(const g2_q4_args &a)
 {
-    const long t = n / 16, c = k / 128;
-    const int r = (int)(n % 16), j = (int)(k % 128 / 32), place = (int)(k % 32 / 8);
-    const unsigned b = codes[g2l_code_at(K, t, c, 16 * place + r) + 4 * j + k % 8 / 2];
-    return q4_value(b >> 4 * (k & 1) & 15) * bf16_f(scales[g2l_scale_at(K, group, t, c, r, (int)(k % 128) / group)]);
+    __shared__ WT ws[128 * Q4_TROW];
+    const WT *W = (const WT *)a.W;
+    const int tid = threadIdx.x, r = tid >> 4, j = tid >> 2 & 3, p = tid & 3;
+    const long chunks = g2l_chunks(a.K), tiles = g2l_tiles(a.N), items = (tiles + 3) / 4 * chunks;
+    for (long i = blockIdx.x; i < items; i += gridDim.x) {
+        const long t0 = i / chunks * 4, c = i % chunks, n = t0 * 16 + (tid & 63);
+#pragma unroll 8
+        for (int k = tid >> 6; k < 128; k += 4)
+            ws[k * Q4_TROW + (tid & 63)] = n < a.N && c * 128 + k < a.K ? W[(c * 128 + k) * a.N + n] : (WT)0.f;
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (t0 + u < tiles) {
+                q4_raw<WT> w;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w.v[e] = ws[(32 * j + 8 * p + e) * Q4_TROW + 16 * u + r];
+                q4_pack8<WT>(a, w, t0 + u, c, r, j, p);
+            }
+        __syncthreads();
+    }
+}
+G2K void g2k_q4_pack_t_f32(const g2_q4_args a) { q4_pack_t_impl<float>(a); }
+G2K void g2k_q4_pack_t_f16(const g2_q4_args a) { q4_pack_t_impl<_Float16>(a); }
+
+/* The eight values of a lane's word of codes. */
+__device__ __forceinline__ void q4_values(unsigned w, float s, float v[8])
+{
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
+    const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
+    v[0] = a[0] * s; v[1] = a[1] * s; v[2] = b[0] * s; v[3] = b[1] * s;
+    v[4] = c[0] * s; v[5] = c[1] * s; v[6] = d[0] * s; v[7] = d[1] * s;
+}
+__device__ __forceinline__ unsigned q4_word(const g2_q4_args &a, long t, long c, int r, int j, int p, float *s)
+{
+    *s = bf16_f(a.scales[g2l_scale_at(a.K, a.group, t, c, r, 32 * j / a.group)]);
+    return j < g2l_chunk_steps(a.K, c) ? *(const unsigned *)(a.codes + g2l_code_at(a.K, t, c, 16 * p + r) + 4 * j) : 0u;
 }
 
-/* One thread per weight. */
+/* To [N,K]: threads as in the laying out. */
 G2K void g2k_q4_read(const g2_q4_args a)
 {
-    for (long i = blockIdx.x * 256l + threadIdx.x; i < (long)a.N * a.K; i += gridDim.x * 256l) {
-        const long n = a.in_out ? i % a.N : i / a.K, k = a.in_out ? i / a.N : i % a.K;
-        a.out[i] = q4_at(a.codes, a.scales, a.K, a.group, n, k);
+    const int tid = threadIdx.x, r = tid >> 4, j = tid >> 2 & 3, p = tid & 3;
+    const long chunks = g2l_chunks(a.K), items = g2l_tiles(a.N) * chunks;
+    for (long i = blockIdx.x * 2l; i < items; i += gridDim.x * 2l) {
+        unsigned w[2];
+        float s[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const long iu = i + u < items ? i + u : items - 1;
+            w[u] = q4_word(a, iu / chunks, iu % chunks, r, j, p, &s[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const long n = (i + u) / chunks * 16 + r, k = (i + u) % chunks * 128 + 32 * j + 8 * p;
+            if (i + u >= items || n >= a.N || k >= a.K) continue;
+            float v[8];
+            q4_values(w[u], s[u], v);
+            float *o = a.out + n * a.K + k;
+            if (k + 8 <= a.K) {
+                *(f32x4u *)o = f32x4{ v[0], v[1], v[2], v[3] };
+                *(f32x4u *)(o + 4) = f32x4{ v[4], v[5], v[6], v[7] };
+            } else
+                for (int e = 0; e < 8; ++e)
+                    if (k + e < a.K) o[e] = v[e];
+        }
     }
 }
 
-/* One work-group per output. */
-G2K void g2k_q4_matvec(const g2_q4mv_args a)
+/* To [K,N], through LDS. */
+G2K void g2k_q4_read_t(const g2_q4_args a)
 {
-    __shared__ float red[4];
-    const long n = blockIdx.x, m = blockIdx.y;
-    float s = 0.f;
-    for (long k = threadIdx.x; k < a.K; k += 256)
-        s = fmaf(q4_at(a.codes, a.scales, a.K, a.group, n, k), a.x[m * a.K + k], s);
-    s = block_sum(s, red);
-    if (threadIdx.x == 0) {
-        if (a.bias) s += a.bias[n];
-        if (a.res) s += a.res[m * a.N + n];
-        a.y[m * a.N + n] = a.gelu ? gelu_f(s) : s;
+    __shared__ float ws[128 * Q4_TROW];
+    const int tid = threadIdx.x, r = tid >> 4, j = tid >> 2 & 3, p = tid & 3;
+    const long chunks = g2l_chunks(a.K), tiles = g2l_tiles(a.N), items = (tiles + 3) / 4 * chunks;
+    for (long i = blockIdx.x; i < items; i += gridDim.x) {
+        const long t0 = i / chunks * 4, c = i % chunks, n = t0 * 16 + (tid & 63);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            float s, v[8];
+            const unsigned w = q4_word(a, t0 + u < tiles ? t0 + u : tiles - 1, c, r, j, p, &s);
+            q4_values(w, s, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ws[(32 * j + 8 * p + e) * Q4_TROW + 16 * u + r] = v[e];
+        }
+        __syncthreads();
+#pragma unroll 8
+        for (int k = tid >> 6; k < 128; k += 4)
+            if (n < a.N && c * 128 + k < a.K) a.out[(c * 128 + k) * a.N + n] = ws[k * Q4_TROW + (tid & 63)];
+        __syncthreads();
     }
 }
+
+/* ---- products: y = x W^T on the matrix cores.  A chunk of 128 columns of a
+ * tile of 16 rows is one 16-byte load a lane; the hardware's conversion makes
+ * fp16 of it (exact; two values an operation) and four 16x16x32 products of
+ * it, one operand the 16 weight rows, the other up to 8 activation rows, each
+ * as two fp16 parts: hi = fp16(x'), lo = fp16(x' - hi), x' the activation
+ * times a power of two that brings the largest of its 128 to 2^14..2^15.  hi +
+ * lo is within 2^-22 of x' (and the power of two within fp32's range, so any
+ * activations keep fp32 accuracy).  A group's scale multiplies its sum, the
+ * power of two a chunk's; all sums are fp32.
+ *
+ * The waves of a work-group take the chunks of the same TR tiles in turn and
+ * each splits only its own chunk of the activations; the sums of the waves
+ * meet in LDS, in order.  */
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+template <int I> __device__ __forceinline__ void q4_half(f16x8 &r, unsigned w)
+{
+    const f16x2 h = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, I);
+    r[2 * I] = h[0];
+    r[2 * I + 1] = h[1];
+}
+__device__ __forceinline__ f16x8 q4_operand(unsigned w)
+{
+    f16x8 r;
+    q4_half<0>(r, w);
+    q4_half<1>(r, w);
+    q4_half<2>(r, w);
+    q4_half<3>(r, w);
+    return r;
+}
+
+/* The power of two (and its inverse) that brings a value of these bits, the
+ * largest of its chunk, to 2^14..2^15; 2^126 at most, where every bit of the
+ * chunk's values lies within the parts' range. */
+struct q4_power { float down, up; };
+__device__ __forceinline__ q4_power q4_power_of(unsigned amax)
+{
+    const unsigned e = amax >> 23 > 15 ? amax >> 23 : 15;
+    return { __uint_as_float((268 - e) << 23), __uint_as_float((e - 14) << 23) };
+}
+
+/* hi and lo parts of two activations */
+__device__ __forceinline__ void q4_split(float a, float b, float down, f16x2 &hi, f16x2 &lo)
+{
+    hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(a * down, b * down));
+    lo[0] = (_Float16)__builtin_fmaf(a, down, -(float)hi[0]);
+    lo[1] = (_Float16)__builtin_fmaf(b, down, -(float)hi[1]);
+}
+
+template <int CTRL> __device__ __forceinline__ float dpp_max(float v)
+{
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true)));
+}
+
+#define Q4_XROW 136 /* halves from row to row of a wave's split activations: 128 and 16 bytes against bank conflicts */
+
+template <int MT> struct q4_x {
+    float v[MT == 1 ? 2 : 16];
+};
+
+/* The chunk's activations: MT == 1: two columns a lane; else lane 8 m + i has
+ * columns 16 i .. 16 i + 15 of row m. */
+template <int MT>
+__device__ __forceinline__ q4_x<MT> q4_load_x(const g2_q4mv_args &a, int m0, int c, int lane)
+{
+    q4_x<MT> x;
+    const int n = MT == 1 ? 2 : 16, m = m0 + (MT == 1 ? 0 : lane >> 3), k = 128 * c + n * (MT == 1 ? lane : lane & 7);
+    const float *p = a.x + (size_t)(m < a.M ? m : a.M - 1) * a.K; /* (a row behind the last: the last, not written) */
+    if (MT == 1 && 128 * c + 128 <= a.K) { /* (uniform) */
+        x.v[0] = p[k];
+        x.v[1] = p[k + 1];
+    } else if (MT > 1 && (128 * c + 128 <= a.K || a.K % 16 == 0)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 q = *(const f32x4u *)(p + (k < a.K ? k : 0) + 4 * i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x.v[(4 * i + e) % n] = k < a.K ? q[e] : 0.f;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < n; ++i) x.v[i] = p[k + i < a.K ? k + i : a.K - 1];
+#pragma unroll
+        for (int i = 0; i < n; ++i) x.v[i] = k + i < a.K ? x.v[i] : 0.f;
+    }
+    return x;
+}
+
+/* Splits them into xs ([part of row][Q4_XROW]); returns the inverse powers of
+ * two of the lane's own rows of the product: MT == 1: row 0; else rows
+ * 2 (lane / 16) and + 1.  Infinities (rare: their own path) are hi, beside lo
+ * 0, and do not count for the power of two; nor does a NaN, which is both. */
+template <int MT>
+__device__ __forceinline__ float q4_largest(float amax)
+{
+    amax = dpp_max<0xB1>(amax);  /* quad: lanes 1 0 3 2 */
+    amax = dpp_max<0x4E>(amax);  /* 2 3 0 1 */
+    amax = dpp_max<0x141>(amax); /* half rows of 8, mirrored */
+    if constexpr (MT == 1) {
+        amax = dpp_max<0x140>(amax); /* rows of 16, mirrored */
+        const int u = __float_as_int(amax);
+        const float r0 = __int_as_float(__builtin_amdgcn_readlane(u, 0)), r1 = __int_as_float(__builtin_amdgcn_readlane(u, 16));
+        const float r2 = __int_as_float(__builtin_amdgcn_readlane(u, 32)), r3 = __int_as_float(__builtin_amdgcn_readlane(u, 48));
+        amax = fmaxf(fmaxf(r0, r1), fmaxf(r2, r3));
+    }
+    return amax;
+}
+
+template <int MT>
+__device__ __forceinline__ void q4_split_x(const q4_x<MT> &x, _Float16 *xs, float *xe, int lane, float e[2])
+{
+    constexpr int N = MT == 1 ? 2 : 16;
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) amax = fmaxf(amax, fabsf(x.v[i]));
+    amax = q4_largest<MT>(amax);
+    const bool odd = __any(amax == INFINITY);
+    if (odd) {
+        amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) amax = fmaxf(amax, fabsf(x.v[i]) < INFINITY ? fabsf(x.v[i]) : 0.f);
+        amax = q4_largest<MT>(amax);
+    }
+    const q4_power own = q4_power_of(__float_as_uint(amax));
+    f16x2 hi[N / 2], lo[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) q4_split(x.v[2 * i], x.v[2 * i + 1], own.down, hi[i], lo[i]);
+    if (odd)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (fabsf(x.v[i]) == INFINITY) {
+                hi[i / 2][i % 2] = (_Float16)x.v[i];
+                lo[i / 2][i % 2] = (_Float16)0.f;
+            }
+    _Float16 *row = xs + (MT == 1 ? 0 : 2 * (lane >> 3)) * Q4_XROW + N * (MT == 1 ? lane : lane & 7);
+    if constexpr (MT == 1) {
+        *(f16x2 *)row = hi[0];
+        *(f16x2 *)(row + Q4_XROW) = lo[0];
+        e[0] = e[1] = own.up;
+    } else {
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            f16x8 h, l;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                h[i] = hi[4 * g + i / 2][i % 2];
+                l[i] = lo[4 * g + i / 2][i % 2];
+            }
+            *(f16x8 *)(row + 8 * g) = h;
+            *(f16x8 *)(row + Q4_XROW + 8 * g) = l;
+        }
+        if ((lane & 7) == 0) xe[lane >> 3] = own.up;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if constexpr (MT > 1) {
+        e[0] = xe[2 * (lane >> 4)];
+        e[1] = xe[2 * (lane >> 4) + 1];
+    }
+}
+
+/* Where a lane finds its weights in a tile.  A chunk of fewer than four steps
+ * is read as if it had four: what lies behind a lane's own bytes meets
+ * activations that are 0, and lanes that would read past the chunk's end read
+ * up to it and move the bytes to their places (q4_shift). */
+struct q4_lane {
+    unsigned whole, part; /* bytes into a chunk of four steps, of fewer */
+    int shift, last;      /* words to move there; the chunk of fewer steps, -1 */
+};
+__device__ __forceinline__ q4_lane q4_lane_of(const g2_q4mv_args &a, int lane)
+{
+    q4_lane l;
+    const int c = (int)g2l_chunks(a.K) - 1, steps = g2l_chunk_steps(a.K, c);
+    const unsigned at = lane * 4 * steps, most = 256 * steps - 16;
+    l.whole = 16 * lane;
+    l.part = at < most ? at : most;
+    l.shift = (at - l.part) / 4;
+    l.last = steps < 4 ? c : -1;
+    return l;
+}
+
+/* One load each of codes and scales, at a uniform base and the lane's offset
+ * and without a branch (behind a branch the compiler waits for every load in
+ * flight; 64-bit addresses per lane had cost as many operations as the
+ * products). */
+template <int G> struct q4_w {
+    u32x4 w;
+    uint16_t s[128 / G];
+};
+template <int G>
+__device__ __forceinline__ q4_w<G> q4_load_w(const uint8_t *codes, const uint16_t *scales, unsigned at, unsigned sat)
+{
+    constexpr int P = 128 / G;
+    typedef uint16_t sv __attribute__((ext_vector_type(P == 1 ? 2 : P)));
+    typedef unsigned int u32x4u __attribute__((ext_vector_type(4), aligned(4)));
+    q4_w<G> r;
+    r.w = *(const u32x4u *)(codes + at);
+    if constexpr (P == 1) r.s[0] = *(const uint16_t *)((const char *)scales + sat);
+    else {
+        const sv v = *(const sv *)((const char *)scales + sat);
+#pragma unroll
+        for (int g = 0; g < P; ++g) r.s[g] = v[g];
+    }
+    return r;
+}
+__device__ __forceinline__ void q4_shift(u32x4 &w, int n)
+{
+    if (n & 1) w = u32x4{ w[1], w[2], w[3], 0u };
+    if (n & 2) w = u32x4{ w[2], w[3], 0u, 0u };
+}
+
+/* Adds a chunk's products to the lane's sums: MT == 1: of row 0; else of rows
+ * 2 (lane / 16) and + 1; column lane % 16 of the tile. */
+template <int MT, int G>
+__device__ __forceinline__ void q4_products(const f16x8 x[4], const u32x4 &w, const uint16_t *scale, const float e[2], float *y)
+{
+    constexpr int P = 128 / G;
+    float s[2] = {};
+#pragma unroll
+    for (int g = 0; g < P; ++g) {
+        f32x4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 4 / P * g; j < 4 / P * (g + 1); ++j)
+            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[j], q4_operand(w[j]), d, 0, 0, 0);
+        const float sc = bf16_f(scale[g]);
+        s[0] = fmaf(sc, d[0] + d[1], s[0]);
+        if constexpr (MT > 1) s[1] = fmaf(sc, d[2] + d[3], s[1]);
+    }
+    y[0] = fmaf(s[0], e[0], y[0]);
+    if constexpr (MT > 1) y[1] = fmaf(s[1], e[1], y[1]);
+}
+template <int MT>
+__device__ __forceinline__ void q4_put(float (*red)[16], int lane, const float *y)
+{
+    if constexpr (MT == 1) {
+        if (lane < 16) red[0][lane] = y[0];
+    } else {
+        red[2 * (lane >> 4)][lane & 15] = y[0];
+        red[2 * (lane >> 4) + 1][lane & 15] = y[1];
+    }
+}
+
+/* The loop over long columns. */
+template <int MT, int KW, int TR, int G>
+__device__ void q4_matvec_impl(const g2_q4mv_args &a)
+{
+    constexpr int ROWS = MT == 1 ? 2 : 16, SB = 32 * (128 / G); /* bytes of a chunk's scales */
+    __shared__ _Float16 xs[KW][ROWS * Q4_XROW];
+    __shared__ float xe[KW][8];
+    __shared__ float red[KW][TR][MT][16];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tiles = (int)g2l_tiles(a.N), t0 = blockIdx.x * TR, m0 = blockIdx.y * 8, chunks = (int)g2l_chunks(a.K);
+    const q4_lane ql = q4_lane_of(a, lane);
+    const unsigned sat = (lane & 15) * (SB / 16);
+    const _Float16 *frag = xs[w] + (lane & (ROWS - 1)) * Q4_XROW + 8 * (lane >> 4);
+    const uint8_t *codes[TR];
+    const uint16_t *scales[TR];
+    float y[TR][2] = {};
+    q4_w<G> wn[TR];
+    q4_x<MT> xn;
+    auto load = [&](int c) {
+        xn = q4_load_x<MT>(a, m0, c, lane);
+#pragma unroll
+        for (int i = 0; i < TR; ++i)
+            wn[i] = q4_load_w<G>(codes[i] + c * 1024l, scales[i] + c * (SB / 2), c == ql.last ? ql.part : ql.whole, sat);
+    };
+#pragma unroll
+    for (int i = 0; i < TR; ++i) {
+        const int t = t0 + i < tiles ? t0 + i : tiles - 1; /* (a tile behind the last: the last again, not written) */
+        codes[i] = a.codes + g2l_code_at(a.K, t, 0, 0);
+        scales[i] = a.scales + g2l_scale_at(a.K, G, t, 0, 0, 0);
+    }
+    if (w < chunks) load(w);
+    for (int c = w; c < chunks; c += KW) {
+        q4_w<G> wc[TR];
+        const q4_x<MT> xc = xn;
+#pragma unroll
+        for (int i = 0; i < TR; ++i) wc[i] = wn[i];
+        if (c + KW < chunks) load(c + KW);
+        float e[2];
+        q4_split_x<MT>(xc, xs[w], xe[w], lane, e);
+        f16x8 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = *(const f16x8 *)(frag + 32 * j);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < TR; ++i) {
+            if (c == ql.last) q4_shift(wc[i].w, ql.shift);
+            q4_products<MT, G>(x, wc[i].w, wc[i].s, e, y[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TR; ++i) q4_put<MT>(red[w][i], lane, y[i]);
+    __syncthreads();
+    for (int o = tid; o < TR * MT * 16; o += KW * 64) {
+        const int r = o & 15, m = o / 16 % MT, i = o / 16 / MT;
+        const long n = (t0 + i) * 16l + r;
+        if (n >= a.N || m0 + m >= a.M) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < KW; ++k) v += red[k][i][m][r];
+        const size_t at = (size_t)(m0 + m) * a.N + n;
+        if (a.bias) v += a.bias[n];
+        if (a.res) v += a.res[at];
+        a.y[at] = a.gelu ? gelu_f(v) : v;
+    }
+}
+#define Q4_MATVEC(MT, KW, TR)                                                                                          \
+    extern "C" __global__ __launch_bounds__(64 * KW) void g2k_q4_mv##MT##_##KW##_##TR##_32(const g2_q4mv_args a)      \
+    { q4_matvec_impl<MT, KW, TR, 32>(a); }                                                                             \
+    extern "C" __global__ __launch_bounds__(64 * KW) void g2k_q4_mv##MT##_##KW##_##TR##_64(const g2_q4mv_args a)      \
+    { q4_matvec_impl<MT, KW, TR, 64>(a); }                                                                             \
+    extern "C" __global__ __launch_bounds__(64 * KW) void g2k_q4_mv##MT##_##KW##_##TR##_128(const g2_q4mv_args a)     \
+    { q4_matvec_impl<MT, KW, TR, 128>(a); }
+Q4_MATVEC(1, 8, 1)
+Q4_MATVEC(1, 16, 1)
+Q4_MATVEC(8, 8, 1)
+Q4_MATVEC(8, 16, 1)
+Q4_MATVEC(8, 8, 2)
+Q4_MATVEC(8, 8, 4)
+
+/* Held form: a wave's chunks of the activations stay in its registers for all
+ * tiles that the work-group takes. */
+template <int NC, int G> struct q4_stage {
+    q4_w<G> w[NC];
+    float bias, res;
+};
+
+template <int MT, int KW, int NC, int G>
+__device__ void q4_held_impl(const g2_q4mv_args &a)
+{
+    constexpr int ROWS = MT == 1 ? 2 : 16, SB = 32 * (128 / G);
+    __shared__ _Float16 xs[KW][ROWS * Q4_XROW];
+    __shared__ float xe[KW][8];
+    __shared__ float red[2][KW][MT][16];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tiles = (int)g2l_tiles(a.N), m0 = blockIdx.y * 8, chunks = (int)g2l_chunks(a.K), step = gridDim.x;
+    const q4_lane ql = q4_lane_of(a, lane);
+    unsigned at[NC], sat[NC];
+    q4_x<MT> xr[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int c = w + KW * i < chunks ? w + KW * i : chunks - 1;
+        xr[i] = q4_load_x<MT>(a, m0, c, lane);
+        at[i] = c * 1024 + (c == ql.last ? ql.part : ql.whole);
+        sat[i] = c * SB + (lane & 15) * (SB / 16);
+    }
+    const size_t tile_codes = g2l_code_at(a.K, 1, 0, 0), tile_scales = g2l_scale_at(a.K, G, 1, 0, 0, 0);
+    /* this thread's output of a tile: row r of the tile, activation row m */
+    const int r = tid & 15, m = tid >> 4, mr = m0 + m < a.M ? m : a.M - 1 - m0;
+    const float *bias = a.bias ? a.bias : a.x, *res = a.res ? a.res + (size_t)m0 * a.N : a.x; /* (readable, not used) */
+    auto load = [&](int t) {
+        q4_stage<NC, G> s;
+        t = t < tiles ? t : tiles - 1;
+        const unsigned left = a.N - 16 * t - 1, n = (unsigned)r < left ? r : left;
+        s.bias = bias[a.bias ? 16l * t + n : 0];
+        s.res = res[a.res ? (size_t)mr * a.N + 16l * t + n : 0];
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+            s.w[i] = q4_load_w<G>(a.codes + t * tile_codes, a.scales + t * tile_scales, at[i], sat[i]);
+        return s;
+    };
+    q4_stage<NC, G> st = load(blockIdx.x);
+    f16x8 x[NC][4];
+    float e[NC][2];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        q4_split_x<MT>(xr[i], xs[w], xe[w], lane, e[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[i][j] = *(const f16x8 *)(xs[w] + (lane & (ROWS - 1)) * Q4_XROW + 8 * (lane >> 4) + 32 * j);
+        __builtin_amdgcn_wave_barrier();
+    }
+    int b = 0;
+    for (int t = blockIdx.x; t < tiles; t += step) {
+        b ^= 1;
+        float y[2] = {};
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            if (w + KW * i < chunks) {
+                if (w + KW * i == ql.last) q4_shift(st.w[i].w, ql.shift);
+                q4_products<MT, G>(x[i], st.w[i].w, st.w[i].s, e[i], y);
+            }
+        }
+        const float add = (a.bias ? st.bias : 0.f) + (a.res ? st.res : 0.f);
+        st = load(t + step);
+        q4_put<MT>(red[b][w], lane, y);
+        __syncthreads();
+        if (m < MT && 16l * t + r < a.N && m0 + m < a.M) {
+            float v = 0.f;
+#pragma unroll
+            for (int k = 0; k < KW; ++k) v += red[b][k][m][r];
+            v += add;
+            a.y[(size_t)(m0 + m) * a.N + 16l * t + r] = a.gelu ? gelu_f(v) : v;
+        }
+    }
+}
+#define Q4_HELD(MT, KW, NC)                                                                                            \
+    extern "C" __global__ __launch_bounds__(64 * KW) void g2k_q4_mvh##MT##_##KW##_##NC##_32(const g2_q4mv_args a)     \
+    { q4_held_impl<MT, KW, NC, 32>(a); }                                                                               \
+    extern "C" __global__ __launch_bounds__(64 * KW) void g2k_q4_mvh##MT##_##KW##_##NC##_64(const g2_q4mv_args a)     \
+    { q4_held_impl<MT, KW, NC, 64>(a); }                                                                               \
+    extern "C" __global__ __launch_bounds__(64 * KW) void g2k_q4_mvh##MT##_##KW##_##NC##_128(const g2_q4mv_args a)    \
+    { q4_held_impl<MT, KW, NC, 128>(a); }
+Q4_HELD(1, 8, 1)
+Q4_HELD(1, 8, 2)
+Q4_HELD(8, 8, 1)
+Q4_HELD(8, 8, 2)
+Q4_HELD(8, 16, 2)
 
 /* ======================================================================
  * 8-bit K/V cache: a block of 16 positions of one head holds the codes
@@ -199,47 +735,289 @@ __device__ __forceinline__ int kv8_length(const int *len, int T_kv, long s)
     return n < 0 ? 0 : n < T_kv ? n : T_kv;
 }
 
-/* One thread per value. */
+/* One thread per four dims of a position, keys and values; positions in the
+ * order of the output. */
 G2K void g2k_kv8_read(const g2_kv8_read_args a)
 {
-    const int D = a.NH * G2L_DH;
-    const long n = (long)a.S * a.T * D;
-    for (long i = blockIdx.x * 256l + threadIdx.x; i < 2 * n; i += gridDim.x * 256l) {
-        const int kv = i >= n;
-        const long j = kv ? i - n : i, s = j / D / a.T;
-        const int c = (int)(j % D), p = a.start + (int)(j / D % a.T), len = kv8_length(a.len, a.T_kv, s);
+    const int quads = a.NH * (G2L_DH / 4);
+    const long n = (long)a.S * a.T * quads;
+    for (long i = blockIdx.x * 256l + threadIdx.x; i < n; i += gridDim.x * 256l) {
+        const long row = n <= UINT32_MAX ? (unsigned)i / (unsigned)quads : i / quads;
+        const int q = (int)(i - row * quads), h = q / (G2L_DH / 4), d = q % (G2L_DH / 4) * 4;
+        const long s = a.S == 1 ? 0 : (unsigned)row / (unsigned)a.T;
+        const int p = a.start + (int)(row - s * a.T), len = kv8_length(a.len, a.T_kv, s);
         if (p >= len) continue;
-        const int h = c / G2L_DH, at = p % G2L_BLOCK * G2L_DH + c % G2L_DH, b = p / G2L_BLOCK;
-        const float v = b < len / G2L_BLOCK
-                            ? (float)a.codes[g2l_kv_code_at(a.NH, a.blocks, s, h, b, kv) + at] *
-                                  a.scales[g2l_kv_scale_at(a.NH, a.blocks, s, h, b, kv)]
-                            : a.last[g2l_kv_last_at(a.NH, s, h, kv) + at];
-        (kv ? a.v : a.k)[j] = v;
+        const int at = p % G2L_BLOCK * G2L_DH + d, b = p / G2L_BLOCK;
+        f32x4 kv[2];
+        if (b < len / G2L_BLOCK) {
+            const size_t c = g2l_kv_code_at(a.NH, a.blocks, s, h, b, 0) + at;
+            const float *sc = a.scales + g2l_kv_scale_at(a.NH, a.blocks, s, h, b, 0);
+#pragma unroll
+            for (int i2 = 0; i2 < 2; ++i2) {
+                const unsigned w = *(const unsigned *)(a.codes + c + i2 * (G2L_BLOCK * G2L_DH));
+                const float f = sc[i2];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) kv[i2][e] = (float)(int8_t)(w >> 8 * e) * f;
+            }
+        } else {
+            const float *l = a.last + g2l_kv_last_at(a.NH, s, h, 0) + at;
+            kv[0] = *(const f32x4 *)l;
+            kv[1] = *(const f32x4 *)(l + G2L_BLOCK * G2L_DH);
+        }
+        *(f32x4u *)(a.k + 4 * i) = kv[0];
+        *(f32x4u *)(a.v + 4 * i) = kv[1];
     }
 }
 
-/* One wave per sequence and head, a lane per dim, one position at a time
- * with the running maximum and sum of the softmax. */
-extern "C" __global__ __launch_bounds__(64) void g2k_kv8_attn(const g2_kv8_attn_args a)
+/* ---- single-query attention.  A wave takes four blocks (64 positions) at a
+ * time: 1 KB of keys and 1 KB of values each, every lane 16 bytes of one
+ * position, so that the codes are used where they were loaded: the four lanes
+ * of a position add up its score, and each weighs its own 16 dims of the
+ * value.  Each position slot (16 a wave) keeps a running maximum and sum of
+ * its own; they meet once, at the end: over the lanes, over the waves in LDS,
+ * and over the parts of a long sequence in a second launch.  Scores are held
+ * in units of log 2, the queries carrying the factor.  */
+struct kv8_sum {
+    float m, l, o[16];
+};
+
+__device__ __forceinline__ float kv8_byte(unsigned w, int i) { return (float)(int8_t)(w >> 8 * i); }
+
+__device__ __forceinline__ float dpp_quad_sum(float v)
 {
-    const int h = blockIdx.x % a.NH, d = threadIdx.x;
-    const long s = blockIdx.x / a.NH;
-    const int len = kv8_length(a.len, a.T_kv, s);
-    const float q = a.q[s * a.q_stride + h * G2L_DH + d];
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    for (int p = 0; p < len; ++p) {
-        const int b = p / G2L_BLOCK, at = p % G2L_BLOCK * G2L_DH + d;
-        float kv[2];
-        for (int i = 0; i < 2; ++i)
-            kv[i] = b < len / G2L_BLOCK ? (float)a.codes[g2l_kv_code_at(a.NH, a.blocks, s, h, b, i) + at] *
-                                              a.scales[g2l_kv_scale_at(a.NH, a.blocks, s, h, b, i)]
-                                        : a.last[g2l_kv_last_at(a.NH, s, h, i) + at];
-        const float x = wave_sum(q * kv[0]) * a.scale, top = fmaxf(m, x), f = expf(m - top), e = expf(x - top);
-        l = l * f + e;
-        o = o * f + e * kv[1];
-        m = top;
+    v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xF, 0xF, false)); /* lanes 1 0 3 2 */
+    return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xF, 0xF, false)); /* 2 3 0 1 */
+}
+
+/* The weight that a state of maximum m has beside one of maximum top (an empty
+ * state's maximum is -infinity; all empty: 0). */
+__device__ __forceinline__ float kv8_factor(float m, float top) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top); }
+
+/* Adds N positions' scores and values (codes times vs, or fp32) to a state. */
+template <int N, typename V>
+__device__ __forceinline__ void kv8_add(kv8_sum &a, const float *s, const float *vs, V value)
+{
+    float top = a.m;
+#pragma unroll
+    for (int u = 0; u < N; ++u) top = fmaxf(top, s[u]);
+    const float base = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f(a.m - base);
+    float p[N], l = 0.f;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        p[u] = __builtin_amdgcn_exp2f(s[u] - base);
+        l += p[u];
+        p[u] *= vs[u];
     }
-    a.out[s * a.out_stride + h * G2L_DH + d] = len ? o / l : 0.f;
+    a.l = fmaf(a.l, f, l);
+    a.m = top;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        float o = a.o[e] * f;
+#pragma unroll
+        for (int u = 0; u < N; ++u) o = fmaf(p[u], value(u, e), o);
+        a.o[e] = o;
+    }
+}
+
+/* Four blocks' codes and scales.  A block behind the last one of the part is
+ * the last again; the first four are asked for before the length is known, by
+ * the bound of the lengths, and may be none of the sequence's. */
+struct kv8_four {
+    u32x4 k[4], v[4];
+    float sk[4], sv[4];
+};
+__device__ __forceinline__ kv8_four kv8_load(const int8_t *codes, const float *scales, int b, int last, int lane)
+{
+    kv8_four r;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int bu = b + u < last ? b + u : last;
+        const int8_t *p = codes + (size_t)bu * (2 * G2L_BLOCK * G2L_DH) + 16 * lane;
+        r.k[u] = *(const u32x4 *)p;
+        r.v[u] = *(const u32x4 *)(p + G2L_BLOCK * G2L_DH);
+        r.sk[u] = scales[2 * bu];
+        r.sv[u] = scales[2 * bu + 1];
+    }
+    return r;
+}
+
+/* Exchange with the lane whose number differs in one bit (4, 8; 16 and 32 below). */
+__device__ __forceinline__ float lane_xor4(float v)
+{
+    const int m = __builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xF, 0xF, false); /* i ^ 7 */
+    return __int_as_float(__builtin_amdgcn_mov_dpp(m, 0x1B, 0xF, 0xF, false));         /* i ^ 3 */
+}
+__device__ __forceinline__ float lane_xor8(float v)
+{
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xF, 0xF, false)); /* rows of 16 turned by 8 */
+}
+/* lo of this lane and its partner's where the lane's bit is 0, hi of both where it is 1 */
+__device__ __forceinline__ float lane_fold32(float lo, float hi)
+{
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(lo), __float_as_uint(hi), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+__device__ __forceinline__ float lane_fold16(float lo, float hi)
+{
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(lo), __float_as_uint(hi), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+__device__ __forceinline__ float slots_max(float v)
+{
+    v = fmaxf(v, lane_xor4(v));
+    v = fmaxf(v, lane_xor8(v));
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+template <int NW>
+__device__ void kv8_attn_impl(const g2_kv8_attn_args &a)
+{
+    __shared__ float part[NW][G2L_PART_FLOATS];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int t = lane >> 2, d0 = 16 * (lane & 3);
+    const int split = blockIdx.x % a.splits, h = blockIdx.x / a.splits % a.NH;
+    const long s = blockIdx.x / a.splits / a.NH;
+    const int8_t *codes = a.codes + g2l_kv_code_at(a.NH, a.blocks, s, h, 0, 0);
+    const float *scales = a.scales + g2l_kv_scale_at(a.NH, a.blocks, s, h, 0, 0);
+    const int b0 = split * a.span, bound = a.T_kv / G2L_BLOCK;
+    kv16 q = kv_load(a.q + s * a.q_stride + h * G2L_DH + d0);
+    kv8_four next = kv8_load(codes, scales, b0 + 4 * w, bound ? bound - 1 : 0, lane);
+    const int len = kv8_length(a.len, a.T_kv, s), full = len / G2L_BLOCK;
+    const int b1 = b0 + a.span < full ? b0 + a.span : full;
+    const float qf = a.scale * 1.44269504f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) q.v[e / 4][e % 4] *= qf;
+    kv8_sum st;
+    st.m = -INFINITY;
+    st.l = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) st.o[e] = 0.f;
+    for (int b = b0 + 4 * w; b < b1; b += 4 * NW) {
+        const kv8_four f = next;
+        if (b + 4 * NW < b1) next = kv8_load(codes, scales, b + 4 * NW, b1 - 1, lane);
+        float x[4], sv[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            float d = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) d = fmaf(q.v[e / 4][e % 4], kv8_byte(f.k[u][e / 4], e % 4), d);
+            x[u] = b + u < b1 ? dpp_quad_sum(d) * f.sk[u] : -INFINITY;
+            sv[u] = b + u < b1 ? f.sv[u] : 0.f;
+        }
+        kv8_add<4>(st, x, sv, [&](int u, int e) { return kv8_byte(f.v[u][e / 4], e % 4); });
+    }
+    /* the block that is not full, in the part that holds its place: the next wave in turn */
+    const int left = len % G2L_BLOCK;
+    if (left && full >= b0 && full < b0 + a.span && w == (full - b0 + 3) / 4 % NW) {
+        const float *p = a.last + g2l_kv_last_at(a.NH, s, h, 0) + t * G2L_DH + d0;
+        kv16 k = {}, v = {};
+        if (t < left) {
+            k = kv_load(p);
+            v = kv_load(p + G2L_BLOCK * G2L_DH);
+        }
+        float d = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) d = fmaf(q.v[e / 4][e % 4], k.v[e / 4][e % 4], d);
+        d = dpp_quad_sum(d);
+        const float x = t < left ? d : -INFINITY, one = 1.f;
+        kv8_add<1>(st, &x, &one, [&](int, int e) { return v.v[e / 4][e % 4]; });
+    }
+    /* the wave's 16 position slots: each step halves the dims that a lane keeps */
+    float top = slots_max(st.m);
+    const float f = kv8_factor(st.m, top);
+    float l = st.l * f;
+    l += lane_xor4(l);
+    l += lane_xor8(l);
+    l = lane_fold16(l, l);
+    l = lane_fold32(l, l);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) st.o[e] *= f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) st.o[e] = lane_fold32(st.o[e], st.o[e + 8]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) st.o[e] = lane_fold16(st.o[e], st.o[e + 4]);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const float lo = st.o[e] + lane_xor8(st.o[e]), hi = st.o[e + 2] + lane_xor8(st.o[e + 2]);
+        st.o[e] = lane & 8 ? hi : lo;
+    }
+    {
+        const float lo = st.o[0] + lane_xor4(st.o[0]), hi = st.o[1] + lane_xor4(st.o[1]);
+        st.o[0] = lane & 4 ? hi : lo;
+    }
+    if (NW > 1 || a.splits > 1) {
+        if (lane == 0) { part[w][0] = top; part[w][1] = l; }
+        part[w][2 + d0 + t] = st.o[0];
+        __syncthreads();
+        if (tid >= 64) return;
+        top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) top = fmaxf(top, part[i][0]);
+        float o = 0.f;
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            const float g = kv8_factor(part[i][0], top);
+            l = fmaf(part[i][1], g, l);
+            o = fmaf(part[i][2 + lane], g, o);
+        }
+        if (a.splits > 1) {
+            float *r = a.part + ((s * a.NH + h) * a.splits + split) * G2L_PART_FLOATS;
+            if (lane == 0) { r[0] = top; r[1] = l; }
+            r[2 + lane] = o;
+            return;
+        }
+        a.out[s * a.out_stride + h * G2L_DH + lane] = len ? o / l : 0.f;
+    } else
+        a.out[s * a.out_stride + h * G2L_DH + d0 + t] = len ? st.o[0] / l : 0.f;
+}
+extern "C" __global__ __launch_bounds__(64) void g2k_kv8_attn1(const g2_kv8_attn_args a) { kv8_attn_impl<1>(a); }
+extern "C" __global__ __launch_bounds__(256) void g2k_kv8_attn4(const g2_kv8_attn_args a) { kv8_attn_impl<4>(a); }
+extern "C" __global__ __launch_bounds__(512) void g2k_kv8_attn8(const g2_kv8_attn_args a) { kv8_attn_impl<8>(a); }
+
+/* Joins the parts of a head: four waves of eight parts each (all their loads
+ * at once: one after the other they took 11 us for 32), then the waves. */
+G2K void g2k_kv8_join(const g2_kv8_attn_args a)
+{
+    __shared__ float part[4][G2L_PART_FLOATS];
+    const int h = blockIdx.x % a.NH, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const long s = blockIdx.x / a.NH;
+    const float *r = a.part + (s * a.NH + h) * a.splits * G2L_PART_FLOATS;
+    float m[G2L_SPLITS / 4], l[G2L_SPLITS / 4], v[G2L_SPLITS / 4], top = -INFINITY, o = 0.f, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < G2L_SPLITS / 4; ++i) {
+        const int n = w * (G2L_SPLITS / 4) + i;
+        const float *p = r + (n < a.splits ? n : a.splits - 1) * G2L_PART_FLOATS;
+        m[i] = p[0];
+        l[i] = p[1];
+        v[i] = p[2 + lane];
+        if (n >= a.splits) m[i] = -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < G2L_SPLITS / 4; ++i) top = fmaxf(top, m[i]);
+#pragma unroll
+    for (int i = 0; i < G2L_SPLITS / 4; ++i) {
+        const float f = kv8_factor(m[i], top);
+        if (w * (G2L_SPLITS / 4) + i >= a.splits) continue;
+        sum = fmaf(l[i], f, sum);
+        o = fmaf(v[i], f, o);
+    }
+    if (lane == 0) { part[w][0] = top; part[w][1] = sum; }
+    part[w][2 + lane] = o;
+    __syncthreads();
+    if (w) return;
+    top = fmaxf(fmaxf(part[0][0], part[1][0]), fmaxf(part[2][0], part[3][0]));
+    sum = o = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float f = kv8_factor(part[i][0], top);
+        sum = fmaf(part[i][1], f, sum);
+        o = fmaf(part[i][2 + lane], f, o);
+    }
+    a.out[s * a.out_stride + h * G2L_DH + lane] = kv8_length(a.len, a.T_kv, s) ? o / sum : 0.f;
 }
 
 /* ======================================================================
@@ -249,41 +1027,74 @@ extern "C" __global__ __launch_bounds__(64) void g2k_kv8_attn(const g2_kv8_attn_
  * one pass over the slice's logits.  Every step is its own fp32 rounding (no
  * fused multiply-add), so equal logits stay equal.
  * ==================================================================== */
-G2K void g2k_logits(const g2_logits_args a)
+template <int THREADS, int QUADS>
+__device__ void logits_impl(const g2_logits_args &a)
 {
 #pragma clang fp contract(off)
-    __shared__ int hits[2 * G2L_SLICE]; /* [slice] counts, [slice] entry of the bias list + 1 */
-    __shared__ float bv[4];
-    __shared__ int bi[4];
+    constexpr int SLICE = THREADS * QUADS * 4;
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    __shared__ i32x4 hits[SLICE / 4], later[SLICE / 4]; /* counts; entry of the bias list + 1 */
+    __shared__ float bv[THREADS / 64];
+    __shared__ int bi[THREADS / 64];
     const int tid = threadIdx.x, row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
-    const int v0 = part * a.slice, nv = a.V - v0 < a.slice ? a.V - v0 : a.slice;
-    for (int i = tid; i < 2 * a.slice; i += 256) hits[i] = 0;
+    const int v0 = part * SLICE, nv = a.V - v0 < SLICE ? a.V - v0 : SLICE;
+    const float *in = a.logits + (size_t)row * a.V + v0;
+    float *out = a.out + (size_t)row * a.V + v0;
+    f32x4 x[QUADS];
+    unsigned allowed[QUADS];
+#pragma unroll
+    for (int q = 0; q < QUADS; ++q) { /* in flight while the ids are counted */
+        const int i = 4 * (tid + THREADS * q);
+        if (i + 4 <= nv) x[q] = *(const f32x4u *)(in + i);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[q][e] = i + e < nv ? in[i + e] : -INFINITY;
+        const int v = v0 + (i < nv ? i : 0);
+        allowed[q] = a.mask ? a.mask[(size_t)row * a.mask_stride + (v >> 5)] >> (v & 31) : 15u;
+    }
+#pragma unroll
+    for (int q = 0; q < QUADS; ++q) {
+        hits[tid + THREADS * q] = i32x4{ 0, 0, 0, 0 };
+        later[tid + THREADS * q] = i32x4{ 0, 0, 0, 0 };
+    }
     __syncthreads();
     if (a.ctx) {
         const int n = a.ctx_len ? clampi(a.ctx_len[row], 0, a.max_ctx) : a.max_ctx;
-        for (int i = tid; i < n; i += 256) {
+        for (int i = tid; i < n; i += THREADS) {
             const unsigned id = (unsigned)a.ctx[(size_t)row * a.max_ctx + i] - (unsigned)v0;
-            if (id < (unsigned)nv) atomicAdd(&hits[id], 1);
+            if (id < (unsigned)nv) atomicAdd((int *)hits + id, 1);
         }
     }
-    for (int i = tid; i < a.n_bias; i += 256) {
+    for (int i = tid; i < a.n_bias; i += THREADS) {
         const unsigned id = (unsigned)a.bias_id[i] - (unsigned)v0;
-        if (id < (unsigned)nv) atomicMax(&hits[a.slice + id], i + 1);
+        if (id < (unsigned)nv) atomicMax((int *)later + id, i + 1);
     }
     __syncthreads();
     float best = -INFINITY;
     int at = -1;
-    for (int i = tid; i < nv; i += 256) {
-        const int v = v0 + i, n = hits[i], e = hits[a.slice + i];
-        float x = a.logits[(size_t)row * a.V + v];
-        if (n) {
-            x = x > 0.f ? x / a.repetition : x * a.repetition;
-            x = x - a.frequency * (float)n - a.presence;
+#pragma unroll
+    for (int q = 0; q < QUADS; ++q) {
+        const int i = 4 * (tid + THREADS * q);
+        const i32x4 n = hits[tid + THREADS * q], l = later[tid + THREADS * q];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float y = x[q][e];
+            if (n[e]) {
+                y = y > 0.f ? y / a.repetition : y * a.repetition;
+                y = y - a.frequency * (float)n[e] - a.presence;
+            }
+            if (l[e]) y = y + a.bias[l[e] - 1];
+            if (!(allowed[q] >> e & 1) || v0 + i + e == a.forbid) y = -INFINITY;
+            x[q][e] = y;
+            if (i + e < nv && y > best) { best = y; at = v0 + i + e; }
         }
-        if (e) x = x + a.bias[e - 1];
-        if (v == a.forbid || (a.mask && !(a.mask[(size_t)row * a.mask_stride + (v >> 5)] >> (v & 31) & 1))) x = -INFINITY;
-        if (a.out) a.out[(size_t)row * a.V + v] = x;
-        if (x > best) { best = x; at = v; }
+        if (a.out) {
+            if (i + 4 <= nv) *(f32x4u *)(out + i) = x[q];
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (i + e < nv) out[i + e] = x[q][e];
+        }
     }
     if (!a.part) return;
     for (int o = 32; o > 0; o >>= 1) {
@@ -294,13 +1105,15 @@ G2K void g2k_logits(const g2_logits_args a)
     if ((tid & 63) == 0) { bv[tid >> 6] = best; bi[tid >> 6] = at; }
     __syncthreads();
     if (tid == 0) {
-        for (int w = 1; w < 4; ++w)
+        for (int w = 1; w < THREADS / 64; ++w)
             if (bv[w] > best || (bv[w] == best && (unsigned)bi[w] < (unsigned)at)) { best = bv[w]; at = bi[w]; }
         float *p = a.part + ((size_t)row * a.parts + part) * 2;
         p[0] = best;
         p[1] = __int_as_float(at);
     }
 }
+G2K void g2k_logits(const g2_logits_args a) { logits_impl<256, 1>(a); }
+extern "C" __global__ __launch_bounds__(1024) void g2k_logits_wide(const g2_logits_args a) { logits_impl<1024, 2>(a); }
 
 /* One wave per row: the best of its slices (at most 64). */
 extern "C" __global__ __launch_bounds__(64) void g2k_logits_pick(const g2_logits_args a)

@@ -88,8 +88,10 @@ G2L_FN size_t g2l_kv_bytes(long S, int NH, long nb)
 #define G2L_SPLITS 32
 #define G2L_PART_FLOATS (2 + G2L_DH)
 
-/* ---- rules on logits: ids of a work-group's slice at most, slices of a row */
-#define G2L_SLICE 4096
+/* ---- rules on logits: ids of a work-group's slice (narrow and wide form),
+ * slices of a row at most */
+#define G2L_SLICE 1024
+#define G2L_SLICE_WIDE 8192
 #define G2L_PARTS 64
 
 #endif
