@@ -120,8 +120,7 @@ extern "C" {
     X(KV8_APPEND, "g2k_kv8_append") X(KV8_READ, "g2k_kv8_read")               \
     X(KV8_ATTN1, "g2k_kv8_attn1") X(KV8_ATTN4, "g2k_kv8_attn4")               \
     X(KV8_ATTN8, "g2k_kv8_attn8") X(KV8_JOIN, "g2k_kv8_join")                 \
-    X(LOGITS, "g2k_logits") X(LOGITS_WIDE, "g2k_logits_wide")                 \
-    X(LOGITS_PICK, "g2k_logits_pick")
+    X(LOGITS, "g2k_logits") X(LOGITS_WIDE, "g2k_logits_wide")
 
 #define G2_ENUM_ENTRY(id, name) G2F_##id,
 enum { G2_KERNEL_LIST(G2_ENUM_ENTRY) G2F_COUNT };

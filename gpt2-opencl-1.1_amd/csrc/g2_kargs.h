@@ -435,12 +435,12 @@ typedef struct {
 } g2_kv8_attn_args;
 
 /* Rules on logits (g2_logit_rules): rows x parts work-groups, each a slice of
- * the ids; part: the best (value, id) of each slice, [rows][parts]. */
+ * the ids; cells: [rows][G2L_CELL], the best key so far and the parts done, 0 between calls. */
 typedef struct {
     const float *logits;
     float *out;
     int *pick;
-    float *part;
+    unsigned long long *cells;
     const int *ctx;
     const int *ctx_len;
     const int *bias_id;

@@ -15,6 +15,7 @@
 #define MAX_SEQ (1 << 24)      /* positions of a cache */
 #define MAX_HEADS 1024
 #define MAX_VOCAB (1 << 18)
+#define MAX_LIST 65535         /* ids of a context, entries of a bias list: counted in 16 bits */
 
 static int aligned(const void *p, size_t a) { return (uintptr_t)p % a == 0; }
 static unsigned cdiv(long a, long b) { return (unsigned)((a + b - 1) / b); }
@@ -56,7 +57,7 @@ static unsigned q4_groups(int N, int K, int in_out)
 {
     const long chunks = g2l_chunks(K), tiles = g2l_tiles(N);
     const long n = in_out ? (tiles + 3) / 4 * chunks : (tiles * chunks + 1) / 2;
-    return n < 1 << 20 ? (unsigned)n : 1u << 20;
+    return n < 1 << 20 ? (unsigned)n : 1u << 20; /* (threads of a launch: below 2^32) */
 }
 
 int g2_quantize_q4(const void *W, int w_dtype, int in_out, uint8_t *codes, uint16_t *scales, int N, int K, int group)
@@ -71,7 +72,7 @@ int g2_quantize_q4(const void *W, int w_dtype, int in_out, uint8_t *codes, uint1
         return g2i_err(G2_E_ARG, "g2_quantize_q4: overlapping buffers");
     if ((rc = ready())) return rc;
     g2_q4_args a = { W, codes, scales, NULL, N, K, group, in_out ? 1 : 0 };
-    if (in_out) return g2i_launch(w_dtype == G2_F16 ? G2F_Q4_PACK_T_F16 : G2F_Q4_PACK_T_F32, q4_groups(N, K, 1), 1, 256, &a);
+    if (in_out) return g2i_launch(w_dtype == G2_F16 ? G2F_Q4_PACK_T_F16 : G2F_Q4_PACK_T_F32, q4_groups(N, K, 1), 1, 1024, &a);
     return g2i_launch(w_dtype == G2_F16 ? G2F_Q4_PACK_F16 : G2F_Q4_PACK_F32, q4_groups(N, K, 0), 1, 256, &a);
 }
 
@@ -85,7 +86,7 @@ int g2_dequantize_q4(const uint8_t *codes, const uint16_t *scales, float *W, int
         return g2i_err(G2_E_ARG, "g2_dequantize_q4: overlapping buffers");
     if ((rc = ready())) return rc;
     g2_q4_args a = { NULL, (uint8_t *)codes, (uint16_t *)scales, W, N, K, group, in_out ? 1 : 0 };
-    return g2i_launch(in_out ? G2F_Q4_READ_T : G2F_Q4_READ, q4_groups(N, K, in_out), 1, 256, &a);
+    return g2i_launch(in_out ? G2F_Q4_READ_T : G2F_Q4_READ, q4_groups(N, K, in_out), 1, in_out ? 1024 : 256, &a);
 }
 
 /* The kernel of a product.  Two forms: the loop (a work-group of 8 or 16 waves
@@ -190,7 +191,7 @@ int g2_kv8_append(const float *qkv, void *cache, const int *pos, const int *coun
         return g2i_err(G2_E_ARG, "g2_kv8_append: %d positions from %d outside the cache of %d", T, pos ? 0 : start, max_seq);
     if (g2i_overlap(qkv, (size_t)n_seq * T * 3 * n_head * 256, cache, g2_kv8_bytes(n_seq, n_head, max_seq)))
         return g2i_err(G2_E_ARG, "g2_kv8_append: overlapping buffers");
-    const long waves = (long)n_seq * n_head * 2 * (T / G2L_BLOCK + 2);
+    const long waves = g2l_append_waves(n_seq, n_head, T);
     if (!fits((waves + 3) * 64)) return g2i_err(G2_E_LIMIT, "g2_kv8_append: too many rows for one call");
     if ((rc = ready())) return rc;
     const long nb = g2l_blocks(max_seq);
@@ -284,7 +285,7 @@ int g2_attn_kv8(const float *q, int q_stride, const void *cache, float *out, int
 
 static int logits_rows(int rows) { return rows >= 1 && rows <= 1 << 16; }
 
-size_t g2_logits_work_bytes(int rows) { return logits_rows(rows) ? (size_t)rows * G2L_PARTS * 2 * sizeof(float) : 0; }
+size_t g2_logits_work_bytes(int rows) { return logits_rows(rows) ? (size_t)rows * G2L_CELL * sizeof(uint64_t) : 0; }
 
 int g2_apply_logit_rules(const float *logits, float *out, int *pick, int rows, int V, const g2_logit_rules *rules,
                          void *work)
@@ -294,6 +295,8 @@ int g2_apply_logit_rules(const float *logits, float *out, int *pick, int rows, i
     if (!logits_rows(rows) || V > MAX_VOCAB)
         return g2i_err(G2_E_LIMIT, "g2_apply_logit_rules: %d rows of %d: at most %d of %d", rows, V, 1 << 16, MAX_VOCAB);
     const g2_logit_rules *r = rules;
+    if (r->max_ctx > MAX_LIST || r->n_bias > MAX_LIST)
+        return g2i_err(G2_E_LIMIT, "g2_apply_logit_rules: context of %d, %d biases: at most %d", r->max_ctx, r->n_bias, MAX_LIST);
     if (r->max_ctx < 0 || r->n_bias < 0 || (r->max_ctx && !r->ctx) || (r->n_bias && (!r->bias_id || !r->bias)))
         return g2i_err(G2_E_ARG, "g2_apply_logit_rules: bad context or bias list");
     if (!(r->repetition >= 0.f) || !isfinite(r->repetition) || !isfinite(r->frequency) || !isfinite(r->presence))
@@ -301,7 +304,7 @@ int g2_apply_logit_rules(const float *logits, float *out, int *pick, int rows, i
     if (r->mask && r->mask_stride != 0 && r->mask_stride < (V + 31) / 32)
         return g2i_err(G2_E_ARG, "g2_apply_logit_rules: mask rows of %d words for %d ids", r->mask_stride, V);
     if (r->forbid < -1 || r->forbid >= V) return g2i_err(G2_E_ARG, "g2_apply_logit_rules: forbidden id %d of %d", r->forbid, V);
-    if (pick && (!work || !aligned(work, 4))) return g2i_err(G2_E_ARG, "g2_apply_logit_rules: a pick needs the workspace");
+    if (pick && (!work || !aligned(work, 8))) return g2i_err(G2_E_ARG, "g2_apply_logit_rules: a pick needs the workspace");
     const size_t n = (size_t)rows * V * 4, nw = pick ? g2_logits_work_bytes(rows) : 0, np = pick ? (size_t)rows * 4 : 0;
     const struct { const void *p; size_t n; } in[] = {
         { r->ctx, r->max_ctx ? (size_t)rows * r->max_ctx * 4 : 0 }, { r->ctx_len, r->ctx_len ? (size_t)rows * 4 : 0 },
@@ -314,19 +317,19 @@ int g2_apply_logit_rules(const float *logits, float *out, int *pick, int rows, i
         bad |= in[i].n && ((out && g2i_overlap(out, n, in[i].p, in[i].n)) ||
                            (pick && (g2i_overlap(pick, np, in[i].p, in[i].n) || g2i_overlap(work, nw, in[i].p, in[i].n))));
     if (bad) return g2i_err(G2_E_ARG, "g2_apply_logit_rules: overlapping buffers");
-    int rc = ready();
+    const int rc = ready();
     if (rc) return rc;
     g2_logits_args a;
     memset(&a, 0, sizeof a);
-    a.logits = logits; a.out = out; a.pick = pick; a.part = pick ? work : NULL;
+    a.logits = logits; a.out = out; a.pick = pick; a.cells = work;
     a.ctx = r->max_ctx ? r->ctx : NULL; a.ctx_len = r->ctx_len; a.max_ctx = r->max_ctx;
     a.bias_id = r->bias_id; a.bias = r->bias; a.n_bias = r->n_bias;
     a.mask = r->mask; a.mask_stride = r->mask_stride; a.forbid = r->forbid;
     a.rows = rows; a.V = V;
     a.repetition = r->repetition > 0.f ? r->repetition : 1.f; a.frequency = r->frequency; a.presence = r->presence;
-    const int wide = cdiv(V, G2L_SLICE) > G2L_PARTS || (long)rows * cdiv(V, G2L_SLICE) > 512;
+    /* slices of 1024 ids, of 8192 where that makes more than 1024 work-groups (us: 16 rows of 50257 7.2, wide 7.4;
+     * 32 rows 8.7, 7.9; 64 rows 14.0, 12.1) */
+    const int wide = (long)rows * cdiv(V, G2L_SLICE) > 1024;
     a.parts = (int)cdiv(V, wide ? G2L_SLICE_WIDE : G2L_SLICE);
-    rc = g2i_launch(wide ? G2F_LOGITS_WIDE : G2F_LOGITS, (unsigned)(rows * a.parts), 1, wide ? 1024 : 256, &a);
-    if (!rc && pick) rc = g2i_launch(G2F_LOGITS_PICK, (unsigned)rows, 1, 64, &a);
-    return rc;
+    return g2i_launch(wide ? G2F_LOGITS_WIDE : G2F_LOGITS, (unsigned)(rows * a.parts), 1, wide ? 1024 : 256, &a);
 }

@@ -35,11 +35,23 @@ __device__ __forceinline__ uint16_t q4_scale(unsigned amax)
     return f_bf16(__uint_as_float(amax) / 6.0f);
 }
 
+/* a / b correctly rounded, for b of 8 significant bits (a bf16 scale) between
+ * 2^-100 and 2^100, from r, the correctly rounded 1 / b: a step on the remainder,
+ * which the fused multiply-add has exactly.  The step's result is within 2^-22
+ * of a last place of a / b before it is rounded; a / b is no nearer than 2^-9 of
+ * one to where the rounding changes, since 25 bits times 8 have 33 and a has
+ * 24.  Where the remainder falls below the normal range, so does a, and the
+ * quotient lies far below the first border between codes. */
+__device__ __forceinline__ float quotient(float a, float b, float r)
+{
+    const float q = a * r;
+    return fmaf(fmaf(-q, b, a), r, q);
+}
+
 /* The codes of eight weights over a scale.  The conversion rounds a value to
  * the nearest code, ties to even and at most 6, as the definition does; it is
- * given the quotient correctly rounded: w / s from the reciprocal and one step
- * on the remainder, exact where neither leaves the normal range (the division
- * itself elsewhere).  A code of -0 becomes 0; a group's scale of 0 or NaN has
+ * given the quotient correctly rounded (the division itself for scales at the
+ * ends of the range).  A code of -0 becomes 0; a group's scale of 0 or NaN has
  * codes 0. */
 __device__ __forceinline__ unsigned q4_codes(const float w[8], float s)
 {
@@ -48,10 +60,7 @@ __device__ __forceinline__ unsigned q4_codes(const float w[8], float s)
         const float r = 1.0f / s;
         float q[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float q0 = w[i] * r;
-            q[i] = fmaf(fmaf(-q0, s, w[i]), r, q0);
-        }
+        for (int i = 0; i < 8; ++i) q[i] = quotient(w[i], s, r);
         c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, q[0], q[1], 1.0f, 0);
         c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, q[2], q[3], 1.0f, 1);
         c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, q[4], q[5], 1.0f, 2);
@@ -121,7 +130,9 @@ __device__ __forceinline__ void q4_pack8(const g2_q4_args &a, const q4_raw<WT> &
 }
 
 /* W [N,K]: a work-group takes chunks of 16 rows x 128 columns, two at a time:
- * thread = row, step, place, eight consecutive columns.  Bounded by HBM. */
+ * thread = row, step, place, eight consecutive columns.  50257 x 768 fp16 28.5
+ * us, 3.5 TB/s (a thread per row and group, which walked its 32 columns one by
+ * one: 204); reading back 30 us, 5.9 TB/s, most of it written (165). */
 template <typename WT>
 __device__ void q4_pack_impl(const g2_q4_args &a)
 {
@@ -146,34 +157,38 @@ G2K void g2k_q4_pack_f32(const g2_q4_args a) { q4_pack_impl<float>(a); }
 G2K void g2k_q4_pack_f16(const g2_q4_args a) { q4_pack_impl<_Float16>(a); }
 
 /* W [K,N]: 64 rows x 128 columns at a time through LDS (64 neighbouring
- * values of a column are one run in memory). */
+ * values of a column are one run in memory), all of a thread's eight loads in
+ * flight: 768 x 768 4.6 us (8.4 with a quarter of the threads). */
 #define Q4_TROW 65
 template <typename WT>
 __device__ void q4_pack_t_impl(const g2_q4_args &a)
 {
     __shared__ WT ws[128 * Q4_TROW];
     const WT *W = (const WT *)a.W;
-    const int tid = threadIdx.x, r = tid >> 4, j = tid >> 2 & 3, p = tid & 3;
+    const int tid = threadIdx.x, u = tid >> 8, r = tid >> 4 & 15, j = tid >> 2 & 3, p = tid & 3;
     const long chunks = g2l_chunks(a.K), tiles = g2l_tiles(a.N), items = (tiles + 3) / 4 * chunks;
     for (long i = blockIdx.x; i < items; i += gridDim.x) {
         const long t0 = i / chunks * 4, c = i % chunks, n = t0 * 16 + (tid & 63);
-#pragma unroll 8
-        for (int k = tid >> 6; k < 128; k += 4)
-            ws[k * Q4_TROW + (tid & 63)] = n < a.N && c * 128 + k < a.K ? W[(c * 128 + k) * a.N + n] : (WT)0.f;
+        const WT *col = W + (n < a.N ? n : a.N - 1);
+        WT v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const long k = c * 128 + (tid >> 6) + 16 * e;
+            v[e] = col[(k < a.K ? k : a.K - 1) * a.N];
+            if (n >= a.N || k >= a.K) v[e] = (WT)0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ws[((tid >> 6) + 16 * e) * Q4_TROW + (tid & 63)] = v[e];
         __syncthreads();
+        q4_raw<WT> w;
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (t0 + u < tiles) {
-                q4_raw<WT> w;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w.v[e] = ws[(32 * j + 8 * p + e) * Q4_TROW + 16 * u + r];
-                q4_pack8<WT>(a, w, t0 + u, c, r, j, p);
-            }
+        for (int e = 0; e < 8; ++e) w.v[e] = ws[(32 * j + 8 * p + e) * Q4_TROW + 16 * u + r];
+        if (t0 + u < tiles) q4_pack8<WT>(a, w, t0 + u, c, r, j, p);
         __syncthreads();
     }
 }
-G2K void g2k_q4_pack_t_f32(const g2_q4_args a) { q4_pack_t_impl<float>(a); }
-G2K void g2k_q4_pack_t_f16(const g2_q4_args a) { q4_pack_t_impl<_Float16>(a); }
+extern "C" __global__ __launch_bounds__(1024) void g2k_q4_pack_t_f32(const g2_q4_args a) { q4_pack_t_impl<float>(a); }
+extern "C" __global__ __launch_bounds__(1024) void g2k_q4_pack_t_f16(const g2_q4_args a) { q4_pack_t_impl<_Float16>(a); }
 
 /* The eight values of a lane's word of codes. */
 __device__ __forceinline__ void q4_values(unsigned w, float s, float v[8])
@@ -221,24 +236,21 @@ G2K void g2k_q4_read(const g2_q4_args a)
 }
 
 /* To [K,N], through LDS. */
-G2K void g2k_q4_read_t(const g2_q4_args a)
+extern "C" __global__ __launch_bounds__(1024) void g2k_q4_read_t(const g2_q4_args a)
 {
     __shared__ float ws[128 * Q4_TROW];
-    const int tid = threadIdx.x, r = tid >> 4, j = tid >> 2 & 3, p = tid & 3;
+    const int tid = threadIdx.x, u = tid >> 8, r = tid >> 4 & 15, j = tid >> 2 & 3, p = tid & 3;
     const long chunks = g2l_chunks(a.K), tiles = g2l_tiles(a.N), items = (tiles + 3) / 4 * chunks;
     for (long i = blockIdx.x; i < items; i += gridDim.x) {
         const long t0 = i / chunks * 4, c = i % chunks, n = t0 * 16 + (tid & 63);
+        float s, v[8];
+        const unsigned w = q4_word(a, t0 + u < tiles ? t0 + u : tiles - 1, c, r, j, p, &s);
+        q4_values(w, s, v);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            float s, v[8];
-            const unsigned w = q4_word(a, t0 + u < tiles ? t0 + u : tiles - 1, c, r, j, p, &s);
-            q4_values(w, s, v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) ws[(32 * j + 8 * p + e) * Q4_TROW + 16 * u + r] = v[e];
-        }
+        for (int e = 0; e < 8; ++e) ws[(32 * j + 8 * p + e) * Q4_TROW + 16 * u + r] = v[e];
         __syncthreads();
-#pragma unroll 8
-        for (int k = tid >> 6; k < 128; k += 4)
+#pragma unroll
+        for (int k = tid >> 6; k < 128; k += 16)
             if (n < a.N && c * 128 + k < a.K) a.out[(c * 128 + k) * a.N + n] = ws[k * Q4_TROW + (tid & 63)];
         __syncthreads();
     }
@@ -254,9 +266,10 @@ G2K void g2k_q4_read_t(const g2_q4_args a)
  * activations keep fp32 accuracy).  A group's scale multiplies its sum, the
  * power of two a chunk's; all sums are fp32.
  *
- * The waves of a work-group take the chunks of the same TR tiles in turn and
- * each splits only its own chunk of the activations; the sums of the waves
- * meet in LDS, in order.  */
+ * Bounded by HBM for large matrices and by the launch and two load latencies
+ * for small ones: 50257 x 1600, groups of 128, 9.9 us in a replayed graph with
+ * matrices that no cache holds, 4.2 TB/s, 8.3 from the cache behind it; 768 x
+ * 768 2.8 us.  Which form a product takes: g2i_q4_form. */
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 template <int I> __device__ __forceinline__ void q4_half(f16x8 &r, unsigned w)
@@ -404,24 +417,15 @@ __device__ __forceinline__ void q4_split_x(const q4_x<MT> &x, _Float16 *xs, floa
     }
 }
 
-/* Where a lane finds its weights in a tile.  A chunk of fewer than four steps
- * is read as if it had four: what lies behind a lane's own bytes meets
- * activations that are 0, and lanes that would read past the chunk's end read
- * up to it and move the bytes to their places (q4_shift). */
+/* Where a lane finds its weights in a chunk. */
 struct q4_lane {
     unsigned whole, part; /* bytes into a chunk of four steps, of fewer */
     int shift, last;      /* words to move there; the chunk of fewer steps, -1 */
 };
 __device__ __forceinline__ q4_lane q4_lane_of(const g2_q4mv_args &a, int lane)
 {
-    q4_lane l;
-    const int c = (int)g2l_chunks(a.K) - 1, steps = g2l_chunk_steps(a.K, c);
-    const unsigned at = lane * 4 * steps, most = 256 * steps - 16;
-    l.whole = 16 * lane;
-    l.part = at < most ? at : most;
-    l.shift = (at - l.part) / 4;
-    l.last = steps < 4 ? c : -1;
-    return l;
+    const int c = (int)g2l_chunks(a.K) - 1;
+    return { 16u * lane, g2l_lane_at(a.K, c, lane), g2l_lane_shift(a.K, c, lane), g2l_chunk_steps(a.K, c) < 4 ? c : -1 };
 }
 
 /* One load each of codes and scales, at a uniform base and the lane's offset
@@ -455,7 +459,10 @@ __device__ __forceinline__ void q4_shift(u32x4 &w, int n)
 }
 
 /* Adds a chunk's products to the lane's sums: MT == 1: of row 0; else of rows
- * 2 (lane / 16) and + 1; column lane % 16 of the tile. */
+ * 2 (lane / 16) and + 1; column lane % 16 of the tile.  The empty statement
+ * keeps the sums of the products' results in the block of the products: moved
+ * behind a branch, the first of them was left without the wait that it needs
+ * after a matrix instruction (test_matrix_waits.py looks for such places). */
 template <int MT, int G>
 __device__ __forceinline__ void q4_products(const f16x8 x[4], const u32x4 &w, const uint16_t *scale, const float e[2], float *y)
 {
@@ -473,6 +480,8 @@ __device__ __forceinline__ void q4_products(const f16x8 x[4], const u32x4 &w, co
     }
     y[0] = fmaf(s[0], e[0], y[0]);
     if constexpr (MT > 1) y[1] = fmaf(s[1], e[1], y[1]);
+    if constexpr (MT > 1) asm volatile("" : "+v"(y[0]), "+v"(y[1]));
+    else asm volatile("" : "+v"(y[0]));
 }
 template <int MT>
 __device__ __forceinline__ void q4_put(float (*red)[16], int lane, const float *y)
@@ -485,12 +494,15 @@ __device__ __forceinline__ void q4_put(float (*red)[16], int lane, const float *
     }
 }
 
-/* The loop over long columns. */
+/* The loop: the waves of a work-group take the chunks of the same TR tiles in
+ * turn, each splits its own chunk of the activations; the sums of the waves
+ * meet in LDS, in order.  The next chunk's loads go out before a chunk's
+ * products. */
 template <int MT, int KW, int TR, int G>
 __device__ void q4_matvec_impl(const g2_q4mv_args &a)
 {
     constexpr int ROWS = MT == 1 ? 2 : 16, SB = 32 * (128 / G); /* bytes of a chunk's scales */
-    __shared__ _Float16 xs[KW][ROWS * Q4_XROW];
+    __shared__ __align__(16) _Float16 xs[KW][ROWS * Q4_XROW];
     __shared__ float xe[KW][8];
     __shared__ float red[KW][TR][MT][16];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -528,11 +540,11 @@ __device__ void q4_matvec_impl(const g2_q4mv_args &a)
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = *(const f16x8 *)(frag + 32 * j);
         __builtin_amdgcn_wave_barrier();
+        if (c == ql.last)
 #pragma unroll
-        for (int i = 0; i < TR; ++i) {
-            if (c == ql.last) q4_shift(wc[i].w, ql.shift);
-            q4_products<MT, G>(x, wc[i].w, wc[i].s, e, y[i]);
-        }
+            for (int i = 0; i < TR; ++i) q4_shift(wc[i].w, ql.shift);
+#pragma unroll
+        for (int i = 0; i < TR; ++i) q4_products<MT, G>(x, wc[i].w, wc[i].s, e, y[i]);
     }
 #pragma unroll
     for (int i = 0; i < TR; ++i) q4_put<MT>(red[w][i], lane, y[i]);
@@ -564,8 +576,11 @@ Q4_MATVEC(8, 16, 1)
 Q4_MATVEC(8, 8, 2)
 Q4_MATVEC(8, 8, 4)
 
-/* Held form: a wave's chunks of the activations stay in its registers for all
- * tiles that the work-group takes. */
+/* The held form: a wave's NC chunks of the activations stay in its registers
+ * for all tiles that the work-group takes in turn; a tile's loads (its bias and
+ * residual with them, since loads return in order) go out a tile ahead; more
+ * tiles ahead are no faster (50257 x 1600 on 512 work-groups 12.4 us with two
+ * and 14.3 with four, 11.9 with one). */
 template <int NC, int G> struct q4_stage {
     q4_w<G> w[NC];
     float bias, res;
@@ -575,7 +590,7 @@ template <int MT, int KW, int NC, int G>
 __device__ void q4_held_impl(const g2_q4mv_args &a)
 {
     constexpr int ROWS = MT == 1 ? 2 : 16, SB = 32 * (128 / G);
-    __shared__ _Float16 xs[KW][ROWS * Q4_XROW];
+    __shared__ __align__(16) _Float16 xs[KW][ROWS * Q4_XROW];
     __shared__ float xe[KW][8];
     __shared__ float red[2][KW][MT][16];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -661,70 +676,69 @@ Q4_HELD(8, 16, 2)
  * NaN scale.
  * ==================================================================== */
 
-/* The 16 dims of a wave's lane: lane l has position l / 4 of the block, dims
- * 16 (l % 4) .. + 15. */
-struct kv16 { f32x4 v[4]; };
-__device__ __forceinline__ kv16 kv_load(const float *p)
-{
-    kv16 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[i] = *(const f32x4u *)(p + 4 * i);
-    return r;
-}
-
-/* One wave per sequence, head, keys or values and block of the call; the
- * first block's wave reads the positions that came before from `last` and
- * then writes there what the call leaves of its last block: in one wave,
- * since both may be the same rows. */
+/* One wave per sequence, head, keys or values and block of the call; load i of
+ * a lane is four dims of position 4 i + lane / 16, so that a load is 256 bytes
+ * of each of four rows, and neighbouring waves have neighbouring heads.  The
+ * first block's wave reads the positions that came before from `last` and then
+ * writes there what the call leaves of its last block: in one wave, since both
+ * may be the same rows.  Four prompts of 1001 rows x 25 heads: 17.3 us, 3.7
+ * TB/s of the keys and values read and the codes written (19.0 with the blocks
+ * of one head side by side, whose loads are 16 rows 19 KB apart); one token:
+ * 3.1, the latency of a load, the maximum over the wave and a store. */
 G2K void g2k_kv8_append(const g2_kv8_append_args a)
 {
-    const int lane = threadIdx.x & 63, t = lane >> 2, d0 = 16 * (lane & 3);
-    const int per = a.T / G2L_BLOCK + 2, D = a.NH * G2L_DH;
-    const long item = blockIdx.x * 4l + (threadIdx.x >> 6);
-    const int i = (int)(item % per), kv = (int)(item / per % 2), h = (int)(item / per / 2 % a.NH);
-    const long s = item / per / 2 / a.NH;
+    const int lane = threadIdx.x & 63, t0 = lane >> 4, d0 = 4 * (lane & 15);
+    const int D = a.NH * G2L_DH;
+    int h, kv, i;
+    long s;
+    g2l_append_item(__builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), a.NH, a.T, &h, &kv, &i, &s);
     if (s >= a.S) return;
     const int p0 = a.pos ? a.pos[s] : a.start;
     int n = a.count ? (a.count[s] < a.T ? a.count[s] : a.T) : a.T;
     if (p0 < 0 || p0 >= a.max_seq || n <= 0) return;
     if (n > a.max_seq - p0) n = a.max_seq - p0;
-    const int end = p0 + n, first = p0 / G2L_BLOCK, b = first + i;
+    const int end = p0 + n, b = p0 / G2L_BLOCK + i;
     const float *rows = a.qkv + (size_t)s * a.T * 3 * D + (1 + kv) * D + h * G2L_DH + d0;
-    float *last = a.last + g2l_kv_last_at(a.NH, s, h, kv) + t * G2L_DH + d0;
+    float *last = a.last + g2l_kv_last_at(a.NH, s, h, kv) + d0;
     if ((b + 1) * G2L_BLOCK <= end) {
-        const int p = b * G2L_BLOCK + t;
-        const kv16 x = kv_load(p < p0 ? last : rows + (size_t)(p - p0) * 3 * D);
+        f32x4 x[4];
         unsigned amax = 0;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const unsigned u = __float_as_uint(x.v[e / 4][e % 4]) & 0x7FFFFFFF;
-            amax = u > amax ? u : amax;
+        for (int u = 0; u < 4; ++u) {
+            const int t = 4 * u + t0, p = b * G2L_BLOCK + t;
+            x[u] = *(const f32x4u *)(p < p0 ? last + t * G2L_DH : rows + (size_t)(p - p0) * 3 * D);
         }
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const unsigned u = __shfl_xor(amax, o);
-            amax = u > amax ? u : amax;
-        }
-        const float sc = amax < 0x7F800000u ? __uint_as_float(amax) / 127.0f : __uint_as_float(0x7FC00000u);
-        u32x4 w;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            unsigned u = 0;
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float r = fminf(fmaxf(rintf(x.v[q][e] / sc), -127.f), 127.f);
-                u |= (sc > 0.f ? (unsigned)(int)r & 255u : 0u) << 8 * e;
+                const unsigned m = __float_as_uint(x[u][e]) & 0x7FFFFFFF;
+                amax = m > amax ? m : amax;
             }
-            w[q] = u;
+        amax = q4_group_max(amax, 128); /* 16 lanes */
+        const unsigned r0 = __builtin_amdgcn_readlane(amax, 0), r1 = __builtin_amdgcn_readlane(amax, 16);
+        const unsigned r2 = __builtin_amdgcn_readlane(amax, 32), r3 = __builtin_amdgcn_readlane(amax, 48);
+        const unsigned m0 = r0 > r1 ? r0 : r1, m1 = r2 > r3 ? r2 : r3;
+        amax = m0 > m1 ? m0 : m1;
+        const float sc = amax < 0x7F800000u ? __uint_as_float(amax) / 127.0f : __uint_as_float(0x7FC00000u);
+        int8_t *codes = a.codes + g2l_kv_code_at(a.NH, a.blocks, s, h, b, kv) + d0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            unsigned w = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float r = fminf(fmaxf(rintf(x[u][e] / sc), -127.f), 127.f);
+                w |= (sc > 0.f ? (unsigned)(int)r & 255u : 0u) << 8 * e;
+            }
+            *(unsigned *)(codes + (4 * u + t0) * G2L_DH) = w;
         }
-        *(u32x4 *)(a.codes + g2l_kv_code_at(a.NH, a.blocks, s, h, b, kv) + 16 * lane) = w;
         if (lane == 0) a.scales[g2l_kv_scale_at(a.NH, a.blocks, s, h, b, kv)] = sc;
     }
-    const int p = end / G2L_BLOCK * G2L_BLOCK + t;
-    if (i == 0 && p >= p0 && p < end) {
-        const kv16 x = kv_load(rows + (size_t)(p - p0) * 3 * D);
+    if (i) return;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) *(f32x4 *)(last + 4 * q) = x.v[q];
+    for (int u = 0; u < 4; ++u) {
+        const int t = 4 * u + t0, p = end / G2L_BLOCK * G2L_BLOCK + t;
+        if (p >= p0 && p < end) *(f32x4 *)(last + t * G2L_DH) = *(const f32x4u *)(rows + (size_t)(p - p0) * 3 * D);
     }
 }
 
@@ -736,7 +750,8 @@ __device__ __forceinline__ int kv8_length(const int *len, int T_kv, long s)
 }
 
 /* One thread per four dims of a position, keys and values; positions in the
- * order of the output. */
+ * order of the output.  Four times 1001 positions x 25 heads 12.4 us, 5.2 TB/s,
+ * four fifths of it written (41 with a thread per value). */
 G2K void g2k_kv8_read(const g2_kv8_read_args a)
 {
     const int quads = a.NH * (G2L_DH / 4);
@@ -776,7 +791,27 @@ G2K void g2k_kv8_read(const g2_kv8_read_args a)
  * value.  Each position slot (16 a wave) keeps a running maximum and sum of
  * its own; they meet once, at the end: over the lanes, over the waves in LDS,
  * and over the parts of a long sequence in a second launch.  Scores are held
- * in units of log 2, the queries carrying the factor.  */
+ * in units of log 2, the queries carrying the factor.
+ *
+ * Bounded by HBM for many or long sequences (48 x 25 heads x 256..1024 23 us,
+ * 4.3 TB/s; 16 heads x 50001 19 us and 4 to join, 4.4 TB/s; a wave for each
+ * head, a position at a time, took 35 ms there), by latency for one short
+ * sequence (12 heads x 701 5.2 us: the launch, the length, two rounds of
+ * loads, the sums over lanes and waves).  The first loads go out before the
+ * length is there and the next four blocks' before the last ones' sums (25
+ * heads x 1024 7.2 us without either, 6.4 with both and the sums over the
+ * lanes without LDS). */
+
+/* The 16 dims of a wave's lane: lane l has position l / 4 of a block, dims 16
+ * (l % 4) .. + 15. */
+struct kv16 { f32x4 v[4]; };
+__device__ __forceinline__ kv16 kv_load(const float *p)
+{
+    kv16 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.v[i] = *(const f32x4u *)(p + 4 * i);
+    return r;
+}
 struct kv8_sum {
     float m, l, o[16];
 };
@@ -882,11 +917,11 @@ __device__ void kv8_attn_impl(const g2_kv8_attn_args &a)
     const long s = blockIdx.x / a.splits / a.NH;
     const int8_t *codes = a.codes + g2l_kv_code_at(a.NH, a.blocks, s, h, 0, 0);
     const float *scales = a.scales + g2l_kv_scale_at(a.NH, a.blocks, s, h, 0, 0);
-    const int b0 = split * a.span, bound = a.T_kv / G2L_BLOCK;
+    const int first = g2l_attn_first(split, a.span, w), bound = a.T_kv / G2L_BLOCK;
     kv16 q = kv_load(a.q + s * a.q_stride + h * G2L_DH + d0);
-    kv8_four next = kv8_load(codes, scales, b0 + 4 * w, bound ? bound - 1 : 0, lane);
+    kv8_four next = kv8_load(codes, scales, first, bound ? bound - 1 : 0, lane);
     const int len = kv8_length(a.len, a.T_kv, s), full = len / G2L_BLOCK;
-    const int b1 = b0 + a.span < full ? b0 + a.span : full;
+    const int b1 = g2l_attn_end(split, a.span, full);
     const float qf = a.scale * 1.44269504f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) q.v[e / 4][e % 4] *= qf;
@@ -895,9 +930,9 @@ __device__ void kv8_attn_impl(const g2_kv8_attn_args &a)
     st.l = 0.f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) st.o[e] = 0.f;
-    for (int b = b0 + 4 * w; b < b1; b += 4 * NW) {
+    for (int b = first; b < b1; b += g2l_attn_step(NW)) {
         const kv8_four f = next;
-        if (b + 4 * NW < b1) next = kv8_load(codes, scales, b + 4 * NW, b1 - 1, lane);
+        if (b + g2l_attn_step(NW) < b1) next = kv8_load(codes, scales, b + g2l_attn_step(NW), b1 - 1, lane);
         float x[4], sv[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -911,7 +946,7 @@ __device__ void kv8_attn_impl(const g2_kv8_attn_args &a)
     }
     /* the block that is not full, in the part that holds its place: the next wave in turn */
     const int left = len % G2L_BLOCK;
-    if (left && full >= b0 && full < b0 + a.span && w == (full - b0 + 3) / 4 % NW) {
+    if (left && g2l_attn_left(split, a.span, full, w, NW)) {
         const float *p = a.last + g2l_kv_last_at(a.NH, s, h, 0) + t * G2L_DH + d0;
         kv16 k = {}, v = {};
         if (t < left) {
@@ -1027,15 +1062,40 @@ G2K void g2k_kv8_join(const g2_kv8_attn_args a)
  * one pass over the slice's logits.  Every step is its own fp32 rounding (no
  * fused multiply-add), so equal logits stay equal.
  * ==================================================================== */
+/* Maximum, minimum over the wave. */
+__device__ __forceinline__ float lanes_max(float v)
+{
+    v = dpp_max<0xB1>(v);  /* quad: lanes 1 0 3 2 */
+    v = dpp_max<0x4E>(v);  /* 2 3 0 1 */
+    return slots_max(v);
+}
+__device__ __forceinline__ unsigned lanes_min(unsigned v)
+{
+#define LANES_MIN(CTRL) { const unsigned o = (unsigned)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, false); v = o < v ? o : v; }
+    LANES_MIN(0xB1) LANES_MIN(0x4E) LANES_MIN(0x141) LANES_MIN(0x140)
+#undef LANES_MIN
+    const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = s[0] < s[1] ? s[0] : s[1];
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return r[0] < r[1] ? r[0] : r[1];
+}
+
+/* A logit and its id as one number: greater for a greater logit, of equal ones
+ * for the lower id; 0 is below all (-infinity and NaN have none). */
+__device__ __forceinline__ unsigned long long logit_key(float v, int id)
+{
+    const unsigned u = __float_as_uint(v + 0.f); /* (-0 counts as 0) */
+    return (unsigned long long)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (unsigned)~id;
+}
+
 template <int THREADS, int QUADS>
 __device__ void logits_impl(const g2_logits_args &a)
 {
 #pragma clang fp contract(off)
     constexpr int SLICE = THREADS * QUADS * 4;
     typedef int i32x4 __attribute__((ext_vector_type(4)));
-    __shared__ i32x4 hits[SLICE / 4], later[SLICE / 4]; /* counts; entry of the bias list + 1 */
-    __shared__ float bv[THREADS / 64];
-    __shared__ int bi[THREADS / 64];
+    __shared__ i32x4 seen[SLICE / 4]; /* an id's times in the context; 65536 times its entry of the bias list + 1 */
+    __shared__ unsigned long long keys[THREADS / 64];
     const int tid = threadIdx.x, row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
     const int v0 = part * SLICE, nv = a.V - v0 < SLICE ? a.V - v0 : SLICE;
     const float *in = a.logits + (size_t)row * a.V + v0;
@@ -1052,42 +1112,53 @@ __device__ void logits_impl(const g2_logits_args &a)
         const int v = v0 + (i < nv ? i : 0);
         allowed[q] = a.mask ? a.mask[(size_t)row * a.mask_stride + (v >> 5)] >> (v & 31) : 15u;
     }
+    /* so are the first entries of the lists, to ids that are none where there are fewer */
+    const int *ctx = a.ctx + (size_t)row * a.max_ctx;
+    int id = -1, bid = -1;
+    if (a.ctx) id = ctx[tid < a.max_ctx ? tid : 0];
+    if (a.n_bias) bid = a.bias_id[tid < a.n_bias ? tid : 0];
+    const int n = !a.ctx ? 0 : a.ctx_len ? clampi(a.ctx_len[row], 0, a.max_ctx) : a.max_ctx;
 #pragma unroll
-    for (int q = 0; q < QUADS; ++q) {
-        hits[tid + THREADS * q] = i32x4{ 0, 0, 0, 0 };
-        later[tid + THREADS * q] = i32x4{ 0, 0, 0, 0 };
-    }
+    for (int q = 0; q < QUADS; ++q) seen[tid + THREADS * q] = i32x4{ 0, 0, 0, 0 };
     __syncthreads();
-    if (a.ctx) {
-        const int n = a.ctx_len ? clampi(a.ctx_len[row], 0, a.max_ctx) : a.max_ctx;
-        for (int i = tid; i < n; i += THREADS) {
-            const unsigned id = (unsigned)a.ctx[(size_t)row * a.max_ctx + i] - (unsigned)v0;
-            if (id < (unsigned)nv) atomicAdd((int *)hits + id, 1);
-        }
-    }
     for (int i = tid; i < a.n_bias; i += THREADS) {
-        const unsigned id = (unsigned)a.bias_id[i] - (unsigned)v0;
-        if (id < (unsigned)nv) atomicMax((int *)later + id, i + 1);
+        const unsigned k = (unsigned)(i == tid ? bid : a.bias_id[i]) - (unsigned)v0;
+        if (k < (unsigned)nv) atomicMax((unsigned *)seen + k, (unsigned)(i + 1) << 16);
+    }
+    if (a.n_bias) __syncthreads();
+    for (int i = tid; i < n; i += THREADS) {
+        const unsigned k = (unsigned)(i == tid ? id : ctx[i]) - (unsigned)v0;
+        if (k < (unsigned)nv) atomicAdd((unsigned *)seen + k, 1u);
     }
     __syncthreads();
     float best = -INFINITY;
-    int at = -1;
+    int at = 0; /* 4 q + e of the best */
 #pragma unroll
     for (int q = 0; q < QUADS; ++q) {
         const int i = 4 * (tid + THREADS * q);
-        const i32x4 n = hits[tid + THREADS * q], l = later[tid + THREADS * q];
+        const i32x4 s = seen[tid + THREADS * q];
+        if (s[0] | s[1] | s[2] | s[3]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float y = x[q][e];
-            if (n[e]) {
-                y = y > 0.f ? y / a.repetition : y * a.repetition;
-                y = y - a.frequency * (float)n[e] - a.presence;
+            for (int e = 0; e < 4; ++e) {
+                float y = x[q][e];
+                const unsigned n = s[e] & 65535, l = (unsigned)s[e] >> 16;
+                if (n) {
+                    y = y > 0.f ? y / a.repetition : y * a.repetition;
+                    y = y - a.frequency * (float)n - a.presence;
+                }
+                if (l) y = y + a.bias[l - 1];
+                x[q][e] = y;
             }
-            if (l[e]) y = y + a.bias[l[e] - 1];
-            if (!(allowed[q] >> e & 1) || v0 + i + e == a.forbid) y = -INFINITY;
-            x[q][e] = y;
-            if (i + e < nv && y > best) { best = y; at = v0 + i + e; }
         }
+        if (a.mask || a.forbid >= 0) { /* (uniform) */
+            const unsigned f = (unsigned)(a.forbid - v0 - i);
+            const unsigned ok = f < 4u ? allowed[q] & ~(1u << f) : allowed[q];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[q][e] = ok >> e & 1 ? x[q][e] : -INFINITY;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) /* (ids behind the slice are -infinity) */
+            if (x[q][e] > best) { best = x[q][e]; at = 4 * q + e; }
         if (a.out) {
             if (i + 4 <= nv) *(f32x4u *)(out + i) = x[q];
             else
@@ -1096,36 +1167,28 @@ __device__ void logits_impl(const g2_logits_args &a)
                     if (i + e < nv) out[i + e] = x[q][e];
         }
     }
-    if (!a.part) return;
-    for (int o = 32; o > 0; o >>= 1) {
-        const float ov = __shfl_xor(best, o);
-        const int oi = __shfl_xor(at, o);
-        if (ov > best || (ov == best && (unsigned)oi < (unsigned)at)) { best = ov; at = oi; }
-    }
-    if ((tid & 63) == 0) { bv[tid >> 6] = best; bi[tid >> 6] = at; }
+    if (!a.pick) return;
+    /* the wave's best value, the lowest id that has it, the slice's best key */
+    const float top = lanes_max(best);
+    const int mine = v0 + 4 * (tid + THREADS * (at >> 2)) + (at & 3);
+    const unsigned low = lanes_min(best == top && best > -INFINITY ? (unsigned)mine : ~0u);
+    unsigned long long key = low == ~0u ? 0 : logit_key(top, (int)low);
+    if ((tid & 63) == 0) keys[tid >> 6] = key;
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < THREADS / 64; ++w)
-            if (bv[w] > best || (bv[w] == best && (unsigned)bi[w] < (unsigned)at)) { best = bv[w]; at = bi[w]; }
-        float *p = a.part + ((size_t)row * a.parts + part) * 2;
-        p[0] = best;
-        p[1] = __int_as_float(at);
+    if (tid) return;
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) key = keys[w] > key ? keys[w] : key;
+    if (a.parts > 1) {
+        unsigned long long *cell = a.cells + G2L_CELL * (size_t)row;
+        /* the maximum has its old value back, so it is done, before the count goes up */
+        const unsigned long long was = __hip_atomic_fetch_max(cell, key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const unsigned long long one = was == ~0ull ? 2 : 1; /* (1: no key is all ones) */
+        if (__hip_atomic_fetch_add(cell + 1, one, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != (unsigned)a.parts - 1) return;
+        key = __hip_atomic_exchange(cell, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(cell + 1, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
+    a.pick[row] = key ? (int)~(unsigned)key : -1;
 }
 G2K void g2k_logits(const g2_logits_args a) { logits_impl<256, 1>(a); }
 extern "C" __global__ __launch_bounds__(1024) void g2k_logits_wide(const g2_logits_args a) { logits_impl<1024, 2>(a); }
 
-/* One wave per row: the best of its slices (at most 64). */
-extern "C" __global__ __launch_bounds__(64) void g2k_logits_pick(const g2_logits_args a)
-{
-    const int i = threadIdx.x, row = blockIdx.x;
-    const float *p = a.part + ((size_t)row * a.parts + i) * 2;
-    float best = i < a.parts ? p[0] : -INFINITY;
-    int at = i < a.parts ? __float_as_int(p[1]) : -1;
-    for (int o = 32; o > 0; o >>= 1) {
-        const float ov = __shfl_xor(best, o);
-        const int oi = __shfl_xor(at, o);
-        if (ov > best || (ov == best && (unsigned)oi < (unsigned)at)) { best = ov; at = oi; }
-    }
-    if (i == 0) a.pick[row] = at;
-}

@@ -47,6 +47,19 @@ G2L_FN size_t g2l_code_at(long K, long t, long c, int lane)
 {
     return ((size_t)t * g2l_steps(K) + 4 * c) * 256 + (size_t)lane * 4 * g2l_chunk_steps(K, c);
 }
+/* Where lane `lane` reads 16 bytes of chunk c, as bytes into the chunk.  A chunk
+ * of fewer than four steps is read as if it had four: what lies behind a lane's
+ * own bytes meets activations that are 0, and lanes that would read past the
+ * chunk's end read up to it and move g2l_lane_shift words to their places. */
+G2L_FN unsigned g2l_lane_at(long K, long c, int lane)
+{
+    const unsigned steps = (unsigned)g2l_chunk_steps(K, c), at = (unsigned)lane * 4 * steps, most = 256 * steps - 16;
+    return at < most ? at : most;
+}
+G2L_FN int g2l_lane_shift(long K, long c, int lane)
+{
+    return (int)((unsigned)lane * 4 * (unsigned)g2l_chunk_steps(K, c) - g2l_lane_at(K, c, lane)) / 4;
+}
 /* element of the scales: row r (0..15) of tile t, group g of chunk c */
 G2L_FN size_t g2l_scale_at(long K, int group, long t, long c, int r, int g)
 {
@@ -88,10 +101,36 @@ G2L_FN size_t g2l_kv_bytes(long S, int NH, long nb)
 #define G2L_SPLITS 32
 #define G2L_PART_FLOATS (2 + G2L_DH)
 
-/* ---- rules on logits: ids of a work-group's slice (narrow and wide form),
- * slices of a row at most */
+/* Work of g2k_kv8_append: wave `item` of a call of T rows has head, keys or
+ * values, the i-th block from the one that holds the first position, sequence
+ * (heads first: neighbouring waves read neighbouring parts of the same rows). */
+G2L_FN unsigned g2l_append_blocks(int T) { return (unsigned)T / G2L_BLOCK + 2; }
+G2L_FN long g2l_append_waves(int S, int NH, int T) { return (long)S * NH * 2 * g2l_append_blocks(T); }
+G2L_FN void g2l_append_item(unsigned item, int NH, int T, int *h, int *kv, int *i, long *s)
+{
+    const unsigned row = item / (unsigned)NH, per = g2l_append_blocks(T);
+    *h = (int)(item % (unsigned)NH);
+    *kv = (int)(row % 2);
+    *i = (int)(row / 2 % per);
+    *s = row / 2 / per;
+}
+/* Work of g2k_kv8_attn*: wave w of nw takes four whole blocks at a time, from
+ * g2l_attn_first on and g2l_attn_step apart, below the end of its part; the
+ * block that is not full is g2l_attn_left's. */
+G2L_FN int g2l_attn_first(int split, int span, int w) { return split * span + 4 * w; }
+G2L_FN int g2l_attn_step(int nw) { return 4 * nw; }
+G2L_FN int g2l_attn_end(int split, int span, int full) { return (split + 1) * span < full ? (split + 1) * span : full; }
+G2L_FN int g2l_attn_left(int split, int span, int full, int w, int nw)
+{
+    const int at = full - split * span;
+    return at >= 0 && at < span && w == (at + 3) / 4 % nw;
+}
+
+/* ---- rules on logits: ids of a work-group's slice (narrow and wide form);
+ * 64-bit words from row to row of the workspace (a cache line: the slices of
+ * all rows meet there) */
 #define G2L_SLICE 1024
 #define G2L_SLICE_WIDE 8192
-#define G2L_PARTS 64
+#define G2L_CELL 16
 
 #endif

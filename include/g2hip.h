@@ -265,12 +265,14 @@ typedef struct {
     int mask_stride;        /*   -infinity; words from row to row, 0: one mask for all   */
     int forbid;             /* an id that is never allowed, -1: none                     */
 } g2_logit_rules;
-/* Bytes of g2_apply_logit_rules' workspace (used where pick is wanted). */
+/* Bytes of g2_apply_logit_rules' workspace (needed where pick is wanted): zero
+ * before its first call, left zero by every call, 8-byte aligned. */
 size_t g2_logits_work_bytes(int rows);
 /* out[rows,V] = logits under the rules (NULL: not wanted; out == logits is
  * legal) and pick[r] = the id of the greatest (NULL: not wanted): the lowest
  * of equal ones, NaN never, -1 where nothing is above -infinity.  The device
- * form of g2_sample_greedy.  1 <= V <= 262144. */
+ * form of g2_sample_greedy.  V up to 262144, max_ctx and n_bias up to 65535,
+ * rows up to 65536. */
 int g2_apply_logit_rules(const float *logits, float *out, int *pick, int rows,
                          int V, const g2_logit_rules *rules, void *work);
 

@@ -125,15 +125,36 @@ def run_matvec(g2, x, codes, scales, N, K, group, bias=None, res=None, gelu=0, s
     return take(y, M * N).reshape(M, N)
 
 
-@pytest.mark.parametrize("M", [1, 2, 3, 7, 8, 9, 16, 21])
-@pytest.mark.parametrize("N,K,group", [(1, 1, 32), (5, 40, 64), (16, 128, 128), (17, 129, 32), (50, 257, 64), (100, 768, 128),
-                                       (768, 768, 64), (333, 1600, 32), (1000, 1601, 128), (33, 6400, 64), (40, 9000, 32), (2563, 100, 32)])
+# sizes on both sides of every border of a form: few and many tiles, short and long columns, whole and partial chunks
+PRODUCTS = [(1, 1, 32), (5, 40, 64), (16, 128, 128), (17, 129, 32), (50, 257, 64), (100, 768, 128), (768, 768, 64), (333, 1600, 32),
+            (1000, 1601, 128), (33, 6400, 64), (40, 9000, 32), (20, 1100, 128), (15, 2100, 32), (18, 2100, 128), (2563, 100, 32)]
+# tiles >= 256, >= 512, >= 2048 with 8 and 16 chunks, 16 waves; every group of 32, 64, 128
+LARGE = [(N, K, G) for N, K in ((4100, 160), (8200, 200), (8195, 2100), (32780, 130), (32770, 1060)) for G in (32, 64, 128)]
+LARGE += [(48, 300, G) for G in (32, 64, 128)] + [(48, 2200, G) for G in (32, 64, 128)] + [(24, 1400, G) for G in (32, 64, 128)]
+ROWS, LARGE_ROWS = [1, 2, 3, 7, 8, 9, 16, 21], [1, 3, 9]
+
+
+def product_cases():
+    return [(M, *s) for s in PRODUCTS for M in ROWS] + [(M, *s) for s in LARGE for M in LARGE_ROWS]
+
+
+_weights = {}
+
+
+def product_weights(g2, N, K, group):
+    """(codes, scales, the values they stand for) of random weights, those of the last sizes kept."""
+    if (N, K, group) not in _weights:
+        _weights.clear()
+        W = (0.02 * rng(N, K).standard_normal((N, K))).astype(np.float32)
+        _weights[N, K, group] = (*packed(g2, W, group), lowbit.values_q4(*lowbit.quantize_q4(W, group), group))
+    return _weights[N, K, group]
+
+
+@pytest.mark.parametrize("N,K,group,M", [(*s, M) for s in PRODUCTS for M in ROWS] + [(*s, M) for s in LARGE for M in LARGE_ROWS])
 def test_matvec_q4(g2, M, N, K, group):
     r = rng(M, N, K)
-    W = (0.02 * r.standard_normal((N, K))).astype(np.float32)
     x, bias, res = (r.standard_normal(n).astype(np.float32) for n in ((M, K), N, (M, N)))
-    codes, scales = packed(g2, W, group)
-    v = lowbit.values_q4(*lowbit.quantize_q4(W, group), group)
+    codes, scales, v = product_weights(g2, N, K, group)
     ref, bound = x.astype(np.float64) @ v.T, matvec_bound(x, v, K)
     tiny = 1e-37
     within(run_matvec(g2, x, codes, scales, N, K, group, shift=1), ref, bound + tiny, "plain")
@@ -363,7 +384,18 @@ def filled_cache(g2, S, NH, max_seq, lens, seed, size=1.0):
     return cache, models
 
 
-@pytest.mark.parametrize("NH,max_seq", [(1, 2100), (12, 1024), (25, 1100), (3, 1003)])
+LENGTHS = [(1, 2100), (12, 1024), (25, 1100), (3, 1003), (20, 14000)]
+BATCHES = [(1, 2, 40, [1]), (4, 3, 64, [0, 1, 15, 64]), (7, 12, 130, [17, 16, 33, 0, 129, 130, 31]), (3, 25, 700, [699, 5, 345]),
+           (40, 4, 90, [(37 * i) % 91 for i in range(40)]), (2, 1, 3000, [2999, 1500]), (70, 12, 50, [(11 * i) % 51 for i in range(70)]),
+           (45, 12, 128, [(29 * i) % 129 for i in range(45)]), (5, 3, 1500, [1490, 1499, 0, 1, 700])]
+
+
+def attention_cases():
+    """(sequences x heads, bound of the lengths) of the tests below."""
+    return [(NH, top) for NH, top in LENGTHS] + [(NH, 64) for NH, _ in LENGTHS] + [(S * NH, m) for S, NH, m, _ in BATCHES]
+
+
+@pytest.mark.parametrize("NH,max_seq", LENGTHS)
 def test_attend_lengths(g2, NH, max_seq):
     top = max_seq
     cache, (m,) = filled_cache(g2, 1, NH, max_seq, [top], NH)
@@ -371,7 +403,7 @@ def test_attend_lengths(g2, NH, max_seq):
     full = m.values()
     # whole blocks are the same at any length; a length inside a block would need its fp32 rows, so lengths are whole
     # blocks and the whole cache
-    for T in [0, 16, 32, 48, 64, 80, 128, 256, 272, 512, 640, 1008, 1024, 1040, 2096, top]:
+    for T in [0, 16, 32, 48, 64, 80, 128, 256, 272, 512, 640, 1008, 1024, 1040, 2096, 5008, 13984, top]:
         if T > top or (T % 16 and T != top):
             continue
         got = run_attend(g2, q, cache, None, T, 1, NH, max_seq, 0.125)
@@ -379,9 +411,7 @@ def test_attend_lengths(g2, NH, max_seq):
         within(got[0], ref, bound, f"length {T}")
 
 
-@pytest.mark.parametrize("S,NH,max_seq,lens", [(1, 2, 40, [1]), (4, 3, 64, [0, 1, 15, 64]), (7, 12, 130, [17, 16, 33, 0, 129, 130, 31]),
-                                               (3, 25, 700, [699, 5, 345]), (40, 4, 90, [(37 * i) % 91 for i in range(40)]),
-                                               (2, 1, 3000, [2999, 1500]), (70, 12, 50, [(11 * i) % 51 for i in range(70)])])
+@pytest.mark.parametrize("S,NH,max_seq,lens", BATCHES)
 def test_attend_batches(g2, S, NH, max_seq, lens):
     cache, models = filled_cache(g2, S, NH, max_seq, lens, 10)
     q = rng(11, S).standard_normal((S, NH, H)).astype(np.float32)
@@ -434,6 +464,13 @@ def test_attend_infinities_and_nan(g2):
     if q[0, 3, 0] > 0:
         assert np.isnan(got[0, 3]).all()  # infinite score: inf - inf
     assert not np.isfinite(got[0, 3]).all() or q[0, 3, 0] < 0
+    qkv = np.ones((13, 3 * D), np.float32)  # the block fills: its keys of head 3 are NaN altogether, no other head's
+    g2.kv8_append(g2.to_device(qkv), cache, None, None, T + 1, 1, 13, NH, max_seq)
+    got = run_attend(g2, q, cache, None, 64, 1, NH, max_seq, 0.125)
+    m.append(T + 1, qkv[:, D:2 * D], qkv[:, 2 * D:])
+    ref, bound = attend_bound(q[0], np.nan_to_num(m.values(), nan=1.0), 0.125, 64)
+    within(got[0, 0], ref[0], bound[0])
+    assert np.isnan(got[0, 1:]).all()
 
 
 def test_attend_beyond_32_bit_offsets(g2):
@@ -473,7 +510,7 @@ def run_rules(g2, l, pick=True, out=True, in_place=False, **kw):
     g2.check(g2._lib.g2_upload(dl.ptr, np.ascontiguousarray(l).ctypes.data, l.nbytes))
     do = dl if in_place else guarded(g2, R * V) if out else None
     dp = g2.to_device(np.full(R + 4, 77, np.int32)) if pick else None
-    work = g2.DevBuf(g2.logits_work_bytes(R)) if pick else None
+    work = g2.to_device(np.zeros(g2.logits_work_bytes(R) + 8, np.uint8)) if pick else None
     dev = {k: g2.to_device(v) if isinstance(v, np.ndarray) else v for k, v in kw.items()}
     g2.apply_logit_rules(dl, do, dp, R, V, g2.logit_rules(**dev), work)
     ids = None
@@ -481,6 +518,7 @@ def run_rules(g2, l, pick=True, out=True, in_place=False, **kw):
         ids = dp.download(np.int32)
         assert (ids[R:] == 77).all()
         ids = ids[:R]
+        assert (work.download(np.uint8) == 0).all()  # left as it has to be for the next call
     return (take(do, R * V).reshape(R, V) if do is not None else None), ids
 
 
@@ -552,6 +590,33 @@ def test_rules_that_leave_nothing(g2):
     same(run_rules(g2, l, out=False, forbid=1999)[1][1:], [-1, -1, -1])
 
 
+def test_calls_give_the_same_bits_again(g2):
+    """No result depends on an order of atomics or on what an earlier call left: calls of other sizes between, the same
+    workspaces."""
+    S, NH, max_seq, V = 3, 5, 3000, 50257
+    lens = [3000, 17, 1600]
+    cache, _ = filled_cache(g2, S, NH, max_seq, lens, 30)
+    small, _ = filled_cache(g2, 2, 3, 2000, [2000, 1999], 31)
+    r = rng(32)
+    q = g2.to_device(r.standard_normal((S, NH * H)).astype(np.float32))
+    dl, work = g2.to_device(np.asarray(lens, np.int32)), g2.DevBuf(g2.kv8_work_bytes(S, NH))
+    out = g2.DevBuf(4 * S * NH * H)
+    logits = g2.to_device(r.standard_normal((30, V)).astype(np.float32))
+    ctx = g2.to_device(r.integers(0, 300, (30, 500)).astype(np.int32))
+    lwork, lo, pick = g2.to_device(np.zeros(g2.logits_work_bytes(30), np.uint8)), g2.DevBuf(120 * V), g2.DevBuf(120)
+    rules = g2.logit_rules(ctx=ctx, max_ctx=500, repetition=1.3, presence=0.1)
+    first = None
+    for turn in range(6):
+        g2.attn_kv8(q, NH * H, cache, out, NH * H, dl, max_seq, S, NH, max_seq, 0.125, work)
+        g2.apply_logit_rules(logits, lo, pick, 30, V, rules, lwork)
+        got = [b.download(np.float32) for b in (out, lo)] + [pick.download(np.int32)]
+        first = first or got
+        for a, b in zip(got, first):
+            same(a.view(np.uint32), b.view(np.uint32))
+        g2.attn_kv8(q, 192, small, out, 192, None, 1999 - turn, 2, 3, 2000, 0.3, work)
+        g2.apply_logit_rules(logits, lo, pick, 3 + turn, 2000 * (turn + 1), rules, lwork)
+
+
 # ------------------------------------------------------------------ together
 
 class Step:
@@ -585,7 +650,7 @@ class Step:
         f = lambda n: g2.DevBuf(4 * n)  # noqa: E731
         self.x, self.n, self.qkv, self.att, self.h = f(S * E), f(S * E), f(S * 3 * E), f(S * E), f(S * 4 * E)
         self.logits, self.out, self.pick = f(S * V), f(S * V), f(S)
-        self.work, self.lwork = g2.DevBuf(g2.kv8_work_bytes(S, NH)), g2.DevBuf(g2.logits_work_bytes(S))
+        self.work, self.lwork = g2.DevBuf(g2.kv8_work_bytes(S, NH)), g2.to_device(np.zeros(g2.logits_work_bytes(S), np.uint8))
         self.ids, self.pos, self.len = g2.DevBuf(4 * S), g2.DevBuf(4 * S), g2.DevBuf(4 * S)
         self.ctx, self.ctx_len = g2.DevBuf(4 * S * max_seq), g2.DevBuf(4 * S)
 

@@ -151,7 +151,7 @@ def test_logit_rule_refusals():
     assert call() == ok and call(out=A) == ok and call(out=None) == ok and call(pick=None, work=None) == ok
     assert call(repetition=0.0) == ok and call(ctx=F, max_ctx=5) == ok and call(mask=F, mask_stride=0) == ok
     assert call(ctx=F, max_ctx=0) == ok and call(forbid=99) == ok
-    for kw in (dict(logits=None), dict(out=None, pick=None), dict(rows=0), dict(V=0), dict(work=None), dict(work=E + 2), dict(out=A + 4),
+    for kw in (dict(logits=None), dict(out=None, pick=None), dict(rows=0), dict(V=0), dict(work=None), dict(work=E + 4), dict(out=A + 4),
                dict(max_ctx=-1), dict(max_ctx=3), dict(n_bias=2), dict(n_bias=2, bias=F), dict(n_bias=2, bias_id=F), dict(n_bias=-1),
                dict(repetition=-1.0), dict(repetition=float("nan")), dict(repetition=float("inf")), dict(frequency=float("inf")),
                dict(presence=float("nan")), dict(mask=F, mask_stride=3), dict(mask=F, mask_stride=-1), dict(forbid=100), dict(forbid=-2),
