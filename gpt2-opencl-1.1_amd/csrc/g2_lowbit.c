@@ -189,7 +189,9 @@ int g2_kv8_append(const float *qkv, void *cache, const int *pos, const int *coun
     if (!qkv) return g2i_err(G2_E_ARG, "g2_kv8_append: NULL buffer");
     if (T < 1 || T > max_seq || (!pos && (start < 0 || start > max_seq - T)))
         return g2i_err(G2_E_ARG, "g2_kv8_append: %d positions from %d outside the cache of %d", T, pos ? 0 : start, max_seq);
-    if (g2i_overlap(qkv, (size_t)n_seq * T * 3 * n_head * 256, cache, g2_kv8_bytes(n_seq, n_head, max_seq)))
+    const size_t size = g2_kv8_bytes(n_seq, n_head, max_seq), ints = (size_t)n_seq * sizeof(int);
+    if (g2i_overlap(qkv, (size_t)n_seq * T * 3 * n_head * 256, cache, size) || (pos && g2i_overlap(pos, ints, cache, size)) ||
+        (count && g2i_overlap(count, ints, cache, size)))
         return g2i_err(G2_E_ARG, "g2_kv8_append: overlapping buffers");
     const long waves = g2l_append_waves(n_seq, n_head, T);
     if (!fits((waves + 3) * 64)) return g2i_err(G2_E_LIMIT, "g2_kv8_append: too many rows for one call");
@@ -210,7 +212,8 @@ int g2_kv8_read(const void *cache, float *k, float *v, const int *len, int T_kv,
     if (T_kv < 0 || T_kv > max_seq || start < 0 || T < 1 || start > max_seq - T)
         return g2i_err(G2_E_ARG, "g2_kv8_read: positions %d..%ld, length %d, cache of %d", start, (long)start + T - 1, T_kv, max_seq);
     const size_t n = (size_t)n_seq * T * n_head * 256, nc = g2_kv8_bytes(n_seq, n_head, max_seq);
-    if (g2i_overlap(k, n, v, n) || g2i_overlap(k, n, cache, nc) || g2i_overlap(v, n, cache, nc))
+    if (g2i_overlap(k, n, v, n) || g2i_overlap(k, n, cache, nc) || g2i_overlap(v, n, cache, nc) ||
+        (len && (g2i_overlap(k, n, len, (size_t)n_seq * 4) || g2i_overlap(v, n, len, (size_t)n_seq * 4))))
         return g2i_err(G2_E_ARG, "g2_kv8_read: overlapping buffers");
     if ((rc = ready())) return rc;
     const long nb = g2l_blocks(max_seq);
@@ -229,7 +232,8 @@ int g2_kv8_read(const void *cache, float *k, float *v, const int *len, int T_kv,
  *  - a wave takes 64 positions at a time: one wave up to 64 (12 heads 3.3, four
  *    waves 3.7), for many heads up to 128 (1600 heads 8.7, 9.9), four up to 512
  *    (200 heads x 512 5.7, eight 6.0), eight beyond (25 x 1024 6.4, four 6.7,
- *    sixteen 6.7). */
+ *    sixteen 6.7), but four for many heads, which fill the chip either way
+ *    (1200 heads x 1024 within 1%) and may be much shorter than the bound. */
 int g2i_kv8_form(long heads, int T_kv, int *span, int *waves)
 {
     const long blocks = g2l_blocks(T_kv) > 0 ? g2l_blocks(T_kv) : 1;
@@ -240,7 +244,8 @@ int g2i_kv8_form(long heads, int T_kv, int *span, int *waves)
     }
     *span = (int)((blocks + splits - 1) / splits);
     splits = (blocks + *span - 1) / *span;
-    *waves = *span <= 4 || (*span <= 8 && heads * splits >= 512) ? 1 : *span <= 32 ? 4 : 8;
+    const int many = heads >= 512;
+    *waves = *span <= 4 || (*span <= 8 && many) ? 1 : *span <= 32 || many ? 4 : 8;
     return (int)splits;
 }
 

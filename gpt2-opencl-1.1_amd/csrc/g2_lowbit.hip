@@ -797,10 +797,9 @@ G2K void g2k_kv8_read(const g2_kv8_read_args a)
  * 4.3 TB/s; 16 heads x 50001 19 us and 4 to join, 4.4 TB/s; a wave for each
  * head, a position at a time, took 35 ms there), by latency for one short
  * sequence (12 heads x 701 5.2 us: the launch, the length, two rounds of
- * loads, the sums over lanes and waves).  The first loads go out before the
- * length is there and the next four blocks' before the last ones' sums (25
- * heads x 1024 7.2 us without either, 6.4 with both and the sums over the
- * lanes without LDS). */
+ * loads, the sums over lanes and waves).  The next four blocks' loads go out
+ * before the last ones' sums, and the sums over the lanes need no LDS (25 heads
+ * x 1024 6.4 us, 7.2 without either). */
 
 /* The 16 dims of a wave's lane: lane l has position l / 4 of a block, dims 16
  * (l % 4) .. + 15. */
@@ -854,9 +853,10 @@ __device__ __forceinline__ void kv8_add(kv8_sum &a, const float *s, const float 
     }
 }
 
-/* Four blocks' codes and scales.  A block behind the last one of the part is
- * the last again; the first four are asked for before the length is known, by
- * the bound of the lengths, and may be none of the sequence's. */
+/* Four blocks' codes and scales; a block behind the last one of the part is the
+ * last again.  (Asking for the first four by the bound of the lengths, before
+ * the length is there, saved 0.1 us where they were needed and cost up to half
+ * the time of many short sequences under a high bound.) */
 struct kv8_four {
     u32x4 k[4], v[4];
     float sk[4], sv[4];
@@ -917,11 +917,12 @@ __device__ void kv8_attn_impl(const g2_kv8_attn_args &a)
     const long s = blockIdx.x / a.splits / a.NH;
     const int8_t *codes = a.codes + g2l_kv_code_at(a.NH, a.blocks, s, h, 0, 0);
     const float *scales = a.scales + g2l_kv_scale_at(a.NH, a.blocks, s, h, 0, 0);
-    const int first = g2l_attn_first(split, a.span, w), bound = a.T_kv / G2L_BLOCK;
+    const int first = g2l_attn_first(split, a.span, w);
     kv16 q = kv_load(a.q + s * a.q_stride + h * G2L_DH + d0);
-    kv8_four next = kv8_load(codes, scales, first, bound ? bound - 1 : 0, lane);
     const int len = kv8_length(a.len, a.T_kv, s), full = len / G2L_BLOCK;
     const int b1 = g2l_attn_end(split, a.span, full);
+    /* (without a branch, which the compiler makes a wait of; a wave without blocks reads one that it does not use) */
+    kv8_four next = kv8_load(codes, scales, first, b1 > 0 ? b1 - 1 : 0, lane);
     const float qf = a.scale * 1.44269504f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) q.v[e / 4][e % 4] *= qf;

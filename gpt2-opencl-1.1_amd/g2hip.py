@@ -343,8 +343,13 @@ def attn_kv8(q, q_stride, cache, out, out_stride, lens, T_kv, n_seq, n_head, max
 
 
 def logits_work_bytes(rows):
-    """Bytes of apply_logit_rules' workspace (needed where a pick is wanted)."""
+    """Bytes of apply_logit_rules' workspace (needed where a pick is wanted; logits_work makes one)."""
     return _lib.g2_logits_work_bytes(rows)
+
+
+def logits_work(rows):
+    """A workspace for apply_logit_rules as it has to be before its first use (zero)."""
+    return to_device(np.zeros(logits_work_bytes(rows), np.uint8))
 
 
 def logit_rules(ctx=None, ctx_len=None, max_ctx=0, repetition=1.0, frequency=0.0, presence=0.0, bias_id=None, bias=None,

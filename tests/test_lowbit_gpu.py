@@ -603,7 +603,7 @@ def test_calls_give_the_same_bits_again(g2):
     out = g2.DevBuf(4 * S * NH * H)
     logits = g2.to_device(r.standard_normal((30, V)).astype(np.float32))
     ctx = g2.to_device(r.integers(0, 300, (30, 500)).astype(np.int32))
-    lwork, lo, pick = g2.to_device(np.zeros(g2.logits_work_bytes(30), np.uint8)), g2.DevBuf(120 * V), g2.DevBuf(120)
+    lwork, lo, pick = g2.logits_work(30), g2.DevBuf(120 * V), g2.DevBuf(120)
     rules = g2.logit_rules(ctx=ctx, max_ctx=500, repetition=1.3, presence=0.1)
     first = None
     for turn in range(6):
@@ -650,7 +650,7 @@ class Step:
         f = lambda n: g2.DevBuf(4 * n)  # noqa: E731
         self.x, self.n, self.qkv, self.att, self.h = f(S * E), f(S * E), f(S * 3 * E), f(S * E), f(S * 4 * E)
         self.logits, self.out, self.pick = f(S * V), f(S * V), f(S)
-        self.work, self.lwork = g2.DevBuf(g2.kv8_work_bytes(S, NH)), g2.to_device(np.zeros(g2.logits_work_bytes(S), np.uint8))
+        self.work, self.lwork = g2.DevBuf(g2.kv8_work_bytes(S, NH)), g2.logits_work(S)
         self.ids, self.pos, self.len = g2.DevBuf(4 * S), g2.DevBuf(4 * S), g2.DevBuf(4 * S)
         self.ctx, self.ctx_len = g2.DevBuf(4 * S * max_seq), g2.DevBuf(4 * S)
 

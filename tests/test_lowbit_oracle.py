@@ -131,10 +131,10 @@ def test_q4_refusals():
 def test_kv8_refusals():
     checked("g2_kv8_append", (A, B, None, None, 3, 2, 4, 12, 64),
             [(0, None, ARG), (1, None, ARG), (1, B + 4, ARG), (4, -1, ARG), (4, 61, ARG), (5, 0, ARG), (6, 0, ARG), (6, 65, ARG),
-             (7, 0, ARG), (7, 1025, LIMIT), (8, 0, ARG), (8, (1 << 24) + 1, LIMIT), (0, B + 64, ARG)])
+             (7, 0, ARG), (7, 1025, LIMIT), (8, 0, ARG), (8, (1 << 24) + 1, LIMIT), (0, B + 64, ARG), (2, B + 16, ARG), (3, B, ARG)])
     checked("g2_kv8_read", (A, B, D, None, 60, 8, 50, 2, 12, 64),
             [(0, None, ARG), (1, None, ARG), (2, None, ARG), (4, 65, ARG), (4, -1, ARG), (5, -1, ARG), (5, 15, ARG), (6, 0, ARG), (7, 0, ARG),
-             (8, 0, ARG), (9, 0, ARG), (1, A, ARG), (2, B, ARG), (0, A + 8, ARG)])
+             (8, 0, ARG), (9, 0, ARG), (1, A, ARG), (2, B, ARG), (0, A + 8, ARG), (3, B, ARG), (3, D + 8, ARG)])
     checked("g2_attn_kv8", (A, 3 * 768, B, D, 768, None, 60, 2, 12, 64, C.c_float(0.125), E),
             [(0, None, ARG), (2, None, ARG), (3, None, ARG), (11, None, ARG), (1, 767, ARG), (4, 767, ARG), (6, 65, ARG), (6, -1, ARG),
              (7, 0, ARG), (8, 0, ARG), (9, 0, ARG), (8, 2000, LIMIT), (2, B + 8, ARG), (3, A + 4, ARG), (3, B, ARG), (3, E, ARG), (11, A, ARG),
