@@ -51,12 +51,12 @@ static int q4_check(const char *fn, const void *codes, const void *scales, int N
     return G2_OK;
 }
 
-/* Work-groups that lay out or read back: 64 rows of 128 columns of [K,N], two
+/* Work-groups that lay out or read back: 32 rows of 128 columns of [K,N], two
  * times 16 of [N,K]; the kernels stride over what is more. */
 static unsigned q4_groups(int N, int K, int in_out)
 {
     const long chunks = g2l_chunks(K), tiles = g2l_tiles(N);
-    const long n = in_out ? (tiles + 3) / 4 * chunks : (tiles * chunks + 1) / 2;
+    const long n = in_out ? (tiles + 1) / 2 * chunks : (tiles * chunks + 1) / 2;
     return n < 1 << 20 ? (unsigned)n : 1u << 20; /* (threads of a launch: below 2^32) */
 }
 
@@ -72,7 +72,7 @@ int g2_quantize_q4(const void *W, int w_dtype, int in_out, uint8_t *codes, uint1
         return g2i_err(G2_E_ARG, "g2_quantize_q4: overlapping buffers");
     if ((rc = ready())) return rc;
     g2_q4_args a = { W, codes, scales, NULL, N, K, group, in_out ? 1 : 0 };
-    if (in_out) return g2i_launch(w_dtype == G2_F16 ? G2F_Q4_PACK_T_F16 : G2F_Q4_PACK_T_F32, q4_groups(N, K, 1), 1, 1024, &a);
+    if (in_out) return g2i_launch(w_dtype == G2_F16 ? G2F_Q4_PACK_T_F16 : G2F_Q4_PACK_T_F32, q4_groups(N, K, 1), 1, 512, &a);
     return g2i_launch(w_dtype == G2_F16 ? G2F_Q4_PACK_F16 : G2F_Q4_PACK_F32, q4_groups(N, K, 0), 1, 256, &a);
 }
 
@@ -86,7 +86,7 @@ int g2_dequantize_q4(const uint8_t *codes, const uint16_t *scales, float *W, int
         return g2i_err(G2_E_ARG, "g2_dequantize_q4: overlapping buffers");
     if ((rc = ready())) return rc;
     g2_q4_args a = { NULL, (uint8_t *)codes, (uint16_t *)scales, W, N, K, group, in_out ? 1 : 0 };
-    return g2i_launch(in_out ? G2F_Q4_READ_T : G2F_Q4_READ, q4_groups(N, K, in_out), 1, in_out ? 1024 : 256, &a);
+    return g2i_launch(in_out ? G2F_Q4_READ_T : G2F_Q4_READ, q4_groups(N, K, in_out), 1, in_out ? 512 : 256, &a);
 }
 
 /* The kernel of a product.  Two forms: the loop (a work-group of 8 or 16 waves
@@ -281,7 +281,7 @@ int g2_attn_kv8(const float *q, int q_stride, const void *cache, float *out, int
     int waves;
     a.splits = g2i_kv8_form(heads, T_kv, &a.span, &waves);
     rc = g2i_launch(waves == 1 ? G2F_KV8_ATTN1 : waves == 4 ? G2F_KV8_ATTN4 : G2F_KV8_ATTN8, (unsigned)(heads * a.splits), 1,
-                    64u * (unsigned)waves, &a);
+                   64u * (unsigned)waves, &a);
     if (!rc && a.splits > 1) rc = g2i_launch(G2F_KV8_JOIN, (unsigned)heads, 1, 256, &a);
     return rc;
 }

@@ -130,9 +130,10 @@ __device__ __forceinline__ void q4_pack8(const g2_q4_args &a, const q4_raw<WT> &
 }
 
 /* W [N,K]: a work-group takes chunks of 16 rows x 128 columns, two at a time:
- * thread = row, step, place, eight consecutive columns.  50257 x 768 fp16 28.5
- * us, 3.5 TB/s (a thread per row and group, which walked its 32 columns one by
- * one: 204); reading back 30 us, 5.9 TB/s, most of it written (165). */
+ * thread = row, step, place, eight consecutive columns.  50257 x 768 fp16 27.6
+ * us, 3.6 TB/s (a thread per row and group, which walked its 32 columns one by
+ * one: 204); loads that do not stay in the L2 were slower (a lane's 32 bytes are
+ * two loads), as were 32-bit quotients in place of the divisions here. */
 template <typename WT>
 __device__ void q4_pack_impl(const g2_q4_args &a)
 {
@@ -156,29 +157,30 @@ __device__ void q4_pack_impl(const g2_q4_args &a)
 G2K void g2k_q4_pack_f32(const g2_q4_args a) { q4_pack_impl<float>(a); }
 G2K void g2k_q4_pack_f16(const g2_q4_args a) { q4_pack_impl<_Float16>(a); }
 
-/* W [K,N]: 64 rows x 128 columns at a time through LDS (64 neighbouring
+/* W [K,N]: 32 rows x 128 columns at a time through LDS (32 neighbouring
  * values of a column are one run in memory), all of a thread's eight loads in
- * flight: 768 x 768 4.6 us (8.4 with a quarter of the threads). */
-#define Q4_TROW 65
+ * flight: 768 x 768 3.7 us, 6400 x 1600 14.9 (4.6 and 22.4 with 64 rows, whose
+ * two work-groups to a CU wait more than these four). */
+#define Q4_TROW 33
 template <typename WT>
 __device__ void q4_pack_t_impl(const g2_q4_args &a)
 {
     __shared__ WT ws[128 * Q4_TROW];
     const WT *W = (const WT *)a.W;
     const int tid = threadIdx.x, u = tid >> 8, r = tid >> 4 & 15, j = tid >> 2 & 3, p = tid & 3;
-    const long chunks = g2l_chunks(a.K), tiles = g2l_tiles(a.N), items = (tiles + 3) / 4 * chunks;
+    const long chunks = g2l_chunks(a.K), tiles = g2l_tiles(a.N), items = (tiles + 1) / 2 * chunks;
     for (long i = blockIdx.x; i < items; i += gridDim.x) {
-        const long t0 = i / chunks * 4, c = i % chunks, n = t0 * 16 + (tid & 63);
+        const long t0 = i / chunks * 2, c = i % chunks, n = t0 * 16 + (tid & 31);
         const WT *col = W + (n < a.N ? n : a.N - 1);
         WT v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const long k = c * 128 + (tid >> 6) + 16 * e;
+            const long k = c * 128 + (tid >> 5) + 16 * e;
             v[e] = col[(k < a.K ? k : a.K - 1) * a.N];
             if (n >= a.N || k >= a.K) v[e] = (WT)0.f;
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ws[((tid >> 6) + 16 * e) * Q4_TROW + (tid & 63)] = v[e];
+        for (int e = 0; e < 8; ++e) ws[((tid >> 5) + 16 * e) * Q4_TROW + (tid & 31)] = v[e];
         __syncthreads();
         q4_raw<WT> w;
 #pragma unroll
@@ -187,8 +189,8 @@ __device__ void q4_pack_t_impl(const g2_q4_args &a)
         __syncthreads();
     }
 }
-extern "C" __global__ __launch_bounds__(1024) void g2k_q4_pack_t_f32(const g2_q4_args a) { q4_pack_t_impl<float>(a); }
-extern "C" __global__ __launch_bounds__(1024) void g2k_q4_pack_t_f16(const g2_q4_args a) { q4_pack_t_impl<_Float16>(a); }
+extern "C" __global__ __launch_bounds__(512) void g2k_q4_pack_t_f32(const g2_q4_args a) { q4_pack_t_impl<float>(a); }
+extern "C" __global__ __launch_bounds__(512) void g2k_q4_pack_t_f16(const g2_q4_args a) { q4_pack_t_impl<_Float16>(a); }
 
 /* The eight values of a lane's word of codes. */
 __device__ __forceinline__ void q4_values(unsigned w, float s, float v[8])
@@ -205,10 +207,16 @@ __device__ __forceinline__ unsigned q4_word(const g2_q4_args &a, long t, long c,
     return j < g2l_chunk_steps(a.K, c) ? *(const unsigned *)(a.codes + g2l_code_at(a.K, t, c, 16 * p + r) + 4 * j) : 0u;
 }
 
-/* To [N,K]: threads as in the laying out. */
+/* To [N,K]: threads as in the laying out; the 16 lanes of a row then take its
+ * 128 columns four at a time, so that a store is 256 bytes of each of four
+ * rows.  Where rows are whole 64-byte pieces the stores do not stay in the L2.
+ * 50257 x 768, values that no cache holds, 26.4 us; with ordinary stores 39.0
+ * (10388 x 3715, whose rows are not, 53.7 and 59.3 the other way round); with a
+ * lane's own 32 bytes in two stores 46.9. */
 G2K void g2k_q4_read(const g2_q4_args a)
 {
-    const int tid = threadIdx.x, r = tid >> 4, j = tid >> 2 & 3, p = tid & 3;
+    const int tid = threadIdx.x, r = tid >> 4, j = tid >> 2 & 3, p = tid & 3, lane = tid & 63, l = tid & 15;
+    const bool whole = a.K % 16 == 0 && (uintptr_t)a.out % 64 == 0;
     const long chunks = g2l_chunks(a.K), items = g2l_tiles(a.N) * chunks;
     for (long i = blockIdx.x * 2l; i < items; i += gridDim.x * 2l) {
         unsigned w[2];
@@ -220,29 +228,37 @@ G2K void g2k_q4_read(const g2_q4_args a)
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const long n = (i + u) / chunks * 16 + r, k = (i + u) % chunks * 128 + 32 * j + 8 * p;
-            if (i + u >= items || n >= a.N || k >= a.K) continue;
-            float v[8];
-            q4_values(w[u], s[u], v);
-            float *o = a.out + n * a.K + k;
-            if (k + 8 <= a.K) {
-                *(f32x4u *)o = f32x4{ v[0], v[1], v[2], v[3] };
-                *(f32x4u *)(o + 4) = f32x4{ v[4], v[5], v[6], v[7] };
-            } else
-                for (int e = 0; e < 8; ++e)
-                    if (k + e < a.K) o[e] = v[e];
+            const long n = (i + u) / chunks * 16 + r, k0 = (i + u) % chunks * 128 + 4 * l;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int from = (lane & 48) + 8 * h + (l >> 1); /* the lane that has columns 64 h + 4 l .. + 3 */
+                const unsigned wh = (unsigned)__shfl((int)w[u], from) >> 16 * (l & 1);
+                const float sh = __shfl(s[u], from);
+                const long k = k0 + 64 * h;
+                if (i + u >= items || n >= a.N || k >= a.K) continue;
+                typedef float f32x2 __attribute__((ext_vector_type(2)));
+                const f32x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(wh, 1.0f, 0), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(wh, 1.0f, 1);
+                const f32x4 v = { lo[0] * sh, lo[1] * sh, hi[0] * sh, hi[1] * sh };
+                float *o = a.out + n * a.K + k;
+                if (whole) __builtin_nontemporal_store(v, (f32x4 *)o);
+                else if (k + 4 <= a.K) *(f32x4u *)o = v;
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (k + e < a.K) o[e] = v[e];
+            }
         }
     }
 }
 
 /* To [K,N], through LDS. */
-extern "C" __global__ __launch_bounds__(1024) void g2k_q4_read_t(const g2_q4_args a)
+extern "C" __global__ __launch_bounds__(512) void g2k_q4_read_t(const g2_q4_args a)
 {
     __shared__ float ws[128 * Q4_TROW];
     const int tid = threadIdx.x, u = tid >> 8, r = tid >> 4 & 15, j = tid >> 2 & 3, p = tid & 3;
-    const long chunks = g2l_chunks(a.K), tiles = g2l_tiles(a.N), items = (tiles + 3) / 4 * chunks;
+    const long chunks = g2l_chunks(a.K), tiles = g2l_tiles(a.N), items = (tiles + 1) / 2 * chunks;
     for (long i = blockIdx.x; i < items; i += gridDim.x) {
-        const long t0 = i / chunks * 4, c = i % chunks, n = t0 * 16 + (tid & 63);
+        const long t0 = i / chunks * 2, c = i % chunks, n = t0 * 16 + (tid & 31);
         float s, v[8];
         const unsigned w = q4_word(a, t0 + u < tiles ? t0 + u : tiles - 1, c, r, j, p, &s);
         q4_values(w, s, v);
@@ -250,8 +266,8 @@ extern "C" __global__ __launch_bounds__(1024) void g2k_q4_read_t(const g2_q4_arg
         for (int e = 0; e < 8; ++e) ws[(32 * j + 8 * p + e) * Q4_TROW + 16 * u + r] = v[e];
         __syncthreads();
 #pragma unroll
-        for (int k = tid >> 6; k < 128; k += 16)
-            if (n < a.N && c * 128 + k < a.K) a.out[(c * 128 + k) * a.N + n] = ws[k * Q4_TROW + (tid & 63)];
+        for (int k = tid >> 5; k < 128; k += 16)
+            if (n < a.N && c * 128 + k < a.K) a.out[(c * 128 + k) * a.N + n] = ws[k * Q4_TROW + (tid & 31)];
         __syncthreads();
     }
 }
@@ -681,8 +697,9 @@ Q4_HELD(8, 16, 2)
  * of each of four rows, and neighbouring waves have neighbouring heads.  The
  * first block's wave reads the positions that came before from `last` and then
  * writes there what the call leaves of its last block: in one wave, since both
- * may be the same rows.  Four prompts of 1001 rows x 25 heads: 17.3 us, 3.7
- * TB/s of the keys and values read and the codes written (19.0 with the blocks
+ * may be the same rows.  Four prompts of 1001 rows x 25 heads: 12.8 us, 5.0
+ * TB/s of the keys and values read and the codes written (17.3 when a reading
+ * back just before had left its values in the L2, and 19.0 then with the blocks
  * of one head side by side, whose loads are 16 rows 19 KB apart); one token:
  * 3.1, the latency of a load, the maximum over the wave and a store. */
 G2K void g2k_kv8_append(const g2_kv8_append_args a)
@@ -779,8 +796,8 @@ G2K void g2k_kv8_read(const g2_kv8_read_args a)
             kv[0] = *(const f32x4 *)l;
             kv[1] = *(const f32x4 *)(l + G2L_BLOCK * G2L_DH);
         }
-        *(f32x4u *)(a.k + 4 * i) = kv[0];
-        *(f32x4u *)(a.v + 4 * i) = kv[1];
+        __builtin_nontemporal_store(kv[0], (f32x4u *)(a.k + 4 * i));
+        __builtin_nontemporal_store(kv[1], (f32x4u *)(a.v + 4 * i));
     }
 }
 
@@ -793,9 +810,9 @@ G2K void g2k_kv8_read(const g2_kv8_read_args a)
  * and over the parts of a long sequence in a second launch.  Scores are held
  * in units of log 2, the queries carrying the factor.
  *
- * Bounded by HBM for many or long sequences (48 x 25 heads x 256..1024 23 us,
- * 4.3 TB/s; 16 heads x 50001 19 us and 4 to join, 4.4 TB/s; a wave for each
- * head, a position at a time, took 35 ms there), by latency for one short
+ * Bounded by HBM for many or long sequences (48 x 25 heads x 1024 28 us, 5.7
+ * TB/s; 16 heads x 50001 18 us and 4 to join, 4.7 TB/s; a wave for each head, a
+ * position at a time, took 35 ms there), by latency for one short
  * sequence (12 heads x 701 5.2 us: the launch, the length, two rounds of
  * loads, the sums over lanes and waves).  The next four blocks' loads go out
  * before the last ones' sums, and the sums over the lanes need no LDS (25 heads
@@ -856,7 +873,9 @@ __device__ __forceinline__ void kv8_add(kv8_sum &a, const float *s, const float 
 /* Four blocks' codes and scales; a block behind the last one of the part is the
  * last again.  (Asking for the first four by the bound of the lengths, before
  * the length is there, saved 0.1 us where they were needed and cost up to half
- * the time of many short sequences under a high bound.) */
+ * the time of many short sequences under a high bound.)  Codes are read once:
+ * loads that do not stay in the L2 (48 x 25 heads x 1024 28.0 us, ordinary ones
+ * 32.8; 16 heads x 50001 21.8, 23.1; a few heads the same). */
 struct kv8_four {
     u32x4 k[4], v[4];
     float sk[4], sv[4];
@@ -868,8 +887,8 @@ __device__ __forceinline__ kv8_four kv8_load(const int8_t *codes, const float *s
     for (int u = 0; u < 4; ++u) {
         const int bu = b + u < last ? b + u : last;
         const int8_t *p = codes + (size_t)bu * (2 * G2L_BLOCK * G2L_DH) + 16 * lane;
-        r.k[u] = *(const u32x4 *)p;
-        r.v[u] = *(const u32x4 *)(p + G2L_BLOCK * G2L_DH);
+        r.k[u] = __builtin_nontemporal_load((const u32x4 *)p);
+        r.v[u] = __builtin_nontemporal_load((const u32x4 *)(p + G2L_BLOCK * G2L_DH));
         r.sk[u] = scales[2 * bu];
         r.sv[u] = scales[2 * bu + 1];
     }

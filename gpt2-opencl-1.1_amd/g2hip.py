@@ -218,8 +218,8 @@ def to_device(arr):
 
 
 def _p(x):
-    if x is None:
-        return None
+    if x is None or type(x) is int:
+        return x
     if isinstance(x, DevBuf):
         return x.ptr
     return int(x)

@@ -176,6 +176,19 @@ def test_matvec_q4_residual_in_place(g2):
     within(take(y, M * N).reshape(M, N), x.astype(np.float64) @ v.T + res, matvec_bound(x, v, K) + 4 * EPS32 * (1 + np.abs(res)) * 40)
 
 
+@pytest.mark.parametrize("M,N,K,group", [(1, 300, 256, 32), (3, 4500, 200, 64), (1, 32800, 96, 128), (9, 32800, 96, 32)])
+def test_matvec_q4_bias_residual_and_gelu(g2, M, N, K, group):
+    """All of the epilogue at once: GELU of the product, the bias and the residual."""
+    r = rng(33, N)
+    W = (0.05 * r.standard_normal((N, K))).astype(np.float32)
+    x, bias, res = (r.standard_normal(n).astype(np.float32) for n in ((M, K), N, (M, N)))
+    codes, scales = packed(g2, W, group)
+    v = lowbit.values_q4(*lowbit.quantize_q4(W, group), group)
+    y = x.astype(np.float64) @ v.T + bias + res
+    bound = 1.13 * (matvec_bound(x, v, K) + 4 * EPS32 * (np.abs(y) + np.abs(bias) + np.abs(res))) + 16 * EPS32 * (1 + np.abs(y))
+    within(run_matvec(g2, x, codes, scales, N, K, group, bias, res, 1), lowbit.gelu(y), bound)
+
+
 @pytest.mark.parametrize("M", [1, 2, 8, 9])
 def test_matvec_q4_range_of_activations(g2, M):
     """Activations of any size: every row scaled differently, columns over 30 orders of magnitude, zeros, denormals."""
