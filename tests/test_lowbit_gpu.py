@@ -165,6 +165,44 @@ def test_matvec_q4(g2, M, N, K, group):
     within(run_matvec(g2, x, codes, scales, N, K, group, bias, None, 1), lowbit.gelu(y), 1.13 * bound + 16 * EPS32 * (1 + np.abs(y)), "GELU")
 
 
+@pytest.mark.parametrize("in_out", [False, True])
+def test_q4_beyond_32_bit_offsets(g2, in_out):
+    """Codes beyond 4 GB, weights and their values beyond 16 and 32: zeros but for the last five columns."""
+    N, K, group, n = 4112, 2 ** 21, 32, 5
+    v = (0.02 * rng(41).standard_normal((N, n))).astype(np.float16)
+    tail = np.zeros((N, group), np.float32)
+    tail[:, -n:] = v
+    want = lowbit.values_q4(*lowbit.quantize_q4(tail, group), group)
+    nc, ns = g2.q4_bytes(N, K, group)
+    assert nc > 2 ** 32
+    W, codes, scales = g2.DevBuf(2 * N * K), g2.DevBuf(nc), g2.DevBuf(ns)
+    g2.check(g2._lib.g2_memset(W.ptr, 0, 2 * N * K))
+    if in_out:
+        vt = np.ascontiguousarray(v.T)
+        g2.check(g2._lib.g2_upload(W.ptr + 2 * N * (K - n), vt.ctypes.data, v.nbytes))
+    else:
+        rows = [0, 1, 700, N - 2, N - 1]  # (a copy for each row: a few rows)
+        want[[r for r in range(N) if r not in rows]] = 0
+        for r in rows:
+            g2.check(g2._lib.g2_upload(W.ptr + 2 * ((r + 1) * K - n), v[r].ctypes.data, 2 * n))
+    g2.quantize_q4(W, g2.F16, in_out, codes, scales, N, K, group)
+    del W
+    out = g2.DevBuf(4 * N * K)
+    g2.dequantize_q4(codes, scales, out, in_out, N, K, group)
+    got = np.empty((40, N) if in_out else (2, K), np.float32)
+    g2.check(g2._lib.g2_download(got.ctypes.data, out.ptr + 4 * N * K - got.nbytes, got.nbytes))
+    assert (got[:-n] == 0).all() if in_out else (got[:, :-n] == 0).all()
+    same(got[-n:].T if in_out else got[:, -n:], want[:, -n:] if in_out else want[-2:, -n:])
+    del out
+    for M in (1, 9):
+        x = rng(42, M).standard_normal((M, K)).astype(np.float32)
+        y = run_matvec(g2, x, codes, scales, N, K, group)
+        xt = x[:, -n:].astype(np.float64)
+        top = np.abs(x[:, -128:]).max(1)[:, None]
+        bound = ((164 + K / 128) * EPS32 + 2.0 ** -22) * (np.abs(xt) @ np.abs(want[:, -n:]).T)
+        within(y, xt @ want[:, -n:].T, bound + 2.0 ** -38 * top * np.abs(want[:, -n:]).sum(1))
+
+
 def test_matvec_q4_residual_in_place(g2):
     M, N, K, group = 3, 200, 300, 64
     r = rng(2)
@@ -520,7 +558,8 @@ def test_attend_beyond_32_bit_offsets(g2):
 def run_rules(g2, l, pick=True, out=True, in_place=False, **kw):
     R, V = l.shape
     dl = guarded(g2, R * V)
-    g2.check(g2._lib.g2_upload(dl.ptr, np.ascontiguousarray(l).ctypes.data, l.nbytes))
+    l = np.ascontiguousarray(l)
+    g2.check(g2._lib.g2_upload(dl.ptr, l.ctypes.data, l.nbytes))
     do = dl if in_place else guarded(g2, R * V) if out else None
     dp = g2.to_device(np.full(R + 4, 77, np.int32)) if pick else None
     work = g2.to_device(np.zeros(g2.logits_work_bytes(R) + 8, np.uint8)) if pick else None
