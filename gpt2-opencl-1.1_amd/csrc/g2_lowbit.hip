@@ -688,16 +688,17 @@ Q4_HELD(8, 16, 2)
  * rint(fp32(x / scale)), scale = fp32(max |x| / 127), and stands for code *
  * scale; the positions of a sequence's last block stand in fp32 until the
  * block is full, so that what a cache holds does not depend on how many
- * positions came at a time.  A block that holds an infinity or NaN gets a
- * NaN scale.
+ * positions came at a time; they are kept there when it is, until the next
+ * block begins, so that a sequence can be cut back to any length in it.  A
+ * block that holds an infinity or NaN gets a NaN scale.
  * ==================================================================== */
 
 /* One wave per sequence, head, keys or values and block of the call; load i of
  * a lane is four dims of position 4 i + lane / 16, so that a load is 256 bytes
  * of each of four rows, and neighbouring waves have neighbouring heads.  The
  * first block's wave reads the positions that came before from `last` and then
- * writes there what the call leaves of its last block: in one wave, since both
- * may be the same rows.  Four prompts of 1001 rows x 25 heads: 12.8 us, 5.0
+ * writes there what the call has of its last block, full or not: in one wave,
+ * since both may be the same rows.  Four prompts of 1001 rows x 25 heads: 12.8 us, 5.0
  * TB/s of the keys and values read and the codes written (17.3 when a reading
  * back just before had left its values in the L2, and 19.0 then with the blocks
  * of one head side by side, whose loads are 16 rows 19 KB apart); one token:
@@ -754,7 +755,7 @@ G2K void g2k_kv8_append(const g2_kv8_append_args a)
     if (i) return;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-        const int t = 4 * u + t0, p = end / G2L_BLOCK * G2L_BLOCK + t;
+        const int t = 4 * u + t0, p = (end - 1) / G2L_BLOCK * G2L_BLOCK + t;
         if (p >= p0 && p < end) *(f32x4 *)(last + t * G2L_DH) = *(const f32x4u *)(rows + (size_t)(p - p0) * 3 * D);
     }
 }

@@ -17,8 +17,8 @@
  * 8-bit cache of S sequences, NH heads of 64 dims, blocks of 16 positions:
  *  codes  [S][NH][blocks][K, V][16][64] int8,
  *  scales [S][NH][blocks][K, V] fp32 (padded to 256 bytes),
- *  last   [S][NH][K, V][16][64] fp32: the positions of the block that is not
- *  full yet.
+ *  last   [S][NH][K, V][16][64] fp32: the positions of the block that was
+ *  appended to last, as they came.
  */
 #ifndef G2_LOWBIT_PLAN_H
 #define G2_LOWBIT_PLAN_H

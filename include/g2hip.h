@@ -222,8 +222,10 @@ int g2_matvec_q4(const float *x, const uint8_t *codes, const uint16_t *scales,
  *   codes  int8 [n_seq][n_head][blocks][K, V][16][64]
  *   scales fp32 [n_seq][n_head][blocks][K, V], padded to 256 bytes
  *   last   fp32 [n_seq][n_head][K, V][16][64]
- * A sequence may be cut back to a length in its last block or to whole blocks
- * and appended to from there. */
+ * A sequence may be cut back, and appended to from there, to any length inside
+ * the block of the position that was appended last (the block may be full), or
+ * to any number of whole blocks before it; after a cut to whole blocks only to
+ * fewer whole blocks, until something is appended. */
 size_t g2_kv8_bytes(int n_seq, int n_head, int max_seq);
 /* g2_split_kv for this cache: rows qkv[n_seq][T][3 D] (keys at column D, values
  * at 2 D) go to positions p .. p + c - 1 of their sequence; p = pos[s], or
