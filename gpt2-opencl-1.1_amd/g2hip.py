@@ -354,9 +354,12 @@ def logits_work(rows):
 
 def logit_rules(ctx=None, ctx_len=None, max_ctx=0, repetition=1.0, frequency=0.0, presence=0.0, bias_id=None, bias=None,
                 n_bias=0, mask=None, mask_stride=0, forbid=-1):
-    """A g2_logit_rules: penalties for the context's ids, a list of biases, a mask of allowed ids, a forbidden id."""
-    return LogitRules(_p(ctx), _p(ctx_len), max_ctx, repetition, frequency, presence, _p(bias_id), _p(bias), n_bias, _p(mask),
-                      mask_stride, forbid)
+    """A g2_logit_rules: penalties for the context's ids, a list of biases, a mask of allowed ids, a forbidden id.
+    It keeps the buffers that it is given alive."""
+    r = LogitRules(_p(ctx), _p(ctx_len), max_ctx, repetition, frequency, presence, _p(bias_id), _p(bias), n_bias, _p(mask),
+                   mask_stride, forbid)
+    r._buffers = (ctx, ctx_len, bias_id, bias, mask)  # (the structure itself holds addresses alone)
+    return r
 
 
 def apply_logit_rules(logits, out, pick, rows, V, rules, work):

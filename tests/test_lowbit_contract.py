@@ -1,0 +1,31 @@
+"""The decode operators in fewer bits, what can be told without a GPU: what the binding keeps alive."""
+import gc
+import weakref
+
+import pytest
+
+import g2hip
+
+
+class Buf(g2hip.DevBuf):
+    """A buffer that owns no memory."""
+
+    def __init__(self, ptr):
+        self.ptr, self.nbytes = ptr, 0
+
+    def free(self):
+        self.ptr = None
+
+
+@pytest.mark.parametrize("name", ["ctx", "ctx_len", "bias_id", "bias", "mask"])
+def test_rules_keep_their_buffers(name):
+    """A structure of rules holds addresses: buffers that only it refers to live as long as it does."""
+    buf = Buf(0x1000)
+    alive = weakref.ref(buf)
+    rules = g2hip.logit_rules(**{name: buf}, max_ctx=3, n_bias=2)
+    del buf
+    gc.collect()
+    assert alive() is not None and getattr(rules, name) == alive().ptr == 0x1000
+    del rules
+    gc.collect()
+    assert alive() is None
