@@ -276,11 +276,16 @@ extern "C" __global__ __launch_bounds__(512) void g2k_q4_read_t(const g2_q4_args
  * tile of 16 rows is one 16-byte load a lane; the hardware's conversion makes
  * fp16 of it (exact; two values an operation) and four 16x16x32 products of
  * it, one operand the 16 weight rows, the other up to 8 activation rows, each
- * as two fp16 parts: hi = fp16(x'), lo = fp16(x' - hi), x' the activation
+ * as two fp16 parts: hi = fp16(x'), lo = fp16(2^11 (x' - hi)), x' the activation
  * times a power of two that brings the largest of its 128 to 2^14..2^15.  hi +
- * lo is within 2^-22 of x' (and the power of two within fp32's range, so any
- * activations keep fp32 accuracy).  A group's scale multiplies its sum, the
- * power of two a chunk's; all sums are fp32.
+ * 2^-11 lo is within 2^-22 of x' where |x'| is 2^-14 or more.  A chunk with an
+ * activation below that (2^-28 of its largest, but not 0) or an infinity is left
+ * to the vector units, which multiply and add in fp32 (q4_add_plain; one in 10^6
+ * rows of normally distributed values): so every activation enters with 2^-22
+ * of its own value.  Such a chunk costs a product 2 to 8 us (6400 x 1600, one and
+ * 8 rows), in the held form, which then takes all chunks so, more (50257 x 1600
+ * 45 and 152 us in all).  A group's scale multiplies its sum, the power of two a
+ * chunk's; all sums are fp32.
  *
  * Bounded by HBM for large matrices and by the launch and two load latencies
  * for small ones: 50257 x 1600, groups of 128, 9.9 us in a replayed graph with
@@ -305,8 +310,7 @@ __device__ __forceinline__ f16x8 q4_operand(unsigned w)
 }
 
 /* The power of two (and its inverse) that brings a value of these bits, the
- * largest of its chunk, to 2^14..2^15; 2^126 at most, where every bit of the
- * chunk's values lies within the parts' range. */
+ * largest of its chunk, to 2^14..2^15; 2^126 at most. */
 struct q4_power { float down, up; };
 __device__ __forceinline__ q4_power q4_power_of(unsigned amax)
 {
@@ -314,13 +318,18 @@ __device__ __forceinline__ q4_power q4_power_of(unsigned amax)
     return { __uint_as_float((268 - e) << 23), __uint_as_float((e - 14) << 23) };
 }
 
-/* hi and lo parts of two activations */
+/* hi and lo parts of two activations (every step but the two conversions is exact) */
+#define Q4_LO 2048.0f
 __device__ __forceinline__ void q4_split(float a, float b, float down, f16x2 &hi, f16x2 &lo)
 {
     hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(a * down, b * down));
-    lo[0] = (_Float16)__builtin_fmaf(a, down, -(float)hi[0]);
-    lo[1] = (_Float16)__builtin_fmaf(b, down, -(float)hi[1]);
+    lo[0] = (_Float16)(__builtin_fmaf(a, down, -(float)hi[0]) * Q4_LO);
+    lo[1] = (_Float16)(__builtin_fmaf(b, down, -(float)hi[1]) * Q4_LO);
 }
+
+/* Whether any lane says so, as one value of the wave (the compiler takes __any's
+ * for a lane's: both sides of its branch then hold their registers at once). */
+__device__ __forceinline__ bool wave_any(bool b) { return __builtin_amdgcn_ballot_w64(b) != 0; }
 
 template <int CTRL> __device__ __forceinline__ float dpp_max(float v)
 {
@@ -331,6 +340,7 @@ template <int CTRL> __device__ __forceinline__ float dpp_max(float v)
 
 template <int MT> struct q4_x {
     float v[MT == 1 ? 2 : 16];
+    bool behind; /* no column of the lane's lies in the matrix */
 };
 
 /* The chunk's activations: MT == 1: two columns a lane; else lane 8 m + i has
@@ -341,6 +351,7 @@ __device__ __forceinline__ q4_x<MT> q4_load_x(const g2_q4mv_args &a, int m0, int
     q4_x<MT> x;
     const int n = MT == 1 ? 2 : 16, m = m0 + (MT == 1 ? 0 : lane >> 3), k = 128 * c + n * (MT == 1 ? lane : lane & 7);
     const float *p = a.x + (size_t)(m < a.M ? m : a.M - 1) * a.K; /* (a row behind the last: the last, not written) */
+    x.behind = k >= a.K;
     if (MT == 1 && 128 * c + 128 <= a.K) { /* (uniform) */
         x.v[0] = p[k];
         x.v[1] = p[k + 1];
@@ -360,52 +371,61 @@ __device__ __forceinline__ q4_x<MT> q4_load_x(const g2_q4mv_args &a, int m0, int
     return x;
 }
 
-/* Splits them into xs ([part of row][Q4_XROW]); returns the inverse powers of
- * two of the lane's own rows of the product: MT == 1: row 0; else rows
- * 2 (lane / 16) and + 1.  Infinities (rare: their own path) are hi, beside lo
- * 0, and do not count for the power of two; nor does a NaN, which is both. */
+/* The largest of the lane's row of the chunk, of magnitudes as bits. */
 template <int MT>
-__device__ __forceinline__ float q4_largest(float amax)
+__device__ __forceinline__ unsigned q4_largest(unsigned amax)
 {
-    amax = dpp_max<0xB1>(amax);  /* quad: lanes 1 0 3 2 */
-    amax = dpp_max<0x4E>(amax);  /* 2 3 0 1 */
-    amax = dpp_max<0x141>(amax); /* half rows of 8, mirrored */
+    amax = q4_group_max(amax, 64); /* 8 lanes */
     if constexpr (MT == 1) {
-        amax = dpp_max<0x140>(amax); /* rows of 16, mirrored */
-        const int u = __float_as_int(amax);
-        const float r0 = __int_as_float(__builtin_amdgcn_readlane(u, 0)), r1 = __int_as_float(__builtin_amdgcn_readlane(u, 16));
-        const float r2 = __int_as_float(__builtin_amdgcn_readlane(u, 32)), r3 = __int_as_float(__builtin_amdgcn_readlane(u, 48));
-        amax = fmaxf(fmaxf(r0, r1), fmaxf(r2, r3));
+        amax = dpp_umax<0x140>(amax); /* rows of 16, mirrored */
+        const unsigned r0 = __builtin_amdgcn_readlane(amax, 0), r1 = __builtin_amdgcn_readlane(amax, 16);
+        const unsigned r2 = __builtin_amdgcn_readlane(amax, 32), r3 = __builtin_amdgcn_readlane(amax, 48);
+        const unsigned m0 = r0 > r1 ? r0 : r1, m1 = r2 > r3 ? r2 : r3;
+        amax = m0 > m1 ? m0 : m1;
     }
     return amax;
 }
 
-template <int MT>
-__device__ __forceinline__ void q4_split_x(const q4_x<MT> &x, _Float16 *xs, float *xe, int lane, float e[2])
+/* The powers of two of the lane's row; plain: whether any row's parts would not
+ * hold a value of it: an infinity, or one below 2^-14 up that is not 0 (at the
+ * least power both parts hold the smallest numbers too).  A NaN counts for
+ * neither: it is a NaN in both parts.  Zeros are told from small values behind
+ * the branch (1600 x 6400, 8 rows, 8.1 us; for every chunk 8.5). */
+struct q4_seen {
+    q4_power own;
+    bool plain;
+};
+template <int MT> __device__ __forceinline__ q4_seen q4_look(const q4_x<MT> &x)
 {
     constexpr int N = MT == 1 ? 2 : 16;
-    float amax = 0.f;
+    float amax = 0.f, least = INFINITY;
 #pragma unroll
-    for (int i = 0; i < N; ++i) amax = fmaxf(amax, fabsf(x.v[i]));
-    amax = q4_largest<MT>(amax);
-    const bool odd = __any(amax == INFINITY);
-    if (odd) {
-        amax = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) amax = fmaxf(amax, fabsf(x.v[i]) < INFINITY ? fabsf(x.v[i]) : 0.f);
-        amax = q4_largest<MT>(amax);
+    for (int i = 0; i < N; ++i) {
+        amax = fmaxf(amax, fabsf(x.v[i]));
+        least = fminf(least, fabsf(x.v[i]));
     }
-    const q4_power own = q4_power_of(__float_as_uint(amax));
+    const unsigned top = q4_largest<MT>(__float_as_uint(amax));
+    q4_seen s = { q4_power_of(top), false };
+    const float low = s.own.up > 0x1p-126f ? s.own.up * 0x1p-14f : 0.f;
+    if (wave_any((top == 0x7F800000u) | ((least < low) & !x.behind))) {
+        bool plain = top == 0x7F800000u;
+#pragma unroll
+        for (int i = 0; i < N; ++i) plain |= (x.v[i] != 0.f) & (fabsf(x.v[i]) < low);
+        s.plain = wave_any(plain);
+    }
+    return s;
+}
+
+/* Splits them into xs ([part of row][Q4_XROW]) and gives the inverse powers of
+ * two of the lane's own rows of the product: MT == 1: row 0; else rows
+ * 2 (lane / 16) and + 1. */
+template <int MT>
+__device__ __forceinline__ void q4_split_x(const q4_x<MT> &x, const q4_power &own, _Float16 *xs, float *xe, int lane, float e[2])
+{
+    constexpr int N = MT == 1 ? 2 : 16;
     f16x2 hi[N / 2], lo[N / 2];
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) q4_split(x.v[2 * i], x.v[2 * i + 1], own.down, hi[i], lo[i]);
-    if (odd)
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (fabsf(x.v[i]) == INFINITY) {
-                hi[i / 2][i % 2] = (_Float16)x.v[i];
-                lo[i / 2][i % 2] = (_Float16)0.f;
-            }
     _Float16 *row = xs + (MT == 1 ? 0 : 2 * (lane >> 3)) * Q4_XROW + N * (MT == 1 ? lane : lane & 7);
     if constexpr (MT == 1) {
         *(f16x2 *)row = hi[0];
@@ -491,14 +511,66 @@ __device__ __forceinline__ void q4_products(const f16x8 x[4], const u32x4 &w, co
         for (int j = 4 / P * g; j < 4 / P * (g + 1); ++j)
             d = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[j], q4_operand(w[j]), d, 0, 0, 0);
         const float sc = bf16_f(scale[g]);
-        s[0] = fmaf(sc, d[0] + d[1], s[0]);
-        if constexpr (MT > 1) s[1] = fmaf(sc, d[2] + d[3], s[1]);
+        s[0] = fmaf(sc, fmaf(d[1], 1.f / Q4_LO, d[0]), s[0]);
+        if constexpr (MT > 1) s[1] = fmaf(sc, fmaf(d[3], 1.f / Q4_LO, d[2]), s[1]);
     }
     y[0] = fmaf(s[0], e[0], y[0]);
     if constexpr (MT > 1) y[1] = fmaf(s[1], e[1], y[1]);
     if constexpr (MT > 1) asm volatile("" : "+v"(y[0]), "+v"(y[1]));
     else asm volatile("" : "+v"(y[0]));
 }
+
+/* Adds chunk c's products to the sums of the TR tiles in fp32: a lane takes the
+ * columns of its own codes, four at a time, for all activation rows, and the four
+ * lanes of a weight row meet. */
+template <int MT, int TR, int G>
+__device__ __forceinline__ void q4_add_plain(const g2_q4mv_args &a, int m0, int c, int lane, const uint8_t *const *codes,
+                                             const uint16_t *const *scales, const q4_lane &ql, float (*y)[2])
+{
+    constexpr int P = 128 / G;
+    const unsigned at = c == ql.last ? ql.part : ql.whole;
+    const int shift = c == ql.last ? ql.shift : 0;
+    float sum[TR][MT] = {};
+#pragma unroll 1
+    for (int j = 0; j < 8; ++j) { /* half a word of codes */
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        const int k = 128 * c + 32 * (j >> 1) + 8 * (lane >> 4) + 4 * (j & 1);
+        const int word = (j >> 1) + shift < 3 ? (j >> 1) + shift : 3; /* (behind K: x is 0) */
+        f32x4 x[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const float *p = a.x + (size_t)(m0 + m < a.M ? m0 + m : a.M - 1) * a.K;
+            if (128 * c + 128 <= a.K || a.K % 4 == 0) { /* (uniform) */
+                x[m] = *(const f32x4u *)(p + (k < a.K ? k : 0));
+                if (k >= a.K) x[m] = f32x4{ 0.f, 0.f, 0.f, 0.f };
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[m][i] = k + i < a.K ? p[k + i < a.K ? k + i : 0] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < TR; ++t) {
+            const unsigned q = *(const unsigned *)(codes[t] + c * 1024l + at + 4 * word) >> 16 * (j & 1);
+            const float s = bf16_f(scales[t][(c * 16l + (lane & 15)) * P + (j >> 1) * P / 4]);
+            const f32x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 0), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 1);
+            const float v[4] = { lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s };
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[t][m] = fmaf(v[i], x[m][i], sum[t][m]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < TR; ++t)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            float v = sum[t][m];
+            v += __shfl_xor(v, 16);
+            v += __shfl_xor(v, 32);
+            y[t][m & 1] += MT == 1 || lane >> 4 == m >> 1 ? v : 0.f;
+        }
+}
+
 template <int MT>
 __device__ __forceinline__ void q4_put(float (*red)[16], int lane, const float *y)
 {
@@ -510,10 +582,29 @@ __device__ __forceinline__ void q4_put(float (*red)[16], int lane, const float *
     }
 }
 
+/* Outputs of the TR tiles from t0 on: the waves' sums, in order, and the epilogue. */
+template <int MT, int KW, int TR>
+__device__ __forceinline__ void q4_outputs(const g2_q4mv_args &a, int t0, int m0, const float (*red)[TR][MT][16])
+{
+    for (int o = threadIdx.x; o < TR * MT * 16; o += KW * 64) {
+        const int r = o & 15, m = o / 16 % MT, i = o / 16 / MT;
+        const long n = (t0 + i) * 16l + r;
+        if (n >= a.N || m0 + m >= a.M) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < KW; ++k) v += red[k][i][m][r];
+        const size_t at = (size_t)(m0 + m) * a.N + n;
+        if (a.bias) v += a.bias[n];
+        if (a.res) v += a.res[at];
+        a.y[at] = a.gelu ? gelu_f(v) : v;
+    }
+}
+
 /* The loop: the waves of a work-group take the chunks of the same TR tiles in
  * turn, each splits its own chunk of the activations; the sums of the waves
  * meet in LDS, in order.  The next chunk's loads go out before a chunk's
- * products. */
+ * products.  Chunks left to fp32 come behind the loop, where their registers
+ * are not beside the loop's. */
 template <int MT, int KW, int TR, int G>
 __device__ void q4_matvec_impl(const g2_q4mv_args &a)
 {
@@ -543,6 +634,7 @@ __device__ void q4_matvec_impl(const g2_q4mv_args &a)
         codes[i] = a.codes + g2l_code_at(a.K, t, 0, 0);
         scales[i] = a.scales + g2l_scale_at(a.K, G, t, 0, 0, 0);
     }
+    bool plain = false;
     if (w < chunks) load(w);
     for (int c = w; c < chunks; c += KW) {
         q4_w<G> wc[TR];
@@ -550,8 +642,13 @@ __device__ void q4_matvec_impl(const g2_q4mv_args &a)
 #pragma unroll
         for (int i = 0; i < TR; ++i) wc[i] = wn[i];
         if (c + KW < chunks) load(c + KW);
+        const q4_seen seen = q4_look<MT>(xc);
+        if (seen.plain) {
+            plain = true;
+            continue;
+        }
         float e[2];
-        q4_split_x<MT>(xc, xs[w], xe[w], lane, e);
+        q4_split_x<MT>(xc, seen.own, xs[w], xe[w], lane, e);
         f16x8 x[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = *(const f16x8 *)(frag + 32 * j);
@@ -562,21 +659,14 @@ __device__ void q4_matvec_impl(const g2_q4mv_args &a)
 #pragma unroll
         for (int i = 0; i < TR; ++i) q4_products<MT, G>(x, wc[i].w, wc[i].s, e, y[i]);
     }
+    if (plain)
+#pragma unroll 1
+        for (int c = w; c < chunks; c += KW)
+            if (q4_look<MT>(q4_load_x<MT>(a, m0, c, lane)).plain) q4_add_plain<MT, TR, G>(a, m0, c, lane, codes, scales, ql, y);
 #pragma unroll
     for (int i = 0; i < TR; ++i) q4_put<MT>(red[w][i], lane, y[i]);
     __syncthreads();
-    for (int o = tid; o < TR * MT * 16; o += KW * 64) {
-        const int r = o & 15, m = o / 16 % MT, i = o / 16 / MT;
-        const long n = (t0 + i) * 16l + r;
-        if (n >= a.N || m0 + m >= a.M) continue;
-        float v = 0.f;
-#pragma unroll
-        for (int k = 0; k < KW; ++k) v += red[k][i][m][r];
-        const size_t at = (size_t)(m0 + m) * a.N + n;
-        if (a.bias) v += a.bias[n];
-        if (a.res) v += a.res[at];
-        a.y[at] = a.gelu ? gelu_f(v) : v;
-    }
+    q4_outputs<MT, KW, TR>(a, t0, m0, red);
 }
 #define Q4_MATVEC(MT, KW, TR)                                                                                          \
     extern "C" __global__ __launch_bounds__(64 * KW) void g2k_q4_mv##MT##_##KW##_##TR##_32(const g2_q4mv_args a)      \
@@ -596,7 +686,8 @@ Q4_MATVEC(8, 8, 4)
  * for all tiles that the work-group takes in turn; a tile's loads (its bias and
  * residual with them, since loads return in order) go out a tile ahead; more
  * tiles ahead are no faster (50257 x 1600 on 512 work-groups 12.4 us with two
- * and 14.3 with four, 11.9 with one). */
+ * and 14.3 with four, 11.9 with one).  A work-group with a chunk that is left to
+ * fp32 takes all of its tiles' products there. */
 template <int NC, int G> struct q4_stage {
     q4_w<G> w[NC];
     float bias, res;
@@ -609,6 +700,7 @@ __device__ void q4_held_impl(const g2_q4mv_args &a)
     __shared__ __align__(16) _Float16 xs[KW][ROWS * Q4_XROW];
     __shared__ float xe[KW][8];
     __shared__ float red[2][KW][MT][16];
+    __shared__ int left[KW]; /* the wave has a chunk that is left to fp32 */
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int tiles = (int)g2l_tiles(a.N), m0 = blockIdx.y * 8, chunks = (int)g2l_chunks(a.K), step = gridDim.x;
     const q4_lane ql = q4_lane_of(a, lane);
@@ -637,11 +729,20 @@ __device__ void q4_held_impl(const g2_q4mv_args &a)
         return s;
     };
     q4_stage<NC, G> st = load(blockIdx.x);
+    q4_power own[NC];
+    bool plain = false;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const q4_seen seen = q4_look<MT>(xr[i]);
+        own[i] = seen.own;
+        plain |= seen.plain;
+    }
+    if (lane == 0) left[w] = plain;
     f16x8 x[NC][4];
     float e[NC][2];
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-        q4_split_x<MT>(xr[i], xs[w], xe[w], lane, e[i]);
+        q4_split_x<MT>(xr[i], own[i], xs[w], xe[w], lane, e[i]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[i][j] = *(const f16x8 *)(xs[w] + (lane & (ROWS - 1)) * Q4_XROW + 8 * (lane >> 4) + 32 * j);
         __builtin_amdgcn_wave_barrier();
@@ -661,6 +762,23 @@ __device__ void q4_held_impl(const g2_q4mv_args &a)
         st = load(t + step);
         q4_put<MT>(red[b][w], lane, y);
         __syncthreads();
+        if (t == (int)blockIdx.x) /* (before the first output) */
+            if (__builtin_expect(__builtin_amdgcn_readfirstlane(wave_any(left[lane % KW])), 0)) {
+                float(*one)[1][MT][16] = (float(*)[1][MT][16])red[0];
+#pragma unroll 1
+                for (; t < tiles; t += step) {
+                    const uint8_t *codes = a.codes + t * tile_codes;
+                    const uint16_t *scales = a.scales + t * tile_scales;
+                    float y[1][2] = {};
+#pragma unroll 1
+                    for (int c = w; c < chunks; c += KW) q4_add_plain<MT, 1, G>(a, m0, c, lane, &codes, &scales, ql, y);
+                    q4_put<MT>(one[w][0], lane, y[0]);
+                    __syncthreads();
+                    q4_outputs<MT, KW, 1>(a, t, m0, one);
+                    __syncthreads();
+                }
+                return;
+            }
         if (m < MT && 16l * t + r < a.N && m0 + m < a.M) {
             float v = 0.f;
 #pragma unroll
@@ -670,18 +788,17 @@ __device__ void q4_held_impl(const g2_q4mv_args &a)
         }
     }
 }
-#define Q4_HELD(MT, KW, NC)                                                                                            \
-    extern "C" __global__ __launch_bounds__(64 * KW) void g2k_q4_mvh##MT##_##KW##_##NC##_32(const g2_q4mv_args a)     \
-    { q4_held_impl<MT, KW, NC, 32>(a); }                                                                               \
-    extern "C" __global__ __launch_bounds__(64 * KW) void g2k_q4_mvh##MT##_##KW##_##NC##_64(const g2_q4mv_args a)     \
-    { q4_held_impl<MT, KW, NC, 64>(a); }                                                                               \
-    extern "C" __global__ __launch_bounds__(64 * KW) void g2k_q4_mvh##MT##_##KW##_##NC##_128(const g2_q4mv_args a)    \
-    { q4_held_impl<MT, KW, NC, 128>(a); }
-Q4_HELD(1, 8, 1)
-Q4_HELD(1, 8, 2)
-Q4_HELD(8, 8, 1)
-Q4_HELD(8, 8, 2)
-Q4_HELD(8, 16, 2)
+/* (WAVES: of a SIMD, which the registers leave resident: see g2i_q4_form) */
+#define Q4_HELD_G(MT, KW, NC, WAVES, G)                                                                                \
+    extern "C" __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(WAVES)))                       \
+    void g2k_q4_mvh##MT##_##KW##_##NC##_##G(const g2_q4mv_args a) { q4_held_impl<MT, KW, NC, G>(a); }
+#define Q4_HELD(MT, KW, NC, WAVES)                                                                                     \
+    Q4_HELD_G(MT, KW, NC, WAVES, 32) Q4_HELD_G(MT, KW, NC, WAVES, 64) Q4_HELD_G(MT, KW, NC, WAVES, 128)
+Q4_HELD(1, 8, 1, 6)
+Q4_HELD(1, 8, 2, 6)
+Q4_HELD(8, 8, 1, 6)
+Q4_HELD(8, 8, 2, 4)
+Q4_HELD(8, 16, 2, 4)
 
 /* ======================================================================
  * 8-bit K/V cache: a block of 16 positions of one head holds the codes

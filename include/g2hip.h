@@ -204,9 +204,10 @@ int g2_quantize_q4(const void *W, int w_dtype, int in_out, uint8_t *codes,
 int g2_dequantize_q4(const uint8_t *codes, const uint16_t *scales, float *W,
                      int in_out, int N, int K, int group);
 /* y[M,N] = act(x[M,K] W^T + bias[n] + residual[m,n]) for M activation rows
- * (one token of M sequences, or M tokens), fp32 accuracy in x and in the sums;
- * bias and residual may be NULL, residual == y is legal; 8 rows share one
- * reading of the weights. */
+ * (one token of M sequences, or M tokens).  Each activation enters within 2^-22
+ * of its own value, whatever the others' sizes; sums are fp32.  bias and
+ * residual may be NULL, residual == y is legal; 8 rows share one reading of the
+ * weights. */
 int g2_matvec_q4(const float *x, const uint8_t *codes, const uint16_t *scales,
                  const float *bias, const float *residual, float *y,
                  int M, int N, int K, int group, int apply_gelu);

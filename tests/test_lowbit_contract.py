@@ -1,10 +1,14 @@
-"""The decode operators in fewer bits, what can be told without a GPU: what the binding keeps alive."""
+"""The decode operators in fewer bits, what can be told without a GPU: what the binding keeps alive, which
+forms the GPU tests reach."""
 import gc
 import weakref
 
 import pytest
 
 import g2hip
+import test_lowbit_addresses as addresses
+import test_lowbit_contract_gpu as gpu
+import test_lowbit_gpu as base
 
 
 class Buf(g2hip.DevBuf):
@@ -29,3 +33,9 @@ def test_rules_keep_their_buffers(name):
     del rules
     gc.collect()
     assert alive() is None
+
+
+def test_every_form_of_a_product_meets_outliers():
+    forms = addresses.q4_form
+    assert {forms(M, N, K)[0] for M, N, K, _ in gpu.OUTLIERS} == {forms(M, N, K)[0] for M, N, K, _ in base.product_cases()}
+    assert len({(forms(M, N, K)[0], G) for M, N, K, G in gpu.OUTLIERS}) == 33

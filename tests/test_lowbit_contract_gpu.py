@@ -1,10 +1,11 @@
 """What the header allows of the decode operators in fewer bits beyond test_lowbit_gpu.py's calls: cutting a sequence
-back from a block that is full."""
+back from a block that is full; activations beside far larger ones."""
 import numpy as np
 import pytest
 
 import test_lowbit_gpu as base
 from oracle import lowbit
+from parity import EPS32
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +87,51 @@ def test_kv8_cut_back_from_an_end_inside_a_block(g2):
         m.raw = m.raw[:, :cut]
         base.check_cache(g2, cache, [m], NH, max_seq)
     assert (cache.download(np.uint8)[n:] == 0xFF).all()
+
+
+# ------------------------------------------------------------------ 4-bit weights: activations of unlike sizes
+
+# every form of a product, each with groups of 32, 64 and 128
+OUTLIERS = [(M, N, K, (32, 64, 128)[(i + j) % 3]) for i in range(3)
+            for j, (M, N, K) in enumerate([(1, 100, 768), (1, 48, 2200), (1, 32780, 130), (1, 32770, 1060), (3, 100, 768), (9, 24, 1400),
+                                           (8, 4100, 160), (2, 8200, 200), (9, 32780, 130), (3, 32770, 1060), (9, 8195, 2100)])]
+
+
+def strict_bound(x, v, K):
+    """|error| of a computed product: each activation enters within 2^-22 of its own value, whatever stands beside it;
+    a sum of K terms goes through at most 160 roundings (128 columns, their groups, the parts of an operand), 4 more
+    and one for each 128 columns; a product below fp32's normal range is off by half its last place."""
+    return ((164 + K / 128) * EPS32 + 2.0 ** -22) * (np.abs(x) @ np.abs(v).T) + (K + 64) * 2.0 ** -149
+
+
+@pytest.mark.parametrize("M,N,K,group", OUTLIERS)
+def test_matvec_q4_activations_beside_larger_ones(g2, M, N, K, group):
+    """Large activations whose weights are 0 (a quarter of the columns) leave the others their own accuracy."""
+    r = base.rng(55, M, N, K)
+    W = (0.02 * r.standard_normal((N, K))).astype(np.float32)
+    zero = r.random(K) < 0.25
+    zero[::128] = True
+    W[:, zero] = 0
+    W[::2] *= r.random((len(W[::2]), K)) < 0.2  # (rows with few weights, so that no large term hides the others)
+    codes, scales = base.packed(g2, W, group)
+    out = g2.DevBuf(4 * N * K)
+    g2.dequantize_q4(codes, scales, out, False, N, K, group)
+    v = out.download(np.float32).reshape(N, K)  # (bit for bit the oracle's: test_q4_layout_and_values)
+    assert (v[:, zero] == 0).all()
+    pick = slice(None) if N < 9000 else r.choice(N, 4000, False)  # rows of the result that are compared
+    v = v[pick].astype(np.float64)
+    for size in (2.0 ** 17, 2.0 ** 20, 1e7, 2.0 ** 30, 2.0 ** 40, 2.0 ** 100, "mixed", "spread"):
+        x = r.standard_normal((M, K))
+        big = r.standard_normal((M, K))
+        if size == "mixed":  # every row and column its own
+            big *= 2.0 ** r.uniform(-10, 100, (M, K))
+        elif size == "spread":  # all columns, down to the smallest numbers
+            big *= 2.0 ** r.uniform(-140, 120, (M, K))
+            x *= 2.0 ** r.uniform(-140, -40, (M, K))
+        else:
+            big *= size * (r.random((M, K)) < 0.1)
+            big[:, ::128] = size
+        x = np.where(zero, big, x).astype(np.float32)
+        got = base.run_matvec(g2, x, codes, scales, N, K, group)[:, pick]
+        x = x.astype(np.float64)
+        base.within(got, x @ v.T, strict_bound(x, v, K), f"beside {size}")
