@@ -273,9 +273,12 @@ typedef struct {
 size_t g2_logits_work_bytes(int rows);
 /* out[rows,V] = logits under the rules (NULL: not wanted; out == logits is
  * legal) and pick[r] = the id of the greatest (NULL: not wanted): the lowest
- * of equal ones, NaN never, -1 where nothing is above -infinity.  The device
- * form of g2_sample_greedy.  V up to 262144, max_ctx and n_bias up to 65535,
- * rows up to 65536. */
+ * of equal ones, NaN never, -1 where nothing is above -infinity.  Where all
+ * logits are finite and above -1e30, a repetition penalty above 1 (or none) and
+ * the end of text as the forbidden id (or none) give the id of
+ * g2_sample_greedy; that call takes a penalty of 1 or less as none, and returns
+ * 0 for a row without a finite logit or with a NaN at id 0.  V up to 262144,
+ * max_ctx and n_bias up to 65535, rows up to 65536. */
 int g2_apply_logit_rules(const float *logits, float *out, int *pick, int rows,
                          int V, const g2_logit_rules *rules, void *work);
 

@@ -135,3 +135,27 @@ def test_matvec_q4_activations_beside_larger_ones(g2, M, N, K, group):
         got = base.run_matvec(g2, x, codes, scales, N, K, group)[:, pick]
         x = x.astype(np.float64)
         base.within(got, x @ v.T, strict_bound(x, v, K), f"beside {size}")
+
+
+# ------------------------------------------------------------------ rules on logits
+
+@pytest.mark.parametrize("penalty", [1.0, 1.3, 3.0])
+def test_rules_pick_as_the_host_sampler(g2, penalty):
+    """The device's choice is g2_sample_greedy's on a model's logits: with and without a penalty, the end of text
+    forbidden or not, ids twice in the context and outside the vocabulary."""
+    cfg = g2.make_config(1, 128, 2)
+    w = g2.synth_weights(cfg, 5)
+    w["wte"] = w["wte"].copy()
+    w["wte"][g2.EOS] *= 40  # (often the greatest logit, so that forbidding it matters)
+    m = g2.Model.from_host(cfg, w, g2.F32, g2.PATH_FUSED)
+    V = cfg.vocab_size
+    r = base.rng(60)
+    for turn in range(4):
+        prompt = r.integers(0, V, 20 + turn).astype(np.int32)
+        m.prefill(prompt)
+        logits = m.logits()
+        top = np.argsort(logits)[::-1][:4 * turn]  # so that the penalty changes the choice
+        ctx = np.concatenate([prompt, prompt[:3], top, [-1, V]]).astype(np.int32)
+        for forbid in (False, True):
+            _, ids = base.run_rules(g2, logits[None], ctx=ctx, max_ctx=len(ctx), repetition=penalty, forbid=g2.EOS if forbid else -1)
+            assert ids[0] == m.sample_greedy(ctx, forbid, penalty)
