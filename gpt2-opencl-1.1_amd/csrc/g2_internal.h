@@ -203,6 +203,9 @@ int g2i_q4_form(int M, int N, int K, int *waves, unsigned *wgs);
 /* g2_attn_kv8's parts of a head, blocks to a part and waves to a work-group. */
 int g2i_kv8_form(long heads, int T_kv, int *span, int *waves);
 
+/* Whether g2_apply_logit_rules takes its wide form, and the slices of a row. */
+int g2i_logits_form(int rows, int V, int *parts);
+
 /* Whether np bytes at p and nq bytes at q share any. */
 static inline int g2i_overlap(const void *p, size_t np, const void *q, size_t nq)
 {

@@ -292,6 +292,16 @@ static int logits_rows(int rows) { return rows >= 1 && rows <= 1 << 16; }
 
 size_t g2_logits_work_bytes(int rows) { return logits_rows(rows) ? (size_t)rows * G2L_CELL * sizeof(uint64_t) : 0; }
 
+/* Whether the rules take the wide slices, and the slices of a row: 1024 ids each,
+ * 8192 where that makes more than 1024 work-groups (us: 16 rows of 50257 7.2,
+ * wide 7.4; 32 rows 8.7, 7.9; 64 rows 14.0, 12.1). */
+int g2i_logits_form(int rows, int V, int *parts)
+{
+    const int wide = (long)rows * cdiv(V, G2L_SLICE) > 1024;
+    *parts = (int)cdiv(V, wide ? G2L_SLICE_WIDE : G2L_SLICE);
+    return wide;
+}
+
 int g2_apply_logit_rules(const float *logits, float *out, int *pick, int rows, int V, const g2_logit_rules *rules,
                          void *work)
 {
@@ -332,9 +342,6 @@ int g2_apply_logit_rules(const float *logits, float *out, int *pick, int rows, i
     a.mask = r->mask; a.mask_stride = r->mask_stride; a.forbid = r->forbid;
     a.rows = rows; a.V = V;
     a.repetition = r->repetition > 0.f ? r->repetition : 1.f; a.frequency = r->frequency; a.presence = r->presence;
-    /* slices of 1024 ids, of 8192 where that makes more than 1024 work-groups (us: 16 rows of 50257 7.2, wide 7.4;
-     * 32 rows 8.7, 7.9; 64 rows 14.0, 12.1) */
-    const int wide = (long)rows * cdiv(V, G2L_SLICE) > 1024;
-    a.parts = (int)cdiv(V, wide ? G2L_SLICE_WIDE : G2L_SLICE);
+    const int wide = g2i_logits_form(rows, V, &a.parts);
     return g2i_launch(wide ? G2F_LOGITS_WIDE : G2F_LOGITS, (unsigned)(rows * a.parts), 1, wide ? 1024 : 256, &a);
 }

@@ -159,3 +159,29 @@ def test_rules_pick_as_the_host_sampler(g2, penalty):
         for forbid in (False, True):
             _, ids = base.run_rules(g2, logits[None], ctx=ctx, max_ctx=len(ctx), repetition=penalty, forbid=g2.EOS if forbid else -1)
             assert ids[0] == m.sample_greedy(ctx, forbid, penalty)
+
+
+# the wide form (more than 1024 narrow slices in all): several slices to a row and one, the last of one id and of nearly all
+WIDE = [(21, 50257), (5, 262144), (130, 8193), (1030, 37), (520, 1025), (200, 8191)]
+
+
+@pytest.mark.parametrize("R,V", WIDE)
+def test_rules_wide(g2, R, V):
+    """test_rules' cases on more rows: all rules at once against the oracle, in place, the choice and the logits alone."""
+    base.test_rules(g2, R, V)
+
+
+@pytest.mark.parametrize("R,V", [(2, 50257), (30, 50257), (130, 8193)])
+def test_rules_ties_across_slices(g2, R, V):
+    """Equal logits on both sides of the slices' borders: the lowest id that is allowed, of 0 and -0 too."""
+    edges = sorted({i for i in (1023, 1024, 8191, 8192, 16384, V - 1) if i < V})
+    for value in (7.0, 0.0):
+        l = -np.abs(base.rng(61, R).standard_normal((R, V))).astype(np.float32) - 1
+        l[:, edges] = value
+        l[:, edges[::2]] = -value if value == 0 else value
+        for n in range(len(edges)):  # the first n of them not allowed
+            allowed = np.ones((1, V), bool)
+            allowed[0, edges[:n]] = False
+            mask = base.bits(allowed, (V + 31) // 32)
+            assert (base.run_rules(g2, l, mask=mask)[1] == edges[n]).all()
+        assert (base.run_rules(g2, l, forbid=edges[0], out=False)[1] == edges[1]).all()
