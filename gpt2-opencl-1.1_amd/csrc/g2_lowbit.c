@@ -95,16 +95,17 @@ int g2_dequantize_q4(const uint8_t *codes, const uint16_t *scales, float *W, int
  * and take tiles in turn).  us in a replayed graph, matrices that no cache
  * holds, groups of 32 (of 128 where two figures stand):
  *  - one row: the loop over single tiles; 16 waves for the few tiles of long
- *    columns (1600 x 6400 5.1, with 8 waves 5.5; 1600 x 1600 3.4 both); the
+ *    columns (1600 x 6400 4.8, with 8 waves 5.1; 1600 x 1600 3.1 both); the
  *    held form from 2048 tiles on, where splitting the activations anew for
- *    each tile costs most (50257 x 1600 11.0 and 9.9, loop 13.9 and 13.0, of 2
- *    tiles 13.5 and 11.2; 50257 x 768 7.4, 8.3; but 16000 x 1600 6.1, 5.5);
+ *    each tile costs most (50257 x 1600 11.4 and 9.7, loop 14.1 and 12.7; 50257
+ *    x 768 7.2, 8.4; but 16000 x 1600 5.9, 5.1);
  *  - up to 8 rows, whose activations take longer to split: 16 waves up to 128
- *    tiles (1600 x 1600 4.4, 4.7; 1600 x 6400 8.2, 9.4); 2 tiles from 256, 4
- *    from 512 on (6400 x 1600 6.2, 5.7, 6.6 for 1, 2, 4; 10000 x 6400 22, 18,
- *    15); held from 2048 tiles (50257 x 1600 14.9, loop 18.8), with 16 waves
- *    and K to 4096 from 512 (12000 x 4000 10.0, loop 11.5).
- * Work-groups of the held form: as many as the registers leave resident. */
+ *    tiles (1600 x 1600 4.1, 4.4; 1600 x 6400 8.1, 9.1); 2 tiles from 256, 4
+ *    from 512 on (6400 x 1600 5.8, 5.7, 6.7 for 1, 2, 4; 10000 x 6400 21, 18,
+ *    16); held from 2048 tiles (50257 x 1600 15.0, loop 24), with 16 waves and K
+ *    to 4096 from 512 (12000 x 4000 9.9, loop 12.0).
+ * Work-groups of the held form: as many as the registers leave resident (80 of
+ * them a lane for 768). */
 int g2i_q4_form(int M, int N, int K, int *waves, unsigned *wgs)
 {
     const long tiles = g2l_tiles(N), chunks = g2l_chunks(K);
@@ -228,7 +229,8 @@ int g2_kv8_read(const void *cache, float *k, float *v, const int *len, int T_kv,
  *  - one launch up to 1024 positions, and for 256 heads and more of any length;
  *    beyond, parts of 256 positions and more, as many as 512 work-groups (16
  *    heads x 2000 9.0 whole, 7.4 in parts; 16 x 4000 10.4 in 3 parts, 7.9 in
- *    15; 25 x 1024 6.4 and 7.1; 256 x 4000 27.0 and 28.3);
+ *    15; 25 x 1024 6.4 and 7.1; 256 x 4000 27.0 and 28.3; numbers of heads that
+ *    do not fill the 256 CUs evenly, 257 to 511, were not measured in parts);
  *  - a wave takes 64 positions at a time: one wave up to 64 (12 heads 3.3, four
  *    waves 3.7), for many heads up to 128 (1600 heads 8.7, 9.9), four up to 512
  *    (200 heads x 512 5.7, eight 6.0), eight beyond (25 x 1024 6.4, four 6.7,

@@ -288,9 +288,9 @@ extern "C" __global__ __launch_bounds__(512) void g2k_q4_read_t(const g2_q4_args
  * chunk's; all sums are fp32.
  *
  * Bounded by HBM for large matrices and by the launch and two load latencies
- * for small ones: 50257 x 1600, groups of 128, 9.9 us in a replayed graph with
- * matrices that no cache holds, 4.2 TB/s, 8.3 from the cache behind it; 768 x
- * 768 2.8 us.  Which form a product takes: g2i_q4_form. */
+ * for small ones: 50257 x 1600, groups of 128, 9.7 us in a replayed graph with
+ * matrices that no cache holds, 4.3 TB/s, 8.5 from the cache behind it; 768 x
+ * 768 2.5 us.  Which form a product takes: g2i_q4_form. */
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 template <int I> __device__ __forceinline__ void q4_half(f16x8 &r, unsigned w)
@@ -815,11 +815,11 @@ Q4_HELD(8, 16, 2, 4)
  * of each of four rows, and neighbouring waves have neighbouring heads.  The
  * first block's wave reads the positions that came before from `last` and then
  * writes there what the call has of its last block, full or not: in one wave,
- * since both may be the same rows.  Four prompts of 1001 rows x 25 heads: 12.8 us, 5.0
+ * since both may be the same rows.  Four prompts of 1001 rows x 25 heads: 13.0 us, 5.0
  * TB/s of the keys and values read and the codes written (17.3 when a reading
  * back just before had left its values in the L2, and 19.0 then with the blocks
  * of one head side by side, whose loads are 16 rows 19 KB apart); one token:
- * 3.1, the latency of a load, the maximum over the wave and a store. */
+ * 3.3, the latency of a load, the maximum over the wave and a store. */
 G2K void g2k_kv8_append(const g2_kv8_append_args a)
 {
     const int lane = threadIdx.x & 63, t0 = lane >> 4, d0 = 4 * (lane & 15);

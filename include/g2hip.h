@@ -253,7 +253,8 @@ int g2_attn_kv8(const float *q, int q_stride, const void *cache, float *out,
                 int max_seq, float scale, float *work);
 
 /* What may become of a row of logits before its token is chosen (pointers are
- * device arrays; NULL or 0 where a rule is not wanted). */
+ * device arrays; NULL or 0 where a rule is not wanted, but -1 for forbid: a
+ * structure of zeros forbids id 0). */
 typedef struct {
     const int *ctx;         /* [rows][max_ctx] ids so far (outside 0..V-1: ignored)      */
     const int *ctx_len;     /* [rows] how many of them count; NULL: max_ctx              */
@@ -269,7 +270,8 @@ typedef struct {
     int forbid;             /* an id that is never allowed, -1: none                     */
 } g2_logit_rules;
 /* Bytes of g2_apply_logit_rules' workspace (needed where pick is wanted): zero
- * before its first call, left zero by every call, 8-byte aligned. */
+ * before its first call, left zero by every call, 8-byte aligned, for one call
+ * alone while it runs. */
 size_t g2_logits_work_bytes(int rows);
 /* out[rows,V] = logits under the rules (NULL: not wanted; out == logits is
  * legal) and pick[r] = the id of the greatest (NULL: not wanted): the lowest
