@@ -256,7 +256,7 @@ def _run_own(s):
         return s["out"]
     if k == "append":
         S, KV, n = c["seqs"], c["kv"], c["high"]
-        g2.kv4_append(p["k_in"], p["v_in"], 2 * KV * DH, g2.F16 if c["f16"] else g2.F32, p["cache"], p["row_start"], p["pos"], 0, S, n,
+        g2.kv4_append(p["k_in"], p["v_in"], 2 * KV * DH, g2.F16 if c["f16"] else g2.F32, p["cache"], p["row_start"], p["pos"], 0, S,
                       s["kv"].shape[0], KV, c["max_seq"])
         g2.kv4_read(p["cache"], p["k"], p["v"], None, p["len"], c["start"] + n, c["start"], n, S, KV, c["max_seq"])
         return s["k"], s["v"]
