@@ -1,0 +1,276 @@
+/*
+ * g2_batch.c -- entry points for several texts at once: packed prompt
+ * attention, the 4-bit K/V cache, beam search (kernels: g2_batch.hip,
+ * layouts: g2_batch_plan.h).
+ *
+ * Every call checks its arguments before it asks for the runtime, so a wrong
+ * call is G2_E_ARG or G2_E_LIMIT without a device too.
+ */
+#include <math.h>
+#include <string.h>
+
+#include "g2_internal.h"
+#include "g2_batch_plan.h"
+
+#define MAX_ROWS (1 << 24)   /* rows of a packed buffer, positions of a cache */
+#define MAX_STRIDE (1 << 24) /* elements from row to row: 31 rows apart is below 2^32 bytes */
+#define MAX_HEADS 1024
+#define MAX_SEQS (1 << 20)
+#define MAX_VOCAB (1 << 18)
+
+static int aligned(const void *p, size_t a) { return (uintptr_t)p % a == 0; }
+static unsigned cdiv(long a, long b) { return (unsigned)((a + b - 1) / b); }
+static int fits(long groups) { return groups <= (long)UINT32_MAX / 256; }
+static int ready(void) { return g2i_ready() ? G2_OK : g2i_err(G2_E_STATE, "g2_init has not been called"); }
+static size_t dsize(int dtype) { return dtype == G2_F16 ? 2 : 4; }
+
+/* bytes from the first element to the last of `rows` rows of n elements */
+static size_t span_of(long rows, long stride, long n, size_t size)
+{
+    return rows < 1 ? 0 : ((size_t)(rows - 1) * (size_t)stride + (size_t)n) * size;
+}
+
+static int heads_check(const char *fn, int n_head, int n_kv)
+{
+    if (n_head < 1 || n_kv < 1 || n_head % n_kv) return g2i_err(G2_E_ARG, "%s: %d heads on %d key heads", fn, n_head, n_kv);
+    if (n_head > MAX_HEADS) return g2i_err(G2_E_LIMIT, "%s: %d heads above %d", fn, n_head, MAX_HEADS);
+    return G2_OK;
+}
+
+/* ---------------------------------------------------------- packed prompts */
+
+int g2_attn_prompt(const void *q, int q_stride, const void *k, const void *v, int kv_stride, void *out, int out_stride,
+                   int dtype, const int *q_start, const int *k_start, int n_seq, int q_rows, int k_rows, int n_head,
+                   int n_kv, float scale)
+{
+    static const char fn[] = "g2_attn_prompt";
+    if (!q || !k || !v || !out) return g2i_err(G2_E_ARG, "%s: NULL buffer", fn);
+    if (dtype != G2_F32 && dtype != G2_F16) return g2i_err(G2_E_ARG, "%s: bad dtype %d", fn, dtype);
+    int rc = heads_check(fn, n_head, n_kv);
+    if (rc) return rc;
+    if (n_seq < 1 || q_rows < 1 || k_rows < 0) return g2i_err(G2_E_ARG, "%s: %d sequences, %d rows, %d keys", fn, n_seq, q_rows, k_rows);
+    if (n_seq > 1 && (!q_start || !k_start)) return g2i_err(G2_E_ARG, "%s: %d sequences need their starts", fn, n_seq);
+    const int nq = n_head * G2B_DH, nk = n_kv * G2B_DH;
+    if ((q_rows > 1 && (q_stride < nq || out_stride < nq)) || (k_rows > 1 && kv_stride < nk))
+        return g2i_err(G2_E_ARG, "%s: strides %d, %d and %d of rows of %d and %d", fn, q_stride, out_stride, kv_stride, nq, nk);
+    if (q_rows > MAX_ROWS || k_rows > MAX_ROWS || n_seq > MAX_SEQS ||
+        (q_rows > 1 && (q_stride > MAX_STRIDE || out_stride > MAX_STRIDE)) || (k_rows > 1 && kv_stride > MAX_STRIDE))
+        return g2i_err(G2_E_LIMIT, "%s: at most %d rows, %d elements apart, and %d sequences", fn, MAX_ROWS, MAX_STRIDE, MAX_SEQS);
+    if (!isfinite(scale)) return g2i_err(G2_E_ARG, "%s: the scale is not finite", fn);
+    const size_t size = dsize(dtype), no = span_of(q_rows, out_stride, nq, size), ns = ((size_t)n_seq + 1) * sizeof(int);
+    if (!aligned(q, size) || !aligned(k, size) || !aligned(v, size) || !aligned(out, size))
+        return g2i_err(G2_E_ARG, "%s: a buffer is not at an element's address", fn);
+    const size_t nkv = span_of(k_rows, kv_stride, nk, size);
+    if (g2i_overlap(out, no, q, span_of(q_rows, q_stride, nq, size)) || g2i_overlap(out, no, k, nkv) || g2i_overlap(out, no, v, nkv) ||
+        (q_start && g2i_overlap(out, no, q_start, ns)) || (k_start && g2i_overlap(out, no, k_start, ns)))
+        return g2i_err(G2_E_ARG, "%s: the output overlaps an input", fn);
+    const long tiles = g2b_row_tiles(q_rows);
+    if (!fits(tiles * n_head)) return g2i_err(G2_E_LIMIT, "%s: too many rows and heads for one call", fn);
+    if ((rc = ready())) return rc;
+    g2_attn_prompt_args a = { q, k, v, out, q_start, k_start, q_rows > 1 ? q_stride : nq, k_rows > 1 ? kv_stride : nk,
+                              q_rows > 1 ? out_stride : nq, n_seq, q_rows, k_rows, n_head, n_kv, (int)tiles, scale };
+    return g2i_launch(dtype == G2_F16 ? G2F_PROMPT_F16 : G2F_PROMPT_F32, (unsigned)(tiles * n_head), 1, 256, &a);
+}
+
+/* -------------------------------------------------------------- 4-bit cache */
+
+static int kv4_sizes(int n_seq, int n_kv, int max_seq)
+{
+    return n_seq >= 1 && n_kv >= 1 && n_kv <= MAX_HEADS && max_seq >= 1 && max_seq <= MAX_ROWS && n_seq <= (1 << 22) / n_kv;
+}
+
+size_t g2_kv4_bytes(int n_seq, int n_kv, int max_seq)
+{
+    return kv4_sizes(n_seq, n_kv, max_seq) ? g2b_bytes(n_seq, n_kv, g2b_tiles(max_seq)) : 0;
+}
+
+size_t g2_kv4_work_bytes(int n_seq, int n_head)
+{
+    return kv4_sizes(n_seq, n_head, 1) ? (size_t)n_seq * n_head * G2B_SPLITS * G2B_PART_FLOATS * sizeof(float) : 0;
+}
+
+static int kv4_check(const char *fn, const void *cache, int n_seq, int n_kv, int max_seq)
+{
+    if (!cache) return g2i_err(G2_E_ARG, "%s: NULL buffer", fn);
+    if (n_seq < 1 || n_kv < 1 || max_seq < 1) return g2i_err(G2_E_ARG, "%s: sizes must be positive", fn);
+    if (!kv4_sizes(n_seq, n_kv, max_seq))
+        return g2i_err(G2_E_LIMIT, "%s: %d sequences x %d heads x %d positions: at most %d heads, %d positions, 4M sequences x heads",
+                       fn, n_seq, n_kv, max_seq, MAX_HEADS, MAX_ROWS);
+    if (!aligned(cache, 16)) return g2i_err(G2_E_ARG, "%s: the cache must be 16-byte aligned", fn);
+    return G2_OK;
+}
+
+int g2_kv4_append(const void *k, const void *v, int stride, int dtype, void *cache, const int *row_start, const int *pos,
+                  int start, int n_seq, int rows, int n_kv, int max_seq)
+{
+    static const char fn[] = "g2_kv4_append";
+    int rc = kv4_check(fn, cache, n_seq, n_kv, max_seq);
+    if (rc) return rc;
+    if (!k || !v) return g2i_err(G2_E_ARG, "%s: NULL buffer", fn);
+    if (dtype != G2_F32 && dtype != G2_F16) return g2i_err(G2_E_ARG, "%s: bad dtype %d", fn, dtype);
+    if (rows < 1 || (rows > 1 && stride < n_kv * G2B_DH))
+        return g2i_err(G2_E_ARG, "%s: %d rows of %d, %d apart", fn, rows, n_kv * G2B_DH, stride);
+    if (rows > MAX_ROWS || (rows > 1 && stride > MAX_STRIDE))
+        return g2i_err(G2_E_LIMIT, "%s: at most %d rows, %d elements apart", fn, MAX_ROWS, MAX_STRIDE);
+    if (!row_start && rows % n_seq) return g2i_err(G2_E_ARG, "%s: %d rows of %d sequences need their starts", fn, rows, n_seq);
+    if (!pos && (start < 0 || start >= max_seq)) return g2i_err(G2_E_ARG, "%s: position %d outside the cache of %d", fn, start, max_seq);
+    const size_t size = dsize(dtype), n = span_of(rows, stride, n_kv * G2B_DH, size), nc = g2_kv4_bytes(n_seq, n_kv, max_seq);
+    if (!aligned(k, size) || !aligned(v, size)) return g2i_err(G2_E_ARG, "%s: a buffer is not at an element's address", fn);
+    if (g2i_overlap(cache, nc, k, n) || g2i_overlap(cache, nc, v, n) || (row_start && g2i_overlap(cache, nc, row_start, ((size_t)n_seq + 1) * 4)) ||
+        (pos && g2i_overlap(cache, nc, pos, (size_t)n_seq * 4)))
+        return g2i_err(G2_E_ARG, "%s: overlapping buffers", fn);
+    const long waves = ((long)rows + 7) / 8 * 2 * n_kv;
+    if (!fits((waves + 3) / 4)) return g2i_err(G2_E_LIMIT, "%s: too many rows for one call", fn);
+    if ((rc = ready())) return rc;
+    g2_kv4_append_args a = { k, v, cache, row_start, pos, rows > 1 ? stride : 0, start, n_seq, rows, row_start ? 0 : rows / n_seq,
+                             n_kv, max_seq, (int)g2b_tiles(max_seq) };
+    return g2i_launch(dtype == G2_F16 ? G2F_KV4_APPEND_F16 : G2F_KV4_APPEND_F32, cdiv(waves, 4), 1, 256, &a);
+}
+
+int g2_kv4_read(const void *cache, float *k, float *v, const int *origin, const int *len, int T_kv, int start, int T,
+                int n_seq, int n_kv, int max_seq)
+{
+    static const char fn[] = "g2_kv4_read";
+    int rc = kv4_check(fn, cache, n_seq, n_kv, max_seq);
+    if (rc) return rc;
+    if (!k || !v) return g2i_err(G2_E_ARG, "%s: NULL buffer", fn);
+    if (T_kv < 0 || T_kv > max_seq || start < 0 || T < 1 || start > max_seq - T)
+        return g2i_err(G2_E_ARG, "%s: positions %d..%ld, length %d, cache of %d", fn, start, (long)start + T - 1, T_kv, max_seq);
+    const size_t n = (size_t)n_seq * T * n_kv * 256, nc = g2_kv4_bytes(n_seq, n_kv, max_seq), nl = (size_t)n_seq * 4;
+    const size_t nt = (size_t)n_seq * max_seq * 4;
+    if (g2i_overlap(k, n, v, n) || g2i_overlap(k, n, cache, nc) || g2i_overlap(v, n, cache, nc) ||
+        (len && (g2i_overlap(k, n, len, nl) || g2i_overlap(v, n, len, nl))) ||
+        (origin && (g2i_overlap(k, n, origin, nt) || g2i_overlap(v, n, origin, nt))))
+        return g2i_err(G2_E_ARG, "%s: overlapping buffers", fn);
+    if ((rc = ready())) return rc;
+    g2_kv4_read_args a = { cache, k, v, origin, len, T_kv, start, T, n_seq, n_kv, max_seq, (int)g2b_tiles(max_seq) };
+    const long threads = (long)(n / 32);
+    return g2i_launch(G2F_KV4_READ, threads > (1l << 20) * 256 ? 1u << 20 : cdiv(threads, 256), 1, 256, &a);
+}
+
+/* Query heads to a pass over their key head's positions, passes to a key head,
+ * parts of the positions and tiles to a part. */
+int g2i_kv4_form(int n_seq, int n_head, int n_kv, int T_kv, int *heads, int *chunks, int *span)
+{
+    const int group = n_head / n_kv;
+    *chunks = (group + 3) / 4;
+    *heads = (group + *chunks - 1) / *chunks;
+    const long tiles = g2b_tiles(T_kv) > 0 ? g2b_tiles(T_kv) : 1, wgs = (long)n_seq * n_kv * *chunks;
+    long splits = 1;
+    if (tiles > 8 && wgs < 512) {
+        splits = tiles / 8 < 1024 / wgs ? tiles / 8 : 1024 / wgs;
+        if (splits > G2B_SPLITS) splits = G2B_SPLITS;
+        if (splits < 1) splits = 1;
+    }
+    *span = (int)((tiles + splits - 1) / splits);
+    return (int)((tiles + *span - 1) / *span);
+}
+
+int g2_attn_kv4(const float *q, int q_stride, const void *cache, float *out, int out_stride, const int *origin,
+                const int *len, int T_kv, int n_seq, int n_head, int n_kv, int max_seq, float scale, float *work)
+{
+    static const char fn[] = "g2_attn_kv4";
+    int rc = heads_check(fn, n_head, n_kv);
+    if (!rc) rc = kv4_check(fn, cache, n_seq, n_kv, max_seq);
+    if (rc) return rc;
+    if (!kv4_sizes(n_seq, n_head, 1)) return g2i_err(G2_E_LIMIT, "%s: %d sequences x %d heads above 4M", fn, n_seq, n_head);
+    if (!q || !out || !work) return g2i_err(G2_E_ARG, "%s: NULL buffer", fn);
+    const int D = n_head * G2B_DH;
+    if (T_kv < 0 || T_kv > max_seq || (n_seq > 1 && (q_stride < D || out_stride < D)))
+        return g2i_err(G2_E_ARG, "%s: length %d of %d, strides %d and %d of rows of %d", fn, T_kv, max_seq, q_stride, out_stride, D);
+    if (!isfinite(scale)) return g2i_err(G2_E_ARG, "%s: the scale is not finite", fn);
+    if (!aligned(q, 4) || !aligned(out, 4) || !aligned(work, 4)) return g2i_err(G2_E_ARG, "%s: a buffer is not at an element's address", fn);
+    const size_t nq = span_of(n_seq, q_stride, D, 4), no = span_of(n_seq, out_stride, D, 4), nl = (size_t)n_seq * 4;
+    const size_t nc = g2_kv4_bytes(n_seq, n_kv, max_seq), nw = g2_kv4_work_bytes(n_seq, n_head), nt = nl * max_seq;
+    if (g2i_overlap(out, no, q, nq) || g2i_overlap(out, no, cache, nc) || g2i_overlap(out, no, work, nw) ||
+        g2i_overlap(work, nw, q, nq) || g2i_overlap(work, nw, cache, nc) ||
+        (len && (g2i_overlap(out, no, len, nl) || g2i_overlap(work, nw, len, nl))) ||
+        (origin && (g2i_overlap(out, no, origin, nt) || g2i_overlap(work, nw, origin, nt))))
+        return g2i_err(G2_E_ARG, "%s: overlapping buffers", fn);
+    if ((rc = ready())) return rc;
+    g2_kv4_attn_args a;
+    memset(&a, 0, sizeof a);
+    a.q = q; a.cache = cache; a.out = out; a.part = work; a.origin = origin; a.len = len;
+    a.q_stride = n_seq > 1 ? q_stride : 0; a.out_stride = n_seq > 1 ? out_stride : 0;
+    a.T_kv = T_kv; a.S = n_seq; a.NH = n_head; a.NKV = n_kv; a.max_seq = max_seq; a.tiles = (int)g2b_tiles(max_seq);
+    a.scale = scale;
+    a.splits = g2i_kv4_form(n_seq, n_head, n_kv, T_kv, &a.heads, &a.chunks, &a.span);
+    const int fid = a.heads == 1 ? G2F_KV4_ATTN1 : a.heads == 2 ? G2F_KV4_ATTN2 : G2F_KV4_ATTN4;
+    rc = g2i_launch(fid, (unsigned)((long)n_seq * n_kv * a.chunks * a.splits), 1, 256, &a);
+    if (!rc && a.splits > 1) rc = g2i_launch(G2F_KV4_JOIN, cdiv((long)n_seq * n_head, 4), 1, 256, &a);
+    return rc;
+}
+
+/* -------------------------------------------------------------- beam search */
+
+static int beam_sizes(int groups, int beams, int V, int n_out)
+{
+    return groups >= 1 && beams >= 1 && V >= 1 && n_out >= 1 && beams <= G2B_MAX_BEAMS && n_out <= G2B_MAX_OUT && V <= MAX_VOCAB &&
+           groups <= (1 << 16) / beams;
+}
+
+size_t g2_beam_work_bytes(int groups, int beams, int V, int n_out)
+{
+    return beam_sizes(groups, beams, V, n_out) ? g2b_beam_bytes((long)groups * beams, g2b_slices(V), n_out) : 0;
+}
+
+int g2_beam_select(const float *logits, const float *score, const int *done, int eos, float *out_score, int *out_parent,
+                   int *out_id, int *out_done, int groups, int beams, int V, int n_out, void *work)
+{
+    static const char fn[] = "g2_beam_select";
+    if (!logits || !score || !out_score || !out_parent || !out_id || !work) return g2i_err(G2_E_ARG, "%s: NULL buffer", fn);
+    if (groups < 1 || beams < 1 || V < 1 || n_out < 1) return g2i_err(G2_E_ARG, "%s: sizes must be positive", fn);
+    if (!beam_sizes(groups, beams, V, n_out))
+        return g2i_err(G2_E_LIMIT, "%s: %d groups of %d beams, %d ids, %d continuations: at most %d beams, %d rows, %d ids, %d continuations",
+                       fn, groups, beams, V, n_out, G2B_MAX_BEAMS, 1 << 16, MAX_VOCAB, G2B_MAX_OUT);
+    if (eos < -1 || eos >= V || (done && eos < 0)) return g2i_err(G2_E_ARG, "%s: end id %d of %d", fn, eos, V);
+    if (!aligned(work, 8)) return g2i_err(G2_E_ARG, "%s: the workspace must be 8-byte aligned", fn);
+    const long rows = (long)groups * beams;
+    const size_t n = (size_t)groups * n_out * 4, nr = (size_t)rows * 4, nw = g2_beam_work_bytes(groups, beams, V, n_out);
+    const struct { const void *p; size_t n; } in[] = { { logits, nr * V }, { score, nr }, { done, done ? nr : 0 } };
+    const struct { const void *p; size_t n; } outs[] = { { out_score, n }, { out_parent, n }, { out_id, n }, { out_done, out_done ? n : 0 }, { work, nw } };
+    for (int i = 0; i < 5; ++i) {
+        int bad = 0;
+        for (int j = 0; j < 3; ++j) bad |= outs[i].n && in[j].n && g2i_overlap(outs[i].p, outs[i].n, in[j].p, in[j].n);
+        for (int j = 0; j < i; ++j) bad |= outs[i].n && outs[j].n && g2i_overlap(outs[i].p, outs[i].n, outs[j].p, outs[j].n);
+        if (bad) return g2i_err(G2_E_ARG, "%s: overlapping buffers", fn);
+    }
+    const int rc = ready();
+    if (rc) return rc;
+    const int slices = g2b_slices(V);
+    g2_beam_args a = { logits, score, done, out_score, out_parent, out_id, out_done, work,
+                       (unsigned long long *)((char *)work + g2b_cands_at(rows, slices)), eos, groups, beams, V, n_out, slices };
+    const int first = g2i_launch(G2F_BEAM_SLICE, (unsigned)(rows * slices), 1, 256, &a);
+    return first ? first : g2i_launch(G2F_BEAM_PICK, (unsigned)groups, 1, 256, &a);
+}
+
+int g2_beam_reorder(const int *ids, int *ids_out, int ids_stride, const int *next, const int *origin, int *origin_out,
+                    int origin_stride, const int *parent, const int *len, int T, int groups, int beams)
+{
+    static const char fn[] = "g2_beam_reorder";
+    const int has_ids = ids || ids_out, has_origin = origin || origin_out;
+    if (!parent || (!has_ids && !has_origin) || (has_ids && (!ids || !ids_out || !next)) || (has_origin && (!origin || !origin_out)))
+        return g2i_err(G2_E_ARG, "%s: NULL buffer", fn);
+    if (groups < 1 || beams < 1) return g2i_err(G2_E_ARG, "%s: sizes must be positive", fn);
+    if (beams > G2B_MAX_BEAMS || groups > (1 << 16) / beams)
+        return g2i_err(G2_E_LIMIT, "%s: %d groups of %d beams: at most %d beams, %d rows", fn, groups, beams, G2B_MAX_BEAMS, 1 << 16);
+    if (T < 0 || (has_ids && T >= ids_stride) || (has_origin && T >= origin_stride))
+        return g2i_err(G2_E_ARG, "%s: %d ints and one more in rows of %d and %d", fn, T, ids_stride, origin_stride);
+    if (T >= MAX_ROWS) return g2i_err(G2_E_LIMIT, "%s: rows of %d: at most %d", fn, T, MAX_ROWS);
+    const long rows = (long)groups * beams;
+    const size_t ni = has_ids ? span_of(rows, ids_stride, T + 1, 4) : 0, no = has_origin ? span_of(rows, origin_stride, T + 1, 4) : 0;
+    const size_t nr = (size_t)rows * 4;
+    const struct { const void *p; size_t n; } in[] = { { parent, nr }, { len, len ? (size_t)groups * 4 : 0 }, { next, has_ids ? nr : 0 } };
+    int bad = (has_ids && ids != ids_out && g2i_overlap(ids, ni, ids_out, ni)) ||
+              (has_origin && origin != origin_out && g2i_overlap(origin, no, origin_out, no)) ||
+              (has_ids && has_origin && (g2i_overlap(ids_out, ni, origin_out, no) || g2i_overlap(ids_out, ni, origin, no) || g2i_overlap(ids, ni, origin_out, no)));
+    for (int i = 0; i < 3; ++i)
+        bad |= in[i].n && ((has_ids && g2i_overlap(ids_out, ni, in[i].p, in[i].n)) || (has_origin && g2i_overlap(origin_out, no, in[i].p, in[i].n)));
+    if (bad) return g2i_err(G2_E_ARG, "%s: overlapping buffers", fn);
+    const long chunks = ((long)T + 1 + 255) / 256;
+    if (!fits(chunks * groups)) return g2i_err(G2_E_LIMIT, "%s: too many ints for one call", fn);
+    const int rc = ready();
+    if (rc) return rc;
+    g2_beam_move_args a = { ids, ids_out, next, origin, origin_out, parent, len, ids_stride, origin_stride, T, groups, beams };
+    return g2i_launch(G2F_BEAM_MOVE, (unsigned)(chunks * groups), 1, 256, &a);
+}

@@ -1,0 +1,773 @@
+/*
+ * g2_batch.hip -- several texts at once (included by g2_kernels.hip behind
+ * g2_lowbit.hip, whose helpers it uses): causal attention of packed prompts,
+ * the 4-bit K/V cache with its single-query attention, beam search.  Layouts
+ * and index functions are in g2_batch_plan.h.
+ */
+namespace gb {
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef _Float16 f16x4u __attribute__((ext_vector_type(4), aligned(2)));
+
+/* ---------------------------------------------------------- packed rows */
+
+/* How many of the n + 1 ascending starts are at or below row (the same row in
+ * every lane): 64 of them probed at a time.  Whatever the list holds, it ends
+ * with a count between 0 and n + 1. */
+__device__ __forceinline__ int starts_below(const int *start, int n, int row, int lane)
+{
+    int lo = 0, left = n + 1; /* the count lies in lo .. lo + left */
+    for (;;) {
+        const int at = g2b_probe(left, lane);
+        const bool in = at < left && start[lo + (at < left ? at : 0)] <= row;
+        const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(in));
+        if (g2b_narrow(&lo, &left, c)) return lo;
+    }
+}
+
+/* The sequence of a lane's row, `row` being one of row0 .. row1 (the same in
+ * every lane); -1 before the first start. */
+__device__ __forceinline__ int seq_of_row(const int *start, int n, int row0, int row1, int row, int lane)
+{
+    int s = starts_below(start, n, row0, lane) - 1;
+    for (int at = s + 1; at <= n; at += 64) {
+        const int b = at + lane <= n ? start[at + lane] : INT_MAX;
+        for (int t = 0; t < 64; ++t) {
+            const int v = __builtin_amdgcn_readlane(b, t);
+            if (v > row1) return s;
+            if (v <= row) s = at + t;
+        }
+    }
+    return s;
+}
+
+/* ======================================================================
+ * Causal attention of packed prompts
+ * ==================================================================== */
+
+/* Eight values as three bf16 parts each, packed in twos: v = p1 + p2 + p3, each
+ * 8 significant bits of what is left, rounded to nearest (so that the products
+ * left out, below 2^-23, have either sign); exactly above 2^-102. */
+__device__ __forceinline__ void parts3(const float (&v)[8], u32x4 (&o)[3])
+{
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        f32x2 r = { v[2 * e], v[2 * e + 1] };
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            const unsigned w = __builtin_bit_cast(unsigned, __builtin_convertvector(r, bf16x2));
+            o[p][e] = w;
+            r[0] -= __uint_as_float(w << 16);
+            r[1] -= __uint_as_float(w & 0xffff0000u);
+        }
+    }
+}
+
+__device__ __forceinline__ f32x16 mma32(const u32x4 &a, const u32x4 &b, const f32x16 &c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma32h(const f16x8 &a, const f16x8 &b, const f32x16 &c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+/* c + a . b, the six products of parts that are above 2^-24 of it, small ones first */
+__device__ __forceinline__ f32x16 mma32_parts(const u32x4 (&a)[3], const u32x4 (&b)[3], f32x16 c)
+{
+    constexpr int pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0};
+#pragma unroll
+    for (int p = 0; p < 6; ++p) c = mma32(a[pa[p]], b[pb[p]], c);
+    return c;
+}
+
+__device__ __forceinline__ float swap_max(float v)
+{
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float swap_sum(float v)
+{
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+__device__ __forceinline__ int lanes_min_int(int v)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o));
+    return v;
+}
+
+__device__ __forceinline__ g2b_row keys_of_row(const g2_attn_prompt_args &a, int row0, int row, int lane)
+{
+    int s = 0, q0 = 0, q1 = a.q_rows, k0 = 0, k1 = a.k_rows;
+    if (a.q_start) s = seq_of_row(a.q_start, a.S, row0, row0 + G2B_ROWS - 1, row, lane);
+    const bool in = s >= 0 && s < a.S;
+    const int i = in ? s : 0;
+    if (a.q_start) { q0 = a.q_start[i]; q1 = a.q_start[i + 1]; }
+    if (a.k_start) { k0 = a.k_start[i]; k1 = a.k_start[i + 1]; }
+    return g2b_row_keys(row, in, q0, q1, k0, k1, a.q_rows, a.k_rows);
+}
+
+/* One wave takes 32 rows of a head (column l % 32 of a lane) against 32 keys at
+ * a time, products transposed: S^T = K Q^T and O^T = V^T P^T with 32x32x16
+ * matrix instructions (lane l supplies A[l % 32][8 (l / 32) ..+7] and B[8 (l /
+ * 32) ..+7][l % 32] and gets D[8 (r / 4) + 4 (l / 32) + r % 4][l % 32], r =
+ * 0..15).  So a lane has its row's scores of 16 of the 32 keys; those of r =
+ * 8u .. 8u + 7 are its operand of the second product's step u if V's operand
+ * takes the keys in the same order, 16 u + 8 (e / 4) + 4 (l / 32) + e % 4. */
+template <typename T> struct prompt_tile;
+template <> struct prompt_tile<float> {
+    f32x4 k[8];
+    float v[2][2][8]; /* [dims 32 t ..][step][key] */
+};
+template <> struct prompt_tile<_Float16> {
+    f16x8 k[4];
+    _Float16 v[2][2][8];
+};
+
+template <typename T>
+__device__ __forceinline__ void prompt_load(prompt_tile<T> &x, const T *k, const T *v, unsigned stride, int n, int lane)
+{
+    const unsigned sb = stride * (unsigned)sizeof(T), m = lane & 31, g = lane >> 5;
+    const char *kb = (const char *)k, *vb = (const char *)v;
+    /* (keys behind the n-th are the n-th again: the mask and zeros take care of them) */
+    const char *kp = kb + (size_t)min((int)m, n - 1) * sb + 8 * g * sizeof(T);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            x.k[2 * s] = *(const f32x4u *)(kp + 64 * s);
+            x.k[2 * s + 1] = *(const f32x4u *)(kp + 64 * s + 16);
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) x.k[s] = *(const f16x8u *)(kp + 32 * s);
+    }
+    if (n >= 32) {
+        const unsigned at = 4 * g * sb + m * (unsigned)sizeof(T);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const char *p = vb + (size_t)(16 * u + 8 * (e / 4) + e % 4) * sb;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) x.v[t][u][e] = *(const T *)(p + at + 32 * t * sizeof(T));
+            }
+    } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int j = 16 * u + 8 * (e / 4) + 4 * (int)g + e % 4;
+                const char *p = vb + (size_t)min(j, n - 1) * sb + m * sizeof(T);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const T y = *(const T *)(p + 32 * t * sizeof(T));
+                    x.v[t][u][e] = j < n ? y : (T)0.f;
+                }
+            }
+    }
+}
+
+template <typename T, int KW>
+__device__ void prompt_impl(const g2_attn_prompt_args &a)
+{
+    constexpr bool F16 = sizeof(T) == 2;
+    __shared__ float red[KW][34][64];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
+    const long item = g2b_item(blockIdx.x, (long)a.tiles * a.NH);
+    const int h = (int)(item / a.tiles), tile = a.tiles - 1 - (int)(item % a.tiles); /* (long rows first) */
+    const int row0 = tile * G2B_ROWS, row = row0 + (lane & 31);
+    const g2b_row mine = keys_of_row(a, row0, row, lane);
+    const bool sees = mine.there && mine.end > mine.lo;
+    const int k0 = __builtin_amdgcn_readfirstlane(lanes_min_int(sees ? mine.lo : INT_MAX));
+    const int k1 = __builtin_amdgcn_readfirstlane(-lanes_min_int(sees ? -mine.end : INT_MAX));
+    const float c = a.scale * 1.44269504f;
+    /* the queries, with the factor in fp32 rows' own values */
+    u32x4 q3[4][3];
+    f16x8 qh[4];
+    {
+        const T *qp = (const T *)a.q + (size_t)min(row, a.q_rows - 1) * a.q_stride + h * G2B_DH + 8 * g;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            if constexpr (F16) qh[s] = *(const f16x8u *)(qp + 16 * s);
+            else {
+                const f32x4 x0 = *(const f32x4u *)(qp + 16 * s), x1 = *(const f32x4u *)(qp + 16 * s + 4);
+                const float x[8] = { x0[0] * c, x0[1] * c, x0[2] * c, x0[3] * c, x1[0] * c, x1[1] * c, x1[2] * c, x1[3] * c };
+                parts3(x, q3[s]);
+            }
+        }
+    }
+    f32x16 o[2] = {};
+    float m = -INFINITY, l = 0.f;
+    const int f = h / (a.NH / a.NKV) * G2B_DH;
+    const T *kp = (const T *)a.k + f, *vp = (const T *)a.v + f;
+    prompt_tile<T> next;
+    const int first = k0 + 32 * w;
+    if (first < k1) prompt_load(next, kp + (size_t)first * a.kv_stride, vp + (size_t)first * a.kv_stride, (unsigned)a.kv_stride, k1 - first, lane);
+    for (int j0 = first; j0 < k1; j0 += 32 * KW) {
+        prompt_tile<T> x = next;
+        const int j1 = j0 + 32 * KW;
+        if (j1 < k1) prompt_load(next, kp + (size_t)j1 * a.kv_stride, vp + (size_t)j1 * a.kv_stride, (unsigned)a.kv_stride, k1 - j1, lane);
+        f32x16 s = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (F16) s = mma32h(x.k[i], qh[i], s);
+            else {
+                const f32x4 y0 = x.k[2 * i], y1 = x.k[2 * i + 1];
+                const float y[8] = { y0[0], y0[1], y0[2], y0[3], y1[0], y1[1], y1[2], y1[3] };
+                u32x4 k3[3];
+                parts3(y, k3);
+                s = mma32_parts(k3, q3[i], s);
+            }
+        }
+        float top = m;
+        if constexpr (F16) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] *= c;
+        }
+        if (wave_any(mine.lo > j0 || mine.end < j0 + 32)) { /* some row does not see all of them */
+            const int at = j0 + 4 * g - mine.lo, n = mine.end - mine.lo;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if ((unsigned)(at + 8 * (r / 4) + r % 4) >= (unsigned)n) s[r] = -INFINITY;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
+        top = swap_max(top);
+        /* (fp16 weights: 2^14 times the weight, so that small ones keep their bits) */
+        const float base = (top == -INFINITY ? 0.f : top) - (F16 ? 14.f : 0.f);
+        if (wave_any(top > m)) {
+            const float down = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+            l *= down;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[t][r] *= down;
+            m = top;
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = __builtin_amdgcn_exp2f(s[r] - base);
+            sum += s[r];
+        }
+        l += sum;
+        /* a value that is not finite must not meet the weights 0 of rows that do not see it */
+        float z = 0.f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z = fmaf((float)x.v[t][u][e], 0.f, z);
+        if (wave_any(z != 0.f)) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (!__builtin_isfinite((float)x.v[t][u][e])) x.v[t][u][e] = (T)0.f;
+            const int n = min(32, k1 - j0);
+#pragma unroll 1
+            for (int i = 0; i < n; ++i) {
+                const bool seen = j0 + i >= mine.lo && j0 + i < mine.end;
+                const T *p = vp + (size_t)(j0 + i) * a.kv_stride + 4 * g;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float y = (float)p[32 * t + 8 * (r / 4) + r % 4];
+                        if (seen && !__builtin_isfinite(y)) o[t][r] += y;
+                    }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            if constexpr (F16) {
+                f16x8 ph;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ph[e] = (_Float16)s[8 * u + e];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    f16x8 vh;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) vh[e] = x.v[t][u][e];
+                    o[t] = mma32h(vh, ph, o[t]);
+                }
+            } else {
+                float p[8];
+                u32x4 p3[3], v3[3];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[e] = s[8 * u + e];
+                parts3(p, p3);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    parts3(x.v[t][u], v3);
+                    o[t] = mma32_parts(v3, p3, o[t]);
+                }
+            }
+        }
+    }
+    l = swap_sum(l);
+    /* the waves' parts meet; wave w writes the dims of its share of the registers */
+    red[w][0][lane] = m;
+    red[w][1][lane] = l;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) red[w][2 + 16 * t + r][lane] = o[t][r];
+    __syncthreads();
+    if (!mine.there) return;
+    float top = -INFINITY, part[KW];
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < KW; ++i) top = fmaxf(top, red[i][0][lane]);
+#pragma unroll
+    for (int i = 0; i < KW; ++i) {
+        part[i] = kv8_factor(red[i][0][lane], top);
+        l = fmaf(red[i][1][lane], part[i], l);
+    }
+    T *out = (T *)a.out + (size_t)row * a.out_stride + h * G2B_DH + 4 * g;
+#pragma unroll
+    for (int i = 0; i < 8 / KW; ++i) {
+        const int q = w * (8 / KW) + i;
+        f32x4 y = {};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int j = 0; j < KW; ++j) y[e] = fmaf(red[j][2 + 4 * q + e][lane], part[j], y[e]);
+            y[e] = sees ? y[e] / l : 0.f;
+        }
+        T *p = out + 32 * (q / 4) + 8 * (q % 4);
+        if constexpr (F16) *(f16x4u *)p = f16x4u{ (_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3] };
+        else *(f32x4u *)p = y;
+    }
+}
+G2K void g2k_prompt_f32(const g2_attn_prompt_args a) { prompt_impl<float, 4>(a); }
+G2K void g2k_prompt_f16(const g2_attn_prompt_args a) { prompt_impl<_Float16, 4>(a); }
+
+/* ======================================================================
+ * 4-bit K/V cache: each position, head and 32 dims on their own, codes and
+ * scale as those of the 4-bit weights.
+ * ==================================================================== */
+
+/* A wave takes 8 rows of keys or values of a head, eight lanes of 8 dims to a
+ * row, neighbouring waves neighbouring heads. */
+template <typename T>
+__device__ void kv4_append_impl(const g2_kv4_append_args &a)
+{
+    const int lane = threadIdx.x & 63, part = lane & 7;
+    const long wave = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = (int)(wave % a.NKV), kv = (int)(wave / a.NKV % 2);
+    const long r0 = wave / a.NKV / 2 * 8;
+    if (r0 >= a.rows) return;
+    const int row = (int)r0 + (lane >> 3);
+    typedef T t8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    const t8 raw = *(const t8 *)((const T *)(kv ? a.v : a.k) + (size_t)min(row, a.rows - 1) * a.stride + h * G2B_DH + 8 * part);
+    int s, q0, q1;
+    if (a.row_start) {
+        s = seq_of_row(a.row_start, a.S, (int)r0, (int)r0 + 7, row, lane);
+        const int i = clampi(s, 0, a.S - 1);
+        q0 = a.row_start[i];
+        q1 = min(a.row_start[i + 1], a.rows);
+    } else {
+        s = row / a.per;
+        q0 = s * a.per;
+        q1 = q0 + a.per;
+    }
+    const bool there = s >= 0 && s < a.S && row >= q0 && row < q1 && row < a.rows;
+    const long p = there ? (long)(a.pos ? a.pos[s] : a.start) + (row - q0) : -1;
+    float x[8];
+    unsigned amax = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        x[e] = (float)raw[e];
+        const unsigned u = __float_as_uint(x[e]) & 0x7FFFFFFF;
+        amax = u > amax ? u : amax;
+    }
+    amax = q4_group_max(amax, 32);
+    const uint16_t sc = q4_scale(amax);
+    const unsigned codes = q4_codes(x, bf16_f(sc));
+    if (p < 0 || p >= a.max_seq) return;
+    unsigned char *t = a.cache + g2b_tile_at(a.NKV, a.tiles, s, h, p / G2B_TILE);
+    const int i = (int)(p % G2B_TILE);
+    *(unsigned *)(t + g2b_code_at(kv, i) + 4 * part) = codes;
+    if (!(part & 3)) *(uint16_t *)(t + g2b_scale_at(kv, i) + 2 * (part >> 2)) = sc;
+}
+G2K void g2k_kv4_append_f32(const g2_kv4_append_args a) { kv4_append_impl<float>(a); }
+G2K void g2k_kv4_append_f16(const g2_kv4_append_args a) { kv4_append_impl<_Float16>(a); }
+
+/* One thread per 8 dims of a position, keys and values, in the order of the output. */
+G2K void g2k_kv4_read(const g2_kv4_read_args a)
+{
+    const int parts = a.NKV * 8;
+    const long n = (long)a.S * a.T * parts;
+    for (long i = blockIdx.x * 256l + threadIdx.x; i < n; i += gridDim.x * 256l) {
+        const long row = i / parts;
+        const int e = (int)(i - row * parts), h = e / 8, part = e % 8;
+        const long s = row / a.T;
+        const int p = a.start + (int)(row - s * a.T);
+        if (p >= kv8_length(a.len, a.T_kv, s)) continue;
+        const int from = a.origin ? a.origin[s * a.max_seq + p] : (int)s;
+        if (from < 0 || from >= a.S) continue;
+        const unsigned char *t = a.cache + g2b_tile_at(a.NKV, a.tiles, from, h, p / G2B_TILE);
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+            float v[8];
+            q4_values(*(const unsigned *)(t + g2b_code_at(kv, p % G2B_TILE) + 4 * part),
+                      bf16_f(*(const uint16_t *)(t + g2b_scale_at(kv, p % G2B_TILE) + 2 * (part >> 2))), v);
+            float *o = (kv ? a.v : a.k) + 8 * i;
+            *(f32x4u *)o = f32x4{ v[0], v[1], v[2], v[3] };
+            *(f32x4u *)(o + 4) = f32x4{ v[4], v[5], v[6], v[7] };
+        }
+    }
+}
+
+/* ---- single-query attention.  A wave takes 64 / LP positions at a time, LP
+ * lanes of DL = 64 / LP dims to a position, for G query heads that share a key
+ * head; each position slot keeps a running maximum and sum of its own. */
+template <int G, int LP>
+__device__ void kv4_attn_impl(const g2_kv4_attn_args &a)
+{
+    constexpr int DL = 64 / LP, SLOTS = 64 / LP, W = DL / 8, NW = 4;
+    __shared__ float part[NW][G][G2B_PART_FLOATS];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int slot = lane / LP, d0 = DL * (lane % LP);
+    const int split = blockIdx.x % a.splits, ch = blockIdx.x / a.splits % a.chunks;
+    const int hk = blockIdx.x / a.splits / a.chunks % a.NKV;
+    const long s = blockIdx.x / a.splits / a.chunks / a.NKV;
+    const int group = a.NH / a.NKV, h0 = hk * group + ch * a.heads;
+    const int nh = min(a.heads, group - ch * a.heads);
+    const int len = kv8_length(a.len, a.T_kv, s);
+    const int p0 = split * a.span * G2B_TILE, p1 = min(len, p0 + a.span * G2B_TILE);
+    float q[G][DL], o[G][DL], m[G], l[G];
+    const float qf = a.scale * 1.44269504f;
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+        const float *p = a.q + s * a.q_stride + (h0 + min(i, nh - 1)) * G2B_DH + d0;
+#pragma unroll
+        for (int e = 0; e < DL; e += 4) {
+            const f32x4 v = *(const f32x4u *)(p + e);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q[i][e + j] = v[j] * qf;
+        }
+#pragma unroll
+        for (int e = 0; e < DL; ++e) o[i][e] = 0.f;
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+    }
+    for (int b = p0 + SLOTS * w; b < p1; b += SLOTS * NW) {
+        const int p = b + slot;
+        const int from = p < p1 ? a.origin ? a.origin[s * a.max_seq + p] : (int)s : -1;
+        const bool there = from >= 0 && from < a.S;
+        const int pc = there ? p : b;
+        const unsigned char *t = a.cache + g2b_tile_at(a.NKV, a.tiles, there ? from : s, hk, pc / G2B_TILE);
+        unsigned kc[W], vc[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            kc[i] = *(const unsigned *)(t + g2b_code_at(0, pc % G2B_TILE) + d0 / 2 + 4 * i);
+            vc[i] = *(const unsigned *)(t + g2b_code_at(1, pc % G2B_TILE) + d0 / 2 + 4 * i);
+        }
+        const float ks = bf16_f(*(const uint16_t *)(t + g2b_scale_at(0, pc % G2B_TILE) + d0 / 32 * 2));
+        const float vs = there ? bf16_f(*(const uint16_t *)(t + g2b_scale_at(1, pc % G2B_TILE) + d0 / 32 * 2)) : 0.f;
+        float x[G], pr[G];
+#pragma unroll
+        for (int i = 0; i < G; ++i) x[i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            float v[8];
+            q4_values(kc[i], 1.f, v);
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[j] = fmaf(q[j][8 * i + e], v[e], x[j]);
+        }
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            float d = x[i] * ks;
+            d += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(d), 0xB1, 0xF, 0xF, false)); /* lanes 1 0 3 2 */
+            if (LP == 4) d += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(d), 0x4E, 0xF, 0xF, false));
+            if (!there) d = -INFINITY;
+            const float top = fmaxf(m[i], d), base = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f(m[i] - base);
+            pr[i] = __builtin_amdgcn_exp2f(d - base);
+            l[i] = fmaf(l[i], f, pr[i]);
+            m[i] = top;
+            pr[i] *= vs;
+#pragma unroll
+            for (int e = 0; e < DL; ++e) o[i][e] *= f;
+        }
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            float v[8];
+            q4_values(vc[i], 1.f, v);
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[j][8 * i + e] = fmaf(pr[j], v[e], o[j][8 * i + e]);
+        }
+    }
+    /* the wave's position slots: each step halves the dims that a lane keeps */
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+        float top = slots_max(m[i]);
+        if (LP == 2) top = fmaxf(top, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(top), 0x4E, 0xF, 0xF, false)));
+        const float f = kv8_factor(m[i], top);
+        float sum = l[i] * f;
+        if (LP == 2) sum += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(sum), 0x4E, 0xF, 0xF, false));
+        sum += lane_xor4(sum);
+        sum += lane_xor8(sum);
+        sum = lane_fold16(sum, sum);
+        sum = lane_fold32(sum, sum);
+        float *v = o[i];
+#pragma unroll
+        for (int e = 0; e < DL; ++e) v[e] *= f;
+        int n = DL / 2;
+#pragma unroll
+        for (int e = 0; e < DL / 2; ++e) v[e] = lane_fold32(v[e], v[e + DL / 2]);
+#pragma unroll
+        for (int e = 0; e < DL / 4; ++e) v[e] = lane_fold16(v[e], v[e + DL / 4]);
+        n = DL / 8;
+#pragma unroll
+        for (int e = 0; e < DL / 8; ++e) {
+            const float lo = v[e] + lane_xor8(v[e]), hi = v[e + n] + lane_xor8(v[e + n]);
+            v[e] = lane & 8 ? hi : lo;
+        }
+        n = DL / 16;
+#pragma unroll
+        for (int e = 0; e < DL / 16; ++e) {
+            const float lo = v[e] + lane_xor4(v[e]), hi = v[e + n] + lane_xor4(v[e + n]);
+            v[e] = lane & 4 ? hi : lo;
+        }
+        if (LP == 2) {
+            const float lo = v[0] + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v[0]), 0x4E, 0xF, 0xF, false));
+            const float hi = v[1] + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v[1]), 0x4E, 0xF, 0xF, false));
+            v[0] = lane & 2 ? hi : lo;
+        }
+        if (lane == 0) { part[w][i][0] = top; part[w][i][1] = sum; }
+        part[w][i][2 + d0 + slot] = v[0];
+    }
+    __syncthreads();
+    for (int i = w; i < nh; i += NW) {
+        float top = -INFINITY, sum = 0.f, y = 0.f;
+#pragma unroll
+        for (int j = 0; j < NW; ++j) top = fmaxf(top, part[j][i][0]);
+#pragma unroll
+        for (int j = 0; j < NW; ++j) {
+            const float f = kv8_factor(part[j][i][0], top);
+            sum = fmaf(part[j][i][1], f, sum);
+            y = fmaf(part[j][i][2 + lane], f, y);
+        }
+        if (a.splits > 1) {
+            float *r = a.part + ((s * a.NH + h0 + i) * a.splits + split) * G2B_PART_FLOATS;
+            if (lane == 0) { r[0] = top; r[1] = sum; }
+            r[2 + lane] = y;
+        } else
+            a.out[s * a.out_stride + (h0 + i) * G2B_DH + lane] = sum == 0.f ? 0.f : y / sum;
+    }
+}
+G2K void g2k_kv4_attn1(const g2_kv4_attn_args a) { kv4_attn_impl<1, 2>(a); }
+G2K void g2k_kv4_attn2(const g2_kv4_attn_args a) { kv4_attn_impl<2, 4>(a); }
+G2K void g2k_kv4_attn4(const g2_kv4_attn_args a) { kv4_attn_impl<4, 4>(a); }
+
+/* Joins the parts of a head, one wave to it. */
+G2K void g2k_kv4_join(const g2_kv4_attn_args a)
+{
+    const int lane = threadIdx.x & 63;
+    const long head = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (head >= (long)a.S * a.NH) return;
+    const float *r = a.part + head * a.splits * G2B_PART_FLOATS;
+    float top = -INFINITY, sum = 0.f, y = 0.f;
+    for (int i = 0; i < a.splits; ++i) top = fmaxf(top, r[i * G2B_PART_FLOATS]);
+    for (int i = 0; i < a.splits; ++i) {
+        const float *p = r + i * G2B_PART_FLOATS, f = kv8_factor(p[0], top);
+        sum = fmaf(p[1], f, sum);
+        y = fmaf(p[2 + lane], f, y);
+    }
+    a.out[head / a.NH * a.out_stride + head % a.NH * G2B_DH + lane] = sum == 0.f ? 0.f : y / sum;
+}
+
+/* ======================================================================
+ * Beam search
+ * ==================================================================== */
+
+__device__ __forceinline__ unsigned long long wave_max_key(unsigned long long v)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const unsigned long long u = __shfl_xor(v, o);
+        v = u > v ? u : v;
+    }
+    return v;
+}
+
+/* A slice of a row: its largest logit, the sum of exponentials below it, and its
+ * n_out greatest logits (of equal ones the lower ids) as keys, 0 for none. */
+G2K void g2k_beam_slice(const g2_beam_args a)
+{
+    __shared__ float red[4];
+    __shared__ unsigned long long best[4];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const long row = blockIdx.x / a.slices;
+    const int slice = blockIdx.x % a.slices, v0 = slice * G2B_SLICE, nv = min(a.V - v0, G2B_SLICE);
+    const float *in = a.logits + row * a.V + v0;
+    float x[16];
+#pragma unroll
+    for (int q = 0; q < 16; ++q) x[q] = tid + 256 * q < nv ? in[tid + 256 * q] : -INFINITY;
+    float top = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) top = fmaxf(top, x[q]);
+    top = wave_max(top);
+    if (lane == 0) red[w] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    __syncthreads();
+    float sum = 0.f;
+    unsigned long long mine = 0; /* the thread's best key */
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+        sum += tid + 256 * q < nv ? expf(x[q] - (top == -INFINITY ? 0.f : top)) : 0.f;
+        if (x[q] > -INFINITY) {
+            const unsigned long long k = logit_key(x[q], v0 + tid + 256 * q);
+            mine = k > mine ? k : mine;
+        }
+    }
+    sum = block_sum(sum, red);
+    const long cell = row * a.slices + slice;
+    if (tid == 0) { a.stats[2 * cell] = top; a.stats[2 * cell + 1] = sum; }
+    for (int n = 0; n < a.n_out; ++n) {
+        const unsigned long long k = wave_max_key(mine);
+        if (lane == 0) best[w] = k;
+        __syncthreads();
+        unsigned long long b = best[0];
+#pragma unroll
+        for (int i = 1; i < 4; ++i) b = best[i] > b ? best[i] : b;
+        if (tid == 0) a.cands[cell * a.n_out + n] = b;
+        if (b && b == mine) { /* its thread goes on to its next */
+            mine = 0;
+#pragma unroll
+            for (int q = 0; q < 16; ++q)
+                if (x[q] > -INFINITY) {
+                    const unsigned long long k2 = logit_key(x[q], v0 + tid + 256 * q);
+                    mine = k2 < b && k2 > mine ? k2 : mine;
+                }
+        }
+        __syncthreads();
+    }
+}
+
+/* A number that orders as a double does (no NaN). */
+__device__ __forceinline__ unsigned long long double_key(double v)
+{
+    const unsigned long long u = __double_as_longlong(v + 0.0);
+    return u >> 63 ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ double key_double(unsigned long long k)
+{
+    return __longlong_as_double(k >> 63 ? k & ~(1ull << 63) : ~k);
+}
+__device__ __forceinline__ float key_logit(unsigned long long k)
+{
+    const unsigned u = (unsigned)(k >> 32);
+    return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
+}
+
+/* The n_out best of a group's candidates: each thread goes over its share of
+ * them once for every one that is taken. */
+G2K void g2k_beam_pick(const g2_beam_args a)
+{
+    __shared__ double lse[G2B_MAX_BEAMS]; /* score - log sum exp; NaN: no continuations */
+    __shared__ unsigned long long bk[4];
+    __shared__ unsigned bf[4];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const long g = blockIdx.x, row0 = g * a.beams;
+    if (tid < a.beams) {
+        const long row = row0 + tid;
+        const float *st = a.stats + 2 * row * a.slices;
+        float top = -INFINITY;
+        double sum = 0.0;
+        for (int i = 0; i < a.slices; ++i) top = fmaxf(top, st[2 * i]);
+        for (int i = 0; i < a.slices; ++i) sum += (double)st[2 * i + 1] * exp((double)st[2 * i] - (double)(top == -INFINITY ? 0.f : top));
+        lse[tid] = a.done && a.done[row] ? __longlong_as_double(0x7ff8000000000000ll) : (double)a.score[row] - ((double)top + log(sum));
+    }
+    __syncthreads();
+    const int per = a.slices * a.n_out, total = a.beams * per;
+    unsigned long long lastk = ~0ull;
+    unsigned lastf = 0;
+    for (int n = 0; n < a.n_out; ++n) {
+        unsigned long long k = 0;
+        unsigned f = ~0u;
+        for (int i = tid; i < total + a.beams; i += 256) {
+            unsigned long long ck;
+            unsigned cf;
+            if (i < total) {
+                const int b = i / per;
+                const unsigned long long c = a.cands[row0 * per + i];
+                const double t = (double)key_logit(c) + lse[b];
+                if (!c || !(t > -INFINITY)) continue;
+                ck = double_key(t);
+                cf = (unsigned)b * (unsigned)a.V + (unsigned)~(unsigned)c;
+            } else {
+                const int b = i - total;
+                if (!a.done || !a.done[row0 + b] || !(a.score[row0 + b] > -INFINITY)) continue;
+                ck = double_key((double)a.score[row0 + b]);
+                cf = (unsigned)b * (unsigned)a.V + (unsigned)a.eos;
+            }
+            if (ck > lastk || (ck == lastk && n && cf <= lastf)) continue; /* taken */
+            if (ck > k || (ck == k && cf < f)) { k = ck; f = cf; }
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const unsigned long long ok = __shfl_xor(k, o);
+            const unsigned of = __shfl_xor(f, o);
+            if (ok > k || (ok == k && of < f)) { k = ok; f = of; }
+        }
+        if (lane == 0) { bk[w] = k; bf[w] = f; }
+        __syncthreads();
+        k = bk[0]; f = bf[0];
+#pragma unroll
+        for (int i = 1; i < 4; ++i)
+            if (bk[i] > k || (bk[i] == k && bf[i] < f)) { k = bk[i]; f = bf[i]; }
+        if (tid == 0) {
+            const long at = g * a.n_out + n;
+            const int parent = k ? (int)(f / (unsigned)a.V) : -1, id = k ? (int)(f % (unsigned)a.V) : -1;
+            a.out_score[at] = k ? (float)key_double(k) : -INFINITY;
+            a.out_parent[at] = parent;
+            a.out_id[at] = id;
+            if (a.out_done) a.out_done[at] = k && (id == a.eos || (a.done && a.done[row0 + parent]));
+        }
+        lastk = k ? k : 1; /* (no key is 1: nothing is left) */
+        lastf = f;
+        __syncthreads();
+    }
+}
+
+/* Columns of a group's tables: a thread reads its column of all beams before it
+ * writes it, so a table may be moved in place. */
+G2K void g2k_beam_move(const g2_beam_move_args a)
+{
+    __shared__ int col[G2B_MAX_BEAMS][256];
+    const int tid = threadIdx.x, chunks = (a.T + 1 + 255) / 256;
+    const long g = blockIdx.x / chunks, row0 = g * a.beams;
+    const int p = (int)(blockIdx.x % chunks) * 256 + tid;
+    const int n = a.len ? clampi(a.len[g], 0, a.T) : a.T;
+    if (p > n) return;
+    for (int which = 0; which < 2; ++which) {
+        const int *in = which ? a.origin : a.ids;
+        int *out = which ? a.origin_out : a.ids_out;
+        const long stride = which ? a.origin_stride : a.ids_stride;
+        if (!out) continue;
+        if (p < n)
+            for (int b = 0; b < a.beams; ++b) col[b][tid] = in[(row0 + b) * stride + p];
+        for (int b = 0; b < a.beams; ++b) {
+            const int from = a.parent[row0 + b];
+            if (from < 0 || from >= a.beams) continue;
+            out[(row0 + b) * stride + p] = p < n ? col[from][tid] : which ? (int)(row0 + b) : a.next[row0 + b];
+        }
+    }
+}
+} // namespace gb

@@ -120,7 +120,14 @@ extern "C" {
     X(KV8_APPEND, "g2k_kv8_append") X(KV8_READ, "g2k_kv8_read")               \
     X(KV8_ATTN1, "g2k_kv8_attn1") X(KV8_ATTN4, "g2k_kv8_attn4")               \
     X(KV8_ATTN8, "g2k_kv8_attn8") X(KV8_JOIN, "g2k_kv8_join")                 \
-    X(LOGITS, "g2k_logits") X(LOGITS_WIDE, "g2k_logits_wide")
+    X(LOGITS, "g2k_logits") X(LOGITS_WIDE, "g2k_logits_wide")                 \
+    X(PROMPT_F32, "g2k_prompt_f32") X(PROMPT_F16, "g2k_prompt_f16")           \
+    X(KV4_APPEND_F32, "g2k_kv4_append_f32")                                   \
+    X(KV4_APPEND_F16, "g2k_kv4_append_f16") X(KV4_READ, "g2k_kv4_read")       \
+    X(KV4_ATTN1, "g2k_kv4_attn1") X(KV4_ATTN2, "g2k_kv4_attn2")               \
+    X(KV4_ATTN4, "g2k_kv4_attn4") X(KV4_JOIN, "g2k_kv4_join")                 \
+    X(BEAM_SLICE, "g2k_beam_slice") X(BEAM_PICK, "g2k_beam_pick")             \
+    X(BEAM_MOVE, "g2k_beam_move")
 
 #define G2_ENUM_ENTRY(id, name) G2F_##id,
 enum { G2_KERNEL_LIST(G2_ENUM_ENTRY) G2F_COUNT };
@@ -205,6 +212,10 @@ int g2i_kv8_form(long heads, int T_kv, int *span, int *waves);
 
 /* Whether g2_apply_logit_rules takes its wide form, and the slices of a row. */
 int g2i_logits_form(int rows, int V, int *parts);
+
+/* g2_attn_kv4's parts of a key head's positions, tiles to a part, query heads to
+ * a pass over them and passes to a key head. */
+int g2i_kv4_form(int n_seq, int n_head, int n_kv, int T_kv, int *heads, int *chunks, int *span);
 
 /* Whether np bytes at p and nq bytes at q share any. */
 static inline int g2i_overlap(const void *p, size_t np, const void *q, size_t nq)

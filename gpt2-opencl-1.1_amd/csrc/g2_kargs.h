@@ -451,4 +451,80 @@ typedef struct {
     float repetition, frequency, presence;
 } g2_logits_args;
 
+/* Packed prompt attention: rows of q (NH heads of 64) against rows of k, v (NKV
+ * heads), sequence s having query rows q_start[s] .. q_start[s+1] - 1 and key
+ * rows k_start[s] .. (NULL: one sequence of all rows).  Strides in elements. */
+typedef struct {
+    const void *q;
+    const void *k;
+    const void *v;
+    void *out;
+    const int *q_start;
+    const int *k_start;
+    int q_stride, kv_stride, out_stride;
+    int S, q_rows, k_rows, NH, NKV, tiles;
+    float scale;
+} g2_attn_prompt_args;
+
+/* 4-bit K/V cache (g2_batch_plan.h).  Append: row r of k, v (NKV heads of 64)
+ * of sequence s goes to position p0 + r - row_start[s], p0 = pos ? pos[s] :
+ * start, row_start NULL: per rows for each sequence. */
+typedef struct {
+    const void *k;
+    const void *v;
+    unsigned char *cache;
+    const int *row_start;
+    const int *pos;
+    int stride, start, S, rows, per, NKV, max_seq, tiles;
+} g2_kv4_append_args;
+
+/* Read: positions start .. start + T - 1 of every sequence to k, v [S][T][64
+ * NKV], those below its length; origin (NULL: its own) says whose slot has a position. */
+typedef struct {
+    const unsigned char *cache;
+    float *k;
+    float *v;
+    const int *origin;
+    const int *len;
+    int T_kv, start, T, S, NKV, max_seq, tiles;
+} g2_kv4_read_args;
+
+/* Single-query attention over the 4-bit cache: chunks of `heads` query heads
+ * that share a key head, in parts of `span` tiles. */
+typedef struct {
+    const float *q;
+    const unsigned char *cache;
+    float *out;
+    float *part;
+    const int *origin;
+    const int *len;
+    int q_stride, out_stride, T_kv, S, NH, NKV, max_seq, tiles, splits, span, chunks, heads;
+    float scale;
+} g2_kv4_attn_args;
+
+/* Beam selection: rows = groups x beams of V logits. */
+typedef struct {
+    const float *logits;
+    const float *score;
+    const int *done;
+    float *out_score;
+    int *out_parent;
+    int *out_id;
+    int *out_done;
+    float *stats;              /* [rows][slices][2] */
+    unsigned long long *cands; /* [rows][slices][n_out] */
+    int eos, groups, beams, V, n_out, slices;
+} g2_beam_args;
+
+typedef struct {
+    const int *ids;
+    int *ids_out;
+    const int *next;
+    const int *origin;
+    int *origin_out;
+    const int *parent;
+    const int *len;
+    int ids_stride, origin_stride, T, groups, beams;
+} g2_beam_move_args;
+
 #endif /* G2_KARGS_H */

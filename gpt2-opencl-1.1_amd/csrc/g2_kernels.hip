@@ -25,6 +25,7 @@
 #include "g2_gemm_plan.h"
 #include "g2_attn_plan.h"
 #include "g2_lowbit_plan.h"
+#include "g2_batch_plan.h"
 
 #define G2K extern "C" __global__ __launch_bounds__(256)
 
@@ -2191,6 +2192,9 @@ G2K void g2k_ln_fold_f16(const g2_lnfold_args a) { ln_fold_impl<_Float16>(a); }
 
 /* 4-bit weights, the 8-bit K/V cache, rules on logits. */
 #include "g2_lowbit.hip"
+
+/* Several texts at once: packed prompts, the 4-bit K/V cache, beam search. */
+#include "g2_batch.hip"
 
 /* The persistent decode step (one cooperative launch per token). */
 #include "g2_step.hip"

@@ -105,6 +105,11 @@ for _n, _a in {
     "g2_kv8_append": [_vp] * 4 + [_i] * 5, "g2_kv8_read": [_vp] * 4 + [_i] * 6,
     "g2_attn_kv8": [_vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _f, _vp],
     "g2_apply_logit_rules": [_vp, _vp, _vp, _i, _i, C.POINTER(LogitRules), _vp],
+    "g2_attn_prompt": [_vp, _i, _vp, _vp, _i, _vp, _i, _i, _vp, _vp] + [_i] * 5 + [_f],
+    "g2_kv4_append": [_vp, _vp, _i, _i, _vp, _vp, _vp] + [_i] * 5, "g2_kv4_read": [_vp] * 5 + [_i] * 6,
+    "g2_attn_kv4": [_vp, _i, _vp, _vp, _i, _vp, _vp] + [_i] * 5 + [_f, _vp],
+    "g2_beam_select": [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp] + [_i] * 4 + [_vp],
+    "g2_beam_reorder": [_vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i],
     "g2_model_uses_graph": [_vp], "g2_read_kv": [_vp, _i, _vp, _vp],
     "g2_config_load": [C.c_char_p, C.POINTER(Config)], "g2_config_parse": [C.c_char_p, C.POINTER(Config)],
     "g2_model_load": [C.c_char_p, _i, _i, C.POINTER(_vp)],
@@ -129,6 +134,9 @@ _sig("g2_q4_scale_bytes", _sz, _i, _i, _i)
 _sig("g2_kv8_bytes", _sz, _i, _i, _i)
 _sig("g2_kv8_work_bytes", _sz, _i, _i)
 _sig("g2_logits_work_bytes", _sz, _i)
+_sig("g2_kv4_bytes", _sz, _i, _i, _i)
+_sig("g2_kv4_work_bytes", _sz, _i, _i)
+_sig("g2_beam_work_bytes", _sz, _i, _i, _i, _i)
 
 
 def last_error():
@@ -365,6 +373,57 @@ def logit_rules(ctx=None, ctx_len=None, max_ctx=0, repetition=1.0, frequency=0.0
 def apply_logit_rules(logits, out, pick, rows, V, rules, work):
     """out = logits under the rules, pick = each row's greatest id; either may be None."""
     check(_lib.g2_apply_logit_rules(_p(logits), _p(out), _p(pick), rows, V, C.byref(rules), _p(work)))
+
+
+# ---------------------------------------------------------------- several texts at once
+
+def attn_prompt(q, q_stride, k, v, kv_stride, out, out_stride, dtype, q_start, k_start, n_seq, q_rows, k_rows, n_head, n_kv, scale):
+    """Causal attention of packed prompts; starts are device arrays of n_seq + 1 ints (None: one sequence of all rows)."""
+    check(_lib.g2_attn_prompt(_p(q), q_stride, _p(k), _p(v), kv_stride, _p(out), out_stride, dtype, _p(q_start), _p(k_start),
+                              n_seq, q_rows, k_rows, n_head, n_kv, scale))
+
+
+def kv4_bytes(n_seq, n_kv, max_seq):
+    """Bytes of a 4-bit K/V cache (0 where the sizes are not supported)."""
+    return _lib.g2_kv4_bytes(n_seq, n_kv, max_seq)
+
+
+def kv4_work_bytes(n_seq, n_head):
+    """Bytes of attn_kv4's workspace."""
+    return _lib.g2_kv4_work_bytes(n_seq, n_head)
+
+
+def kv4_append(k, v, stride, dtype, cache, row_start, pos, start, n_seq, rows, n_kv, max_seq):
+    """Appends rows of keys and values (packed by row_start, or None: rows / n_seq each) at pos (device array, or None: start)."""
+    check(_lib.g2_kv4_append(_p(k), _p(v), stride, dtype, _p(cache), _p(row_start), _p(pos), start, n_seq, rows, n_kv, max_seq))
+
+
+def kv4_read(cache, k, v, origin, lens, T_kv, start, T, n_seq, n_kv, max_seq):
+    """Keys and values at positions start .. start + T - 1 that lie below a sequence's length, fp32."""
+    check(_lib.g2_kv4_read(_p(cache), _p(k), _p(v), _p(origin), _p(lens), T_kv, start, T, n_seq, n_kv, max_seq))
+
+
+def attn_kv4(q, q_stride, cache, out, out_stride, origin, lens, T_kv, n_seq, n_head, n_kv, max_seq, scale, work):
+    """Attention of one query row per sequence over the 4-bit cache; origin: whose slot has a position (None: its own)."""
+    check(_lib.g2_attn_kv4(_p(q), q_stride, _p(cache), _p(out), out_stride, _p(origin), _p(lens), T_kv, n_seq, n_head, n_kv,
+                           max_seq, scale, _p(work)))
+
+
+def beam_work_bytes(groups, beams, V, n_out):
+    """Bytes of beam_select's workspace."""
+    return _lib.g2_beam_work_bytes(groups, beams, V, n_out)
+
+
+def beam_select(logits, score, done, eos, out_score, out_parent, out_id, out_done, groups, beams, V, n_out, work):
+    """The n_out best continuations of each group's beams: scores, beams, ids, whether they have ended."""
+    check(_lib.g2_beam_select(_p(logits), _p(score), _p(done), eos, _p(out_score), _p(out_parent), _p(out_id), _p(out_done),
+                              groups, beams, V, n_out, _p(work)))
+
+
+def beam_reorder(ids, ids_out, ids_stride, next_ids, origin, origin_out, origin_stride, parent, lens, T, groups, beams):
+    """The beams' ids and origins in their parents' order, with the step's ids and rows behind them."""
+    check(_lib.g2_beam_reorder(_p(ids), _p(ids_out), ids_stride, _p(next_ids), _p(origin), _p(origin_out), origin_stride,
+                               _p(parent), _p(lens), T, groups, beams))
 
 
 # ---------------------------------------------------------------- host-only

@@ -284,6 +284,102 @@ size_t g2_logits_work_bytes(int rows);
 int g2_apply_logit_rules(const float *logits, float *out, int *pick, int rows,
                          int V, const g2_logit_rules *rules, void *work);
 
+/* ---- several texts at once (no counterpart in the reference) ----------------
+ * Prompts of different lengths in one call, a 4-bit K/V cache that beams can
+ * share, and a step of beam search on the device.  Conventions as in the
+ * section before: no buffer of the library, arguments checked also before
+ * g2_init, outputs that overlap inputs refused except where a line allows it,
+ * device arrays of starts, lengths, positions and rows cut off or left out by
+ * the kernels. */
+
+/* Causal attention of whole prompts that stand one behind the other in q, k
+ * and v (the fused g2_attn_1q for every row): sequence s has the query rows
+ * q_start[s] .. q_start[s+1]-1 and the key rows k_start[s] .. k_start[s+1]-1,
+ * both lists n_seq + 1 ascending ints on the device (q_start == k_start is
+ * legal; NULL, for n_seq 1: all rows).  With nq query and nk key rows, query i
+ * sees the keys j <= i + nk - nq: its own prefix where nk == nq, also nk - nq
+ * keys that were there before where there are more; a row that sees no key
+ * gives zeros.  Rows outside all sequences are left as they were.  n_head
+ * heads of 64 dims, n_kv key heads (a divisor; head h uses key head h / (n_head
+ * / n_kv)).  Rows begin strides apart, in elements of dtype (G2_F32 or G2_F16,
+ * for q, k, v and out alike): a row of qkv products serves, its queries first.
+ * fp32 rows enter whole (products of magnitudes below 2^-102 may lose their
+ * last bits), sums are fp32; of fp16 rows the softmax's weights are rounded to
+ * fp16 for the second product.  A key with an infinity or NaN makes the rows
+ * that see it NaN, a value with one counts where it is seen. */
+int g2_attn_prompt(const void *q, int q_stride, const void *k, const void *v, int kv_stride,
+                   void *out, int out_stride, int dtype, const int *q_start, const int *k_start,
+                   int n_seq, int q_rows, int k_rows, int n_head, int n_kv, float scale);
+
+/* 4-bit K/V cache of n_seq sequences, n_kv key heads of 64 dims, max_seq
+ * positions: E2M1 codes (as g2_quantize_q4's) and a bf16 scale for each
+ * position, head and 32 dims, 36 bytes for a key or value instead of 256.
+ * Every position stands for itself: a sequence may be cut back to any length
+ * and written over from there.  One buffer, 16-byte aligned, no initial state:
+ * g2_kv4_bytes of it (0 if the sizes are not supported), in tiles of 32
+ * positions [n_seq][n_kv][ceil(max_seq/32)]:
+ *   codes  [K, V][32][32 bytes], an even dim in the low half of a byte
+ *   scales bf16 [K, V][32][2]
+ * scale = bf16(max |x| / 6) of 32 dims, code = the value nearest to x / scale
+ * (fp32), ties to the even code; 32 dims with an infinity, a NaN or a magnitude
+ * above 2^96 read back as NaN. */
+size_t g2_kv4_bytes(int n_seq, int n_kv, int max_seq);
+/* Appends rows of keys and values (dtype G2_F32 or G2_F16, n_kv heads of 64,
+ * stride elements from row to row): sequence s's are rows row_start[s] ..
+ * row_start[s+1]-1 of `rows` (device, as q_start above; NULL: rows / n_seq
+ * each), and go to positions p, p + 1, ..., p = pos[s], or start where pos is
+ * NULL.  Positions outside 0..max_seq-1 are left out. */
+int g2_kv4_append(const void *k, const void *v, int stride, int dtype, void *cache,
+                  const int *row_start, const int *pos, int start, int n_seq, int rows,
+                  int n_kv, int max_seq);
+/* The values at positions start .. start + T - 1 of every sequence, k and v
+ * [n_seq][T][64 n_kv] fp32.  A sequence's length is len[s] at most T_kv, or T_kv
+ * where len is NULL; rows at or behind it are left as they were.  origin, a
+ * device array [n_seq][max_seq], names the sequence whose slot holds a
+ * position (NULL: its own): beams share what they have in common.  A position
+ * whose origin is not in 0..n_seq-1 is not there. */
+int g2_kv4_read(const void *cache, float *k, float *v, const int *origin, const int *len,
+                int T_kv, int start, int T, int n_seq, int n_kv, int max_seq);
+/* Bytes of g2_attn_kv4's workspace (0 if the sizes are not supported). */
+size_t g2_kv4_work_bytes(int n_seq, int n_head);
+/* Attention of one query row per sequence over its cached positions
+ * (g2_attn_kv8 over this cache, with n_kv key heads as in g2_attn_prompt): rows,
+ * strides and lengths as there, origin as in g2_kv4_read.  No position: zeros.
+ * work: g2_kv4_work_bytes, 4-byte aligned, for this call alone while it runs. */
+int g2_attn_kv4(const float *q, int q_stride, const void *cache, float *out, int out_stride,
+                const int *origin, const int *len, int T_kv, int n_seq, int n_head, int n_kv,
+                int max_seq, float scale, float *work);
+
+/* Bytes of g2_beam_select's workspace (0 if the sizes are not supported). */
+size_t g2_beam_work_bytes(int groups, int beams, int V, int n_out);
+/* A step of beam search: for each group the n_out continuations of its beams
+ * with the greatest sums of log-probabilities, greatest first; of equal ones
+ * the lower beam's, then the lower id's first.  logits [groups * beams][V], score
+ * [groups * beams] the beams' sums so far; a continuation's is score + logit -
+ * log sum exp(logits), compared in 64 bits.  done (NULL: none) marks beams that
+ * have ended: such a beam goes on as it is, with id eos and its own score.
+ * out_score, out_parent (a beam of the group), out_id and out_done (NULL: not
+ * wanted; 1 where the beam had ended or the id is eos) are [groups * n_out].
+ * eos -1: no id ends a beam (done must be NULL).  A beam of score -infinity or
+ * NaN, or whose logits hold a NaN or +infinity, has no continuations; where there
+ * are fewer than n_out above -infinity, parent and id are -1, the score
+ * -infinity.  With n_out == beams and scores of 0, -infinity, -infinity ... one
+ * beam starts a group.  beams up to 32, n_out up to 64, V up to 262144, groups *
+ * beams up to 65536.  work: 8-byte aligned, for this call alone while it runs. */
+int g2_beam_select(const float *logits, const float *score, const int *done, int eos,
+                   float *out_score, int *out_parent, int *out_id, int *out_done,
+                   int groups, int beams, int V, int n_out, void *work);
+/* What beams carry along, after a selection of n_out == beams: row b of each
+ * group gets the first n ints of row parent[b] of the group and one more; n =
+ * len[group] at most T, or T where len is NULL (T below both strides).  ids gets
+ * next[b], its tokens; origin the row's own number group * beams + b, where
+ * g2_kv4_append puts the token's key and value.  Either table may be NULL, out
+ * may be the table itself; a row whose parent is outside 0..beams-1 is left as
+ * it was, and so are ints behind the new one. */
+int g2_beam_reorder(const int *ids, int *ids_out, int ids_stride, const int *next,
+                    const int *origin, int *origin_out, int origin_stride,
+                    const int *parent, const int *len, int T, int groups, int beams);
+
 /* ---- configuration, weights, model (main.c:272-331, 1137-1512, 1739-1904) -- */
 
 typedef struct {

@@ -1,0 +1,83 @@
+"""CPU check of the index arithmetic of the operators for several texts at once and of the host's choice of forms.
+
+tests/native/batch_addr.cpp compiles the kernels' own index functions (csrc/g2_batch_plan.h) with g++ and walks the
+cache's tiles, the pieces of work, the search of a row's sequence (in lists of starts, and in lists in no order, whose
+probes have to stay inside) and the keys that a row sees; a planted mistake must be caught.  No GPU is involved."""
+import ctypes as C
+import os
+import shutil
+import subprocess
+
+import pytest
+
+import g2hip
+import test_batch_gpu as gpu
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CSRC = os.path.join(ROOT, "gpt2-opencl-1.1_amd", "csrc")
+
+
+@pytest.fixture(scope="module")
+def walk(tmp_path_factory):
+    if not shutil.which("g++"):
+        pytest.skip("g++ not available")
+    out = str(tmp_path_factory.mktemp("batch") / "batch_addr")
+    subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-I" + CSRC, "-o", out, os.path.join(ROOT, "tests", "native", "batch_addr.cpp")],
+                   check=True)
+
+    def run(*args):
+        return subprocess.run([out, *map(str, args)], capture_output=True, text=True).stdout.strip()
+
+    return run
+
+
+@pytest.mark.parametrize("S,NKV,max_seq", [(1, 1, 1), (1, 3, 32), (2, 5, 33), (3, 25, 1000), (7, 12, 1024)])
+def test_cache(walk, S, NKV, max_seq):
+    assert walk("cache", S, NKV, max_seq) == "ok"
+    assert g2hip.kv4_bytes(S, NKV, max_seq) == S * NKV * -(-max_seq // 32) * 2304
+    assert walk("cache", S, NKV, max_seq, 1) != "ok"
+
+
+@pytest.mark.parametrize("n", [1, 7, 8, 9, 15, 16, 17, 100, 1023, 4001])
+def test_items(walk, n):
+    assert walk("items", n) == "ok"
+
+
+@pytest.mark.parametrize("n", [2, 3, 63, 64, 65, 66, 128, 129, 1000, 4096, 4097, 5000])
+def test_search(walk, n):
+    assert walk("search", n, n) == "ok"
+
+
+def test_rows(walk):
+    for seed in range(3):
+        assert walk("rows", seed) == "ok"
+
+
+def test_beam_workspace(walk):
+    for G, B, V, n in ((1, 1, 1, 1), (1, 4, 50257, 4), (16, 8, 50257, 8), (3, 7, 4097, 64), (2048, 32, 262144, 64)):
+        assert walk("beams", G * B, -(-V // 4096), n) == "ok"
+        assert g2hip.beam_work_bytes(G, B, V, n) >= G * B * -(-V // 4096) * 8 * (1 + n)
+
+
+def kv4_form(S, NH, NKV, T):
+    fn = g2hip._lib.g2i_kv4_form
+    fn.argtypes = [C.c_int] * 4 + [C.POINTER(C.c_int)] * 3
+    heads, chunks, span = C.c_int(), C.c_int(), C.c_int()
+    return fn(S, NH, NKV, T, C.byref(heads), C.byref(chunks), C.byref(span)), heads.value, chunks.value, span.value
+
+
+def test_attention_parts():
+    for NKV in (1, 2, 3, 5, 12, 25, 512):
+        for group in (1, 2, 3, 4, 5, 7, 8, 9, 16, 25):
+            for S in (1, 3, 48, 1000):
+                for T in (0, 1, 31, 32, 33, 256, 257, 700, 1024, 5000, 50001, 1 << 24):
+                    splits, heads, chunks, span = kv4_form(S, NKV * group, NKV, T)
+                    tiles = max(1, -(-T // 32))
+                    assert 1 <= splits <= 32 and (splits - 1) * span < tiles <= splits * span
+                    assert 1 <= heads <= 4 and (chunks - 1) * heads < group <= chunks * heads
+                    assert S * NKV * chunks * splits * 256 < 2 ** 32
+
+
+def test_every_form_of_the_attention_is_tested():
+    got = {(f[0] > 1, min(f[1], 3)) for f in (kv4_form(*c) for c in gpu.attention_cases())}
+    assert got >= {(False, 1), (False, 2), (False, 3), (True, 1), (True, 3)}
