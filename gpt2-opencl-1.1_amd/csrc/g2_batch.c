@@ -39,6 +39,14 @@ static int heads_check(const char *fn, int n_head, int n_kv)
 
 /* ---------------------------------------------------------- packed prompts */
 
+int g2i_prompt_form(int rows, int n_head, int n_kv, long *tiles)
+{
+    const long queries = (long)rows * (n_head / n_kv);
+    const int many = (queries + 127) / 128 * n_kv >= 256;
+    *tiles = (queries + (many ? 127 : 31)) / (many ? 128 : 32);
+    return many;
+}
+
 int g2_attn_prompt(const void *q, int q_stride, const void *k, const void *v, int kv_stride, void *out, int out_stride,
                    int dtype, const int *q_start, const int *k_start, int n_seq, int q_rows, int k_rows, int n_head,
                    int n_kv, float scale)
@@ -64,12 +72,15 @@ int g2_attn_prompt(const void *q, int q_stride, const void *k, const void *v, in
     if (g2i_overlap(out, no, q, span_of(q_rows, q_stride, nq, size)) || g2i_overlap(out, no, k, nkv) || g2i_overlap(out, no, v, nkv) ||
         (q_start && g2i_overlap(out, no, q_start, ns)) || (k_start && g2i_overlap(out, no, k_start, ns)))
         return g2i_err(G2_E_ARG, "%s: the output overlaps an input", fn);
-    const long tiles = g2b_row_tiles(q_rows);
-    if (!fits(tiles * n_head)) return g2i_err(G2_E_LIMIT, "%s: too many rows and heads for one call", fn);
+    long tiles;
+    const int many = g2i_prompt_form(q_rows, n_head, n_kv, &tiles);
+    if (!fits(tiles * n_kv) || (long)q_rows * (n_head / n_kv) > INT32_MAX - 128) return g2i_err(G2_E_LIMIT, "%s: too many rows and heads for one call", fn);
     if ((rc = ready())) return rc;
     g2_attn_prompt_args a = { q, k, v, out, q_start, k_start, q_rows > 1 ? q_stride : nq, k_rows > 1 ? kv_stride : nk,
                               q_rows > 1 ? out_stride : nq, n_seq, q_rows, k_rows, n_head, n_kv, (int)tiles, scale };
-    return g2i_launch(dtype == G2_F16 ? G2F_PROMPT_F16 : G2F_PROMPT_F32, (unsigned)(tiles * n_head), 1, 256, &a);
+    const int fid = many ? (dtype == G2_F16 ? G2F_PROMPT_TILE_F16 : G2F_PROMPT_TILE_F32)
+                         : (dtype == G2_F16 ? G2F_PROMPT_SPLIT_F16 : G2F_PROMPT_SPLIT_F32);
+    return g2i_launch(fid, (unsigned)(tiles * n_kv), 1, 256, &a);
 }
 
 /* -------------------------------------------------------------- 4-bit cache */

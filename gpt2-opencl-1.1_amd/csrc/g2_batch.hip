@@ -101,10 +101,10 @@ __device__ __forceinline__ int lanes_min_int(int v)
     return v;
 }
 
-__device__ __forceinline__ g2b_row keys_of_row(const g2_attn_prompt_args &a, int row0, int row, int lane)
+__device__ __forceinline__ g2b_row keys_of_row(const g2_attn_prompt_args &a, int row0, int row1, int row, int lane)
 {
     int s = 0, q0 = 0, q1 = a.q_rows, k0 = 0, k1 = a.k_rows;
-    if (a.q_start) s = seq_of_row(a.q_start, a.S, row0, row0 + G2B_ROWS - 1, row, lane);
+    if (a.q_start) s = seq_of_row(a.q_start, a.S, row0, row1, row, lane);
     const bool in = s >= 0 && s < a.S;
     const int i = in ? s : 0;
     if (a.q_start) { q0 = a.q_start[i]; q1 = a.q_start[i + 1]; }
@@ -112,219 +112,271 @@ __device__ __forceinline__ g2b_row keys_of_row(const g2_attn_prompt_args &a, int
     return g2b_row_keys(row, in, q0, q1, k0, k1, a.q_rows, a.k_rows);
 }
 
-/* One wave takes 32 rows of a head (column l % 32 of a lane) against 32 keys at
- * a time, products transposed: S^T = K Q^T and O^T = V^T P^T with 32x32x16
- * matrix instructions (lane l supplies A[l % 32][8 (l / 32) ..+7] and B[8 (l /
- * 32) ..+7][l % 32] and gets D[8 (r / 4) + 4 (l / 32) + r % 4][l % 32], r =
- * 0..15).  So a lane has its row's scores of 16 of the 32 keys; those of r =
- * 8u .. 8u + 7 are its operand of the second product's step u if V's operand
- * takes the keys in the same order, 16 u + 8 (e / 4) + 4 (l / 32) + e % 4. */
-template <typename T> struct prompt_tile;
-template <> struct prompt_tile<float> {
-    f32x4 k[8];
-    float v[2][2][8]; /* [dims 32 t ..][step][key] */
-};
-template <> struct prompt_tile<_Float16> {
-    f16x8 k[4];
-    _Float16 v[2][2][8];
+/* One wave takes 32 queries (column l % 32 of a lane) against 32 keys at a time,
+ * products transposed: S^T = K Q^T and O^T = V^T P^T with 32x32x16 matrix
+ * instructions (lane l supplies A[l % 32][8 (l / 32) ..+7] and B[8 (l / 32)
+ * ..+7][l % 32] and gets D[8 (r / 4) + 4 (l / 32) + r % 4][l % 32], r = 0..15).
+ * So a lane has its query's scores of 16 of the 32 keys; those of r = 8u .. 8u +
+ * 7 are its operand of the second product's step u if V's operand takes the
+ * keys in the same order, 16 u + 8 (e / 4) + 4 (l / 32) + e % 4.
+ *
+ * Queries are the rows' heads that share a key head, row by row: 32
+ * of them are fewer rows where heads are grouped, so less is masked. */
+template <typename T> struct prompt_op; /* an operand of one instruction, 8 values a lane */
+template <> struct prompt_op<float> { u32x4 p[3]; };
+template <> struct prompt_op<_Float16> { f16x8 p; };
+
+__device__ __forceinline__ f32x16 prompt_mma(const prompt_op<float> &a, const prompt_op<float> &b, const f32x16 &c) { return mma32_parts(a.p, b.p, c); }
+__device__ __forceinline__ f32x16 prompt_mma(const prompt_op<_Float16> &a, const prompt_op<_Float16> &b, const f32x16 &c) { return mma32h(a.p, b.p, c); }
+__device__ __forceinline__ void prompt_pack(const float (&v)[8], prompt_op<float> &o) { parts3(v, o.p); }
+__device__ __forceinline__ void prompt_pack(const _Float16 (&v)[8], prompt_op<_Float16> &o)
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o.p[e] = v[e];
+}
+
+/* A lane's query: its row's keys, its operands of the four steps of 16 dims, its
+ * state, where its output goes. */
+template <typename T> struct prompt_query {
+    g2b_row keys;
+    int row, head, k0, k1; /* k0 .. k1 - 1: what the wave's queries see together */
+    bool sees;
+    prompt_op<T> q[4];
+    f32x16 o[2]; /* dims 32 t + 8 (r / 4) + 4 (l / 32) + r % 4 */
+    float m, l;
 };
 
 template <typename T>
-__device__ __forceinline__ void prompt_load(prompt_tile<T> &x, const T *k, const T *v, unsigned stride, int n, int lane)
+__device__ __forceinline__ void prompt_start(prompt_query<T> &y, const g2_attn_prompt_args &a, int hk, int first, int lane)
 {
-    const unsigned sb = stride * (unsigned)sizeof(T), m = lane & 31, g = lane >> 5;
-    const char *kb = (const char *)k, *vb = (const char *)v;
-    /* (keys behind the n-th are the n-th again: the mask and zeros take care of them) */
-    const char *kp = kb + (size_t)min((int)m, n - 1) * sb + 8 * g * sizeof(T);
-    if constexpr (sizeof(T) == 4) {
+    const int group = a.NH / a.NKV, g = lane >> 5;
+    const int at = first + (lane & 31), row1 = (first + 31) / group;
+    y.row = at / group;
+    y.head = hk * group + at % group;
+    y.keys = keys_of_row(a, first / group, row1, y.row, lane);
+    y.sees = y.keys.there && y.keys.end > y.keys.lo;
+    y.k0 = __builtin_amdgcn_readfirstlane(lanes_min_int(y.sees ? y.keys.lo : INT_MAX));
+    y.k1 = __builtin_amdgcn_readfirstlane(-lanes_min_int(y.sees ? -y.keys.end : INT_MAX));
+    const T *qp = (const T *)a.q + (size_t)min(y.row, a.q_rows - 1) * a.q_stride + y.head * G2B_DH + 8 * g;
+    const float c = a.scale * 1.44269504f; /* scores in units of log 2; fp32 queries carry the factor */
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            x.k[2 * s] = *(const f32x4u *)(kp + 64 * s);
-            x.k[2 * s + 1] = *(const f32x4u *)(kp + 64 * s + 16);
+    for (int s = 0; s < 4; ++s) {
+        if constexpr (sizeof(T) == 2) y.q[s].p = *(const f16x8u *)(qp + 16 * s);
+        else {
+            const f32x4 x0 = *(const f32x4u *)(qp + 16 * s), x1 = *(const f32x4u *)(qp + 16 * s + 4);
+            const float x[8] = { x0[0] * c, x0[1] * c, x0[2] * c, x0[3] * c, x1[0] * c, x1[1] * c, x1[2] * c, x1[3] * c };
+            prompt_pack(x, y.q[s]);
         }
-    } else {
-#pragma unroll
-        for (int s = 0; s < 4; ++s) x.k[s] = *(const f16x8u *)(kp + 32 * s);
     }
-    if (n >= 32) {
-        const unsigned at = 4 * g * sb + m * (unsigned)sizeof(T);
+    y.o[0] = y.o[1] = f32x16{};
+    y.m = -INFINITY;
+    y.l = 0.f;
+}
+
+/* Scores of the keys j0 .. j0 + 31 to weights, with the state's maximum and sum. */
+template <typename T>
+__device__ __forceinline__ void prompt_weights(prompt_query<T> &y, f32x16 &s, int j0, float c, int g)
+{
+    constexpr bool F16 = sizeof(T) == 2;
+    if constexpr (F16) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int r = 0; r < 16; ++r) s[r] *= c;
+    }
+    if (wave_any(y.keys.lo > j0 || y.keys.end < j0 + 32)) { /* some query does not see all of them */
+        const int at = j0 + 4 * g - y.keys.lo, n = y.keys.end - y.keys.lo;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const char *p = vb + (size_t)(16 * u + 8 * (e / 4) + e % 4) * sb;
+        for (int r = 0; r < 16; ++r)
+            if ((unsigned)(at + 8 * (r / 4) + r % 4) >= (unsigned)n) s[r] = -INFINITY;
+    }
+    float top = y.m;
 #pragma unroll
-                for (int t = 0; t < 2; ++t) x.v[t][u][e] = *(const T *)(p + at + 32 * t * sizeof(T));
-            }
-    } else {
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
+    top = swap_max(top);
+    if (wave_any(top > y.m)) {
+        const float down = y.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(y.m - top);
+        y.l *= down;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int j = 16 * u + 8 * (e / 4) + 4 * (int)g + e % 4;
-                const char *p = vb + (size_t)min(j, n - 1) * sb + m * sizeof(T);
+            for (int r = 0; r < 16; ++r) y.o[t][r] *= down;
+        y.m = top;
+    }
+    /* (fp16 weights: 2^14 times the weight, so that small ones keep their bits) */
+    const float base = (top == -INFINITY ? 0.f : top) - (F16 ? 14.f : 0.f);
+    float sum = 0.f;
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const T y = *(const T *)(p + 32 * t * sizeof(T));
-                    x.v[t][u][e] = j < n ? y : (T)0.f;
-                }
+    for (int r = 0; r < 16; ++r) {
+        s[r] = __builtin_amdgcn_exp2f(s[r] - base);
+        sum += s[r];
+    }
+    y.l += sum;
+}
+
+/* The operand of the weights of step u. */
+__device__ __forceinline__ void prompt_weight_op(const f32x16 &s, int u, prompt_op<float> &p)
+{
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = s[8 * u + e];
+    parts3(x, p.p);
+}
+__device__ __forceinline__ void prompt_weight_op(const f32x16 &s, int u, prompt_op<_Float16> &p)
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p.p[e] = (_Float16)s[8 * u + e];
+}
+
+/* Whether one of eight values is not finite; such values are then 0: they must not
+ * meet the weights 0 of queries that do not see them.  prompt_odd adds them to
+ * the queries that do. */
+template <typename T> __device__ __forceinline__ float prompt_look(const T (&v)[8], float z)
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z = fmaf((float)v[e], 0.f, z);
+    return z;
+}
+template <typename T> __device__ __forceinline__ void prompt_clean(T (&v)[8])
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = __builtin_isfinite((float)v[e]) ? v[e] : (T)0.f;
+}
+template <typename T>
+__device__ __forceinline__ void prompt_odd(prompt_query<T> &y, const T *v, long stride, int j0, int n, int g)
+{
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+        const bool seen = j0 + i >= y.keys.lo && j0 + i < y.keys.end;
+        const T *p = v + (size_t)(j0 + i) * stride + 4 * g;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float x = (float)p[32 * t + 8 * (r / 4) + r % 4];
+                if (seen && !__builtin_isfinite(x)) y.o[t][r] += x;
             }
     }
 }
 
-template <typename T, int KW>
-__device__ void prompt_impl(const g2_attn_prompt_args &a)
+template <typename T> __device__ __forceinline__ void prompt_store(T *p, const f32x4 &y)
 {
-    constexpr bool F16 = sizeof(T) == 2;
-    __shared__ float red[KW][34][64];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
-    const long item = g2b_item(blockIdx.x, (long)a.tiles * a.NH);
-    const int h = (int)(item / a.tiles), tile = a.tiles - 1 - (int)(item % a.tiles); /* (long rows first) */
-    const int row0 = tile * G2B_ROWS, row = row0 + (lane & 31);
-    const g2b_row mine = keys_of_row(a, row0, row, lane);
-    const bool sees = mine.there && mine.end > mine.lo;
-    const int k0 = __builtin_amdgcn_readfirstlane(lanes_min_int(sees ? mine.lo : INT_MAX));
-    const int k1 = __builtin_amdgcn_readfirstlane(-lanes_min_int(sees ? -mine.end : INT_MAX));
-    const float c = a.scale * 1.44269504f;
-    /* the queries, with the factor in fp32 rows' own values */
-    u32x4 q3[4][3];
-    f16x8 qh[4];
-    {
-        const T *qp = (const T *)a.q + (size_t)min(row, a.q_rows - 1) * a.q_stride + h * G2B_DH + 8 * g;
+    if constexpr (sizeof(T) == 2) *(f16x4u *)p = f16x4u{ (_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3] };
+    else *(f32x4u *)p = y;
+}
+
+/* Eight values of a key's dims, of a dim's keys (in the second product's order):
+ * keys from the n-th on are the n-th again, and 0 among the values. */
+template <typename T> __device__ __forceinline__ void prompt_load_k(T (&x)[8], const T *p)
+{
+    if constexpr (sizeof(T) == 4) {
+        const f32x4 a = *(const f32x4u *)p, b = *(const f32x4u *)(p + 4);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            if constexpr (F16) qh[s] = *(const f16x8u *)(qp + 16 * s);
-            else {
-                const f32x4 x0 = *(const f32x4u *)(qp + 16 * s), x1 = *(const f32x4u *)(qp + 16 * s + 4);
-                const float x[8] = { x0[0] * c, x0[1] * c, x0[2] * c, x0[3] * c, x1[0] * c, x1[1] * c, x1[2] * c, x1[3] * c };
-                parts3(x, q3[s]);
-            }
+        for (int e = 0; e < 4; ++e) { x[e] = a[e]; x[4 + e] = b[e]; }
+    } else {
+        const f16x8 a = *(const f16x8u *)p;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = a[e];
+    }
+}
+/* (rows: the first key's, the same in every lane; at: the lane's dim and its key 4 (l / 32) in elements) */
+template <typename T>
+__device__ __forceinline__ void prompt_load_v(T (&x)[8], const T *rows, unsigned dim, int key0, long stride, int n)
+{
+    if (n >= 32) {
+        const unsigned at = (unsigned)key0 * (unsigned)stride + dim;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = (rows + (size_t)(8 * (e / 4) + e % 4) * stride)[at];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int j = key0 + 8 * (e / 4) + e % 4;
+            const T v = rows[(size_t)min(j, n - 1) * stride + dim];
+            x[e] = j < n ? v : (T)0.f;
         }
     }
-    f32x16 o[2] = {};
-    float m = -INFINITY, l = 0.f;
-    const int f = h / (a.NH / a.NKV) * G2B_DH;
-    const T *kp = (const T *)a.k + f, *vp = (const T *)a.v + f;
-    prompt_tile<T> next;
-    const int first = k0 + 32 * w;
-    if (first < k1) prompt_load(next, kp + (size_t)first * a.kv_stride, vp + (size_t)first * a.kv_stride, (unsigned)a.kv_stride, k1 - first, lane);
-    for (int j0 = first; j0 < k1; j0 += 32 * KW) {
-        prompt_tile<T> x = next;
+}
+
+/* ---- few queries: a work-group takes 32 of them, its four waves every fourth 32
+ * keys each, whose rows they read as the operands that they are (a key's dims
+ * 16 bytes at a time, a value's dims side by side, so that eight loads are
+ * eight keys of a dim); the waves' states meet at the end. */
+template <typename T>
+__device__ void prompt_split_impl(const g2_attn_prompt_args &a)
+{
+    constexpr int KW = 4;
+    __shared__ float red[KW][34][64];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
+    const long item = g2b_item(blockIdx.x, (long)a.tiles * a.NKV);
+    const int hk = (int)(item / a.tiles), tile = a.tiles - 1 - (int)(item % a.tiles); /* (long rows first) */
+    prompt_query<T> y;
+    prompt_start(y, a, hk, tile * 32, lane);
+    const float c = a.scale * 1.44269504f;
+    const long stride = a.kv_stride;
+    const T *kp = (const T *)a.k + hk * G2B_DH, *vp = (const T *)a.v + hk * G2B_DH;
+    T k[4][8], v[2][2][8];
+    auto load_k = [&](int j0) {
+        const T *p = kp + (size_t)j0 * stride + (size_t)min(lane & 31, y.k1 - j0 - 1) * stride + 8 * g;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) prompt_load_k(k[s], p + 16 * s);
+    };
+    auto load_v = [&](int j0) {
+        const int n = y.k1 - j0;
+        const T *p = vp + (size_t)j0 * stride;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (n >= 32) prompt_load_v(v[t][u], p + (size_t)(16 * u) * stride, 32 * t + (lane & 31), 4 * g, stride, 32);
+                else prompt_load_v(v[t][u], p, 32 * t + (lane & 31), 16 * u + 4 * g, stride, n);
+            }
+    };
+    int j0 = y.k0 < y.k1 ? y.k0 + 32 * w : y.k1;
+    if (j0 < y.k1) { load_k(j0); load_v(j0); }
+    for (; j0 < y.k1; j0 += 32 * KW) {
         const int j1 = j0 + 32 * KW;
-        if (j1 < k1) prompt_load(next, kp + (size_t)j1 * a.kv_stride, vp + (size_t)j1 * a.kv_stride, (unsigned)a.kv_stride, k1 - j1, lane);
         f32x16 s = {};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if constexpr (F16) s = mma32h(x.k[i], qh[i], s);
-            else {
-                const f32x4 y0 = x.k[2 * i], y1 = x.k[2 * i + 1];
-                const float y[8] = { y0[0], y0[1], y0[2], y0[3], y1[0], y1[1], y1[2], y1[3] };
-                u32x4 k3[3];
-                parts3(y, k3);
-                s = mma32_parts(k3, q3[i], s);
-            }
+            prompt_op<T> x;
+            prompt_pack(k[i], x);
+            s = prompt_mma(x, y.q[i], s);
         }
-        float top = m;
-        if constexpr (F16) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] *= c;
-        }
-        if (wave_any(mine.lo > j0 || mine.end < j0 + 32)) { /* some row does not see all of them */
-            const int at = j0 + 4 * g - mine.lo, n = mine.end - mine.lo;
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if ((unsigned)(at + 8 * (r / 4) + r % 4) >= (unsigned)n) s[r] = -INFINITY;
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
-        top = swap_max(top);
-        /* (fp16 weights: 2^14 times the weight, so that small ones keep their bits) */
-        const float base = (top == -INFINITY ? 0.f : top) - (F16 ? 14.f : 0.f);
-        if (wave_any(top > m)) {
-            const float down = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-            l *= down;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[t][r] *= down;
-            m = top;
-        }
-        float sum = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[r] = __builtin_amdgcn_exp2f(s[r] - base);
-            sum += s[r];
-        }
-        l += sum;
-        /* a value that is not finite must not meet the weights 0 of rows that do not see it */
+        if (j1 < y.k1) load_k(j1);
+        prompt_weights(y, s, j0, c, g);
         float z = 0.f;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) z = fmaf((float)x.v[t][u][e], 0.f, z);
+            for (int u = 0; u < 2; ++u) z = prompt_look(v[t][u], z);
         if (wave_any(z != 0.f)) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (!__builtin_isfinite((float)x.v[t][u][e])) x.v[t][u][e] = (T)0.f;
-            const int n = min(32, k1 - j0);
-#pragma unroll 1
-            for (int i = 0; i < n; ++i) {
-                const bool seen = j0 + i >= mine.lo && j0 + i < mine.end;
-                const T *p = vp + (size_t)(j0 + i) * a.kv_stride + 4 * g;
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float y = (float)p[32 * t + 8 * (r / 4) + r % 4];
-                        if (seen && !__builtin_isfinite(y)) o[t][r] += y;
-                    }
-            }
+                for (int u = 0; u < 2; ++u) prompt_clean(v[t][u]);
+            prompt_odd(y, vp, stride, j0, min(32, y.k1 - j0), g);
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            if constexpr (F16) {
-                f16x8 ph;
+            prompt_op<T> p, x;
+            prompt_weight_op(s, u, p);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) ph[e] = (_Float16)s[8 * u + e];
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    f16x8 vh;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) vh[e] = x.v[t][u][e];
-                    o[t] = mma32h(vh, ph, o[t]);
-                }
-            } else {
-                float p[8];
-                u32x4 p3[3], v3[3];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) p[e] = s[8 * u + e];
-                parts3(p, p3);
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    parts3(x.v[t][u], v3);
-                    o[t] = mma32_parts(v3, p3, o[t]);
-                }
+            for (int t = 0; t < 2; ++t) {
+                prompt_pack(v[t][u], x);
+                y.o[t] = prompt_mma(x, p, y.o[t]);
             }
         }
+        if (j1 < y.k1) load_v(j1);
     }
-    l = swap_sum(l);
+    y.l = swap_sum(y.l);
     /* the waves' parts meet; wave w writes the dims of its share of the registers */
-    red[w][0][lane] = m;
-    red[w][1][lane] = l;
+    red[w][0][lane] = y.m;
+    red[w][1][lane] = y.l;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) red[w][2 + 16 * t + r][lane] = o[t][r];
+        for (int r = 0; r < 16; ++r) red[w][2 + 16 * t + r][lane] = y.o[t][r];
     __syncthreads();
-    if (!mine.there) return;
-    float top = -INFINITY, part[KW];
-    l = 0.f;
+    if (!y.keys.there) return;
+    float top = -INFINITY, part[KW], l = 0.f;
 #pragma unroll
     for (int i = 0; i < KW; ++i) top = fmaxf(top, red[i][0][lane]);
 #pragma unroll
@@ -332,24 +384,124 @@ __device__ void prompt_impl(const g2_attn_prompt_args &a)
         part[i] = kv8_factor(red[i][0][lane], top);
         l = fmaf(red[i][1][lane], part[i], l);
     }
-    T *out = (T *)a.out + (size_t)row * a.out_stride + h * G2B_DH + 4 * g;
+    T *out = (T *)a.out + (size_t)y.row * a.out_stride + y.head * G2B_DH + 4 * g;
 #pragma unroll
     for (int i = 0; i < 8 / KW; ++i) {
         const int q = w * (8 / KW) + i;
-        f32x4 y = {};
+        f32x4 x = {};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
 #pragma unroll
-            for (int j = 0; j < KW; ++j) y[e] = fmaf(red[j][2 + 4 * q + e][lane], part[j], y[e]);
-            y[e] = sees ? y[e] / l : 0.f;
+            for (int j = 0; j < KW; ++j) x[e] = fmaf(red[j][2 + 4 * q + e][lane], part[j], x[e]);
+            x[e] = y.sees ? x[e] / l : 0.f;
         }
-        T *p = out + 32 * (q / 4) + 8 * (q % 4);
-        if constexpr (F16) *(f16x4u *)p = f16x4u{ (_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3] };
-        else *(f32x4u *)p = y;
+        prompt_store(out + 32 * (q / 4) + 8 * (q % 4), x);
     }
 }
-G2K void g2k_prompt_f32(const g2_attn_prompt_args a) { prompt_impl<float, 4>(a); }
-G2K void g2k_prompt_f16(const g2_attn_prompt_args a) { prompt_impl<_Float16, 4>(a); }
+extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g2k_prompt_split_f32(const g2_attn_prompt_args a) { prompt_split_impl<float>(a); }
+extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g2k_prompt_split_f16(const g2_attn_prompt_args a) { prompt_split_impl<_Float16>(a); }
+
+/* ---- many queries: a work-group takes 128 of them, 32 a wave, and its waves
+ * read each 32 keys and values together, once, as operands in LDS: unit (part,
+ * step, lane) of 16 bytes is what the lane reads of it, so that reads and
+ * writes are both one row of units.  Two stages: the next keys are on their
+ * way from memory while the products of these run, and one barrier stands
+ * between. */
+template <typename T>
+__device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
+{
+    constexpr int P = sizeof(T) == 4 ? 3 : 1, UNITS = P * 256; /* of keys, and of values */
+    __shared__ u32x4 lds[2][2 * UNITS];
+    __shared__ int range[4][2], odd[2][4];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
+    const long item = g2b_item(blockIdx.x, (long)a.tiles * a.NKV);
+    const int hk = (int)(item / a.tiles), tile = a.tiles - 1 - (int)(item % a.tiles); /* (long rows first) */
+    prompt_query<T> y;
+    prompt_start(y, a, hk, tile * 128 + 32 * w, lane);
+    if (lane == 0) { range[w][0] = y.k0; range[w][1] = y.k1; }
+    __syncthreads();
+    const int k0 = __builtin_amdgcn_readfirstlane(min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0])));
+    const int k1 = __builtin_amdgcn_readfirstlane(max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1])));
+    const float c = a.scale * 1.44269504f;
+    const long stride = a.kv_stride;
+    const T *kp = (const T *)a.k + hk * G2B_DH, *vp = (const T *)a.v + hk * G2B_DH;
+    /* this thread's share: dims 8 (tid / 32) ..+7 of key tid % 32; of dim lane, the keys that lanes of half w % 2 take in step w / 2 */
+    T k[8], v[8];
+    auto load = [&](int j0) {
+        const int n = k1 - j0;
+        prompt_load_k(k, kp + (size_t)j0 * stride + (size_t)min(tid & 31, n - 1) * stride + 8 * (tid >> 5));
+        if (n >= 32) prompt_load_v(v, vp + (size_t)(j0 + 16 * (w >> 1) + 4 * (w & 1)) * stride, lane, 0, stride, 32);
+        else prompt_load_v(v, vp + (size_t)j0 * stride, lane, 16 * (w >> 1) + 4 * (w & 1), stride, n);
+    };
+    auto stage = [&](int b) {
+        const bool any = wave_any(prompt_look(v, 0.f) != 0.f);
+        if (any) prompt_clean(v);
+        if (lane == 0) odd[b][w] = any;
+        prompt_op<T> x, z;
+        prompt_pack(k, x);
+        prompt_pack(v, z);
+        u32x4 *kd = lds[b] + tid, *vd = lds[b] + UNITS + (lane >> 5) * 128 + (w >> 1) * 64 + (w & 1) * 32 + (lane & 31);
+        if constexpr (P == 3) {
+#pragma unroll
+            for (int i = 0; i < 3; ++i) { kd[256 * i] = x.p[i]; vd[256 * i] = z.p[i]; }
+        } else {
+            *kd = __builtin_bit_cast(u32x4, x.p);
+            *vd = __builtin_bit_cast(u32x4, z.p);
+        }
+    };
+    auto fetch = [&](const u32x4 *p, prompt_op<T> &x) {
+        if constexpr (P == 3) {
+#pragma unroll
+            for (int i = 0; i < 3; ++i) x.p[i] = p[256 * i];
+        } else x.p = __builtin_bit_cast(f16x8, *p);
+    };
+    if (k0 < k1) {
+        load(k0);
+        stage(0);
+    }
+    __syncthreads();
+    int b = 0;
+    for (int j0 = k0; j0 < k1; j0 += 32, b ^= 1) {
+        const bool more = j0 + 32 < k1;
+        if (more) load(j0 + 32);
+        if (j0 < y.k1 && j0 + 32 > y.k0) { /* (the wave's queries see some of them) */
+            const u32x4 *kd = lds[b] + lane, *vd = lds[b] + UNITS + lane;
+            f32x16 s = {};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                prompt_op<T> x;
+                fetch(kd + 64 * i, x);
+                s = prompt_mma(x, y.q[i], s);
+            }
+            prompt_weights(y, s, j0, c, g);
+            if (__builtin_amdgcn_readfirstlane(odd[b][0] | odd[b][1] | odd[b][2] | odd[b][3])) prompt_odd(y, vp, stride, j0, min(32, k1 - j0), g);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                prompt_op<T> p, x;
+                prompt_weight_op(s, u, p);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    fetch(vd + 128 * t + 64 * u, x);
+                    y.o[t] = prompt_mma(x, p, y.o[t]);
+                }
+            }
+        }
+        if (more) stage(b ^ 1);
+        __syncthreads();
+    }
+    if (!y.keys.there) return;
+    const float l = swap_sum(y.l);
+    T *out = (T *)a.out + (size_t)y.row * a.out_stride + y.head * G2B_DH + 4 * g;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        f32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = y.sees ? y.o[q / 4][4 * (q % 4) + e] / l : 0.f;
+        prompt_store(out + 32 * (q / 4) + 8 * (q % 4), x);
+    }
+}
+extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g2k_prompt_tile_f32(const g2_attn_prompt_args a) { prompt_tile_impl<float>(a); }
+extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g2k_prompt_tile_f16(const g2_attn_prompt_args a) { prompt_tile_impl<_Float16>(a); }
 
 /* ======================================================================
  * 4-bit K/V cache: each position, head and 32 dims on their own, codes and

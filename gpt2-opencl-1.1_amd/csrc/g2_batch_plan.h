@@ -43,9 +43,7 @@ G2B_FN unsigned g2b_scale_at(int kv, int p) { return G2B_SCALES + (unsigned)(kv 
 #define G2B_SPLITS 32
 #define G2B_PART_FLOATS (2 + G2B_DH)
 
-/* ---- packed prompts: a work-group takes G2B_ROWS packed rows of a head, whatever sequences they are of */
-#define G2B_ROWS 32
-G2B_FN long g2b_row_tiles(long rows) { return (rows + G2B_ROWS - 1) / G2B_ROWS; }
+/* ---- packed prompts */
 
 /* Search of a list of `left` ascending values from its entry lo on, 64 probes at a
  * time: probe `lane`'s entry, counted from lo, and what c probes at or below

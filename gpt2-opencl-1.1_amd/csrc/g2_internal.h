@@ -121,7 +121,10 @@ extern "C" {
     X(KV8_ATTN1, "g2k_kv8_attn1") X(KV8_ATTN4, "g2k_kv8_attn4")               \
     X(KV8_ATTN8, "g2k_kv8_attn8") X(KV8_JOIN, "g2k_kv8_join")                 \
     X(LOGITS, "g2k_logits") X(LOGITS_WIDE, "g2k_logits_wide")                 \
-    X(PROMPT_F32, "g2k_prompt_f32") X(PROMPT_F16, "g2k_prompt_f16")           \
+    X(PROMPT_SPLIT_F32, "g2k_prompt_split_f32")                               \
+    X(PROMPT_SPLIT_F16, "g2k_prompt_split_f16")                               \
+    X(PROMPT_TILE_F32, "g2k_prompt_tile_f32")                                 \
+    X(PROMPT_TILE_F16, "g2k_prompt_tile_f16")                                 \
     X(KV4_APPEND_F32, "g2k_kv4_append_f32")                                   \
     X(KV4_APPEND_F16, "g2k_kv4_append_f16") X(KV4_READ, "g2k_kv4_read")       \
     X(KV4_ATTN1, "g2k_kv4_attn1") X(KV4_ATTN2, "g2k_kv4_attn2")               \
@@ -212,6 +215,10 @@ int g2i_kv8_form(long heads, int T_kv, int *span, int *waves);
 
 /* Whether g2_apply_logit_rules takes its wide form, and the slices of a row. */
 int g2i_logits_form(int rows, int V, int *parts);
+
+/* Whether g2_attn_prompt takes the form for many queries (128 to a work-group,
+ * else 32), and the work-groups of a key head. */
+int g2i_prompt_form(int rows, int n_head, int n_kv, long *tiles);
 
 /* g2_attn_kv4's parts of a key head's positions, tiles to a part, query heads to
  * a pass over them and passes to a key head. */
