@@ -48,21 +48,22 @@ __device__ __forceinline__ int seq_of_row(const int *start, int n, int row0, int
  * Causal attention of packed prompts
  * ==================================================================== */
 
-/* Eight values as three bf16 parts each, packed in twos: v = p1 + p2 + p3, each
- * 8 significant bits of what is left, rounded to nearest (so that the products
- * left out, below 2^-23, have either sign); exactly above 2^-102. */
+/* Eight values as three bf16 parts each, packed in twos: v = p1 + p2 + p3, 8
+ * significant bits each, exactly above 2^-102.  The first is cut off (rounded, it
+ * would leave the range of finite values at its end), the others are rounded to
+ * nearest, so that the products left out, below 2^-21, have either sign. */
 __device__ __forceinline__ void parts3(const float (&v)[8], u32x4 (&o)[3])
 {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        f32x2 r = { v[2 * e], v[2 * e + 1] };
-#pragma unroll
-        for (int p = 0; p < 3; ++p) {
-            const unsigned w = __builtin_bit_cast(unsigned, __builtin_convertvector(r, bf16x2));
-            o[p][e] = w;
-            r[0] -= __uint_as_float(w << 16);
-            r[1] -= __uint_as_float(w & 0xffff0000u);
-        }
+        const unsigned a = __float_as_uint(v[2 * e]), b = __float_as_uint(v[2 * e + 1]);
+        o[0][e] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+        f32x2 r = { v[2 * e] - __uint_as_float(a & 0xffff0000u), v[2 * e + 1] - __uint_as_float(b & 0xffff0000u) };
+        const unsigned w = __builtin_bit_cast(unsigned, __builtin_convertvector(r, bf16x2));
+        o[1][e] = w;
+        r[0] -= __uint_as_float(w << 16);
+        r[1] -= __uint_as_float(w & 0xffff0000u);
+        o[2][e] = __builtin_bit_cast(unsigned, __builtin_convertvector(r, bf16x2));
     }
 }
 
@@ -74,7 +75,7 @@ __device__ __forceinline__ f32x16 mma32h(const f16x8 &a, const f16x8 &b, const f
 {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
-/* c + a . b, the six products of parts that are above 2^-24 of it, small ones first */
+/* c + a . b, the six products of parts that are above 2^-21 of it, small ones first */
 __device__ __forceinline__ f32x16 mma32_parts(const u32x4 (&a)[3], const u32x4 (&b)[3], f32x16 c)
 {
     constexpr int pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0};
@@ -135,6 +136,50 @@ __device__ __forceinline__ void prompt_pack(const _Float16 (&v)[8], prompt_op<_F
     for (int e = 0; e < 8; ++e) o.p[e] = v[e];
 }
 
+/* Eight values of a row's dims, at any element's address. */
+template <typename T> __device__ __forceinline__ void prompt_load_k(T (&x)[8], const T *p)
+{
+    if constexpr (sizeof(T) == 4) {
+        const f32x4 a = *(const f32x4u *)p, b = *(const f32x4u *)(p + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { x[e] = a[e]; x[4 + e] = b[e]; }
+    } else {
+        const f16x8 a = *(const f16x8u *)p;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = a[e];
+    }
+}
+
+/* The rows of keys or values from j0 on, up to 32 and below k1, as a buffer:
+ * what is read behind the last of them is 0. */
+template <typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t prompt_rows(const T *p, int j0, int k1, long stride)
+{
+    const int n = min(32, k1 - j0);
+    const unsigned bytes = ((unsigned)(n - 1) * (unsigned)stride + G2B_DH) * (unsigned)sizeof(T);
+    return __builtin_amdgcn_make_buffer_rsrc((void *)(p + (size_t)j0 * stride), (short)0, bytes, 0x00020000);
+}
+/* A dim's values of the eight keys that a lane of half g takes in step u (in the
+ * second product's order): where its values are, from the buffer's begin. */
+template <typename T> __device__ __forceinline__ void prompt_value_at(unsigned (&at)[8], int u, int g, int dim, long stride)
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) at[e] = ((unsigned)(16 * u + 8 * (e / 4) + 4 * g + e % 4) * (unsigned)stride + (unsigned)dim) * (unsigned)sizeof(T);
+}
+template <typename T> __device__ __forceinline__ void prompt_load_v(T (&x)[8], __amdgpu_buffer_rsrc_t rows, const unsigned (&at)[8], int more)
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if constexpr (sizeof(T) == 4) x[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows, (int)at[e] + more, 0, 0));
+        else x[e] = __builtin_bit_cast(_Float16, __builtin_amdgcn_raw_buffer_load_b16(rows, (int)at[e] + more, 0, 0));
+    }
+}
+
+/* Scores in units of log 2; not 0, which would make NaN of the masked ones. */
+__device__ __forceinline__ float prompt_unit(float scale) { return fmaxf(fabsf(scale) * 1.44269504f, 0x1p-126f); }
+/* The weight of a state of maximum m beside one of maximum top (an empty one's is -infinity). */
+__device__ __forceinline__ float prompt_factor(float m, float top, float c) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * c); }
+
 /* A lane's query: its row's keys, its operands of the four steps of 16 dims, its
  * state, where its output goes. */
 template <typename T> struct prompt_query {
@@ -158,42 +203,47 @@ __device__ __forceinline__ void prompt_start(prompt_query<T> &y, const g2_attn_p
     y.k0 = __builtin_amdgcn_readfirstlane(lanes_min_int(y.sees ? y.keys.lo : INT_MAX));
     y.k1 = __builtin_amdgcn_readfirstlane(-lanes_min_int(y.sees ? -y.keys.end : INT_MAX));
     const T *qp = (const T *)a.q + (size_t)min(y.row, a.q_rows - 1) * a.q_stride + y.head * G2B_DH + 8 * g;
-    const float c = a.scale * 1.44269504f; /* scores in units of log 2; fp32 queries carry the factor */
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-        if constexpr (sizeof(T) == 2) y.q[s].p = *(const f16x8u *)(qp + 16 * s);
-        else {
-            const f32x4 x0 = *(const f32x4u *)(qp + 16 * s), x1 = *(const f32x4u *)(qp + 16 * s + 4);
-            const float x[8] = { x0[0] * c, x0[1] * c, x0[2] * c, x0[3] * c, x1[0] * c, x1[1] * c, x1[2] * c, x1[3] * c };
-            prompt_pack(x, y.q[s]);
-        }
+        T x[8];
+        prompt_load_k(x, qp + 16 * s);
+        if (a.scale < 0.f)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = -x[e]; /* (the unit is positive: prompt_unit) */
+        prompt_pack(x, y.q[s]);
     }
+    /* (loaded now: a wait for them inside the loop would wait for the keys, too) */
+    if constexpr (sizeof(T) == 2)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) asm volatile("" : "+v"(y.q[s].p));
     y.o[0] = y.o[1] = f32x16{};
     y.m = -INFINITY;
     y.l = 0.f;
 }
 
-/* Scores of the keys j0 .. j0 + 31 to weights, with the state's maximum and sum. */
+/* Scores of the keys j0 .. j0 + 31 to weights, with the state's maximum and sum.
+ * The state follows the maximum only where a query's grew by more than 2^8: then
+ * the sums are scaled down to it, else weights up to 2^8 are as good (fp16
+ * weights are 2^6 times that, so that small ones keep their bits: 2^14 at most,
+ * exact down to 2^-20 of the largest). */
 template <typename T>
 __device__ __forceinline__ void prompt_weights(prompt_query<T> &y, f32x16 &s, int j0, float c, int g)
 {
     constexpr bool F16 = sizeof(T) == 2;
-    if constexpr (F16) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] *= c;
-    }
     if (wave_any(y.keys.lo > j0 || y.keys.end < j0 + 32)) { /* some query does not see all of them */
         const int at = j0 + 4 * g - y.keys.lo, n = y.keys.end - y.keys.lo;
 #pragma unroll
         for (int r = 0; r < 16; ++r)
             if ((unsigned)(at + 8 * (r / 4) + r % 4) >= (unsigned)n) s[r] = -INFINITY;
     }
-    float top = y.m;
+    float top = s[0];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
     top = swap_max(top);
-    if (wave_any(top > y.m)) {
-        const float down = y.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(y.m - top);
+    const bool grew = top * c > y.m * c + 8.f; /* (an empty state's maximum is -infinity) */
+    if (wave_any(grew)) {
+        if (!grew) top = y.m; /* (each query by itself: its result does not depend on its neighbours') */
+        const float down = prompt_factor(y.m, top, c);
         y.l *= down;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -201,12 +251,20 @@ __device__ __forceinline__ void prompt_weights(prompt_query<T> &y, f32x16 &s, in
             for (int r = 0; r < 16; ++r) y.o[t][r] *= down;
         y.m = top;
     }
-    /* (fp16 weights: 2^14 times the weight, so that small ones keep their bits) */
-    const float base = (top == -INFINITY ? 0.f : top) - (F16 ? 14.f : 0.f);
+    /* The exponent as one operation on the score: what the rounding of m c adds is the
+     * same factor for all weights of a query, and has to be a small one. */
+    const float up = F16 ? 6.f : 0.f, mc = y.m == -INFINITY ? 0.f : y.m * c, base = up - mc;
+    const bool far = !(fabsf(mc) < 0x1p28f);
     float sum = 0.f;
+    if (wave_any(far)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = far ? fmaf(s[r] - y.m, c, up) : fmaf(s[r], c, base);
+    } else
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, base);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        s[r] = __builtin_amdgcn_exp2f(s[r] - base);
+        s[r] = __builtin_amdgcn_exp2f(s[r]);
         sum += s[r];
     }
     y.l += sum;
@@ -263,38 +321,6 @@ template <typename T> __device__ __forceinline__ void prompt_store(T *p, const f
     else *(f32x4u *)p = y;
 }
 
-/* Eight values of a key's dims, of a dim's keys (in the second product's order):
- * keys from the n-th on are the n-th again, and 0 among the values. */
-template <typename T> __device__ __forceinline__ void prompt_load_k(T (&x)[8], const T *p)
-{
-    if constexpr (sizeof(T) == 4) {
-        const f32x4 a = *(const f32x4u *)p, b = *(const f32x4u *)(p + 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { x[e] = a[e]; x[4 + e] = b[e]; }
-    } else {
-        const f16x8 a = *(const f16x8u *)p;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = a[e];
-    }
-}
-/* (rows: the first key's, the same in every lane; at: the lane's dim and its key 4 (l / 32) in elements) */
-template <typename T>
-__device__ __forceinline__ void prompt_load_v(T (&x)[8], const T *rows, unsigned dim, int key0, long stride, int n)
-{
-    if (n >= 32) {
-        const unsigned at = (unsigned)key0 * (unsigned)stride + dim;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = (rows + (size_t)(8 * (e / 4) + e % 4) * stride)[at];
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int j = key0 + 8 * (e / 4) + e % 4;
-            const T v = rows[(size_t)min(j, n - 1) * stride + dim];
-            x[e] = j < n ? v : (T)0.f;
-        }
-    }
-}
-
 /* ---- few queries: a work-group takes 32 of them, its four waves every fourth 32
  * keys each, whose rows they read as the operands that they are (a key's dims
  * 16 bytes at a time, a value's dims side by side, so that eight loads are
@@ -305,29 +331,29 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
     constexpr int KW = 4;
     __shared__ float red[KW][34][64];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
-    const long item = g2b_item(blockIdx.x, (long)a.tiles * a.NKV);
-    const int hk = (int)(item / a.tiles), tile = a.tiles - 1 - (int)(item % a.tiles); /* (long rows first) */
+    int hk;
+    long tile;
+    g2b_prompt_item(blockIdx.x, a.NKV, a.tiles, &hk, &tile);
     prompt_query<T> y;
-    prompt_start(y, a, hk, tile * 32, lane);
-    const float c = a.scale * 1.44269504f;
+    prompt_start(y, a, hk, (int)tile * 32, lane);
+    const float c = prompt_unit(a.scale);
     const long stride = a.kv_stride;
     const T *kp = (const T *)a.k + hk * G2B_DH, *vp = (const T *)a.v + hk * G2B_DH;
     T k[4][8], v[2][2][8];
+    unsigned at[2][8];
+    prompt_value_at<T>(at[0], 0, g, lane & 31, stride);
+    prompt_value_at<T>(at[1], 1, g, lane & 31, stride);
     auto load_k = [&](int j0) {
         const T *p = kp + (size_t)j0 * stride + (size_t)min(lane & 31, y.k1 - j0 - 1) * stride + 8 * g;
 #pragma unroll
         for (int s = 0; s < 4; ++s) prompt_load_k(k[s], p + 16 * s);
     };
     auto load_v = [&](int j0) {
-        const int n = y.k1 - j0;
-        const T *p = vp + (size_t)j0 * stride;
+        const __amdgpu_buffer_rsrc_t rows = prompt_rows(vp, j0, y.k1, stride);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                if (n >= 32) prompt_load_v(v[t][u], p + (size_t)(16 * u) * stride, 32 * t + (lane & 31), 4 * g, stride, 32);
-                else prompt_load_v(v[t][u], p, 32 * t + (lane & 31), 16 * u + 4 * g, stride, n);
-            }
+            for (int t = 0; t < 2; ++t) prompt_load_v(v[t][u], rows, at[u], 32 * t * (int)sizeof(T));
     };
     int j0 = y.k0 < y.k1 ? y.k0 + 32 * w : y.k1;
     if (j0 < y.k1) { load_k(j0); load_v(j0); }
@@ -381,7 +407,7 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
     for (int i = 0; i < KW; ++i) top = fmaxf(top, red[i][0][lane]);
 #pragma unroll
     for (int i = 0; i < KW; ++i) {
-        part[i] = kv8_factor(red[i][0][lane], top);
+        part[i] = prompt_factor(red[i][0][lane], top, c);
         l = fmaf(red[i][1][lane], part[i], l);
     }
     T *out = (T *)a.out + (size_t)y.row * a.out_stride + y.head * G2B_DH + 4 * g;
@@ -414,24 +440,25 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
     __shared__ u32x4 lds[2][2 * UNITS];
     __shared__ int range[4][2], odd[2][4];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
-    const long item = g2b_item(blockIdx.x, (long)a.tiles * a.NKV);
-    const int hk = (int)(item / a.tiles), tile = a.tiles - 1 - (int)(item % a.tiles); /* (long rows first) */
+    int hk;
+    long tile;
+    g2b_prompt_item(blockIdx.x, a.NKV, a.tiles, &hk, &tile);
     prompt_query<T> y;
-    prompt_start(y, a, hk, tile * 128 + 32 * w, lane);
+    prompt_start(y, a, hk, (int)tile * 128 + 32 * w, lane);
     if (lane == 0) { range[w][0] = y.k0; range[w][1] = y.k1; }
     __syncthreads();
     const int k0 = __builtin_amdgcn_readfirstlane(min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0])));
     const int k1 = __builtin_amdgcn_readfirstlane(max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1])));
-    const float c = a.scale * 1.44269504f;
+    const float c = prompt_unit(a.scale);
     const long stride = a.kv_stride;
     const T *kp = (const T *)a.k + hk * G2B_DH, *vp = (const T *)a.v + hk * G2B_DH;
     /* this thread's share: dims 8 (tid / 32) ..+7 of key tid % 32; of dim lane, the keys that lanes of half w % 2 take in step w / 2 */
     T k[8], v[8];
+    unsigned at[8];
+    prompt_value_at<T>(at, w >> 1, w & 1, lane, stride);
     auto load = [&](int j0) {
-        const int n = k1 - j0;
-        prompt_load_k(k, kp + (size_t)j0 * stride + (size_t)min(tid & 31, n - 1) * stride + 8 * (tid >> 5));
-        if (n >= 32) prompt_load_v(v, vp + (size_t)(j0 + 16 * (w >> 1) + 4 * (w & 1)) * stride, lane, 0, stride, 32);
-        else prompt_load_v(v, vp + (size_t)j0 * stride, lane, 16 * (w >> 1) + 4 * (w & 1), stride, n);
+        prompt_load_k(k, kp + (size_t)j0 * stride + (size_t)min(tid & 31, k1 - j0 - 1) * stride + 8 * (tid >> 5));
+        prompt_load_v(v, prompt_rows(vp, j0, k1, stride), at, 0);
     };
     auto stage = [&](int b) {
         const bool any = wave_any(prompt_look(v, 0.f) != 0.f);

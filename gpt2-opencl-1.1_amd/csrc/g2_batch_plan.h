@@ -83,12 +83,16 @@ G2B_FN g2b_row g2b_row_keys(int row, int in, int q0, int q1, int k0, int k1, int
     return r;
 }
 
-/* Work-group b of n: its piece of work.  Work-group b runs on XCD b % 8; each
- * XCD gets neighbouring pieces, so that what they share stays in its L2. */
-G2B_FN long g2b_item(long b, long n)
+/* Work-group b of tiles * NKV: its key head and tile of queries.  Work-group b
+ * runs on XCD b % 8.  The last tiles, whose rows see most keys, come first, all
+ * heads of a tile side by side; of the heads, 8 n of them keep to XCD head % 8,
+ * whose L2 then has their keys, and the rest go where there is room. */
+G2B_FN void g2b_prompt_item(long b, int NKV, long tiles, int *head, long *tile)
 {
-    const long x = b % 8, per = n / 8, more = n % 8;
-    return x * per + (x < more ? x : more) + b / 8;
+    const long rank = b / NKV;
+    const int j = (int)(b % NKV), x = (int)(b % 8), fixed = NKV / 8 * 8;
+    *tile = tiles - 1 - rank;
+    *head = j < fixed ? j / 8 * 8 + x : fixed + j % 8;
 }
 
 /* ---- beam search: ids of a work-group's slice of a row, most beams and candidates of a group */

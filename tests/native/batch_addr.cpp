@@ -1,7 +1,7 @@
 // CPU walk of the index arithmetic of the operators for several texts at once
 // (g2_batch_plan.h), for test_batch_addresses.py.  Prints "ok" or the first mistake.
 //   cache S NKV max_seq [mistake]  the parts of a cache buffer
-//   items n                        every piece of work is one work-group's
+//   items NKV tiles                every piece of work is one work-group's
 //   search n seed                  counts in ordered lists, an end in others
 //   rows seed                      the keys of a row, whatever its starts hold
 //   beams rows slices n_out        the parts of the selection's workspace
@@ -45,12 +45,16 @@ static int cache(long S, int NKV, long max_seq, int mistake)
     return 1;
 }
 
-static int items(long n)
+static int items(int NKV, long tiles)
 {
-    std::vector<unsigned char> seen(n, 0);
-    for (long b = 0; b < n; ++b) {
-        const long i = g2b_item(b, n);
-        if (i < 0 || i >= n || seen[i]++) return bad("a piece outside or twice", b, i, n);
+    std::vector<unsigned char> seen(NKV * tiles, 0);
+    for (long b = 0; b < NKV * tiles; ++b) {
+        int h;
+        long t;
+        g2b_prompt_item(b, NKV, tiles, &h, &t);
+        if (h < 0 || h >= NKV || t < 0 || t >= tiles || seen[h * tiles + t]++) return bad("a piece outside or twice", b, h, t);
+        if (h < NKV / 8 * 8 && h % 8 != b % 8) return bad("a head on another XCD", b, h, t);
+        if (t != tiles - 1 - b / NKV) return bad("tiles in another order", b, h, t);
     }
     return 1;
 }
@@ -136,7 +140,7 @@ int main(int n, char **v)
     auto arg = [&](int i) { return i < n ? std::atol(v[i]) : 0; };
     int ok = 0;
     if (n > 1 && !std::strcmp(v[1], "cache")) ok = cache(arg(2), (int)arg(3), arg(4), (int)arg(5));
-    else if (n > 1 && !std::strcmp(v[1], "items")) ok = items(arg(2));
+    else if (n > 1 && !std::strcmp(v[1], "items")) ok = items((int)arg(2), arg(3));
     else if (n > 1 && !std::strcmp(v[1], "search")) ok = search((int)arg(2), (int)arg(3));
     else if (n > 1 && !std::strcmp(v[1], "rows")) ok = rows((int)arg(2));
     else if (n > 1 && !std::strcmp(v[1], "beams")) ok = beams(arg(2), (int)arg(3), (int)arg(4));

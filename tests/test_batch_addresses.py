@@ -38,9 +38,10 @@ def test_cache(walk, S, NKV, max_seq):
     assert walk("cache", S, NKV, max_seq, 1) != "ok"
 
 
-@pytest.mark.parametrize("n", [1, 7, 8, 9, 15, 16, 17, 100, 1023, 4001])
-def test_items(walk, n):
-    assert walk("items", n) == "ok"
+@pytest.mark.parametrize("NKV", [1, 2, 4, 5, 7, 8, 9, 12, 16, 20, 25, 40, 1023])
+def test_items(walk, NKV):
+    for tiles in (1, 2, 7, 8, 9, 63, 250):
+        assert walk("items", NKV, tiles) == "ok"
 
 
 @pytest.mark.parametrize("n", [2, 3, 63, 64, 65, 66, 128, 129, 1000, 4096, 4097, 5000])

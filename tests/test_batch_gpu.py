@@ -23,13 +23,13 @@ def ints(g2, x):
 # ------------------------------------------------------------------ packed prompts
 
 def prompt_bound(mass, top, T, f16, out):
-    """|error| of a computed row.  A score is a sum of 64 products, each of six products of parts (what they leave out is
-    below 2^-22 of it), so it goes through at most 6 * 64 + 2 roundings, each 2^-24 of the sum of |q k|; a weight's relative error is twice
+    """|error| of a computed row.  A score is a sum of 64 products, each of six products of parts (a second
+    part is below 2^-7 of its value, a third below 2^-15, so what they leave out is below 2 * 2^-22 + 2^-30 of it), so it goes through at most 6 * 64 + 2 roundings, each 2^-24 of the sum of |q k|; a weight's relative error is twice
     that (its own and the largest's) and 2^-21 for its exponent's product with log2 e, the exponential and the
     sum's share; the weighted sum of T keys goes through 6 T roundings and the joining of at most eight parts 16, and
     as many in the sum of the weights.  fp16: scores of exact products, a weight rounded by 2^-11, the output by 2^-11 of itself
     (or the half of fp16's smallest step)."""
-    score = (386 * EPS32 + (0 if f16 else 2.0 ** -22)) * top[..., None] * 2
+    score = (386 * EPS32 + (0 if f16 else 2.0 ** -21 + 2.0 ** -30)) * top[..., None] * 2
     w = np.expm1(np.minimum(score, 1)) + 2.0 ** -21 * (1 + top[..., None]) + (12 * T + 32) * EPS32
     if f16:
         return (w + 2.0 ** -11) * mass * 1.001 + 2.0 ** -11 * np.abs(out) + 2.0 ** -25
