@@ -220,9 +220,19 @@ static int beam_sizes(int groups, int beams, int V, int n_out)
            groups <= (1 << 16) / beams;
 }
 
+int g2i_beam_form(int rows, int V, int *slices)
+{
+    const int wide = (long)rows * cdiv(V, G2B_SLICE) > 1024;
+    *slices = (int)cdiv(V, wide ? G2B_SLICE_WIDE : G2B_SLICE);
+    return wide;
+}
+
 size_t g2_beam_work_bytes(int groups, int beams, int V, int n_out)
 {
-    return beam_sizes(groups, beams, V, n_out) ? g2b_beam_bytes((long)groups * beams, g2b_slices(V), n_out) : 0;
+    int slices;
+    if (!beam_sizes(groups, beams, V, n_out)) return 0;
+    g2i_beam_form(groups * beams, V, &slices);
+    return g2b_beam_bytes(groups, (long)groups * beams, slices, n_out);
 }
 
 int g2_beam_select(const float *logits, const float *score, const int *done, int eos, float *out_score, int *out_parent,
@@ -248,11 +258,17 @@ int g2_beam_select(const float *logits, const float *score, const int *done, int
     }
     const int rc = ready();
     if (rc) return rc;
-    const int slices = g2b_slices(V);
-    g2_beam_args a = { logits, score, done, out_score, out_parent, out_id, out_done, work,
-                       (unsigned long long *)((char *)work + g2b_cands_at(rows, slices)), eos, groups, beams, V, n_out, slices };
-    const int first = g2i_launch(G2F_BEAM_SLICE, (unsigned)(rows * slices), 1, 256, &a);
-    return first ? first : g2i_launch(G2F_BEAM_PICK, (unsigned)groups, 1, 256, &a);
+    char *p = work;
+    g2_beam_args a;
+    memset(&a, 0, sizeof a);
+    a.logits = logits; a.score = score; a.done = done;
+    a.out_score = out_score; a.out_parent = out_parent; a.out_id = out_id; a.out_done = out_done;
+    a.eos = eos; a.groups = groups; a.beams = beams; a.V = V; a.n_out = n_out;
+    const int wide = g2i_beam_form((int)rows, V, &a.slices);
+    a.counts = work;
+    a.stats = (unsigned long long *)(p + g2b_stats_at(groups));
+    a.cands = (unsigned long long *)(p + g2b_cands_at(groups, rows, a.slices));
+    return g2i_launch(wide ? G2F_BEAM_SELECT_WIDE : G2F_BEAM_SELECT, (unsigned)(rows * a.slices), 1, 256, &a);
 }
 
 int g2_beam_reorder(const int *ids, int *ids_out, int ids_stride, const int *next, const int *origin, int *origin_out,
@@ -279,9 +295,11 @@ int g2_beam_reorder(const int *ids, int *ids_out, int ids_stride, const int *nex
         bad |= in[i].n && ((has_ids && g2i_overlap(ids_out, ni, in[i].p, in[i].n)) || (has_origin && g2i_overlap(origin_out, no, in[i].p, in[i].n)));
     if (bad) return g2i_err(G2_E_ARG, "%s: overlapping buffers", fn);
     const long chunks = ((long)T + 1 + 255) / 256;
-    if (!fits(chunks * groups)) return g2i_err(G2_E_LIMIT, "%s: too many ints for one call", fn);
+    if (!fits(chunks * rows)) return g2i_err(G2_E_LIMIT, "%s: too many ints for one call", fn);
     const int rc = ready();
     if (rc) return rc;
     g2_beam_move_args a = { ids, ids_out, next, origin, origin_out, parent, len, ids_stride, origin_stride, T, groups, beams };
-    return g2i_launch(G2F_BEAM_MOVE, (unsigned)(chunks * groups), 1, 256, &a);
+    if ((has_ids && ids == ids_out) || (has_origin && origin == origin_out))
+        return g2i_launch(G2F_BEAM_MOVE, (unsigned)(chunks * groups), 1, 256, &a);
+    return g2i_launch(G2F_BEAM_COPY, (unsigned)(chunks * rows), 1, 256, &a);
 }

@@ -774,72 +774,13 @@ G2K void g2k_kv4_join(const g2_kv4_attn_args a)
  * Beam search
  * ==================================================================== */
 
-__device__ __forceinline__ unsigned long long wave_max_key(unsigned long long v)
-{
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const unsigned long long u = __shfl_xor(v, o);
-        v = u > v ? u : v;
-    }
-    return v;
-}
+/* Candidates are few once a bound is known that n of them reach: the n-th
+ * greatest of the lanes' own greatest is one, whatever the rest.  What reaches it
+ * is put down in LDS, in any order, and each candidate counts those above it. */
 
-/* A slice of a row: its largest logit, the sum of exponentials below it, and its
- * n_out greatest logits (of equal ones the lower ids) as keys, 0 for none. */
-G2K void g2k_beam_slice(const g2_beam_args a)
-{
-    __shared__ float red[4];
-    __shared__ unsigned long long best[4];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const long row = blockIdx.x / a.slices;
-    const int slice = blockIdx.x % a.slices, v0 = slice * G2B_SLICE, nv = min(a.V - v0, G2B_SLICE);
-    const float *in = a.logits + row * a.V + v0;
-    float x[16];
-#pragma unroll
-    for (int q = 0; q < 16; ++q) x[q] = tid + 256 * q < nv ? in[tid + 256 * q] : -INFINITY;
-    float top = -INFINITY;
-#pragma unroll
-    for (int q = 0; q < 16; ++q) top = fmaxf(top, x[q]);
-    top = wave_max(top);
-    if (lane == 0) red[w] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    __syncthreads();
-    float sum = 0.f;
-    unsigned long long mine = 0; /* the thread's best key */
-#pragma unroll
-    for (int q = 0; q < 16; ++q) {
-        sum += tid + 256 * q < nv ? expf(x[q] - (top == -INFINITY ? 0.f : top)) : 0.f;
-        if (x[q] > -INFINITY) {
-            const unsigned long long k = logit_key(x[q], v0 + tid + 256 * q);
-            mine = k > mine ? k : mine;
-        }
-    }
-    sum = block_sum(sum, red);
-    const long cell = row * a.slices + slice;
-    if (tid == 0) { a.stats[2 * cell] = top; a.stats[2 * cell + 1] = sum; }
-    for (int n = 0; n < a.n_out; ++n) {
-        const unsigned long long k = wave_max_key(mine);
-        if (lane == 0) best[w] = k;
-        __syncthreads();
-        unsigned long long b = best[0];
-#pragma unroll
-        for (int i = 1; i < 4; ++i) b = best[i] > b ? best[i] : b;
-        if (tid == 0) a.cands[cell * a.n_out + n] = b;
-        if (b && b == mine) { /* its thread goes on to its next */
-            mine = 0;
-#pragma unroll
-            for (int q = 0; q < 16; ++q)
-                if (x[q] > -INFINITY) {
-                    const unsigned long long k2 = logit_key(x[q], v0 + tid + 256 * q);
-                    mine = k2 < b && k2 > mine ? k2 : mine;
-                }
-        }
-        __syncthreads();
-    }
-}
+#define BEAM_LIST 512 /* candidates that LDS holds; a slice or group with more (many equal ones) takes them one by one */
 
-/* A number that orders as a double does (no NaN). */
+/* A number that orders as a double does (no NaN), 0 below all. */
 __device__ __forceinline__ unsigned long long double_key(double v)
 {
     const unsigned long long u = __double_as_longlong(v + 0.0);
@@ -854,99 +795,292 @@ __device__ __forceinline__ float key_logit(unsigned long long k)
     const unsigned u = (unsigned)(k >> 32);
     return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
 }
-
-/* The n_out best of a group's candidates: each thread goes over its share of
- * them once for every one that is taken. */
-G2K void g2k_beam_pick(const g2_beam_args a)
+__device__ __forceinline__ unsigned long long ld_agent64(const unsigned long long *p)
 {
-    __shared__ double lse[G2B_MAX_BEAMS]; /* score - log sum exp; NaN: no continuations */
-    __shared__ unsigned long long bk[4];
-    __shared__ unsigned bf[4];
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void st_agent64(unsigned long long *p, unsigned long long v)
+{
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+/* A candidate: its total as a key, and beam V + id, lower first of equal ones. */
+struct beam_cand {
+    unsigned long long k;
+    unsigned f;
+};
+__device__ __forceinline__ bool beam_above(const beam_cand &a, const beam_cand &b) { return a.k > b.k || (a.k == b.k && a.f < b.f); }
+
+union beam_lds {
+    struct {
+        float top[4], sum[4], bound[4];
+        unsigned long long list[BEAM_LIST];
+    } slice;
+    struct {
+        double lse[G2B_MAX_BEAMS]; /* score - log sum exp; NaN: no continuations */
+        unsigned long long list[BEAM_LIST];
+        unsigned flat[BEAM_LIST];
+        unsigned long long bound;
+    } pick;
+};
+
+/* The last of a group's work-groups: the n_out best of all its slices' candidates. */
+template <int SLICE>
+__device__ void beam_pick(const g2_beam_args &a, long g, beam_lds &lds, int *count)
+{
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const long g = blockIdx.x, row0 = g * a.beams;
-    if (tid < a.beams) {
-        const long row = row0 + tid;
-        const float *st = a.stats + 2 * row * a.slices;
+    const long row0 = g * a.beams;
+    for (int b = w; b < a.beams; b += 4) {
+        const unsigned long long *st = a.stats + (row0 + b) * a.slices;
         float top = -INFINITY;
+        for (int i = lane; i < a.slices; i += 64) top = fmaxf(top, __uint_as_float((unsigned)ld_agent64(st + i)));
+        top = wave_max(top);
+        const double base = top == -INFINITY ? 0.0 : (double)top;
         double sum = 0.0;
-        for (int i = 0; i < a.slices; ++i) top = fmaxf(top, st[2 * i]);
-        for (int i = 0; i < a.slices; ++i) sum += (double)st[2 * i + 1] * exp((double)st[2 * i] - (double)(top == -INFINITY ? 0.f : top));
-        lse[tid] = a.done && a.done[row] ? __longlong_as_double(0x7ff8000000000000ll) : (double)a.score[row] - ((double)top + log(sum));
+        for (int i = lane; i < a.slices; i += 64) {
+            const unsigned long long v = ld_agent64(st + i);
+            sum += (double)__uint_as_float((unsigned)(v >> 32)) * exp((double)__uint_as_float((unsigned)v) - base);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+        if (lane == 0)
+            lds.pick.lse[b] = a.done && a.done[row0 + b] ? __longlong_as_double(0x7ff8000000000000ll) : (double)a.score[row0 + b] - ((double)top + log(sum));
     }
+    if (tid == 0) { lds.pick.bound = 1; *count = 0; }
     __syncthreads();
-    const int per = a.slices * a.n_out, total = a.beams * per;
-    unsigned long long lastk = ~0ull;
-    unsigned lastf = 0;
-    for (int n = 0; n < a.n_out; ++n) {
-        unsigned long long k = 0;
-        unsigned f = ~0u;
-        for (int i = tid; i < total + a.beams; i += 256) {
-            unsigned long long ck;
-            unsigned cf;
-            if (i < total) {
-                const int b = i / per;
-                const unsigned long long c = a.cands[row0 * per + i];
-                const double t = (double)key_logit(c) + lse[b];
-                if (!c || !(t > -INFINITY)) continue;
-                ck = double_key(t);
-                cf = (unsigned)b * (unsigned)a.V + (unsigned)~(unsigned)c;
-            } else {
-                const int b = i - total;
-                if (!a.done || !a.done[row0 + b] || !(a.score[row0 + b] > -INFINITY)) continue;
-                ck = double_key((double)a.score[row0 + b]);
-                cf = (unsigned)b * (unsigned)a.V + (unsigned)a.eos;
+    /* list l: a slice's candidates, greatest first, or (behind them) an ended beam as it is */
+    const int slices = a.beams * a.slices, lists = slices + a.beams, n = a.n_out;
+    const unsigned long long *cands = a.cands + row0 * a.slices * n;
+    auto get = [&](int l, int j) {
+        beam_cand c = { 0, ~0u };
+        if (l < slices) {
+            const unsigned long long k = ld_agent64(cands + (long)l * n + j);
+            const int b = l / a.slices;
+            const double t = (double)key_logit(k) + lds.pick.lse[b];
+            if (k && t > -INFINITY) {
+                c.k = double_key(t);
+                c.f = (unsigned)b * (unsigned)a.V + ~(unsigned)k;
             }
-            if (ck > lastk || (ck == lastk && n && cf <= lastf)) continue; /* taken */
-            if (ck > k || (ck == k && cf < f)) { k = ck; f = cf; }
+        } else if (l < lists && j == 0 && a.done) {
+            const int b = l - slices;
+            const float score = a.score[row0 + b];
+            if (a.done[row0 + b] && score > -INFINITY) {
+                c.k = double_key((double)score);
+                c.f = (unsigned)b * (unsigned)a.V + (unsigned)a.eos;
+            }
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const unsigned long long ok = __shfl_xor(k, o);
-            const unsigned of = __shfl_xor(f, o);
-            if (ok > k || (ok == k && of < f)) { k = ok; f = of; }
+        return c;
+    };
+    unsigned long long best = 0;
+    for (int l = tid; l < lists; l += 256) {
+        const unsigned long long k = get(l, 0).k;
+        best = k > best ? k : best;
+    }
+    lds.pick.list[tid] = best;
+    __syncthreads();
+    int above = 0;
+    for (int i = 0; i < 256; ++i) {
+        const unsigned long long k = lds.pick.list[i];
+        above += k > best || (k == best && i < tid);
+    }
+    if (above == n - 1 && best) lds.pick.bound = best;
+    __syncthreads();
+    const unsigned long long bound = lds.pick.bound;
+    for (int l = tid; l < lists; l += 256)
+        for (int j = 0; j < n; ++j) {
+            const beam_cand c = get(l, j);
+            if (c.k < bound) break;
+            const int at = atomicAdd(count, 1);
+            if (at < BEAM_LIST) { lds.pick.list[at] = c.k; lds.pick.flat[at] = c.f; }
         }
-        if (lane == 0) { bk[w] = k; bf[w] = f; }
+    __syncthreads();
+    const int total = *count;
+    auto put = [&](int i, const beam_cand &c) {
+        const long at = g * n + i;
+        const int parent = c.k ? (int)(c.f / (unsigned)a.V) : -1, id = c.k ? (int)(c.f % (unsigned)a.V) : -1;
+        a.out_score[at] = c.k ? (float)key_double(c.k) : -INFINITY;
+        a.out_parent[at] = parent;
+        a.out_id[at] = id;
+        if (a.out_done) a.out_done[at] = c.k && (id == a.eos || (a.done && a.done[row0 + parent]));
+    };
+    const beam_cand none = { 0, ~0u };
+    if (total <= BEAM_LIST) {
+        for (int i = tid; i < total; i += 256) {
+            const beam_cand c = { lds.pick.list[i], lds.pick.flat[i] };
+            int at = 0;
+            for (int j = 0; j < total; ++j) {
+                const beam_cand o = { lds.pick.list[j], lds.pick.flat[j] };
+                at += beam_above(o, c);
+            }
+            if (at < n) put(at, c);
+        }
+        for (int i = total + tid; i < n; i += 256) put(i, none);
+        return;
+    }
+    beam_cand last = { ~0ull, 0 };
+    for (int i = 0; i < n; ++i) { /* one by one: the best that is below the last one */
+        beam_cand c = none;
+        for (int l = tid; l < lists; l += 256)
+            for (int j = 0; j < n; ++j) {
+                const beam_cand x = get(l, j);
+                if (x.k < bound) break;
+                if ((i == 0 || beam_above(last, x)) && beam_above(x, c)) c = x;
+            }
         __syncthreads();
-        k = bk[0]; f = bf[0];
-#pragma unroll
-        for (int i = 1; i < 4; ++i)
-            if (bk[i] > k || (bk[i] == k && bf[i] < f)) { k = bk[i]; f = bf[i]; }
-        if (tid == 0) {
-            const long at = g * a.n_out + n;
-            const int parent = k ? (int)(f / (unsigned)a.V) : -1, id = k ? (int)(f % (unsigned)a.V) : -1;
-            a.out_score[at] = k ? (float)key_double(k) : -INFINITY;
-            a.out_parent[at] = parent;
-            a.out_id[at] = id;
-            if (a.out_done) a.out_done[at] = k && (id == a.eos || (a.done && a.done[row0 + parent]));
-        }
-        lastk = k ? k : 1; /* (no key is 1: nothing is left) */
-        lastf = f;
+        lds.pick.list[tid] = c.k;
+        lds.pick.flat[tid] = c.f;
         __syncthreads();
+        for (int t = 0; t < 256; ++t) {
+            const beam_cand x = { lds.pick.list[t], lds.pick.flat[t] };
+            if (beam_above(x, c)) c = x;
+        }
+        if (tid == 0) put(i, c);
+        last = c; /* (at least n reach the bound) */
     }
 }
 
-/* Columns of a group's tables: a thread reads its column of all beams before it
- * writes it, so a table may be moved in place. */
+/* A slice of a row: its largest logit, the sum of exponentials below it, and its
+ * n_out greatest logits (of equal ones the lower ids) as keys, 0 for none; then
+ * the group's last work-group picks.  What one work-group leaves for another goes
+ * to the coherence point and is there before the count goes up. */
+template <int QUADS>
+__device__ void beam_select_impl(const g2_beam_args &a)
+{
+    constexpr int SLICE = 1024 * QUADS, Q = 4 * QUADS;
+    __shared__ beam_lds lds;
+    __shared__ int count, last;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = a.n_out;
+    const long row = blockIdx.x / a.slices;
+    const int slice = blockIdx.x % a.slices, v0 = slice * SLICE, nv = min(a.V - v0, SLICE);
+    const float *in = a.logits + row * a.V + v0;
+    float x[Q];
+#pragma unroll
+    for (int q = 0; q < QUADS; ++q) {
+        const int i = 4 * (tid + 256 * q);
+        if (i + 4 <= nv) {
+            const f32x4 v = *(const f32x4u *)(in + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * q + e] = v[e];
+        } else
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * q + e] = i + e < nv ? in[i + e] : -INFINITY;
+    }
+    if (tid == 0) count = 0;
+    float mine = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) mine = fmaxf(mine, x[q]);
+    const float top = lanes_max(mine), base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f; /* (NaN where a logit is; ids behind the row add nothing) */
+#pragma unroll
+    for (int q = 0; q < Q; ++q) sum += __builtin_amdgcn_exp2f((x[q] - base) * 1.44269504f);
+    sum = wave_sum(sum);
+    /* the n-th greatest of the lanes' greatest, equal ones together */
+    float bound = -INFINITY;
+    int left = n;
+    for (float v = mine; left > 0;) {
+        bound = lanes_max(v);
+        if (!(bound > -INFINITY)) break;
+        left -= __builtin_popcountll(__builtin_amdgcn_ballot_w64(v == bound));
+        v = v == bound ? -INFINITY : v;
+    }
+    if (lane == 0) { lds.slice.top[w] = top; lds.slice.sum[w] = sum; lds.slice.bound[w] = bound; }
+    __syncthreads();
+    bound = fmaxf(fmaxf(lds.slice.bound[0], lds.slice.bound[1]), fmaxf(lds.slice.bound[2], lds.slice.bound[3]));
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+        if (x[q] >= bound && x[q] > -INFINITY) {
+            const int at = atomicAdd(&count, 1);
+            if (at < BEAM_LIST) lds.slice.list[at] = logit_key(x[q], v0 + 4 * (tid + 256 * (q / 4)) + q % 4);
+        }
+    __syncthreads();
+    const int total = count;
+    const long cell = row * a.slices + slice;
+    unsigned long long *cands = a.cands + cell * n;
+    if (total <= BEAM_LIST) {
+        for (int i = tid; i < total; i += 256) {
+            const unsigned long long k = lds.slice.list[i];
+            int at = 0;
+            for (int j = 0; j < total; ++j) at += lds.slice.list[j] > k;
+            if (at < n) st_agent64(cands + at, k);
+        }
+        for (int i = total + tid; i < n; i += 256) st_agent64(cands + i, 0);
+    } else {
+        unsigned long long below = ~0ull;
+        for (int i = 0; i < n; ++i) { /* one by one: the greatest key below the last one */
+            unsigned long long k = 0;
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+                if (x[q] > -INFINITY) {
+                    const unsigned long long y = logit_key(x[q], v0 + 4 * (tid + 256 * (q / 4)) + q % 4);
+                    k = y < below && y > k ? y : k;
+                }
+            __syncthreads();
+            lds.slice.list[tid] = k;
+            __syncthreads();
+            for (int t = 0; t < 256; ++t) k = lds.slice.list[t] > k ? lds.slice.list[t] : k;
+            if (tid == 0) st_agent64(cands + i, k);
+            below = k;
+        }
+    }
+    if (tid == 0) {
+        float m = -INFINITY, l = 0.f;
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, lds.slice.top[i]);
+        for (int i = 0; i < 4; ++i) l += lds.slice.sum[i] * (lds.slice.top[i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((lds.slice.top[i] - m) * 1.44269504f));
+        st_agent64(a.stats + cell, (unsigned long long)__float_as_uint(l) << 32 | __float_as_uint(m));
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    const long g = row / a.beams;
+    if (tid == 0) {
+        unsigned *cell = a.counts + g * G2B_COUNT_INTS;
+        last = __hip_atomic_fetch_add(cell, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(a.beams * a.slices) - 1;
+        if (last) __hip_atomic_store(cell, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (last) beam_pick<SLICE>(a, g, lds, &count);
+}
+G2K void g2k_beam_select(const g2_beam_args a) { beam_select_impl<1>(a); }
+G2K void g2k_beam_select_wide(const g2_beam_args a) { beam_select_impl<4>(a); }
+
+/* Rows of the tables in their parents' order, 256 ints of a row to a work-group. */
+G2K void g2k_beam_copy(const g2_beam_move_args a)
+{
+    const int chunks = (a.T + 1 + 255) / 256;
+    const long row = blockIdx.x / chunks;
+    const int g = (int)(row / a.beams), p = (int)(blockIdx.x % chunks) * 256 + threadIdx.x;
+    const int n = a.len ? clampi(a.len[g], 0, a.T) : a.T;
+    const int from = a.parent[row];
+    if (p > n || from < 0 || from >= a.beams) return;
+    const long src = (long)g * a.beams + from;
+    int id = 0, at = 0;
+    if (a.ids_out) id = p < n ? a.ids[src * a.ids_stride + p] : a.next[row];
+    if (a.origin_out) at = p < n ? a.origin[src * a.origin_stride + p] : (int)row;
+    if (a.ids_out) a.ids_out[row * a.ids_stride + p] = id;
+    if (a.origin_out) a.origin_out[row * a.origin_stride + p] = at;
+}
+
+/* The same where a table is moved in place: a thread reads its column of all
+ * beams before it writes it. */
 G2K void g2k_beam_move(const g2_beam_move_args a)
 {
-    __shared__ int col[G2B_MAX_BEAMS][256];
+    __shared__ int col[2][G2B_MAX_BEAMS][256];
     const int tid = threadIdx.x, chunks = (a.T + 1 + 255) / 256;
     const long g = blockIdx.x / chunks, row0 = g * a.beams;
     const int p = (int)(blockIdx.x % chunks) * 256 + tid;
     const int n = a.len ? clampi(a.len[g], 0, a.T) : a.T;
     if (p > n) return;
-    for (int which = 0; which < 2; ++which) {
-        const int *in = which ? a.origin : a.ids;
-        int *out = which ? a.origin_out : a.ids_out;
-        const long stride = which ? a.origin_stride : a.ids_stride;
-        if (!out) continue;
-        if (p < n)
-            for (int b = 0; b < a.beams; ++b) col[b][tid] = in[(row0 + b) * stride + p];
+    if (p < n)
+#pragma unroll 4
         for (int b = 0; b < a.beams; ++b) {
-            const int from = a.parent[row0 + b];
-            if (from < 0 || from >= a.beams) continue;
-            out[(row0 + b) * stride + p] = p < n ? col[from][tid] : which ? (int)(row0 + b) : a.next[row0 + b];
+            if (a.ids_out) col[0][b][tid] = a.ids[(row0 + b) * a.ids_stride + p];
+            if (a.origin_out) col[1][b][tid] = a.origin[(row0 + b) * a.origin_stride + p];
         }
+#pragma unroll 4
+    for (int b = 0; b < a.beams; ++b) {
+        const int from = a.parent[row0 + b];
+        if (from < 0 || from >= a.beams) continue;
+        if (a.ids_out) a.ids_out[(row0 + b) * a.ids_stride + p] = p < n ? col[0][from][tid] : a.next[row0 + b];
+        if (a.origin_out) a.origin_out[(row0 + b) * a.origin_stride + p] = p < n ? col[1][from][tid] : (int)(row0 + b);
     }
 }
 } // namespace gb

@@ -95,18 +95,22 @@ G2B_FN void g2b_prompt_item(long b, int NKV, long tiles, int *head, long *tile)
     *head = j < fixed ? j / 8 * 8 + x : fixed + j % 8;
 }
 
-/* ---- beam search: ids of a work-group's slice of a row, most beams and candidates of a group */
-#define G2B_SLICE 4096
+/* ---- beam search: ids of a work-group's slice of a row (narrow and wide form),
+ * most beams and continuations of a group; ints from count to count (a cache
+ * line: the work-groups of a group meet there) */
+#define G2B_SLICE 1024
+#define G2B_SLICE_WIDE 4096
 #define G2B_MAX_BEAMS 32
 #define G2B_MAX_OUT 64
-G2B_FN int g2b_slices(int V) { return (V + G2B_SLICE - 1) / G2B_SLICE; }
-/* The workspace: for each row and slice its largest logit and sum of
- * exponentials (2 floats), then `n_out` candidates (8 bytes each: a logit's
- * order and its id). */
-G2B_FN size_t g2b_cands_at(long rows, int slices) { return ((size_t)rows * slices * 8 + 255) / 256 * 256; }
-G2B_FN size_t g2b_beam_bytes(long rows, int slices, int n_out)
+#define G2B_COUNT_INTS 16
+/* The workspace: a count of work-groups for each group (0 between calls), for
+ * each row and slice its largest logit and sum of exponentials (8 bytes), then
+ * n_out candidates (8 bytes each: a logit's order and its id). */
+G2B_FN size_t g2b_stats_at(long groups) { return (size_t)groups * G2B_COUNT_INTS * 4; }
+G2B_FN size_t g2b_cands_at(long groups, long rows, int slices) { return g2b_stats_at(groups) + (size_t)rows * slices * 8; }
+G2B_FN size_t g2b_beam_bytes(long groups, long rows, int slices, int n_out)
 {
-    return g2b_cands_at(rows, slices) + (size_t)rows * slices * n_out * 8;
+    return g2b_cands_at(groups, rows, slices) + (size_t)rows * slices * n_out * 8;
 }
 
 #endif

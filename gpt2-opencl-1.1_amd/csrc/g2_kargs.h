@@ -511,7 +511,8 @@ typedef struct {
     int *out_parent;
     int *out_id;
     int *out_done;
-    float *stats;              /* [rows][slices][2] */
+    unsigned *counts;          /* [groups][G2B_COUNT_INTS] */
+    unsigned long long *stats; /* [rows][slices]: largest logit, sum */
     unsigned long long *cands; /* [rows][slices][n_out] */
     int eos, groups, beams, V, n_out, slices;
 } g2_beam_args;

@@ -410,8 +410,13 @@ def attn_kv4(q, q_stride, cache, out, out_stride, origin, lens, T_kv, n_seq, n_h
 
 
 def beam_work_bytes(groups, beams, V, n_out):
-    """Bytes of beam_select's workspace."""
+    """Bytes of beam_select's workspace (beam_work makes one)."""
     return _lib.g2_beam_work_bytes(groups, beams, V, n_out)
+
+
+def beam_work(groups, beams, V, n_out):
+    """A workspace for beam_select as it has to be before its first use (zero)."""
+    return to_device(np.zeros(beam_work_bytes(groups, beams, V, n_out), np.uint8))
 
 
 def beam_select(logits, score, done, eos, out_score, out_parent, out_id, out_done, groups, beams, V, n_out, work):

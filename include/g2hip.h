@@ -350,7 +350,9 @@ int g2_attn_kv4(const float *q, int q_stride, const void *cache, float *out, int
                 const int *origin, const int *len, int T_kv, int n_seq, int n_head, int n_kv,
                 int max_seq, float scale, float *work);
 
-/* Bytes of g2_beam_select's workspace (0 if the sizes are not supported). */
+/* Bytes of g2_beam_select's workspace (0 if the sizes are not supported): zero
+ * before its first call and before one of other sizes, 8-byte aligned, for one
+ * call alone while it runs. */
 size_t g2_beam_work_bytes(int groups, int beams, int V, int n_out);
 /* A step of beam search: for each group the n_out continuations of its beams
  * with the greatest sums of log-probabilities, greatest first; of equal ones
@@ -365,7 +367,7 @@ size_t g2_beam_work_bytes(int groups, int beams, int V, int n_out);
  * are fewer than n_out above -infinity, parent and id are -1, the score
  * -infinity.  With n_out == beams and scores of 0, -infinity, -infinity ... one
  * beam starts a group.  beams up to 32, n_out up to 64, V up to 262144, groups *
- * beams up to 65536.  work: 8-byte aligned, for this call alone while it runs. */
+ * beams up to 65536. */
 int g2_beam_select(const float *logits, const float *score, const int *done, int eos,
                    float *out_score, int *out_parent, int *out_id, int *out_done,
                    int groups, int beams, int V, int n_out, void *work);

@@ -4,7 +4,7 @@
 //   items NKV tiles                every piece of work is one work-group's
 //   search n seed                  counts in ordered lists, an end in others
 //   rows seed                      the keys of a row, whatever its starts hold
-//   beams rows slices n_out        the parts of the selection's workspace
+//   beams groups rows slices n_out the parts of the selection's workspace
 #include <climits>
 #include <cstdio>
 #include <cstdlib>
@@ -128,10 +128,11 @@ static int rows(int seed)
     return 1;
 }
 
-static int beams(long n, int slices, int n_out)
+static int beams(long groups, long n, int slices, int n_out)
 {
-    const size_t at = g2b_cands_at(n, slices), all = g2b_beam_bytes(n, slices, n_out);
-    if (at % 8 || at < (size_t)n * slices * 8 || all != at + (size_t)n * slices * n_out * 8) return bad("parts", n, slices, n_out);
+    const size_t st = g2b_stats_at(groups), at = g2b_cands_at(groups, n, slices), all = g2b_beam_bytes(groups, n, slices, n_out);
+    if (st % 8 || at % 8 || st < (size_t)groups * 4 || at < st + (size_t)n * slices * 8 || all != at + (size_t)n * slices * n_out * 8)
+        return bad("parts", n, slices, n_out);
     return 1;
 }
 
@@ -143,7 +144,7 @@ int main(int n, char **v)
     else if (n > 1 && !std::strcmp(v[1], "items")) ok = items((int)arg(2), arg(3));
     else if (n > 1 && !std::strcmp(v[1], "search")) ok = search((int)arg(2), (int)arg(3));
     else if (n > 1 && !std::strcmp(v[1], "rows")) ok = rows((int)arg(2));
-    else if (n > 1 && !std::strcmp(v[1], "beams")) ok = beams(arg(2), (int)arg(3), (int)arg(4));
+    else if (n > 1 && !std::strcmp(v[1], "beams")) ok = beams(arg(2), arg(3), (int)arg(4), (int)arg(5));
     if (ok) std::printf("ok\n");
     return ok ? 0 : 1;
 }

@@ -440,10 +440,12 @@ def select(g2, logits, score, done, eos, beams, n_out, want_done=True):
     n = G * n_out
     ds = ints(g2, done) if done is not None else None
     os, op, oi, od = guarded(g2, n), guarded(g2, n), guarded(g2, n), guarded(g2, n)
-    work = g2.to_device(np.full(g2.beam_work_bytes(G, beams, V, n_out) + 64, 0xAB, np.uint8))
+    nw = g2.beam_work_bytes(G, beams, V, n_out)
+    work = g2.to_device(np.concatenate([np.zeros(nw, np.uint8), np.full(64, 0xAB, np.uint8)]))
     g2.beam_select(g2.to_device(logits.astype(np.float32)), g2.to_device(np.asarray(score, np.float32)), ds, eos, os, op, oi,
                    od if want_done else None, G, beams, V, n_out, work)
-    assert (work.download(np.uint8)[-64:] == 0xAB).all()
+    left = work.download(np.uint8)
+    assert (left[nw:nw + 64] == 0xAB).all() and (left[:64 * G] == 0).all()
     s = take(os, n).reshape(G, n_out)
     p, i, d = (take(x, n).view(np.int32).reshape(G, n_out) for x in (op, oi, od))
     return s, p, i, d
@@ -464,7 +466,8 @@ def check_select(g2, logits, score, done, eos, beams, n_out):
 
 
 @pytest.mark.parametrize("G,beams,V,n_out", [(1, 1, 1, 1), (1, 1, 5, 8), (2, 3, 7, 4), (1, 4, 4095, 4), (3, 5, 4096, 10), (2, 2, 4097, 2), (1, 8, 50257, 8),
-                                             (5, 8, 9000, 16), (1, 32, 1000, 64), (2, 32, 5000, 32), (1, 1, 50257, 64), (40, 4, 300, 4), (1, 3, 262144, 5)])
+                                             (5, 8, 9000, 16), (1, 32, 1000, 64), (2, 32, 5000, 32), (1, 1, 50257, 64), (40, 4, 300, 4), (1, 3, 262144, 5),
+                                             (65, 16, 700, 16), (4, 8, 50257, 8), (300, 4, 1030, 3), (33, 1, 33000, 64)])
 def test_select(g2, G, beams, V, n_out):
     r = rng(G, beams, V, n_out)
     logits = 3 * r.standard_normal((G * beams, V))
@@ -484,6 +487,8 @@ def test_select_ties(g2):
         check_select(g2, logits, np.zeros(8), None, 3, 4, 12)
         logits[:, 11] = -0.0
         check_select(g2, logits, np.zeros(8), np.array([0, 1, 0, 0, 1, 1, 1, 1]), 3, 4, 64)
+    check_select(g2, np.zeros((1100, 1024)), np.zeros(1100), None, -1, 11, 64)  # (the wide form, more equal ones than its lists hold)
+    check_select(g2, np.zeros((264, 5000)), np.zeros(264), None, -1, 8, 33)
 
 
 def test_select_beside_each_other(g2):
@@ -590,10 +595,11 @@ class Search:
         for g in range(G):
             ids[g * B:(g + 1) * B, :self.lens[g]] = self.prompts[g]
         dids, dorigin = g2.to_device(ids), g2.to_device(origin.astype(np.int32))
-        score, work = g2.to_device(np.zeros(R, np.float32)), g2.to_device(np.zeros(g2.beam_work_bytes(G, B, self.V, B), np.uint8))
+        score = g2.to_device(np.zeros(R, np.float32))
+        first, work = g2.beam_work(G, 1, self.V, B), g2.beam_work(G, B, self.V, B)
         parent, nxt, done, new, ended = (ints(g2, np.zeros(R)) for _ in range(5))
         # the first choice is among one beam's continuations
-        g2.beam_select(g2.to_device(l), g2.to_device(np.zeros(G, np.float32)), None, self.eos, score, parent, nxt, done, G, 1, self.V, B, work)
+        g2.beam_select(g2.to_device(l), g2.to_device(np.zeros(G, np.float32)), None, self.eos, score, parent, nxt, done, G, 1, self.V, B, first)
         n = np.array(self.lens, np.int32)
         g2.beam_reorder(dids, dids, self.max_seq, nxt, dorigin, dorigin, self.max_seq, parent, ints(g2, n), int(n.max()), G, B)
         awork = g2.to_device(np.zeros(g2.kv4_work_bytes(R, self.NH) // 4, np.float32))
@@ -672,7 +678,7 @@ def test_captured_and_replayed(g2):
             self.origin, self.ids = ints(g2, np.zeros((R, M))), ints(g2, np.zeros((R, M)))
             self.logits, self.score, self.done = g2.DevBuf(4 * R * V), g2.DevBuf(4 * R), ints(g2, [0] * R)
             self.new, self.parent, self.next, self.ended = (g2.DevBuf(4 * R) for _ in range(4))
-            self.n, self.bwork = ints(g2, [0] * G), g2.DevBuf(g2.beam_work_bytes(G, B, V, B))
+            self.n, self.bwork = ints(g2, [0] * G), g2.beam_work(G, B, V, B)
             self.k, self.v = g2.to_device(np.zeros(R * M * NKV * H, np.float32)), g2.to_device(np.zeros(R * M * NKV * H, np.float32))
 
         def upload(self, seed):
