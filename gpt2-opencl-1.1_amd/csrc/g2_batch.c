@@ -220,11 +220,15 @@ static int beam_sizes(int groups, int beams, int V, int n_out)
            groups <= (1 << 16) / beams;
 }
 
+/* Slices of 4096 ids while that makes at most 256 work-groups (one for each CU), else
+ * of 16384, else of 28672 (us: 4 rows of 50257 8.9 with 4096; 16 rows 14.8 with
+ * 28672, 10.1 with 16384; 64 rows 12.7, 10.4; 128 rows 11.4 with 28672, 13.5 with
+ * 16384; 512 rows 40, 39). */
 int g2i_beam_form(int rows, int V, int *slices)
 {
-    const int wide = (long)rows * cdiv(V, G2B_SLICE) > 1024;
-    *slices = (int)cdiv(V, wide ? G2B_SLICE_WIDE : G2B_SLICE);
-    return wide;
+    const int times = (long)rows * cdiv(V, G2B_SLICE) <= 256 ? 1 : (long)rows * cdiv(V, 4 * G2B_SLICE) <= 256 ? 4 : 7;
+    *slices = (int)cdiv(V, times * G2B_SLICE);
+    return times;
 }
 
 size_t g2_beam_work_bytes(int groups, int beams, int V, int n_out)
@@ -264,11 +268,11 @@ int g2_beam_select(const float *logits, const float *score, const int *done, int
     a.logits = logits; a.score = score; a.done = done;
     a.out_score = out_score; a.out_parent = out_parent; a.out_id = out_id; a.out_done = out_done;
     a.eos = eos; a.groups = groups; a.beams = beams; a.V = V; a.n_out = n_out;
-    const int wide = g2i_beam_form((int)rows, V, &a.slices);
+    const int times = g2i_beam_form((int)rows, V, &a.slices);
     a.counts = work;
     a.stats = (unsigned long long *)(p + g2b_stats_at(groups));
     a.cands = (unsigned long long *)(p + g2b_cands_at(groups, rows, a.slices));
-    return g2i_launch(wide ? G2F_BEAM_SELECT_WIDE : G2F_BEAM_SELECT, (unsigned)(rows * a.slices), 1, 256, &a);
+    return g2i_launch(times == 1 ? G2F_BEAM_SELECT1 : times == 4 ? G2F_BEAM_SELECT4 : G2F_BEAM_SELECT7, (unsigned)(rows * a.slices), 1, 1024, &a);
 }
 
 int g2_beam_reorder(const int *ids, int *ids_out, int ids_stride, const int *next, const int *origin, int *origin_out,

@@ -774,11 +774,14 @@ G2K void g2k_kv4_join(const g2_kv4_attn_args a)
  * Beam search
  * ==================================================================== */
 
-/* Candidates are few once a bound is known that n of them reach: the n-th
- * greatest of the lanes' own greatest is one, whatever the rest.  What reaches it
- * is put down in LDS, in any order, and each candidate counts those above it. */
+/* Candidates are few once a bound is known that n of them reach.  One is the
+ * least of the greatest of G >= n groups: of values that are spread over the
+ * groups, about G (1 + 1/2 + ... + 1/G) reach it (54 for 16).  What reaches it is
+ * put down in LDS, in any order, and each candidate counts those above it. */
 
-#define BEAM_LIST 512 /* candidates that LDS holds; a slice or group with more (many equal ones) takes them one by one */
+#define BEAM_THREADS 1024
+#define BEAM_WAVES (BEAM_THREADS / 64)
+#define BEAM_LIST 1024 /* candidates that LDS holds; a slice or group with more (many equal ones) takes them one by one */
 
 /* A number that orders as a double does (no NaN), 0 below all. */
 __device__ __forceinline__ unsigned long long double_key(double v)
@@ -804,138 +807,228 @@ __device__ __forceinline__ void st_agent64(unsigned long long *p, unsigned long 
     __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-/* A candidate: its total as a key, and beam V + id, lower first of equal ones. */
+/* A candidate: its total as a key (0: none), and its beam and id, which order as beam
+ * V + id does; lower first of equal ones. */
 struct beam_cand {
     unsigned long long k;
     unsigned f;
 };
+#define BEAM_ID_BITS 18 /* (V is 2^18 at most) */
 __device__ __forceinline__ bool beam_above(const beam_cand &a, const beam_cand &b) { return a.k > b.k || (a.k == b.k && a.f < b.f); }
+
+__device__ __forceinline__ float lanes_sum(float v)
+{
+    v = dpp_quad_sum(v);
+    v += lane_xor4(v);
+    v += lane_xor8(v);
+    v = lane_fold16(v, v);
+    return lane_fold32(v, v);
+}
+/* The least of the greatest of the wave's 2^log groups, those that have something
+ * above -infinity, and how many those are; lanes that differ in their high bits
+ * are of different groups. */
+struct beam_groups {
+    float least;
+    int count;
+};
+__device__ __forceinline__ beam_groups beam_bound(float v, int log)
+{
+    const int most = 6 - log;
+    auto step = [&](int i, float o) { v = i < most ? fmaxf(v, o) : fminf(v, o); };
+    beam_groups r = { 0.f, 0 };
+    auto meet = [&](int i) { /* the groups are whole */
+        if (i != most) return;
+        r.count = __builtin_popcountll(__builtin_amdgcn_ballot_w64(v > -INFINITY)) >> most;
+        v = v > -INFINITY ? v : INFINITY;
+    };
+    step(0, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xF, 0xF, false))); /* lanes 1 0 3 2 */
+    step(1, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xF, 0xF, false))); /* 2 3 0 1 */
+    meet(2);
+    step(2, lane_xor4(v));
+    meet(3);
+    step(3, lane_xor8(v));
+    meet(4);
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(s[0]);
+    step(4, __uint_as_float(s[1]));
+    meet(5);
+    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(t[0]);
+    step(5, __uint_as_float(t[1]));
+    meet(6);
+    r.least = v;
+    return r;
+}
+/* The groups of a wave that make n of `full` waves (16 at most, then there are fewer than n). */
+__device__ __forceinline__ int beam_groups_log(int n, int full) { return n <= full ? 0 : n <= 2 * full ? 1 : n <= 4 * full ? 2 : n <= 8 * full ? 3 : 4; }
+/* The work-group's bound from those of its waves: -infinity where they have fewer than n groups. */
+__device__ __forceinline__ float beam_bound_of(const float *least, const int *count, int n)
+{
+    float v = INFINITY;
+    int all = 0;
+#pragma unroll
+    for (int i = 0; i < BEAM_WAVES; ++i) {
+        v = fminf(v, least[i]);
+        all += count[i];
+    }
+    return all >= n ? v : -INFINITY;
+}
+/* How many of LDS's first n keys are above k, and how many are k; the list is a multiple of 8 long, 0 behind the n-th. */
+__device__ __forceinline__ int beam_rank(const unsigned long long *list, int n, unsigned long long k, int &same)
+{
+    typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+    int at = 0;
+    same = 0;
+    for (int j = 0; j < n; j += 8) {
+        u64x2 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = *(const u64x2 *)(list + j + 2 * i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            at += (v[i][0] > k) + (v[i][1] > k);
+            same += (v[i][0] == k) + (v[i][1] == k);
+        }
+    }
+    return at;
+}
 
 union beam_lds {
     struct {
-        float top[4], sum[4], bound[4];
-        unsigned long long list[BEAM_LIST];
+        alignas(16) float top[BEAM_WAVES], sum[BEAM_WAVES], bound[BEAM_WAVES];
+        alignas(16) int groups[BEAM_WAVES];
+        alignas(16) unsigned long long list[BEAM_LIST + 8];
     } slice;
     struct {
         double lse[G2B_MAX_BEAMS]; /* score - log sum exp; NaN: no continuations */
-        unsigned long long list[BEAM_LIST];
+        alignas(16) unsigned long long list[BEAM_LIST + 8];
         unsigned flat[BEAM_LIST];
-        unsigned long long bound;
+        alignas(16) float bound[BEAM_WAVES];
+        alignas(16) int groups[BEAM_WAVES];
+        /* (below: what is taken one by one) */
+        unsigned long long best[BEAM_WAVES];
+        unsigned best_flat[BEAM_WAVES];
     } pick;
 };
 
-/* The last of a group's work-groups: the n_out best of all its slices' candidates. */
-template <int SLICE>
-__device__ void beam_pick(const g2_beam_args &a, long g, beam_lds &lds, int *count)
+/* The last of a group's work-groups: the n_out best of all its slices' candidates.
+ * One work-group, once: what it costs are its waits for memory (one, for sums and
+ * candidates together) and instructions that no one has run before. */
+__device__ void beam_pick(const g2_beam_args &a, unsigned g, beam_lds &lds, int *count)
 {
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const long row0 = g * a.beams;
-    for (int b = w; b < a.beams; b += 4) {
-        const unsigned long long *st = a.stats + (row0 + b) * a.slices;
-        float top = -INFINITY;
-        for (int i = lane; i < a.slices; i += 64) top = fmaxf(top, __uint_as_float((unsigned)ld_agent64(st + i)));
-        top = wave_max(top);
-        const double base = top == -INFINITY ? 0.0 : (double)top;
-        double sum = 0.0;
-        for (int i = lane; i < a.slices; i += 64) {
-            const unsigned long long v = ld_agent64(st + i);
-            sum += (double)__uint_as_float((unsigned)(v >> 32)) * exp((double)__uint_as_float((unsigned)v) - base);
-        }
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = a.n_out;
+    const unsigned row0 = g * (unsigned)a.beams, beams = (unsigned)a.beams, slices = (unsigned)a.slices;
+    /* candidate c: entry c % n of a list; the beams' first slices first, so that a group
+     * of the bound has candidates of several beams; behind them the ended beams as they are */
+    const unsigned listed = beams * slices * (unsigned)n, all = a.done ? listed + beams : listed;
+    auto load = [&](unsigned c, unsigned &beam) {
+        const unsigned l = c / (unsigned)n, s = l / beams;
+        beam = l - s * beams;
+        return ld_agent64(a.cands + ((size_t)(row0 + beam) * slices + s) * (unsigned)n + (c - l * (unsigned)n));
+    };
+    unsigned beam0 = 0;
+    const unsigned long long key0 = (unsigned)tid < listed ? load((unsigned)tid, beam0) : 0;
+#pragma unroll 1
+    for (int b = w; b < a.beams; b += BEAM_WAVES) { /* (a row has 64 slices at most) */
+        const unsigned long long v = lane < a.slices ? ld_agent64(a.stats + (size_t)(row0 + (unsigned)b) * slices + (unsigned)lane) : 0xFF800000ull;
+        const float top = __uint_as_float((unsigned)v), most = lanes_max(top);
+        double sum = (double)(__uint_as_float((unsigned)(v >> 32)) * (top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((top - most) * 1.44269504f)));
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
         if (lane == 0)
-            lds.pick.lse[b] = a.done && a.done[row0 + b] ? __longlong_as_double(0x7ff8000000000000ll) : (double)a.score[row0 + b] - ((double)top + log(sum));
+            lds.pick.lse[b] = a.done && a.done[row0 + (unsigned)b] ? __longlong_as_double(0x7ff8000000000000ll) : (double)a.score[row0 + (unsigned)b] - ((double)most + log(sum));
     }
-    if (tid == 0) { lds.pick.bound = 1; *count = 0; }
+    if (tid == 0) *count = 0;
     __syncthreads();
-    /* list l: a slice's candidates, greatest first, or (behind them) an ended beam as it is */
-    const int slices = a.beams * a.slices, lists = slices + a.beams, n = a.n_out;
-    const unsigned long long *cands = a.cands + row0 * a.slices * n;
-    auto get = [&](int l, int j) {
-        beam_cand c = { 0, ~0u };
-        if (l < slices) {
-            const unsigned long long k = ld_agent64(cands + (long)l * n + j);
-            const int b = l / a.slices;
-            const double t = (double)key_logit(k) + lds.pick.lse[b];
-            if (k && t > -INFINITY) {
-                c.k = double_key(t);
-                c.f = (unsigned)b * (unsigned)a.V + ~(unsigned)k;
-            }
-        } else if (l < lists && j == 0 && a.done) {
-            const int b = l - slices;
-            const float score = a.score[row0 + b];
-            if (a.done[row0 + b] && score > -INFINITY) {
-                c.k = double_key((double)score);
-                c.f = (unsigned)b * (unsigned)a.V + (unsigned)a.eos;
-            }
-        }
+    auto cand = [&](unsigned beam, unsigned long long k) { /* from its logit's key */
+        const double t = (double)key_logit(k) + lds.pick.lse[beam];
+        beam_cand c = { 0, beam << BEAM_ID_BITS | ((1u << BEAM_ID_BITS) - 1 & ~(unsigned)k) };
+        if (k && t > -INFINITY) c.k = double_key(t);
         return c;
     };
-    unsigned long long best = 0;
-    for (int l = tid; l < lists; l += 256) {
-        const unsigned long long k = get(l, 0).k;
-        best = k > best ? k : best;
-    }
-    lds.pick.list[tid] = best;
-    __syncthreads();
-    int above = 0;
-    for (int i = 0; i < 256; ++i) {
-        const unsigned long long k = lds.pick.list[i];
-        above += k > best || (k == best && i < tid);
-    }
-    if (above == n - 1 && best) lds.pick.bound = best;
-    __syncthreads();
-    const unsigned long long bound = lds.pick.bound;
-    for (int l = tid; l < lists; l += 256)
-        for (int j = 0; j < n; ++j) {
-            const beam_cand c = get(l, j);
-            if (c.k < bound) break;
-            const int at = atomicAdd(count, 1);
-            if (at < BEAM_LIST) { lds.pick.list[at] = c.k; lds.pick.flat[at] = c.f; }
+    auto get = [&](unsigned c) {
+        unsigned beam;
+        if (c < listed) {
+            const unsigned long long k = load(c, beam);
+            return cand(beam, k);
         }
+        beam = c - listed;
+        beam_cand e = { 0, beam << BEAM_ID_BITS | (unsigned)a.eos };
+        const float score = a.score[row0 + beam];
+        if (a.done[row0 + beam] && score > -INFINITY) e.k = double_key((double)score);
+        return e;
+    };
+    beam_cand c0 = { 0, 0 };
+    if ((unsigned)tid < listed) c0 = cand(beam0, key0);
+    else if ((unsigned)tid < all) c0 = get((unsigned)tid);
+    float best = c0.k ? (float)key_double(c0.k) : -INFINITY;
+#pragma unroll 1
+    for (unsigned c = (unsigned)tid + BEAM_THREADS; c < all; c += BEAM_THREADS) {
+        const beam_cand x = get(c);
+        if (x.k) best = fmaxf(best, (float)key_double(x.k));
+    }
+    const int full = min((int)(listed / 64), BEAM_WAVES);
+    beam_groups own = { INFINITY, 0 };
+    if (w < full) own = beam_bound(best, beam_groups_log(n, full));
+    if (lane == 0) { lds.pick.bound[w] = own.least; lds.pick.groups[w] = own.count; }
+    __syncthreads();
+    /* (rounded to 32 bits a total keeps its place among the others, but for equal ones) */
+    const float bound = beam_bound_of(lds.pick.bound, lds.pick.groups, n);
+    auto reaches = [&](const beam_cand &c) { return c.k && (float)key_double(c.k) >= bound; };
+    auto add = [&](const beam_cand &c) {
+        if (!reaches(c)) return;
+        const int at = atomicAdd(count, 1);
+        if (at < BEAM_LIST) { lds.pick.list[at] = c.k; lds.pick.flat[at] = c.f; }
+    };
+    add(c0);
+#pragma unroll 1
+    for (unsigned c = (unsigned)tid + BEAM_THREADS; c < all; c += BEAM_THREADS) add(get(c));
     __syncthreads();
     const int total = *count;
     auto put = [&](int i, const beam_cand &c) {
-        const long at = g * n + i;
-        const int parent = c.k ? (int)(c.f / (unsigned)a.V) : -1, id = c.k ? (int)(c.f % (unsigned)a.V) : -1;
+        const size_t at = (size_t)g * (unsigned)n + (unsigned)i;
+        const int parent = c.k ? (int)(c.f >> BEAM_ID_BITS) : -1, id = c.k ? (int)(c.f & ((1u << BEAM_ID_BITS) - 1)) : -1;
         a.out_score[at] = c.k ? (float)key_double(c.k) : -INFINITY;
         a.out_parent[at] = parent;
         a.out_id[at] = id;
-        if (a.out_done) a.out_done[at] = c.k && (id == a.eos || (a.done && a.done[row0 + parent]));
+        if (a.out_done) a.out_done[at] = c.k && (id == a.eos || (a.done && a.done[row0 + (unsigned)parent]));
     };
     const beam_cand none = { 0, ~0u };
     if (total <= BEAM_LIST) {
-        for (int i = tid; i < total; i += 256) {
-            const beam_cand c = { lds.pick.list[i], lds.pick.flat[i] };
-            int at = 0;
-            for (int j = 0; j < total; ++j) {
-                const beam_cand o = { lds.pick.list[j], lds.pick.flat[j] };
-                at += beam_above(o, c);
-            }
+        if (tid < 8) lds.pick.list[total + tid] = 0;
+        __syncthreads();
+        if (tid < total) {
+            const beam_cand c = { lds.pick.list[tid], lds.pick.flat[tid] };
+            int same, at = beam_rank(lds.pick.list, total, c.k, same);
+            if (same > 1 && at < n)
+#pragma unroll 1
+                for (int j = 0; j < total; ++j) at += lds.pick.list[j] == c.k && lds.pick.flat[j] < c.f;
             if (at < n) put(at, c);
-        }
-        for (int i = total + tid; i < n; i += 256) put(i, none);
+        } else if (tid < n) put(tid, none);
         return;
     }
     beam_cand last = { ~0ull, 0 };
+#pragma unroll 1
     for (int i = 0; i < n; ++i) { /* one by one: the best that is below the last one */
         beam_cand c = none;
-        for (int l = tid; l < lists; l += 256)
-            for (int j = 0; j < n; ++j) {
-                const beam_cand x = get(l, j);
-                if (x.k < bound) break;
-                if ((i == 0 || beam_above(last, x)) && beam_above(x, c)) c = x;
-            }
+#pragma unroll 1
+        for (unsigned l = (unsigned)tid; l < all; l += BEAM_THREADS) {
+            const beam_cand x = get(l);
+            if (reaches(x) && (i == 0 || beam_above(last, x)) && beam_above(x, c)) c = x;
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const beam_cand x = { __shfl_xor(c.k, o), __shfl_xor(c.f, o) };
+            if (beam_above(x, c)) c = x;
+        }
         __syncthreads();
-        lds.pick.list[tid] = c.k;
-        lds.pick.flat[tid] = c.f;
+        if (lane == 0) { lds.pick.best[w] = c.k; lds.pick.best_flat[w] = c.f; }
         __syncthreads();
-        for (int t = 0; t < 256; ++t) {
-            const beam_cand x = { lds.pick.list[t], lds.pick.flat[t] };
+        for (int t = 0; t < BEAM_WAVES; ++t) {
+            const beam_cand x = { lds.pick.best[t], lds.pick.best_flat[t] };
             if (beam_above(x, c)) c = x;
         }
         if (tid == 0) put(i, c);
-        last = c; /* (at least n reach the bound) */
+        last = c.k ? c : beam_cand{ 1, 0 }; /* (no key is 1: nothing is left) */
     }
 }
 
@@ -946,17 +1039,17 @@ __device__ void beam_pick(const g2_beam_args &a, long g, beam_lds &lds, int *cou
 template <int QUADS>
 __device__ void beam_select_impl(const g2_beam_args &a)
 {
-    constexpr int SLICE = 1024 * QUADS, Q = 4 * QUADS;
+    constexpr int SLICE = 4 * BEAM_THREADS * QUADS, Q = 4 * QUADS;
     __shared__ beam_lds lds;
     __shared__ int count, last;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = a.n_out;
-    const long row = blockIdx.x / a.slices;
-    const int slice = blockIdx.x % a.slices, v0 = slice * SLICE, nv = min(a.V - v0, SLICE);
-    const float *in = a.logits + row * a.V + v0;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = a.n_out;
+    const unsigned row = blockIdx.x / (unsigned)a.slices, slice = blockIdx.x - row * (unsigned)a.slices;
+    const int v0 = (int)slice * SLICE, nv = min(a.V - v0, SLICE);
+    const float *in = a.logits + (size_t)row * (unsigned)a.V + v0;
     float x[Q];
 #pragma unroll
     for (int q = 0; q < QUADS; ++q) {
-        const int i = 4 * (tid + 256 * q);
+        const int i = 4 * (tid + BEAM_THREADS * q);
         if (i + 4 <= nv) {
             const f32x4 v = *(const f32x4u *)(in + i);
 #pragma unroll
@@ -973,37 +1066,33 @@ __device__ void beam_select_impl(const g2_beam_args &a)
     float sum = 0.f; /* (NaN where a logit is; ids behind the row add nothing) */
 #pragma unroll
     for (int q = 0; q < Q; ++q) sum += __builtin_amdgcn_exp2f((x[q] - base) * 1.44269504f);
-    sum = wave_sum(sum);
-    /* the n-th greatest of the lanes' greatest, equal ones together */
-    float bound = -INFINITY;
-    int left = n;
-    for (float v = mine; left > 0;) {
-        bound = lanes_max(v);
-        if (!(bound > -INFINITY)) break;
-        left -= __builtin_popcountll(__builtin_amdgcn_ballot_w64(v == bound));
-        v = v == bound ? -INFINITY : v;
-    }
-    if (lane == 0) { lds.slice.top[w] = top; lds.slice.sum[w] = sum; lds.slice.bound[w] = bound; }
+    sum = lanes_sum(sum);
+    /* (groups of the waves that have ids for every lane; without one the slice is short) */
+    const int full = min(nv / 256, BEAM_WAVES);
+    beam_groups own = { INFINITY, 0 };
+    if (w < full) own = beam_bound(mine, beam_groups_log(n, full));
+    if (lane == 0) { lds.slice.top[w] = top; lds.slice.sum[w] = sum; lds.slice.bound[w] = own.least; lds.slice.groups[w] = own.count; }
     __syncthreads();
-    bound = fmaxf(fmaxf(lds.slice.bound[0], lds.slice.bound[1]), fmaxf(lds.slice.bound[2], lds.slice.bound[3]));
+    const float bound = beam_bound_of(lds.slice.bound, lds.slice.groups, n);
 #pragma unroll
     for (int q = 0; q < Q; ++q)
         if (x[q] >= bound && x[q] > -INFINITY) {
             const int at = atomicAdd(&count, 1);
-            if (at < BEAM_LIST) lds.slice.list[at] = logit_key(x[q], v0 + 4 * (tid + 256 * (q / 4)) + q % 4);
+            if (at < BEAM_LIST) lds.slice.list[at] = logit_key(x[q], v0 + 4 * (tid + BEAM_THREADS * (q / 4)) + q % 4);
         }
     __syncthreads();
     const int total = count;
-    const long cell = row * a.slices + slice;
-    unsigned long long *cands = a.cands + cell * n;
+    const size_t cell = blockIdx.x;
+    unsigned long long *cands = a.cands + cell * (unsigned)n;
     if (total <= BEAM_LIST) {
-        for (int i = tid; i < total; i += 256) {
-            const unsigned long long k = lds.slice.list[i];
-            int at = 0;
-            for (int j = 0; j < total; ++j) at += lds.slice.list[j] > k;
+        if (tid < 8) lds.slice.list[total + tid] = 0;
+        __syncthreads();
+        if (tid < total) {
+            const unsigned long long k = lds.slice.list[tid];
+            int same; /* (one: ids differ) */
+            const int at = beam_rank(lds.slice.list, total, k, same);
             if (at < n) st_agent64(cands + at, k);
-        }
-        for (int i = total + tid; i < n; i += 256) st_agent64(cands + i, 0);
+        } else if (tid < n) st_agent64(cands + tid, 0);
     } else {
         unsigned long long below = ~0ull;
         for (int i = 0; i < n; ++i) { /* one by one: the greatest key below the last one */
@@ -1011,36 +1100,46 @@ __device__ void beam_select_impl(const g2_beam_args &a)
 #pragma unroll
             for (int q = 0; q < Q; ++q)
                 if (x[q] > -INFINITY) {
-                    const unsigned long long y = logit_key(x[q], v0 + 4 * (tid + 256 * (q / 4)) + q % 4);
+                    const unsigned long long y = logit_key(x[q], v0 + 4 * (tid + BEAM_THREADS * (q / 4)) + q % 4);
                     k = y < below && y > k ? y : k;
                 }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) {
+                const unsigned long long y = __shfl_xor(k, o);
+                k = y > k ? y : k;
+            }
             __syncthreads();
-            lds.slice.list[tid] = k;
+            if (lane == 0) lds.slice.list[w] = k;
             __syncthreads();
-            for (int t = 0; t < 256; ++t) k = lds.slice.list[t] > k ? lds.slice.list[t] : k;
+            for (int t = 0; t < BEAM_WAVES; ++t) k = lds.slice.list[t] > k ? lds.slice.list[t] : k;
             if (tid == 0) st_agent64(cands + i, k);
             below = k;
         }
     }
     if (tid == 0) {
         float m = -INFINITY, l = 0.f;
-        for (int i = 0; i < 4; ++i) m = fmaxf(m, lds.slice.top[i]);
-        for (int i = 0; i < 4; ++i) l += lds.slice.sum[i] * (lds.slice.top[i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((lds.slice.top[i] - m) * 1.44269504f));
+#pragma unroll
+        for (int i = 0; i < BEAM_WAVES; ++i) m = fmaxf(m, lds.slice.top[i]);
+#pragma unroll
+        for (int i = 0; i < BEAM_WAVES; ++i) l += lds.slice.sum[i] * (lds.slice.top[i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((lds.slice.top[i] - m) * 1.44269504f));
         st_agent64(a.stats + cell, (unsigned long long)__float_as_uint(l) << 32 | __float_as_uint(m));
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    const long g = row / a.beams;
+    const unsigned g = row / (unsigned)a.beams;
     if (tid == 0) {
-        unsigned *cell = a.counts + g * G2B_COUNT_INTS;
+        unsigned *cell = a.counts + (size_t)g * G2B_COUNT_INTS;
         last = __hip_atomic_fetch_add(cell, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(a.beams * a.slices) - 1;
         if (last) __hip_atomic_store(cell, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (last) beam_pick<SLICE>(a, g, lds, &count);
+    if (last) beam_pick(a, g, lds, &count);
 }
-G2K void g2k_beam_select(const g2_beam_args a) { beam_select_impl<1>(a); }
-G2K void g2k_beam_select_wide(const g2_beam_args a) { beam_select_impl<4>(a); }
+#define BEAM_SELECT(NAME, QUADS) \
+    extern "C" __global__ __launch_bounds__(BEAM_THREADS) void NAME(const g2_beam_args a) { beam_select_impl<QUADS>(a); }
+BEAM_SELECT(g2k_beam_select1, 1)
+BEAM_SELECT(g2k_beam_select4, 4)
+BEAM_SELECT(g2k_beam_select7, 7)
 
 /* Rows of the tables in their parents' order, 256 ints of a row to a work-group. */
 G2K void g2k_beam_copy(const g2_beam_move_args a)

@@ -95,11 +95,10 @@ G2B_FN void g2b_prompt_item(long b, int NKV, long tiles, int *head, long *tile)
     *head = j < fixed ? j / 8 * 8 + x : fixed + j % 8;
 }
 
-/* ---- beam search: ids of a work-group's slice of a row (narrow and wide form),
+/* ---- beam search: ids of a work-group's slice of a row,
  * most beams and continuations of a group; ints from count to count (a cache
  * line: the work-groups of a group meet there) */
-#define G2B_SLICE 1024
-#define G2B_SLICE_WIDE 4096
+#define G2B_SLICE 4096 /* times 1, 4 or 7 */
 #define G2B_MAX_BEAMS 32
 #define G2B_MAX_OUT 64
 #define G2B_COUNT_INTS 16

@@ -129,8 +129,8 @@ extern "C" {
     X(KV4_APPEND_F16, "g2k_kv4_append_f16") X(KV4_READ, "g2k_kv4_read")       \
     X(KV4_ATTN1, "g2k_kv4_attn1") X(KV4_ATTN2, "g2k_kv4_attn2")               \
     X(KV4_ATTN4, "g2k_kv4_attn4") X(KV4_JOIN, "g2k_kv4_join")                 \
-    X(BEAM_SELECT, "g2k_beam_select")                                         \
-    X(BEAM_SELECT_WIDE, "g2k_beam_select_wide")                               \
+    X(BEAM_SELECT1, "g2k_beam_select1") X(BEAM_SELECT4, "g2k_beam_select4")   \
+    X(BEAM_SELECT7, "g2k_beam_select7")                                       \
     X(BEAM_COPY, "g2k_beam_copy") X(BEAM_MOVE, "g2k_beam_move")
 
 #define G2_ENUM_ENTRY(id, name) G2F_##id,
@@ -225,7 +225,7 @@ int g2i_prompt_form(int rows, int n_head, int n_kv, long *tiles);
  * a pass over them and passes to a key head. */
 int g2i_kv4_form(int n_seq, int n_head, int n_kv, int T_kv, int *heads, int *chunks, int *span);
 
-/* Whether g2_beam_select takes its wide form, and the slices of a row. */
+/* 4096 ids to a slice of g2_beam_select times this (1, 4, 7), and the slices of a row. */
 int g2i_beam_form(int rows, int V, int *slices);
 
 /* Whether np bytes at p and nq bytes at q share any. */

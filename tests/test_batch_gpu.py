@@ -467,7 +467,8 @@ def check_select(g2, logits, score, done, eos, beams, n_out):
 
 @pytest.mark.parametrize("G,beams,V,n_out", [(1, 1, 1, 1), (1, 1, 5, 8), (2, 3, 7, 4), (1, 4, 4095, 4), (3, 5, 4096, 10), (2, 2, 4097, 2), (1, 8, 50257, 8),
                                              (5, 8, 9000, 16), (1, 32, 1000, 64), (2, 32, 5000, 32), (1, 1, 50257, 64), (40, 4, 300, 4), (1, 3, 262144, 5),
-                                             (65, 16, 700, 16), (4, 8, 50257, 8), (300, 4, 1030, 3), (33, 1, 33000, 64)])
+                                             (65, 16, 700, 16), (4, 8, 50257, 8), (300, 4, 1030, 3), (33, 1, 33000, 64), (600, 1, 1000, 5), (4, 6, 50257, 20),
+                                             (2, 3, 260, 33), (1, 2, 520, 64), (70, 8, 29000, 9), (12, 8, 10000, 8)])
 def test_select(g2, G, beams, V, n_out):
     r = rng(G, beams, V, n_out)
     logits = 3 * r.standard_normal((G * beams, V))
