@@ -160,20 +160,22 @@ int g2_kv4_read(const void *cache, float *k, float *v, const int *origin, const 
 }
 
 /* Query heads to a pass over their key head's positions, passes to a key head,
- * parts of the positions and tiles to a part. */
-int g2i_kv4_form(int n_seq, int n_head, int n_kv, int T_kv, int *heads, int *chunks, int *span)
+ * parts of the positions and tiles to a part, waves to a work-group. */
+int g2i_kv4_form(int n_seq, int n_head, int n_kv, int T_kv, int *heads, int *chunks, int *span, int *waves)
 {
     const int group = n_head / n_kv;
-    *chunks = (group + 3) / 4;
+    const long tiles = g2b_tiles(T_kv) > 0 ? g2b_tiles(T_kv) : 1;
+    int most = 4;
+    *chunks = (group + most - 1) / most;
     *heads = (group + *chunks - 1) / *chunks;
-    const long tiles = g2b_tiles(T_kv) > 0 ? g2b_tiles(T_kv) : 1, wgs = (long)n_seq * n_kv * *chunks;
+    const long wgs = (long)n_seq * n_kv * *chunks;
     long splits = 1;
-    if (tiles > 8 && wgs < 512) {
-        splits = tiles / 8 < 1024 / wgs ? tiles / 8 : 1024 / wgs;
+    if (tiles > 32 && wgs < 256) {
+        splits = tiles / 8 < 512 / wgs ? tiles / 8 : 512 / wgs;
         if (splits > G2B_SPLITS) splits = G2B_SPLITS;
-        if (splits < 1) splits = 1;
     }
     *span = (int)((tiles + splits - 1) / splits);
+    *waves = *span <= 2 && *heads == 1 ? 1 : *span <= 8 ? 4 : 8;
     return (int)((tiles + *span - 1) / *span);
 }
 
@@ -205,10 +207,13 @@ int g2_attn_kv4(const float *q, int q_stride, const void *cache, float *out, int
     a.q_stride = n_seq > 1 ? q_stride : 0; a.out_stride = n_seq > 1 ? out_stride : 0;
     a.T_kv = T_kv; a.S = n_seq; a.NH = n_head; a.NKV = n_kv; a.max_seq = max_seq; a.tiles = (int)g2b_tiles(max_seq);
     a.scale = scale;
-    a.splits = g2i_kv4_form(n_seq, n_head, n_kv, T_kv, &a.heads, &a.chunks, &a.span);
-    const int fid = a.heads == 1 ? G2F_KV4_ATTN1 : a.heads == 2 ? G2F_KV4_ATTN2 : G2F_KV4_ATTN4;
-    rc = g2i_launch(fid, (unsigned)((long)n_seq * n_kv * a.chunks * a.splits), 1, 256, &a);
-    if (!rc && a.splits > 1) rc = g2i_launch(G2F_KV4_JOIN, cdiv((long)n_seq * n_head, 4), 1, 256, &a);
+    int waves;
+    a.splits = g2i_kv4_form(n_seq, n_head, n_kv, T_kv, &a.heads, &a.chunks, &a.span, &waves);
+    const int fid = a.heads == 1 ? (waves == 1 ? G2F_KV4_ATTN1_1 : waves == 4 ? G2F_KV4_ATTN1_4 : G2F_KV4_ATTN1_8)
+                  : a.heads == 2 ? (waves == 4 ? G2F_KV4_ATTN2_4 : G2F_KV4_ATTN2_8)
+                                 : (waves == 4 ? G2F_KV4_ATTN4_4 : G2F_KV4_ATTN4_8);
+    rc = g2i_launch(fid + (origin ? 1 : 0), (unsigned)((long)n_seq * n_kv * a.chunks * a.splits), 1, 64u * (unsigned)waves, &a);
+    if (!rc && a.splits > 1) rc = g2i_launch(G2F_KV4_JOIN, (unsigned)(n_seq * n_head), 1, 256, &a);
     return rc;
 }
 

@@ -607,88 +607,161 @@ G2K void g2k_kv4_read(const g2_kv4_read_args a)
     }
 }
 
-/* ---- single-query attention.  A wave takes 64 / LP positions at a time, LP
- * lanes of DL = 64 / LP dims to a position, for G query heads that share a key
- * head; each position slot keeps a running maximum and sum of its own. */
-template <int G, int LP>
+/* ---- single-query attention.  A wave takes U times 64 / LP positions at a time,
+ * LP lanes of DL = 64 / LP dims to a position, for G query heads that share a key
+ * head: codes are used where they were loaded, a score is the sum over LP lanes,
+ * and each position slot keeps a running maximum and sum of its own, which
+ * follows the maximum only where it grew by more than 2^8.  The slots meet once,
+ * at the end: over the lanes, over the waves in LDS, and over the parts of a long
+ * sequence in a second launch.  The next positions' loads go out before the last
+ * ones' sums. */
+template <int W, int U> struct kv4_in {
+    unsigned k[U][W], v[U][W];
+    unsigned ks[U], vs[U]; /* bf16 */
+    bool there[U];
+};
+
+template <int G, int LP, int NW, int U, bool ORIGIN>
 __device__ void kv4_attn_impl(const g2_kv4_attn_args &a)
 {
-    constexpr int DL = 64 / LP, SLOTS = 64 / LP, W = DL / 8, NW = 4;
+    constexpr int DL = 64 / LP, SLOTS = 64 / LP, W = DL / 8, STEP = SLOTS * U;
+    typedef unsigned words __attribute__((ext_vector_type(W)));
     __shared__ float part[NW][G][G2B_PART_FLOATS];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int slot = lane / LP, d0 = DL * (lane % LP);
-    const int split = blockIdx.x % a.splits, ch = blockIdx.x / a.splits % a.chunks;
-    const int hk = blockIdx.x / a.splits / a.chunks % a.NKV;
-    const long s = blockIdx.x / a.splits / a.chunks / a.NKV;
-    const int group = a.NH / a.NKV, h0 = hk * group + ch * a.heads;
-    const int nh = min(a.heads, group - ch * a.heads);
-    const int len = kv8_length(a.len, a.T_kv, s);
-    const int p0 = split * a.span * G2B_TILE, p1 = min(len, p0 + a.span * G2B_TILE);
+    const unsigned split = blockIdx.x % (unsigned)a.splits, rest = blockIdx.x / (unsigned)a.splits;
+    const int ch = (int)(rest % (unsigned)a.chunks), hk = (int)(rest / (unsigned)a.chunks % (unsigned)a.NKV);
+    const int s = (int)(rest / (unsigned)a.chunks / (unsigned)a.NKV);
+    const int group = a.NH / a.NKV, h0 = hk * group + ch * a.heads, nh = min(a.heads, group - ch * a.heads);
+    const int len = __builtin_amdgcn_readfirstlane(kv8_length(a.len, a.T_kv, s));
+    const int p0 = (int)split * a.span * G2B_TILE, p1 = min(len, p0 + a.span * G2B_TILE);
+    const unsigned char *cache = a.cache + g2b_tile_at(a.NKV, a.tiles, s, hk, 0);
+    const size_t seq = (size_t)a.NKV * (unsigned)a.tiles * G2B_TILE_BYTES;
+    const unsigned code0 = (unsigned)d0 / 2, scale0 = (unsigned)d0 / 32 * 2;
+    int from[U]; /* of the step that is loaded next */
+    auto origins = [&](int b) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int p = b + u * SLOTS + slot;
+            from[u] = p < p1 ? a.origin[(size_t)(unsigned)s * (unsigned)a.max_seq + (unsigned)p] : -1;
+        }
+    };
+    typedef kv4_in<W, U> in_t;
+    auto load = [&](in_t &x, int b) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int bu = min(b + u * SLOTS, p1 - 1) / SLOTS * SLOTS, p = b + u * SLOTS + slot, i = (bu + slot) % G2B_TILE;
+            const unsigned char *t;
+            if constexpr (ORIGIN) {
+                x.there[u] = (unsigned)from[u] < (unsigned)a.S;
+                t = a.cache + g2b_tile_at(a.NKV, a.tiles, 0, hk, bu / G2B_TILE) + (size_t)(x.there[u] ? (unsigned)from[u] : 0u) * seq;
+            } else {
+                x.there[u] = p < p1;
+                t = cache + (size_t)(unsigned)(bu / G2B_TILE) * G2B_TILE_BYTES;
+            }
+            const words *kp = (const words *)(t + (g2b_code_at(0, i) + code0)), *vp = (const words *)(t + (g2b_code_at(1, i) + code0));
+            words k, v;
+            if constexpr (ORIGIN) { k = *kp; v = *vp; }
+            else { k = __builtin_nontemporal_load(kp); v = __builtin_nontemporal_load(vp); }
+#pragma unroll
+            for (int j = 0; j < W; ++j) { x.k[u][j] = k[j]; x.v[u][j] = v[j]; }
+            x.ks[u] = *(const uint16_t *)(t + (g2b_scale_at(0, i) + scale0));
+            x.vs[u] = *(const uint16_t *)(t + (g2b_scale_at(1, i) + scale0));
+        }
+    };
     float q[G][DL], o[G][DL], m[G], l[G];
     const float qf = a.scale * 1.44269504f;
 #pragma unroll
     for (int i = 0; i < G; ++i) {
-        const float *p = a.q + s * a.q_stride + (h0 + min(i, nh - 1)) * G2B_DH + d0;
+        const float *p = a.q + (size_t)(unsigned)s * (unsigned)a.q_stride + (h0 + min(i, nh - 1)) * G2B_DH + d0;
 #pragma unroll
         for (int e = 0; e < DL; e += 4) {
             const f32x4 v = *(const f32x4u *)(p + e);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) q[i][e + j] = v[j] * qf;
+            for (int j = 0; j < 4; ++j) q[i][e + j] = v[j];
         }
+    }
+    in_t next;
+    int b = p0 + STEP * w;
+    if (b < p1) {
+        if constexpr (ORIGIN) origins(b);
+        load(next, b);
+        if constexpr (ORIGIN) origins(b + STEP * NW);
+    }
 #pragma unroll
-        for (int e = 0; e < DL; ++e) o[i][e] = 0.f;
+    for (int i = 0; i < G; ++i) {
+#pragma unroll
+        for (int e = 0; e < DL; ++e) { q[i][e] *= qf; o[i][e] = 0.f; }
         m[i] = -INFINITY;
         l[i] = 0.f;
     }
-    for (int b = p0 + SLOTS * w; b < p1; b += SLOTS * NW) {
-        const int p = b + slot;
-        const int from = p < p1 ? a.origin ? a.origin[s * a.max_seq + p] : (int)s : -1;
-        const bool there = from >= 0 && from < a.S;
-        const int pc = there ? p : b;
-        const unsigned char *t = a.cache + g2b_tile_at(a.NKV, a.tiles, there ? from : s, hk, pc / G2B_TILE);
-        unsigned kc[W], vc[W];
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-            kc[i] = *(const unsigned *)(t + g2b_code_at(0, pc % G2B_TILE) + d0 / 2 + 4 * i);
-            vc[i] = *(const unsigned *)(t + g2b_code_at(1, pc % G2B_TILE) + d0 / 2 + 4 * i);
+    for (; b < p1; b += STEP * NW) {
+        const in_t x = next;
+        if (b + STEP * NW < p1) {
+            load(next, b + STEP * NW);
+            if constexpr (ORIGIN) origins(b + 2 * STEP * NW);
         }
-        const float ks = bf16_f(*(const uint16_t *)(t + g2b_scale_at(0, pc % G2B_TILE) + d0 / 32 * 2));
-        const float vs = there ? bf16_f(*(const uint16_t *)(t + g2b_scale_at(1, pc % G2B_TILE) + d0 / 32 * 2)) : 0.f;
-        float x[G], pr[G];
+        float sc[U][G];
 #pragma unroll
-        for (int i = 0; i < G; ++i) x[i] = 0.f;
+        for (int u = 0; u < U; ++u) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-            float v[8];
-            q4_values(kc[i], 1.f, v);
+            for (int j = 0; j < G; ++j) sc[u][j] = 0.f;
 #pragma unroll
-            for (int j = 0; j < G; ++j)
+            for (int i = 0; i < W; ++i) {
+                float v[8];
+                q4_values(x.k[u][i], 1.f, v);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[j] = fmaf(q[j][8 * i + e], v[e], x[j]);
+                for (int j = 0; j < G; ++j)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sc[u][j] = fmaf(q[j][8 * i + e], v[e], sc[u][j]);
+            }
+        }
+        bool grew = false;
+        float top[G];
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+            top[j] = m[j];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float d = sc[u][j] * __uint_as_float(x.ks[u] << 16);
+                d += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(d), 0xB1, 0xF, 0xF, false)); /* lanes 1 0 3 2 */
+                if (LP == 4) d += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(d), 0x4E, 0xF, 0xF, false));
+                sc[u][j] = x.there[u] ? d : -INFINITY;
+                top[j] = fmaxf(top[j], sc[u][j]);
+            }
+            grew |= top[j] > m[j] + 8.f; /* (an empty state's maximum is -infinity) */
+        }
+        if (wave_any(grew)) {
+#pragma unroll
+            for (int j = 0; j < G; ++j) {
+                const float f = kv8_factor(m[j], top[j]);
+                m[j] = top[j];
+                l[j] *= f;
+#pragma unroll
+                for (int e = 0; e < DL; ++e) o[j][e] *= f;
+            }
         }
 #pragma unroll
-        for (int i = 0; i < G; ++i) {
-            float d = x[i] * ks;
-            d += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(d), 0xB1, 0xF, 0xF, false)); /* lanes 1 0 3 2 */
-            if (LP == 4) d += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(d), 0x4E, 0xF, 0xF, false));
-            if (!there) d = -INFINITY;
-            const float top = fmaxf(m[i], d), base = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f(m[i] - base);
-            pr[i] = __builtin_amdgcn_exp2f(d - base);
-            l[i] = fmaf(l[i], f, pr[i]);
-            m[i] = top;
-            pr[i] *= vs;
+        for (int j = 0; j < G; ++j) {
+            const float base = m[j] == -INFINITY ? 0.f : m[j];
 #pragma unroll
-            for (int e = 0; e < DL; ++e) o[i][e] *= f;
+            for (int u = 0; u < U; ++u) {
+                const float p = __builtin_amdgcn_exp2f(sc[u][j] - base);
+                l[j] += p;
+                sc[u][j] = p * __uint_as_float(x.there[u] ? x.vs[u] << 16 : 0u);
+            }
         }
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-            float v[8];
-            q4_values(vc[i], 1.f, v);
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int j = 0; j < G; ++j)
+            for (int i = 0; i < W; ++i) {
+                float v[8];
+                q4_values(x.v[u][i], 1.f, v);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o[j][8 * i + e] = fmaf(pr[j], v[e], o[j][8 * i + e]);
-        }
+                for (int j = 0; j < G; ++j)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[j][8 * i + e] = fmaf(sc[u][j], v[e], o[j][8 * i + e]);
+            }
     }
     /* the wave's position slots: each step halves the dims that a lane keeps */
 #pragma unroll
@@ -705,21 +778,18 @@ __device__ void kv4_attn_impl(const g2_kv4_attn_args &a)
         float *v = o[i];
 #pragma unroll
         for (int e = 0; e < DL; ++e) v[e] *= f;
-        int n = DL / 2;
 #pragma unroll
         for (int e = 0; e < DL / 2; ++e) v[e] = lane_fold32(v[e], v[e + DL / 2]);
 #pragma unroll
         for (int e = 0; e < DL / 4; ++e) v[e] = lane_fold16(v[e], v[e + DL / 4]);
-        n = DL / 8;
 #pragma unroll
         for (int e = 0; e < DL / 8; ++e) {
-            const float lo = v[e] + lane_xor8(v[e]), hi = v[e + n] + lane_xor8(v[e + n]);
+            const float lo = v[e] + lane_xor8(v[e]), hi = v[e + DL / 8] + lane_xor8(v[e + DL / 8]);
             v[e] = lane & 8 ? hi : lo;
         }
-        n = DL / 16;
 #pragma unroll
         for (int e = 0; e < DL / 16; ++e) {
-            const float lo = v[e] + lane_xor4(v[e]), hi = v[e + n] + lane_xor4(v[e + n]);
+            const float lo = v[e] + lane_xor4(v[e]), hi = v[e + DL / 16] + lane_xor4(v[e + DL / 16]);
             v[e] = lane & 4 ? hi : lo;
         }
         if (LP == 2) {
@@ -742,32 +812,66 @@ __device__ void kv4_attn_impl(const g2_kv4_attn_args &a)
             y = fmaf(part[j][i][2 + lane], f, y);
         }
         if (a.splits > 1) {
-            float *r = a.part + ((s * a.NH + h0 + i) * a.splits + split) * G2B_PART_FLOATS;
+            float *r = a.part + (((size_t)(unsigned)s * (unsigned)a.NH + (unsigned)(h0 + i)) * (unsigned)a.splits + split) * G2B_PART_FLOATS;
             if (lane == 0) { r[0] = top; r[1] = sum; }
             r[2 + lane] = y;
         } else
-            a.out[s * a.out_stride + (h0 + i) * G2B_DH + lane] = sum == 0.f ? 0.f : y / sum;
+            a.out[(size_t)(unsigned)s * (unsigned)a.out_stride + (h0 + i) * G2B_DH + lane] = sum == 0.f ? 0.f : y / sum;
     }
 }
-G2K void g2k_kv4_attn1(const g2_kv4_attn_args a) { kv4_attn_impl<1, 2>(a); }
-G2K void g2k_kv4_attn2(const g2_kv4_attn_args a) { kv4_attn_impl<2, 4>(a); }
-G2K void g2k_kv4_attn4(const g2_kv4_attn_args a) { kv4_attn_impl<4, 4>(a); }
+#define KV4_ATTN(G, LP, NW, U)                                                                                         \
+    extern "C" __global__ __launch_bounds__(64 * NW) void g2k_kv4_attn##G##_##NW(const g2_kv4_attn_args a)            \
+    { kv4_attn_impl<G, LP, NW, U, false>(a); }                                                                         \
+    extern "C" __global__ __launch_bounds__(64 * NW) void g2k_kv4_attn##G##_##NW##_o(const g2_kv4_attn_args a)        \
+    { kv4_attn_impl<G, LP, NW, U, true>(a); }
+KV4_ATTN(1, 2, 1, 2)
+KV4_ATTN(1, 2, 4, 2)
+KV4_ATTN(1, 2, 8, 2)
+KV4_ATTN(2, 4, 4, 2)
+KV4_ATTN(2, 4, 8, 2)
+KV4_ATTN(4, 4, 4, 2)
+KV4_ATTN(4, 4, 8, 2)
 
-/* Joins the parts of a head, one wave to it. */
+/* Joins the parts of a head: four waves of eight parts each, all their loads at
+ * once, then the waves. */
 G2K void g2k_kv4_join(const g2_kv4_attn_args a)
 {
-    const int lane = threadIdx.x & 63;
-    const long head = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (head >= (long)a.S * a.NH) return;
-    const float *r = a.part + head * a.splits * G2B_PART_FLOATS;
-    float top = -INFINITY, sum = 0.f, y = 0.f;
-    for (int i = 0; i < a.splits; ++i) top = fmaxf(top, r[i * G2B_PART_FLOATS]);
-    for (int i = 0; i < a.splits; ++i) {
-        const float *p = r + i * G2B_PART_FLOATS, f = kv8_factor(p[0], top);
-        sum = fmaf(p[1], f, sum);
-        y = fmaf(p[2 + lane], f, y);
+    __shared__ float part[4][G2B_PART_FLOATS];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const float *r = a.part + (size_t)blockIdx.x * (unsigned)a.splits * G2B_PART_FLOATS;
+    float m[G2B_SPLITS / 4], l[G2B_SPLITS / 4], v[G2B_SPLITS / 4], top = -INFINITY, o = 0.f, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < G2B_SPLITS / 4; ++i) {
+        const int n = w * (G2B_SPLITS / 4) + i;
+        const float *p = r + min(n, a.splits - 1) * G2B_PART_FLOATS;
+        m[i] = p[0];
+        l[i] = p[1];
+        v[i] = p[2 + lane];
+        if (n >= a.splits) m[i] = -INFINITY;
     }
-    a.out[head / a.NH * a.out_stride + head % a.NH * G2B_DH + lane] = sum == 0.f ? 0.f : y / sum;
+#pragma unroll
+    for (int i = 0; i < G2B_SPLITS / 4; ++i) top = fmaxf(top, m[i]);
+#pragma unroll
+    for (int i = 0; i < G2B_SPLITS / 4; ++i) {
+        if (w * (G2B_SPLITS / 4) + i >= a.splits) continue;
+        const float f = kv8_factor(m[i], top);
+        sum = fmaf(l[i], f, sum);
+        o = fmaf(v[i], f, o);
+    }
+    if (lane == 0) { part[w][0] = top; part[w][1] = sum; }
+    part[w][2 + lane] = o;
+    __syncthreads();
+    if (w) return;
+    top = fmaxf(fmaxf(part[0][0], part[1][0]), fmaxf(part[2][0], part[3][0]));
+    sum = o = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float f = kv8_factor(part[i][0], top);
+        sum = fmaf(part[i][1], f, sum);
+        o = fmaf(part[i][2 + lane], f, o);
+    }
+    const unsigned s = blockIdx.x / (unsigned)a.NH, h = blockIdx.x - s * (unsigned)a.NH;
+    a.out[(size_t)s * (unsigned)a.out_stride + h * G2B_DH + lane] = sum == 0.f ? 0.f : o / sum;
 }
 
 /* ======================================================================

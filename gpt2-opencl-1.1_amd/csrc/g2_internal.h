@@ -43,6 +43,12 @@ extern "C" {
     X(Q4_MVH##MT##_##KW##_##NC##_64, "g2k_q4_mvh" #MT "_" #KW "_" #NC "_64")  \
     X(Q4_MVH##MT##_##KW##_##NC##_128, "g2k_q4_mvh" #MT "_" #KW "_" #NC "_128")
 
+/* Attention over the 4-bit cache for up to G query heads in NW waves: positions
+ * in their own sequence's slot, and through a table of origins. */
+#define G2_KV4_LIST(X, G, NW)                                                 \
+    X(KV4_ATTN##G##_##NW, "g2k_kv4_attn" #G "_" #NW)                          \
+    X(KV4_ATTN##G##_##NW##_O, "g2k_kv4_attn" #G "_" #NW "_o")
+
 /* Kernel table: index -> symbol name in the gfx950 code object. */
 #define G2_KERNEL_LIST(X)                                                     \
     X(MVSK4_F32, "g2k_mvsk_f32_4") X(MVSK4_F16, "g2k_mvsk_f16_4")       \
@@ -127,8 +133,10 @@ extern "C" {
     X(PROMPT_TILE_F16, "g2k_prompt_tile_f16")                                 \
     X(KV4_APPEND_F32, "g2k_kv4_append_f32")                                   \
     X(KV4_APPEND_F16, "g2k_kv4_append_f16") X(KV4_READ, "g2k_kv4_read")       \
-    X(KV4_ATTN1, "g2k_kv4_attn1") X(KV4_ATTN2, "g2k_kv4_attn2")               \
-    X(KV4_ATTN4, "g2k_kv4_attn4") X(KV4_JOIN, "g2k_kv4_join")                 \
+    G2_KV4_LIST(X, 1, 1) G2_KV4_LIST(X, 1, 4) G2_KV4_LIST(X, 1, 8)            \
+    G2_KV4_LIST(X, 2, 4) G2_KV4_LIST(X, 2, 8)                                 \
+    G2_KV4_LIST(X, 4, 4) G2_KV4_LIST(X, 4, 8)                                 \
+    X(KV4_JOIN, "g2k_kv4_join")                                               \
     X(BEAM_SELECT1, "g2k_beam_select1") X(BEAM_SELECT4, "g2k_beam_select4")   \
     X(BEAM_SELECT7, "g2k_beam_select7")                                       \
     X(BEAM_COPY, "g2k_beam_copy") X(BEAM_MOVE, "g2k_beam_move")
@@ -222,8 +230,8 @@ int g2i_logits_form(int rows, int V, int *parts);
 int g2i_prompt_form(int rows, int n_head, int n_kv, long *tiles);
 
 /* g2_attn_kv4's parts of a key head's positions, tiles to a part, query heads to
- * a pass over them and passes to a key head. */
-int g2i_kv4_form(int n_seq, int n_head, int n_kv, int T_kv, int *heads, int *chunks, int *span);
+ * a pass over them, passes to a key head, waves to a work-group. */
+int g2i_kv4_form(int n_seq, int n_head, int n_kv, int T_kv, int *heads, int *chunks, int *span, int *waves);
 
 /* 4096 ids to a slice of g2_beam_select times this (1, 4, 7), and the slices of a row. */
 int g2i_beam_form(int rows, int V, int *slices);

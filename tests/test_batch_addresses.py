@@ -78,9 +78,10 @@ def test_every_form_of_the_selection_is_tested():
 
 def kv4_form(S, NH, NKV, T):
     fn = g2hip._lib.g2i_kv4_form
-    fn.argtypes = [C.c_int] * 4 + [C.POINTER(C.c_int)] * 3
-    heads, chunks, span = C.c_int(), C.c_int(), C.c_int()
-    return fn(S, NH, NKV, T, C.byref(heads), C.byref(chunks), C.byref(span)), heads.value, chunks.value, span.value
+    fn.argtypes = [C.c_int] * 4 + [C.POINTER(C.c_int)] * 4
+    heads, chunks, span, waves = C.c_int(), C.c_int(), C.c_int(), C.c_int()
+    splits = fn(S, NH, NKV, T, C.byref(heads), C.byref(chunks), C.byref(span), C.byref(waves))
+    return splits, heads.value, chunks.value, span.value, waves.value
 
 
 def test_attention_parts():
@@ -88,13 +89,15 @@ def test_attention_parts():
         for group in (1, 2, 3, 4, 5, 7, 8, 9, 16, 25):
             for S in (1, 3, 48, 1000):
                 for T in (0, 1, 31, 32, 33, 256, 257, 700, 1024, 5000, 50001, 1 << 24):
-                    splits, heads, chunks, span = kv4_form(S, NKV * group, NKV, T)
+                    splits, heads, chunks, span, waves = kv4_form(S, NKV * group, NKV, T)
                     tiles = max(1, -(-T // 32))
                     assert 1 <= splits <= 32 and (splits - 1) * span < tiles <= splits * span
                     assert 1 <= heads <= 4 and (chunks - 1) * heads < group <= chunks * heads
-                    assert S * NKV * chunks * splits * 256 < 2 ** 32
+                    assert waves in (1, 4, 8) and (waves > 1 or heads == 1) and S * NKV * chunks * splits * 64 * waves < 2 ** 32
 
 
 def test_every_form_of_the_attention_is_tested():
-    got = {(f[0] > 1, min(f[1], 3)) for f in (kv4_form(*c) for c in gpu.attention_cases())}
-    assert got >= {(False, 1), (False, 2), (False, 3), (True, 1), (True, 3)}
+    got = {(f[0] > 1, f[1] if f[1] < 3 else 4, f[4]) for f in (kv4_form(*c) for c in gpu.attention_cases())}
+    assert {f[1:] for f in got} == {(1, 1), (1, 4), (1, 8), (2, 4), (2, 8), (4, 4), (4, 8)} and {f[0] for f in got} == {False, True}
+    through = {(f[1] if f[1] < 3 else 4, f[4]) for f in (kv4_form(*c) for c in gpu.ORIGINS)}
+    assert through == {f[1:] for f in got}
