@@ -155,28 +155,45 @@ int g2_kv4_read(const void *cache, float *k, float *v, const int *origin, const 
         return g2i_err(G2_E_ARG, "%s: overlapping buffers", fn);
     if ((rc = ready())) return rc;
     g2_kv4_read_args a = { cache, k, v, origin, len, T_kv, start, T, n_seq, n_kv, max_seq, (int)g2b_tiles(max_seq) };
-    const long threads = (long)(n / 32);
+    const long threads = (long)(n / 16);
     return g2i_launch(G2F_KV4_READ, threads > (1l << 20) * 256 ? 1u << 20 : cdiv(threads, 256), 1, 256, &a);
 }
 
 /* Query heads to a pass over their key head's positions, passes to a key head,
- * parts of the positions and tiles to a part, waves to a work-group. */
+ * parts of the positions and tiles to a part, waves to a work-group.  us, one call
+ * after the other, caches that no cache holds where they are large:
+ *  - up to four heads share a pass, fewer where that leaves less than 200
+ *    work-groups: the sums of four heads take four times as long as one's, and
+ *    a CU for each pays more than the codes read again (64 sequences of 2 x 8
+ *    heads x 1000 12.0 with 4, 12.9 with 2, 15.7 with 1; 30 of 4 x 4 x 128 5.3,
+ *    4.2, 5.0; one of 4 x 4 x 1000 11.4, 7.7, 5.6);
+ *  - parts above 1024 positions, of 256 and more, as many as 256 work-groups
+ *    (12 heads x 4000 7.1 in 16 parts, 8.0 in 32, 8.6 in 4; 16 x 50000 on 4 key
+ *    heads 13.0 in 16, 14.0 in 32);
+ *  - waves of 64 positions a step, each of which costs the same at the end: one up
+ *    to 128 positions, for many heads up to 256 (3600 heads x 200 15.6, four 20.1;
+ *    360 x 128 4.2, 4.9), eight from 800 for few heads (96 x 901 6.3, four 6.5; 256
+ *    passes of two heads x 2000 12.1, 14.6), four else (12 x 700 5.0, eight 5.3;
+ *    1200 x 640 14.4, eight 17.5, one 15.3). */
 int g2i_kv4_form(int n_seq, int n_head, int n_kv, int T_kv, int *heads, int *chunks, int *span, int *waves)
 {
     const int group = n_head / n_kv;
     const long tiles = g2b_tiles(T_kv) > 0 ? g2b_tiles(T_kv) : 1;
-    int most = 4;
-    *chunks = (group + most - 1) / most;
-    *heads = (group + *chunks - 1) / *chunks;
-    const long wgs = (long)n_seq * n_kv * *chunks;
-    long splits = 1;
+    long wgs, splits = 1;
+    for (int most = 4;; most /= 2) {
+        *chunks = (group + most - 1) / most;
+        *heads = (group + *chunks - 1) / *chunks;
+        wgs = (long)n_seq * n_kv * *chunks;
+        if (wgs >= 200 || most == 1) break;
+    }
     if (tiles > 32 && wgs < 256) {
-        splits = tiles / 8 < 512 / wgs ? tiles / 8 : 512 / wgs;
+        splits = tiles / 8 < 256 / wgs ? tiles / 8 : 256 / wgs;
         if (splits > G2B_SPLITS) splits = G2B_SPLITS;
     }
     *span = (int)((tiles + splits - 1) / splits);
-    *waves = *span <= 2 && *heads == 1 ? 1 : *span <= 8 ? 4 : 8;
-    return (int)((tiles + *span - 1) / *span);
+    splits = (tiles + *span - 1) / *span;
+    *waves = *heads == 1 && *span <= (wgs * splits >= 1024 ? 8 : 4) ? 1 : *span > 24 && wgs * splits < 512 ? 8 : 4;
+    return (int)splits;
 }
 
 int g2_attn_kv4(const float *q, int q_stride, const void *cache, float *out, int out_stride, const int *origin,

@@ -581,29 +581,31 @@ __device__ void kv4_append_impl(const g2_kv4_append_args &a)
 G2K void g2k_kv4_append_f32(const g2_kv4_append_args a) { kv4_append_impl<float>(a); }
 G2K void g2k_kv4_append_f16(const g2_kv4_append_args a) { kv4_append_impl<_Float16>(a); }
 
-/* One thread per 8 dims of a position, keys and values, in the order of the output. */
+/* One thread per four dims of a position, keys and values, in the order of the
+ * output, which does not stay in the L2. */
 G2K void g2k_kv4_read(const g2_kv4_read_args a)
 {
-    const int parts = a.NKV * 8;
-    const long n = (long)a.S * a.T * parts;
+    const unsigned quads = (unsigned)a.NKV * (G2B_DH / 4);
+    const long n = (long)a.S * a.T * quads;
     for (long i = blockIdx.x * 256l + threadIdx.x; i < n; i += gridDim.x * 256l) {
-        const long row = i / parts;
-        const int e = (int)(i - row * parts), h = e / 8, part = e % 8;
-        const long s = row / a.T;
-        const int p = a.start + (int)(row - s * a.T);
+        const long row = n <= UINT32_MAX ? (unsigned)i / quads : i / quads;
+        const unsigned e = (unsigned)(i - row * quads), d = e % (G2B_DH / 4) * 4;
+        const int h = (int)(e / (G2B_DH / 4)), s = a.S == 1 ? 0 : (int)((unsigned)row / (unsigned)a.T);
+        const int p = a.start + (int)(row - (long)s * a.T);
         if (p >= kv8_length(a.len, a.T_kv, s)) continue;
-        const int from = a.origin ? a.origin[s * a.max_seq + p] : (int)s;
-        if (from < 0 || from >= a.S) continue;
+        const int from = a.origin ? a.origin[(size_t)(unsigned)s * (unsigned)a.max_seq + (unsigned)p] : s;
+        if ((unsigned)from >= (unsigned)a.S) continue;
         const unsigned char *t = a.cache + g2b_tile_at(a.NKV, a.tiles, from, h, p / G2B_TILE);
+        f32x4 v[2];
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
-            float v[8];
-            q4_values(*(const unsigned *)(t + g2b_code_at(kv, p % G2B_TILE) + 4 * part),
-                      bf16_f(*(const uint16_t *)(t + g2b_scale_at(kv, p % G2B_TILE) + 2 * (part >> 2))), v);
-            float *o = (kv ? a.v : a.k) + 8 * i;
-            *(f32x4u *)o = f32x4{ v[0], v[1], v[2], v[3] };
-            *(f32x4u *)(o + 4) = f32x4{ v[4], v[5], v[6], v[7] };
+            const unsigned c = *(const uint16_t *)(t + g2b_code_at(kv, p % G2B_TILE) + d / 2);
+            const float sc = bf16_f(*(const uint16_t *)(t + g2b_scale_at(kv, p % G2B_TILE) + d / 32 * 2));
+            const f32x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
+            v[kv] = f32x4{ lo[0] * sc, lo[1] * sc, hi[0] * sc, hi[1] * sc };
         }
+        __builtin_nontemporal_store(v[0], (f32x4u *)(a.k + 4 * i));
+        __builtin_nontemporal_store(v[1], (f32x4u *)(a.v + 4 * i));
     }
 }
 

@@ -374,10 +374,12 @@ def attention_cases():
     """(S, NH, NKV, T) on both sides of every border of a form."""
     return [(1, 1, 1, 1), (1, 1, 1, 33), (2, 4, 4, 100), (1, 2, 1, 64), (3, 6, 2, 65), (2, 4, 1, 129), (1, 5, 1, 200), (1, 7, 1, 31), (2, 16, 2, 257),
             (1, 12, 12, 701), (5, 25, 25, 300), (1, 16, 4, 3000), (1, 1, 1, 5000), (600, 1, 1, 40), (40, 16, 16, 70), (520, 2, 2, 300), (1, 9, 3, 1025),
-            (8, 12, 12, 1024), (3, 2, 1, 600), (2, 6, 3, 2500)]
+            (8, 12, 12, 1024), (3, 2, 1, 600), (2, 6, 3, 2500), (1100, 1, 1, 200), (200, 3, 1, 70), (210, 4, 1, 900), (110, 8, 2, 800), (101, 4, 2, 100),
+            (100, 4, 2, 1030), (205, 5, 1, 40), (128, 8, 2, 1100)]
 
 
-ORIGINS = [(4, 4, 4, 40), (8, 12, 12, 901), (6, 8, 2, 300), (3, 5, 1, 1500), (2, 1, 1, 4000), (5, 3, 3, 100), (4, 4, 2, 100), (4, 2, 1, 500), (3, 8, 2, 70)]
+ORIGINS = [(4, 4, 4, 40), (8, 12, 12, 901), (6, 8, 2, 300), (3, 5, 1, 1500), (2, 1, 1, 4000), (5, 3, 3, 200), (104, 4, 2, 100), (104, 4, 2, 900), (210, 4, 1, 70),
+           (208, 4, 1, 801)]
 
 
 @pytest.mark.parametrize("S,NH,NKV,T", attention_cases())
