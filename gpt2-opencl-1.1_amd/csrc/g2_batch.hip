@@ -102,15 +102,45 @@ __device__ __forceinline__ int lanes_min_int(int v)
     return v;
 }
 
-__device__ __forceinline__ g2b_row keys_of_row(const g2_attn_prompt_args &a, int row0, int row1, int row, int lane)
+/* Where a work-group's tile of queries is.  With up to 63 sequences the tiles are the
+ * sequences' own, deepest first: a tile's depth, its place in its sequence, is what
+ * its rows see, so long work begins first, and the starts are read once, an entry
+ * to a lane.  With more sequences, which are short ones, tiles are cut from all
+ * rows in their order, and each row's sequence is searched. */
+struct prompt_place {
+    int first;          /* the tile's first query: in its sequence, or of all */
+    int q0, q1, k0, k1; /* the sequence's rows and keys */
+    bool own;
+};
+__device__ __forceinline__ prompt_place prompt_find(const g2_attn_prompt_args &a, int size, int rank, int lane)
 {
-    int s = 0, q0 = 0, q1 = a.q_rows, k0 = 0, k1 = a.k_rows;
-    if (a.q_start) s = seq_of_row(a.q_start, a.S, row0, row1, row, lane);
-    const bool in = s >= 0 && s < a.S;
-    const int i = in ? s : 0;
-    if (a.q_start) { q0 = a.q_start[i]; q1 = a.q_start[i + 1]; }
-    if (a.k_start) { k0 = a.k_start[i]; k1 = a.k_start[i + 1]; }
-    return g2b_row_keys(row, in, q0, q1, k0, k1, a.q_rows, a.k_rows);
+    prompt_place r = { (a.tiles - 1 - rank) * size, 0, 0, 0, 0, a.S < 64 };
+    if (!r.own) return r;
+    const int group = a.NH / a.NKV, at = min(lane, a.S);
+    const int qs = a.q_start ? a.q_start[at] : at ? a.q_rows : 0, ks = a.k_start ? a.k_start[at] : at ? a.k_rows : 0;
+    const int q0 = g2b_clamp(qs, a.q_rows), q1 = __shfl_down(q0, 1), n = lane < a.S ? max(0, q1 - q0) : 0;
+    const int tiles = (int)(((unsigned)n * (unsigned)group + (unsigned)size - 1) / (unsigned)size);
+    unsigned long long mask = 1;
+    int depth;
+    if (a.S == 1) depth = __builtin_amdgcn_readfirstlane(tiles) - 1 - rank;
+    else {
+        depth = -lanes_min_int(-tiles);
+        for (;;) {
+            --depth;
+            mask = __builtin_amdgcn_ballot_w64(tiles > depth);
+            const int c = __builtin_popcountll(mask);
+            if (depth < 0 || rank < c) break;
+            rank -= c;
+        }
+        mask = __builtin_amdgcn_ballot_w64(mask >> lane & 1 && __builtin_popcountll(mask & ((1ull << lane) - 1)) == rank);
+    }
+    const int s = depth < 0 ? 0 : __builtin_ctzll(mask);
+    r.first = depth * size; /* (below 0: no work is left) */
+    r.q0 = __builtin_amdgcn_readlane(qs, s);
+    r.q1 = __builtin_amdgcn_readlane(qs, s + 1);
+    r.k0 = __builtin_amdgcn_readlane(ks, s);
+    r.k1 = __builtin_amdgcn_readlane(ks, s + 1);
+    return r;
 }
 
 /* One wave takes 32 queries (column l % 32 of a lane) against 32 keys at a time,
@@ -159,20 +189,40 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t prompt_rows(const T *p, int j0
     const unsigned bytes = ((unsigned)(n - 1) * (unsigned)stride + G2B_DH) * (unsigned)sizeof(T);
     return __builtin_amdgcn_make_buffer_rsrc((void *)(p + (size_t)j0 * stride), (short)0, bytes, 0x00020000);
 }
-/* A dim's values of the eight keys that a lane of half g takes in step u (in the
- * second product's order): where its values are, from the buffer's begin. */
-template <typename T> __device__ __forceinline__ void prompt_value_at(unsigned (&at)[8], int u, int g, int dim, long stride)
+/* Two dims' values of the eight keys that a lane of half g takes in step u (in the
+ * second product's order): where they are, from the buffer's begin. */
+template <typename T> __device__ __forceinline__ void prompt_value_at(unsigned (&at)[8], int u, int g, int pair, long stride)
 {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) at[e] = ((unsigned)(16 * u + 8 * (e / 4) + 4 * g + e % 4) * (unsigned)stride + (unsigned)dim) * (unsigned)sizeof(T);
+    for (int e = 0; e < 8; ++e) at[e] = ((unsigned)(16 * u + 8 * (e / 4) + 4 * g + e % 4) * (unsigned)stride + 2u * (unsigned)pair) * (unsigned)sizeof(T);
 }
-template <typename T> __device__ __forceinline__ void prompt_load_v(T (&x)[8], __amdgpu_buffer_rsrc_t rows, const unsigned (&at)[8], int more)
+/* (fp16 pairs: `even` where they are at a multiple of four bytes, which a load of both asks for) */
+__device__ __forceinline__ void prompt_load_v(float (&x)[2][8], __amdgpu_buffer_rsrc_t rows, const unsigned (&at)[8], int)
 {
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        if constexpr (sizeof(T) == 4) x[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows, (int)at[e] + more, 0, 0));
-        else x[e] = __builtin_bit_cast(_Float16, __builtin_amdgcn_raw_buffer_load_b16(rows, (int)at[e] + more, 0, 0));
+        const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rows, (int)at[e], 0, 0));
+        x[0][e] = __uint_as_float(v[0]);
+        x[1][e] = __uint_as_float(v[1]);
     }
+}
+__device__ __forceinline__ void prompt_load_v(_Float16 (&x)[2][8], __amdgpu_buffer_rsrc_t rows, const unsigned (&at)[8], int even)
+{
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    if (even)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const f16x2 v = __builtin_bit_cast(f16x2, __builtin_amdgcn_raw_buffer_load_b32(rows, (int)at[e], 0, 0));
+            x[0][e] = v[0];
+            x[1][e] = v[1];
+        }
+    else
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[0][e] = __builtin_bit_cast(_Float16, __builtin_amdgcn_raw_buffer_load_b16(rows, (int)at[e], 0, 0));
+            x[1][e] = __builtin_bit_cast(_Float16, __builtin_amdgcn_raw_buffer_load_b16(rows, (int)at[e] + 2, 0, 0));
+        }
 }
 
 /* Scores in units of log 2; not 0, which would make NaN of the masked ones. */
@@ -187,18 +237,26 @@ template <typename T> struct prompt_query {
     int row, head, k0, k1; /* k0 .. k1 - 1: what the wave's queries see together */
     bool sees;
     prompt_op<T> q[4];
-    f32x16 o[2]; /* dims 32 t + 8 (r / 4) + 4 (l / 32) + r % 4 */
+    f32x16 o[2];
     float m, l;
 };
 
 template <typename T>
-__device__ __forceinline__ void prompt_start(prompt_query<T> &y, const g2_attn_prompt_args &a, int hk, int first, int lane)
+__device__ __forceinline__ void prompt_start(prompt_query<T> &y, const g2_attn_prompt_args &a, int hk, const prompt_place &place, int off, int lane)
 {
-    const int group = a.NH / a.NKV, g = lane >> 5;
-    const int at = first + (lane & 31), row1 = (first + 31) / group;
-    y.row = at / group;
-    y.head = hk * group + at % group;
-    y.keys = keys_of_row(a, first / group, row1, y.row, lane);
+    const int group = a.NH / a.NKV, g = lane >> 5, first = place.first + off;
+    const unsigned at = (unsigned)(first + (lane & 31));
+    y.row = (int)(at / (unsigned)group);
+    y.head = hk * group + (int)(at % (unsigned)group);
+    if (place.own) {
+        y.row += max(place.q0, 0);
+        y.keys = g2b_row_keys(y.row, 1, place.q0, place.q1, place.k0, place.k1, a.q_rows, a.k_rows);
+    } else {
+        const int s = seq_of_row(a.q_start, a.S, (int)((unsigned)first / (unsigned)group), (int)((unsigned)(first + 31) / (unsigned)group), y.row, lane);
+        const bool in = s >= 0 && s < a.S;
+        const int i = in ? s : 0;
+        y.keys = g2b_row_keys(y.row, in, a.q_start[i], a.q_start[i + 1], a.k_start[i], a.k_start[i + 1], a.q_rows, a.k_rows);
+    }
     y.sees = y.keys.there && y.keys.end > y.keys.lo;
     y.k0 = __builtin_amdgcn_readfirstlane(lanes_min_int(y.sees ? y.keys.lo : INT_MAX));
     y.k1 = __builtin_amdgcn_readfirstlane(-lanes_min_int(y.sees ? -y.keys.end : INT_MAX));
@@ -304,21 +362,26 @@ __device__ __forceinline__ void prompt_odd(prompt_query<T> &y, const T *v, long 
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
         const bool seen = j0 + i >= y.keys.lo && j0 + i < y.keys.end;
-        const T *p = v + (size_t)(j0 + i) * stride + 4 * g;
+        const T *p = v + (size_t)(j0 + i) * stride + 8 * g;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float x = (float)p[32 * t + 8 * (r / 4) + r % 4];
+                const float x = (float)p[16 * (r / 4) + 2 * (r % 4) + t];
                 if (seen && !__builtin_isfinite(x)) y.o[t][r] += x;
             }
     }
 }
 
-template <typename T> __device__ __forceinline__ void prompt_store(T *p, const f32x4 &y)
+/* Eight dims of a row: quads of registers, of tile 0 and 1, side by side. */
+template <typename T> __device__ __forceinline__ void prompt_store(T *p, const f32x4 &a, const f32x4 &b)
 {
-    if constexpr (sizeof(T) == 2) *(f16x4u *)p = f16x4u{ (_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3] };
-    else *(f32x4u *)p = y;
+    if constexpr (sizeof(T) == 2)
+        *(f16x8u *)p = f16x8u{ (_Float16)a[0], (_Float16)b[0], (_Float16)a[1], (_Float16)b[1], (_Float16)a[2], (_Float16)b[2], (_Float16)a[3], (_Float16)b[3] };
+    else {
+        *(f32x4u *)p = f32x4{ a[0], b[0], a[1], b[1] };
+        *(f32x4u *)(p + 4) = f32x4{ a[2], b[2], a[3], b[3] };
+    }
 }
 
 /* ---- few queries: a work-group takes 32 of them, its four waves every fourth 32
@@ -335,11 +398,13 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
     long tile;
     g2b_prompt_item(blockIdx.x, a.NKV, a.tiles, &hk, &tile);
     prompt_query<T> y;
-    prompt_start(y, a, hk, (int)tile * 32, lane);
+    const prompt_place place = prompt_find(a, 32, a.tiles - 1 - (int)tile, lane);
+    if (place.first < 0) return;
+    prompt_start(y, a, hk, place, 0, lane);
     const float c = prompt_unit(a.scale);
     const long stride = a.kv_stride;
     const T *kp = (const T *)a.k + hk * G2B_DH, *vp = (const T *)a.v + hk * G2B_DH;
-    T k[4][8], v[2][2][8];
+    T k[4][8], v[2][2][8]; /* v: step, dim of the pair, key */
     unsigned at[2][8];
     prompt_value_at<T>(at[0], 0, g, lane & 31, stride);
     prompt_value_at<T>(at[1], 1, g, lane & 31, stride);
@@ -351,9 +416,7 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
     auto load_v = [&](int j0) {
         const __amdgpu_buffer_rsrc_t rows = prompt_rows(vp, j0, y.k1, stride);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) prompt_load_v(v[t][u], rows, at[u], 32 * t * (int)sizeof(T));
+        for (int u = 0; u < 2; ++u) prompt_load_v(v[u], rows, at[u], a.even);
     };
     int j0 = y.k0 < y.k1 ? y.k0 + 32 * w : y.k1;
     if (j0 < y.k1) { load_k(j0); load_v(j0); }
@@ -372,12 +435,12 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) z = prompt_look(v[t][u], z);
+            for (int u = 0; u < 2; ++u) z = prompt_look(v[u][t], z);
         if (wave_any(z != 0.f)) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) prompt_clean(v[t][u]);
+                for (int u = 0; u < 2; ++u) prompt_clean(v[u][t]);
             prompt_odd(y, vp, stride, j0, min(32, y.k1 - j0), g);
         }
 #pragma unroll
@@ -386,7 +449,7 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
             prompt_weight_op(s, u, p);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                prompt_pack(v[t][u], x);
+                prompt_pack(v[u][t], x);
                 y.o[t] = prompt_mma(x, p, y.o[t]);
             }
         }
@@ -410,41 +473,41 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
         part[i] = prompt_factor(red[i][0][lane], top, c);
         l = fmaf(red[i][1][lane], part[i], l);
     }
-    T *out = (T *)a.out + (size_t)y.row * a.out_stride + y.head * G2B_DH + 4 * g;
+    T *out = (T *)a.out + (size_t)y.row * a.out_stride + y.head * G2B_DH + 8 * g;
+    f32x4 x[2] = {};
 #pragma unroll
-    for (int i = 0; i < 8 / KW; ++i) {
-        const int q = w * (8 / KW) + i;
-        f32x4 x = {};
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
 #pragma unroll
-            for (int j = 0; j < KW; ++j) x[e] = fmaf(red[j][2 + 4 * q + e][lane], part[j], x[e]);
-            x[e] = y.sees ? x[e] / l : 0.f;
+            for (int j = 0; j < KW; ++j) x[t][e] = fmaf(red[j][2 + 16 * t + 4 * w + e][lane], part[j], x[t][e]);
+            x[t][e] = y.sees ? x[t][e] / l : 0.f;
         }
-        prompt_store(out + 32 * (q / 4) + 8 * (q % 4), x);
-    }
+    prompt_store(out + 16 * w, x[0], x[1]);
 }
 extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g2k_prompt_split_f32(const g2_attn_prompt_args a) { prompt_split_impl<float>(a); }
 extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g2k_prompt_split_f16(const g2_attn_prompt_args a) { prompt_split_impl<_Float16>(a); }
 
 /* ---- many queries: a work-group takes 128 of them, 32 a wave, and its waves
- * read each 32 keys and values together, once, as operands in LDS: unit (part,
- * step, lane) of 16 bytes is what the lane reads of it, so that reads and
- * writes are both one row of units.  Two stages: the next keys are on their
- * way from memory while the products of these run, and one barrier stands
- * between. */
-template <typename T>
+ * read KT times 32 keys and values together, once, as operands in LDS: unit
+ * (part, step, lane) of 16 bytes is what the lane reads of it, so that reads and
+ * writes are both rows of units.  Two stages: the next keys are on their way from
+ * memory while the products of these run, and one barrier stands between.  Of 32
+ * keys two waves bring the keys, two the values (a step each), in turns. */
+template <typename T, int KT>
 __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
 {
-    constexpr int P = sizeof(T) == 4 ? 3 : 1, UNITS = P * 256; /* of keys, and of values */
-    __shared__ u32x4 lds[2][2 * UNITS];
-    __shared__ int range[4][2], odd[2][4];
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
+    constexpr int P = sizeof(T) == 4 ? 3 : 1, UNITS = P * 256; /* of 32 keys, and of their values */
+    __shared__ u32x4 lds[2][KT][2 * UNITS];
+    __shared__ int range[4][2], odd[2][KT][2];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, m = lane & 31;
     int hk;
     long tile;
     g2b_prompt_item(blockIdx.x, a.NKV, a.tiles, &hk, &tile);
     prompt_query<T> y;
-    prompt_start(y, a, hk, (int)tile * 128 + 32 * w, lane);
+    const prompt_place place = prompt_find(a, 128, a.tiles - 1 - (int)tile, lane);
+    if (place.first < 0) return;
+    prompt_start(y, a, hk, place, 32 * w, lane);
     if (lane == 0) { range[w][0] = y.k0; range[w][1] = y.k1; }
     __syncthreads();
     const int k0 = __builtin_amdgcn_readfirstlane(min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0])));
@@ -452,35 +515,50 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
     const float c = prompt_unit(a.scale);
     const long stride = a.kv_stride;
     const T *kp = (const T *)a.k + hk * G2B_DH, *vp = (const T *)a.v + hk * G2B_DH;
-    /* this thread's share: dims 8 (tid / 32) ..+7 of key tid % 32; of dim lane, the keys that lanes of half w % 2 take in step w / 2 */
-    T k[8], v[8];
+    T x[KT][2][8]; /* this lane's share: two chunks of a key's dims, or two dims of eight keys */
     unsigned at[8];
-    prompt_value_at<T>(at, w >> 1, w & 1, lane, stride);
+    prompt_value_at<T>(at, w & 1, g, m, stride);
+    auto brings_keys = [&](int i) { return ((w >> 1) ^ i) & 1; };
+    const int chunk = 4 * (w & 1) + 2 * g;
     auto load = [&](int j0) {
-        prompt_load_k(k, kp + (size_t)j0 * stride + (size_t)min(tid & 31, k1 - j0 - 1) * stride + 8 * (tid >> 5));
-        prompt_load_v(v, prompt_rows(vp, j0, k1, stride), at, 0);
-    };
-    auto stage = [&](int b) {
-        const bool any = wave_any(prompt_look(v, 0.f) != 0.f);
-        if (any) prompt_clean(v);
-        if (lane == 0) odd[b][w] = any;
-        prompt_op<T> x, z;
-        prompt_pack(k, x);
-        prompt_pack(v, z);
-        u32x4 *kd = lds[b] + tid, *vd = lds[b] + UNITS + (lane >> 5) * 128 + (w >> 1) * 64 + (w & 1) * 32 + (lane & 31);
-        if constexpr (P == 3) {
 #pragma unroll
-            for (int i = 0; i < 3; ++i) { kd[256 * i] = x.p[i]; vd[256 * i] = z.p[i]; }
-        } else {
-            *kd = __builtin_bit_cast(u32x4, x.p);
-            *vd = __builtin_bit_cast(u32x4, z.p);
+        for (int i = 0; i < KT; ++i) {
+            const int j = min(j0 + 32 * i, k1 - 1); /* (keys behind the last are masked) */
+            if (brings_keys(i)) {
+                const T *p = kp + (size_t)j * stride + (size_t)min(m, k1 - j - 1) * stride + 8 * chunk;
+                prompt_load_k(x[i][0], p);
+                prompt_load_k(x[i][1], p + 8);
+            } else prompt_load_v(x[i], prompt_rows(vp, j, k1, stride), at, a.even);
         }
     };
-    auto fetch = [&](const u32x4 *p, prompt_op<T> &x) {
+    auto put = [&](u32x4 *p, const T (&v)[8]) {
+        prompt_op<T> z;
+        prompt_pack(v, z);
         if constexpr (P == 3) {
 #pragma unroll
-            for (int i = 0; i < 3; ++i) x.p[i] = p[256 * i];
-        } else x.p = __builtin_bit_cast(f16x8, *p);
+            for (int i = 0; i < 3; ++i) p[256 * i] = z.p[i];
+        } else *p = __builtin_bit_cast(u32x4, z.p);
+    };
+    auto stage = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < KT; ++i) {
+            if (brings_keys(i)) {
+                put(lds[b][i] + chunk * 32 + m, x[i][0]);
+                put(lds[b][i] + chunk * 32 + 32 + m, x[i][1]);
+            } else {
+                const bool any = wave_any(prompt_look(x[i][1], prompt_look(x[i][0], 0.f)) != 0.f);
+                if (any) { prompt_clean(x[i][0]); prompt_clean(x[i][1]); }
+                if (lane == 0) odd[b][i][w & 1] = any;
+                put(lds[b][i] + UNITS + (w & 1) * 64 + lane, x[i][0]);
+                put(lds[b][i] + UNITS + 128 + (w & 1) * 64 + lane, x[i][1]);
+            }
+        }
+    };
+    auto fetch = [&](const u32x4 *p, prompt_op<T> &z) {
+        if constexpr (P == 3) {
+#pragma unroll
+            for (int i = 0; i < 3; ++i) z.p[i] = p[256 * i];
+        } else z.p = __builtin_bit_cast(f16x8, *p);
     };
     if (k0 < k1) {
         load(k0);
@@ -488,28 +566,32 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
     }
     __syncthreads();
     int b = 0;
-    for (int j0 = k0; j0 < k1; j0 += 32, b ^= 1) {
-        const bool more = j0 + 32 < k1;
-        if (more) load(j0 + 32);
-        if (j0 < y.k1 && j0 + 32 > y.k0) { /* (the wave's queries see some of them) */
-            const u32x4 *kd = lds[b] + lane, *vd = lds[b] + UNITS + lane;
-            f32x16 s = {};
+    for (int j0 = k0; j0 < k1; j0 += 32 * KT, b ^= 1) {
+        const bool more = j0 + 32 * KT < k1;
+        if (more) load(j0 + 32 * KT);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                prompt_op<T> x;
-                fetch(kd + 64 * i, x);
-                s = prompt_mma(x, y.q[i], s);
+        for (int i = 0; i < KT; ++i) {
+            const int j = j0 + 32 * i;
+            if (j >= y.k1 || j + 32 <= y.k0) continue; /* (none of the wave's queries sees any of them) */
+            const u32x4 *kd = lds[b][i] + lane, *vd = kd + UNITS;
+            f32x16 s = {};
+            {
+                prompt_op<T> z[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) fetch(kd + 64 * t, z[t]);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) s = prompt_mma(z[t], y.q[t], s);
             }
-            prompt_weights(y, s, j0, c, g);
-            if (__builtin_amdgcn_readfirstlane(odd[b][0] | odd[b][1] | odd[b][2] | odd[b][3])) prompt_odd(y, vp, stride, j0, min(32, k1 - j0), g);
+            prompt_weights(y, s, j, c, g);
+            if (__builtin_amdgcn_readfirstlane(odd[b][i][0] | odd[b][i][1])) prompt_odd(y, vp, stride, j, min(32, k1 - j), g);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                prompt_op<T> p, x;
+                prompt_op<T> p, z;
                 prompt_weight_op(s, u, p);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    fetch(vd + 128 * t + 64 * u, x);
-                    y.o[t] = prompt_mma(x, p, y.o[t]);
+                    fetch(vd + 128 * t + 64 * u, z);
+                    y.o[t] = prompt_mma(z, p, y.o[t]);
                 }
             }
         }
@@ -518,17 +600,19 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
     }
     if (!y.keys.there) return;
     const float l = swap_sum(y.l);
-    T *out = (T *)a.out + (size_t)y.row * a.out_stride + y.head * G2B_DH + 4 * g;
+    T *out = (T *)a.out + (size_t)y.row * a.out_stride + y.head * G2B_DH + 8 * g;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-        f32x4 x;
+    for (int q = 0; q < 4; ++q) {
+        f32x4 v[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = y.sees ? y.o[q / 4][4 * (q % 4) + e] / l : 0.f;
-        prompt_store(out + 32 * (q / 4) + 8 * (q % 4), x);
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[t][e] = y.sees ? y.o[t][4 * q + e] / l : 0.f;
+        prompt_store(out + 16 * q, v[0], v[1]);
     }
 }
-extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g2k_prompt_tile_f32(const g2_attn_prompt_args a) { prompt_tile_impl<float>(a); }
-extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g2k_prompt_tile_f16(const g2_attn_prompt_args a) { prompt_tile_impl<_Float16>(a); }
+extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void g2k_prompt_tile_f32(const g2_attn_prompt_args a) { prompt_tile_impl<float, 1>(a); }
+extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void g2k_prompt_tile_f16(const g2_attn_prompt_args a) { prompt_tile_impl<_Float16, 2>(a); }
 
 /* ======================================================================
  * 4-bit K/V cache: each position, head and 32 dims on their own, codes and

@@ -86,13 +86,17 @@ G2B_FN g2b_row g2b_row_keys(int row, int in, int q0, int q1, int k0, int k1, int
 /* Work-group b of tiles * NKV: its key head and tile of queries.  Work-group b
  * runs on XCD b % 8.  The last tiles, whose rows see most keys, come first, all
  * heads of a tile side by side; of the heads, 8 n of them keep to XCD head % 8,
- * whose L2 then has their keys, and the rest go where there is room. */
+ * whose L2 then has their keys, and the rest go where there is room.  Of each 32
+ * work-groups of an XCD (one for each of its CUs) every other 32 are turned
+ * round, so that a CU gets a shorter one behind a longer one. */
 G2B_FN void g2b_prompt_item(long b, int NKV, long tiles, int *head, long *tile)
 {
-    const long rank = b / NKV;
-    const int j = (int)(b % NKV), x = (int)(b % 8), fixed = NKV / 8 * 8;
+    const long x = b % 8, k = b / 8, turn = k / 32, n = NKV * tiles;
+    const long i = turn % 2 && (turn + 1) * 256 <= n ? 8 * (turn * 32 + 31 - k % 32) + x : b;
+    const long rank = i / NKV;
+    const int j = (int)(i % NKV), fixed = NKV / 8 * 8;
     *tile = tiles - 1 - rank;
-    *head = j < fixed ? j / 8 * 8 + x : fixed + j % 8;
+    *head = j < fixed ? j / 8 * 8 + (int)x : fixed + j % 8;
 }
 
 /* ---- beam search: ids of a work-group's slice of a row,

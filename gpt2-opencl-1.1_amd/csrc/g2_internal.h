@@ -227,7 +227,7 @@ int g2i_logits_form(int rows, int V, int *parts);
 
 /* Whether g2_attn_prompt takes the form for many queries (128 to a work-group,
  * else 32), and the work-groups of a key head. */
-int g2i_prompt_form(int rows, int n_head, int n_kv, long *tiles);
+int g2i_prompt_form(int rows, int n_seq, int n_head, int n_kv, long *tiles);
 
 /* g2_attn_kv4's parts of a key head's positions, tiles to a part, query heads to
  * a pass over them, passes to a key head, waves to a work-group. */

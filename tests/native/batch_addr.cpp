@@ -54,7 +54,7 @@ static int items(int NKV, long tiles)
         g2b_prompt_item(b, NKV, tiles, &h, &t);
         if (h < 0 || h >= NKV || t < 0 || t >= tiles || seen[h * tiles + t]++) return bad("a piece outside or twice", b, h, t);
         if (h < NKV / 8 * 8 && h % 8 != b % 8) return bad("a head on another XCD", b, h, t);
-        if (t != tiles - 1 - b / NKV) return bad("tiles in another order", b, h, t);
+        if (labs(tiles - 1 - t - b / NKV) * NKV > 256 + NKV) return bad("tiles in another order", b, h, t);
     }
     return 1;
 }
