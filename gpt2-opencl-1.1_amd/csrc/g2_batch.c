@@ -39,13 +39,13 @@ static int heads_check(const char *fn, int n_head, int n_kv)
 
 /* ---------------------------------------------------------- packed prompts */
 
-int g2i_prompt_form(int rows, int n_seq, int n_head, int n_kv, long *tiles)
+int g2i_prompt_form(int f16, int q_rows, int k_rows, int n_seq, int n_head, int n_kv, long *tiles)
 {
-    const long queries = (long)rows * (n_head / n_kv);
-    const int many = (queries + 127) / 128 * n_kv >= 256, size = many ? 128 : 32;
+    const long queries = (long)q_rows * (n_head / n_kv);
+    const int many = (queries + 127) / 128 * n_kv >= (f16 ? 300 : 512), size = many ? 128 : 32;
     /* (tiles of up to 63 sequences are their own, the last of each may not be full) */
     *tiles = n_seq > 1 && n_seq < 64 ? queries / size + n_seq : (queries + size - 1) / size;
-    return many;
+    return !many ? PF_SPLIT : f16 && (k_rows / n_seq >= 1500 || *tiles * n_kv < 1024) ? PF_DUO : PF_TILE;
 }
 
 int g2_attn_prompt(const void *q, int q_stride, const void *k, const void *v, int kv_stride, void *out, int out_stride,
@@ -74,15 +74,15 @@ int g2_attn_prompt(const void *q, int q_stride, const void *k, const void *v, in
         (q_start && g2i_overlap(out, no, q_start, ns)) || (k_start && g2i_overlap(out, no, k_start, ns)))
         return g2i_err(G2_E_ARG, "%s: the output overlaps an input", fn);
     long tiles;
-    const int many = g2i_prompt_form(q_rows, n_seq, n_head, n_kv, &tiles);
-    if (!fits(tiles * n_kv) || (long)q_rows * (n_head / n_kv) > INT32_MAX - 128) return g2i_err(G2_E_LIMIT, "%s: too many rows and heads for one call", fn);
+    const int f16 = dtype == G2_F16, form = g2i_prompt_form(f16, q_rows, k_rows, n_seq, n_head, n_kv, &tiles);
+    if (!fits(2 * tiles * n_kv) || (long)q_rows * (n_head / n_kv) > INT32_MAX - 128) return g2i_err(G2_E_LIMIT, "%s: too many rows and heads for one call", fn);
     if ((rc = ready())) return rc;
     g2_attn_prompt_args a = { q, k, v, out, q_start, k_start, q_rows > 1 ? q_stride : nq, k_rows > 1 ? kv_stride : nk,
                               q_rows > 1 ? out_stride : nq, n_seq, q_rows, k_rows, n_head, n_kv, (int)tiles,
                               aligned(v, 4) && (k_rows <= 1 || kv_stride % 2 == 0), scale };
-    const int fid = many ? (dtype == G2_F16 ? G2F_PROMPT_TILE_F16 : G2F_PROMPT_TILE_F32)
-                         : (dtype == G2_F16 ? G2F_PROMPT_SPLIT_F16 : G2F_PROMPT_SPLIT_F32);
-    return g2i_launch(fid, (unsigned)(tiles * n_kv), 1, 256, &a);
+    const int fid = form == PF_SPLIT ? (f16 ? G2F_PROMPT_SPLIT_F16 : G2F_PROMPT_SPLIT_F32)
+                  : form == PF_DUO ? G2F_PROMPT_DUO_F16 : f16 ? G2F_PROMPT_TILE_F16 : G2F_PROMPT_TILE_F32;
+    return g2i_launch(fid, (unsigned)(tiles * n_kv), 1, form == PF_DUO ? 512 : 256, &a);
 }
 
 /* -------------------------------------------------------------- 4-bit cache */

@@ -190,38 +190,42 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t prompt_rows(const T *p, int j0
     return __builtin_amdgcn_make_buffer_rsrc((void *)(p + (size_t)j0 * stride), (short)0, bytes, 0x00020000);
 }
 /* Two dims' values of the eight keys that a lane of half g takes in step u (in the
- * second product's order): where they are, from the buffer's begin. */
-template <typename T> __device__ __forceinline__ void prompt_value_at(unsigned (&at)[8], int u, int g, int pair, long stride)
+ * second product's order): where the first of them is, from the buffer's begin.
+ * (Where the others are is added up for each load: eight registers held for it
+ * cost the fp32 tiles a wave.) */
+template <typename T> __device__ __forceinline__ unsigned prompt_value_at(int u, int g, int pair, long stride)
 {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) at[e] = ((unsigned)(16 * u + 8 * (e / 4) + 4 * g + e % 4) * (unsigned)stride + 2u * (unsigned)pair) * (unsigned)sizeof(T);
+    return ((unsigned)(16 * u + 4 * g) * (unsigned)stride + 2u * (unsigned)pair) * (unsigned)sizeof(T);
 }
-/* (fp16 pairs: `even` where they are at a multiple of four bytes, which a load of both asks for) */
-__device__ __forceinline__ void prompt_load_v(float (&x)[2][8], __amdgpu_buffer_rsrc_t rows, const unsigned (&at)[8], int)
+__device__ __forceinline__ void prompt_load_v(float (&x)[2][8], __amdgpu_buffer_rsrc_t rows, unsigned at, long stride, int)
 {
     typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    asm volatile("" : "+v"(at));
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rows, (int)at[e], 0, 0));
+        const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rows, (int)(at + (unsigned)(8 * (e / 4) + e % 4) * (unsigned)stride * 4u), 0, 0));
         x[0][e] = __uint_as_float(v[0]);
         x[1][e] = __uint_as_float(v[1]);
     }
 }
-__device__ __forceinline__ void prompt_load_v(_Float16 (&x)[2][8], __amdgpu_buffer_rsrc_t rows, const unsigned (&at)[8], int even)
+/* (fp16 pairs: `even` where they are at a multiple of four bytes, which a load of both asks for) */
+__device__ __forceinline__ void prompt_load_v(_Float16 (&x)[2][8], __amdgpu_buffer_rsrc_t rows, unsigned at, long stride, int even)
 {
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    asm volatile("" : "+v"(at));
     if (even)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const f16x2 v = __builtin_bit_cast(f16x2, __builtin_amdgcn_raw_buffer_load_b32(rows, (int)at[e], 0, 0));
+            const f16x2 v = __builtin_bit_cast(f16x2, __builtin_amdgcn_raw_buffer_load_b32(rows, (int)(at + (unsigned)(8 * (e / 4) + e % 4) * (unsigned)stride * 2u), 0, 0));
             x[0][e] = v[0];
             x[1][e] = v[1];
         }
     else
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            x[0][e] = __builtin_bit_cast(_Float16, __builtin_amdgcn_raw_buffer_load_b16(rows, (int)at[e], 0, 0));
-            x[1][e] = __builtin_bit_cast(_Float16, __builtin_amdgcn_raw_buffer_load_b16(rows, (int)at[e] + 2, 0, 0));
+            const int p = (int)(at + (unsigned)(8 * (e / 4) + e % 4) * (unsigned)stride * 2u);
+            x[0][e] = __builtin_bit_cast(_Float16, __builtin_amdgcn_raw_buffer_load_b16(rows, p, 0, 0));
+            x[1][e] = __builtin_bit_cast(_Float16, __builtin_amdgcn_raw_buffer_load_b16(rows, p + 2, 0, 0));
         }
 }
 
@@ -238,7 +242,7 @@ template <typename T> struct prompt_query {
     bool sees;
     prompt_op<T> q[4];
     f32x16 o[2];
-    float m, l;
+    float m, l, base; /* base: added to a score in units of log 2, this time */
 };
 
 template <typename T>
@@ -285,9 +289,8 @@ __device__ __forceinline__ void prompt_start(prompt_query<T> &y, const g2_attn_p
  * weights are 2^6 times that, so that small ones keep their bits: 2^14 at most,
  * exact down to 2^-20 of the largest). */
 template <typename T>
-__device__ __forceinline__ void prompt_weights(prompt_query<T> &y, f32x16 &s, int j0, float c, int g)
+__device__ __forceinline__ void prompt_follow(prompt_query<T> &y, f32x16 &s, int j0, float c, int g)
 {
-    constexpr bool F16 = sizeof(T) == 2;
     if (wave_any(y.keys.lo > j0 || y.keys.end < j0 + 32)) { /* some query does not see all of them */
         const int at = j0 + 4 * g - y.keys.lo, n = y.keys.end - y.keys.lo;
 #pragma unroll
@@ -309,23 +312,28 @@ __device__ __forceinline__ void prompt_weights(prompt_query<T> &y, f32x16 &s, in
             for (int r = 0; r < 16; ++r) y.o[t][r] *= down;
         y.m = top;
     }
-    /* The exponent as one operation on the score: what the rounding of m c adds is the
-     * same factor for all weights of a query, and has to be a small one. */
-    const float up = F16 ? 6.f : 0.f, mc = y.m == -INFINITY ? 0.f : y.m * c, base = up - mc;
-    const bool far = !(fabsf(mc) < 0x1p28f);
-    float sum = 0.f;
+    /* The exponent will be one operation on the score: what the rounding of m c adds is
+     * the same factor for all weights of a query.  Where it could be a large one, the
+     * scores become differences now. */
+    const bool far = !(fabsf(y.m * c) < 0x1p28f) && y.m != -INFINITY;
     if (wave_any(far)) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = far ? fmaf(s[r] - y.m, c, up) : fmaf(s[r], c, base);
-    } else
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, base);
+        for (int r = 0; r < 16; ++r) s[r] = far ? s[r] - y.m : s[r];
+        y.base = far ? 0.f : y.m;
+    } else y.base = y.m;
+    y.base = (sizeof(T) == 2 ? 6.f : 0.f) - (y.base == -INFINITY ? 0.f : y.base * c);
+}
+/* Scores to weights, and their sum. */
+template <typename T>
+__device__ __forceinline__ void prompt_weights(prompt_query<T> &y, f32x16 &s, float c)
+{
+    float sum[2] = {};
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        s[r] = __builtin_amdgcn_exp2f(s[r]);
-        sum += s[r];
+        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, y.base));
+        sum[r & 1] += s[r];
     }
-    y.l += sum;
+    y.l += sum[0] + sum[1];
 }
 
 /* The operand of the weights of step u. */
@@ -345,11 +353,25 @@ __device__ __forceinline__ void prompt_weight_op(const f32x16 &s, int u, prompt_
 /* Whether one of eight values is not finite; such values are then 0: they must not
  * meet the weights 0 of queries that do not see them.  prompt_odd adds them to
  * the queries that do. */
-template <typename T> __device__ __forceinline__ float prompt_look(const T (&v)[8], float z)
+__device__ __forceinline__ bool prompt_look(const float (&v)[2][8])
 {
+    float z[2] = {};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) z = fmaf((float)v[e], 0.f, z);
-    return z;
+    for (int e = 0; e < 8; ++e) {
+        z[0] = fmaf(v[0][e], 0.f, z[0]);
+        z[1] = fmaf(v[1][e], 0.f, z[1]);
+    }
+    return wave_any(z[0] + z[1] != 0.f);
+}
+__device__ __forceinline__ bool prompt_look(const _Float16 (&v)[2][8])
+{
+    _Float16 z0 = 0, z1 = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        z0 = __builtin_fmaf16(v[0][e], (_Float16)0.f, z0);
+        z1 = __builtin_fmaf16(v[1][e], (_Float16)0.f, z1);
+    }
+    return wave_any(z0 + z1 != (_Float16)0.f);
 }
 template <typename T> __device__ __forceinline__ void prompt_clean(T (&v)[8])
 {
@@ -384,30 +406,42 @@ template <typename T> __device__ __forceinline__ void prompt_store(T *p, const f
     }
 }
 
+template <typename T> __device__ __forceinline__ void prompt_out(const prompt_query<T> &y, const g2_attn_prompt_args &a, float l, int g)
+{
+    const float one = 1.f / l;
+    T *out = (T *)a.out + (size_t)y.row * a.out_stride + y.head * G2B_DH + 8 * g;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        f32x4 v[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[t][e] = y.sees ? y.o[t][4 * q + e] * one : 0.f;
+        prompt_store(out + 16 * q, v[0], v[1]);
+    }
+}
+
 /* ---- few queries: a work-group takes 32 of them, its four waves every fourth 32
  * keys each, whose rows they read as the operands that they are (a key's dims
  * 16 bytes at a time, a value's dims side by side, so that eight loads are
  * eight keys of a dim); the waves' states meet at the end. */
-template <typename T>
+template <typename T, int KW>
 __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
 {
-    constexpr int KW = 4;
     __shared__ float red[KW][34][64];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     int hk;
     long tile;
     g2b_prompt_item(blockIdx.x, a.NKV, a.tiles, &hk, &tile);
     prompt_query<T> y;
-    const prompt_place place = prompt_find(a, 32, a.tiles - 1 - (int)tile, lane);
+    const prompt_place place = prompt_find(a, 128 / KW, a.tiles - 1 - (int)tile, lane);
     if (place.first < 0) return;
-    prompt_start(y, a, hk, place, 0, lane);
+    prompt_start(y, a, hk, place, KW == 1 ? 32 * w : 0, lane);
     const float c = prompt_unit(a.scale);
     const long stride = a.kv_stride;
     const T *kp = (const T *)a.k + hk * G2B_DH, *vp = (const T *)a.v + hk * G2B_DH;
     T k[4][8], v[2][2][8]; /* v: step, dim of the pair, key */
-    unsigned at[2][8];
-    prompt_value_at<T>(at[0], 0, g, lane & 31, stride);
-    prompt_value_at<T>(at[1], 1, g, lane & 31, stride);
+    const unsigned at[2] = { prompt_value_at<T>(0, g, lane & 31, stride), prompt_value_at<T>(1, g, lane & 31, stride) };
     auto load_k = [&](int j0) {
         const T *p = kp + (size_t)j0 * stride + (size_t)min(lane & 31, y.k1 - j0 - 1) * stride + 8 * g;
 #pragma unroll
@@ -416,9 +450,9 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
     auto load_v = [&](int j0) {
         const __amdgpu_buffer_rsrc_t rows = prompt_rows(vp, j0, y.k1, stride);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) prompt_load_v(v[u], rows, at[u], a.even);
+        for (int u = 0; u < 2; ++u) prompt_load_v(v[u], rows, at[u], stride, a.even);
     };
-    int j0 = y.k0 < y.k1 ? y.k0 + 32 * w : y.k1;
+    int j0 = y.k0 < y.k1 ? y.k0 + (KW == 1 ? 0 : 32 * w) : y.k1;
     if (j0 < y.k1) { load_k(j0); load_v(j0); }
     for (; j0 < y.k1; j0 += 32 * KW) {
         const int j1 = j0 + 32 * KW;
@@ -430,13 +464,10 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
             s = prompt_mma(x, y.q[i], s);
         }
         if (j1 < y.k1) load_k(j1);
-        prompt_weights(y, s, j0, c, g);
-        float z = 0.f;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) z = prompt_look(v[u][t], z);
-        if (wave_any(z != 0.f)) {
+        prompt_follow(y, s, j0, c, g);
+        prompt_weights(y, s, c);
+        const bool odd0 = prompt_look(v[0]), odd1 = prompt_look(v[1]);
+        if (odd0 || odd1) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -456,6 +487,10 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
         if (j1 < y.k1) load_v(j1);
     }
     y.l = swap_sum(y.l);
+    if constexpr (KW == 1) {
+        if (y.keys.there) prompt_out(y, a, y.l, g);
+        return;
+    }
     /* the waves' parts meet; wave w writes the dims of its share of the registers */
     red[w][0][lane] = y.m;
     red[w][1][lane] = y.l;
@@ -473,6 +508,7 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
         part[i] = prompt_factor(red[i][0][lane], top, c);
         l = fmaf(red[i][1][lane], part[i], l);
     }
+    const float one = 1.f / l;
     T *out = (T *)a.out + (size_t)y.row * a.out_stride + y.head * G2B_DH + 8 * g;
     f32x4 x[2] = {};
 #pragma unroll
@@ -481,12 +517,12 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
         for (int e = 0; e < 4; ++e) {
 #pragma unroll
             for (int j = 0; j < KW; ++j) x[t][e] = fmaf(red[j][2 + 16 * t + 4 * w + e][lane], part[j], x[t][e]);
-            x[t][e] = y.sees ? x[t][e] / l : 0.f;
+            x[t][e] = y.sees ? x[t][e] * one : 0.f;
         }
     prompt_store(out + 16 * w, x[0], x[1]);
 }
-extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g2k_prompt_split_f32(const g2_attn_prompt_args a) { prompt_split_impl<float>(a); }
-extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g2k_prompt_split_f16(const g2_attn_prompt_args a) { prompt_split_impl<_Float16>(a); }
+extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g2k_prompt_split_f32(const g2_attn_prompt_args a) { prompt_split_impl<float, 4>(a); }
+extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g2k_prompt_split_f16(const g2_attn_prompt_args a) { prompt_split_impl<_Float16, 4>(a); }
 
 /* ---- many queries: a work-group takes 128 of them, 32 a wave, and its waves
  * read KT times 32 keys and values together, once, as operands in LDS: unit
@@ -494,13 +530,16 @@ extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
  * writes are both rows of units.  Two stages: the next keys are on their way from
  * memory while the products of these run, and one barrier stands between.  Of 32
  * keys two waves bring the keys, two the values (a step each), in turns. */
-template <typename T, int KT>
+template <typename T, int KT, int KW>
 __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
 {
     constexpr int P = sizeof(T) == 4 ? 3 : 1, UNITS = P * 256; /* of 32 keys, and of their values */
-    __shared__ u32x4 lds[2][KT][2 * UNITS];
-    __shared__ int range[4][2], odd[2][KT][2];
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, m = lane & 31;
+    __shared__ u32x4 all[KW][2][KT][2 * UNITS];
+    __shared__ int range[4][2], odds[KW][2][KT][2];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3, kw = wave >> 2;
+    const int g = lane >> 5, m = lane & 31;
+    auto &lds = all[kw];
+    auto &odd = odds[kw];
     int hk;
     long tile;
     g2b_prompt_item(blockIdx.x, a.NKV, a.tiles, &hk, &tile);
@@ -508,7 +547,7 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
     const prompt_place place = prompt_find(a, 128, a.tiles - 1 - (int)tile, lane);
     if (place.first < 0) return;
     prompt_start(y, a, hk, place, 32 * w, lane);
-    if (lane == 0) { range[w][0] = y.k0; range[w][1] = y.k1; }
+    if (lane == 0 && kw == 0) { range[w][0] = y.k0; range[w][1] = y.k1; }
     __syncthreads();
     const int k0 = __builtin_amdgcn_readfirstlane(min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0])));
     const int k1 = __builtin_amdgcn_readfirstlane(max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1])));
@@ -516,8 +555,7 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
     const long stride = a.kv_stride;
     const T *kp = (const T *)a.k + hk * G2B_DH, *vp = (const T *)a.v + hk * G2B_DH;
     T x[KT][2][8]; /* this lane's share: two chunks of a key's dims, or two dims of eight keys */
-    unsigned at[8];
-    prompt_value_at<T>(at, w & 1, g, m, stride);
+    const unsigned at = prompt_value_at<T>(w & 1, g, m, stride);
     auto brings_keys = [&](int i) { return ((w >> 1) ^ i) & 1; };
     const int chunk = 4 * (w & 1) + 2 * g;
     auto load = [&](int j0) {
@@ -528,7 +566,7 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
                 const T *p = kp + (size_t)j * stride + (size_t)min(m, k1 - j - 1) * stride + 8 * chunk;
                 prompt_load_k(x[i][0], p);
                 prompt_load_k(x[i][1], p + 8);
-            } else prompt_load_v(x[i], prompt_rows(vp, j, k1, stride), at, a.even);
+            } else prompt_load_v(x[i], prompt_rows(vp, j, k1, stride), at, stride, a.even);
         }
     };
     auto put = [&](u32x4 *p, const T (&v)[8]) {
@@ -546,7 +584,7 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
                 put(lds[b][i] + chunk * 32 + m, x[i][0]);
                 put(lds[b][i] + chunk * 32 + 32 + m, x[i][1]);
             } else {
-                const bool any = wave_any(prompt_look(x[i][1], prompt_look(x[i][0], 0.f)) != 0.f);
+                const bool any = prompt_look(x[i]);
                 if (any) { prompt_clean(x[i][0]); prompt_clean(x[i][1]); }
                 if (lane == 0) odd[b][i][w & 1] = any;
                 put(lds[b][i] + UNITS + (w & 1) * 64 + lane, x[i][0]);
@@ -560,15 +598,17 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
             for (int i = 0; i < 3; ++i) z.p[i] = p[256 * i];
         } else z.p = __builtin_bit_cast(f16x8, *p);
     };
-    if (k0 < k1) {
-        load(k0);
+    /* (the groups of four waves take every KW-th piece; all go through as many barriers) */
+    constexpr int STEP = 32 * KT * KW;
+    int j0 = k0 + 32 * KT * kw, b = 0;
+    if (j0 < k1) {
+        load(j0);
         stage(0);
     }
     __syncthreads();
-    int b = 0;
-    for (int j0 = k0; j0 < k1; j0 += 32 * KT, b ^= 1) {
-        const bool more = j0 + 32 * KT < k1;
-        if (more) load(j0 + 32 * KT);
+    for (int left = k1 - k0; KW == 1 ? j0 < k1 : left > 0; left -= STEP, j0 += STEP, b ^= 1) {
+        const bool more = j0 + STEP < k1;
+        if (more) load(j0 + STEP);
 #pragma unroll
         for (int i = 0; i < KT; ++i) {
             const int j = j0 + 32 * i;
@@ -582,7 +622,8 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
 #pragma unroll
                 for (int t = 0; t < 4; ++t) s = prompt_mma(z[t], y.q[t], s);
             }
-            prompt_weights(y, s, j, c, g);
+            prompt_follow(y, s, j, c, g);
+            prompt_weights(y, s, c);
             if (__builtin_amdgcn_readfirstlane(odd[b][i][0] | odd[b][i][1])) prompt_odd(y, vp, stride, j, min(32, k1 - j), g);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -598,21 +639,35 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
         if (more) stage(b ^ 1);
         __syncthreads();
     }
-    if (!y.keys.there) return;
-    const float l = swap_sum(y.l);
-    T *out = (T *)a.out + (size_t)y.row * a.out_stride + y.head * G2B_DH + 8 * g;
+    y.l = swap_sum(y.l);
+    if constexpr (KW > 1) { /* the groups' states meet where the keys were */
+        static_assert(KW == 2 && sizeof(all) >= 34 * 256 * sizeof(float), "one state a query in LDS");
+        float *red = (float *)all + w * 64 + lane;
+        if (kw) {
+            red[0] = y.m;
+            red[256] = y.l;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        f32x4 v[2];
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) red[256 * (2 + 16 * t + r)] = y.o[t][r];
+        }
+        __syncthreads();
+        if (kw) return;
+        const float top = fmaxf(y.m, red[0]), mine = prompt_factor(y.m, top, c), other = prompt_factor(red[0], top, c);
+        y.l = y.l * mine + red[256] * other;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[t][e] = y.sees ? y.o[t][4 * q + e] / l : 0.f;
-        prompt_store(out + 16 * q, v[0], v[1]);
+            for (int r = 0; r < 16; ++r) y.o[t][r] = y.o[t][r] * mine + red[256 * (2 + 16 * t + r)] * other;
     }
+    if (y.keys.there) prompt_out(y, a, y.l, g);
 }
-extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void g2k_prompt_tile_f32(const g2_attn_prompt_args a) { prompt_tile_impl<float, 1>(a); }
-extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void g2k_prompt_tile_f16(const g2_attn_prompt_args a) { prompt_tile_impl<_Float16, 2>(a); }
+#define PROMPT_TILE(NAME, T, KT, KW, WAVES)                                                                            \
+    extern "C" __global__ __launch_bounds__(256 * KW) __attribute__((amdgpu_waves_per_eu(WAVES)))                      \
+    void NAME(const g2_attn_prompt_args a) { prompt_tile_impl<T, KT, KW>(a); }
+PROMPT_TILE(g2k_prompt_tile_f32, float, 1, 1, 3)
+PROMPT_TILE(g2k_prompt_tile_f16, _Float16, 2, 1, 4)
+PROMPT_TILE(g2k_prompt_duo_f16, _Float16, 2, 2, 4)
 
 /* ======================================================================
  * 4-bit K/V cache: each position, head and 32 dims on their own, codes and

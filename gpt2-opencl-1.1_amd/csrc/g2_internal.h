@@ -131,6 +131,7 @@ extern "C" {
     X(PROMPT_SPLIT_F16, "g2k_prompt_split_f16")                               \
     X(PROMPT_TILE_F32, "g2k_prompt_tile_f32")                                 \
     X(PROMPT_TILE_F16, "g2k_prompt_tile_f16")                                 \
+    X(PROMPT_DUO_F16, "g2k_prompt_duo_f16")                                   \
     X(KV4_APPEND_F32, "g2k_kv4_append_f32")                                   \
     X(KV4_APPEND_F16, "g2k_kv4_append_f16") X(KV4_READ, "g2k_kv4_read")       \
     G2_KV4_LIST(X, 1, 1) G2_KV4_LIST(X, 1, 4) G2_KV4_LIST(X, 1, 8)            \
@@ -225,9 +226,10 @@ int g2i_kv8_form(long heads, int T_kv, int *span, int *waves);
 /* Whether g2_apply_logit_rules takes its wide form, and the slices of a row. */
 int g2i_logits_form(int rows, int V, int *parts);
 
-/* Whether g2_attn_prompt takes the form for many queries (128 to a work-group,
- * else 32), and the work-groups of a key head. */
-int g2i_prompt_form(int rows, int n_seq, int n_head, int n_kv, long *tiles);
+/* g2_attn_prompt's form, and the work-groups of a key head: 32 queries to a
+ * work-group, 128, or 128 in two groups of waves that share the keys. */
+enum { PF_SPLIT, PF_TILE, PF_DUO };
+int g2i_prompt_form(int f16, int q_rows, int k_rows, int n_seq, int n_head, int n_kv, long *tiles);
 
 /* g2_attn_kv4's parts of a key head's positions, tiles to a part, query heads to
  * a pass over them, passes to a key head, waves to a work-group. */
