@@ -197,36 +197,44 @@ template <typename T> __device__ __forceinline__ unsigned prompt_value_at(int u,
 {
     return ((unsigned)(16 * u + 4 * g) * (unsigned)stride + 2u * (unsigned)pair) * (unsigned)sizeof(T);
 }
-__device__ __forceinline__ void prompt_load_v(float (&x)[2][8], __amdgpu_buffer_rsrc_t rows, unsigned at, long stride, int)
+/* (fp16 values stay the pairs that they are in memory) */
+template <typename T> struct prompt_pairs;
+template <> struct prompt_pairs<float> { float x[2][8]; };
+template <> struct prompt_pairs<_Float16> { unsigned x[8]; };
+__device__ __forceinline__ void prompt_load_v(prompt_pairs<float> &v, __amdgpu_buffer_rsrc_t rows, unsigned at, long stride, int)
 {
     typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
     asm volatile("" : "+v"(at));
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rows, (int)(at + (unsigned)(8 * (e / 4) + e % 4) * (unsigned)stride * 4u), 0, 0));
-        x[0][e] = __uint_as_float(v[0]);
-        x[1][e] = __uint_as_float(v[1]);
+        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rows, (int)(at + (unsigned)(8 * (e / 4) + e % 4) * (unsigned)stride * 4u), 0, 0));
+        v.x[0][e] = __uint_as_float(w[0]);
+        v.x[1][e] = __uint_as_float(w[1]);
     }
 }
-/* (fp16 pairs: `even` where they are at a multiple of four bytes, which a load of both asks for) */
-__device__ __forceinline__ void prompt_load_v(_Float16 (&x)[2][8], __amdgpu_buffer_rsrc_t rows, unsigned at, long stride, int even)
+/* (`even` where pairs are at multiples of four bytes, which a load of both asks for) */
+__device__ __forceinline__ void prompt_load_v(prompt_pairs<_Float16> &v, __amdgpu_buffer_rsrc_t rows, unsigned at, long stride, int even)
 {
-    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
     asm volatile("" : "+v"(at));
     if (even)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const f16x2 v = __builtin_bit_cast(f16x2, __builtin_amdgcn_raw_buffer_load_b32(rows, (int)(at + (unsigned)(8 * (e / 4) + e % 4) * (unsigned)stride * 2u), 0, 0));
-            x[0][e] = v[0];
-            x[1][e] = v[1];
-        }
+        for (int e = 0; e < 8; ++e)
+            v.x[e] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(rows, (int)(at + (unsigned)(8 * (e / 4) + e % 4) * (unsigned)stride * 2u), 0, 0);
     else
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int p = (int)(at + (unsigned)(8 * (e / 4) + e % 4) * (unsigned)stride * 2u);
-            x[0][e] = __builtin_bit_cast(_Float16, __builtin_amdgcn_raw_buffer_load_b16(rows, p, 0, 0));
-            x[1][e] = __builtin_bit_cast(_Float16, __builtin_amdgcn_raw_buffer_load_b16(rows, p + 2, 0, 0));
+            v.x[e] = (unsigned)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rows, p, 0, 0) | (unsigned)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rows, p + 2, 0, 0) << 16;
         }
+}
+/* The operand of dim t of the pairs. */
+__device__ __forceinline__ void prompt_pack(const prompt_pairs<float> &v, int t, prompt_op<float> &o) { parts3(v.x[t], o.p); }
+__device__ __forceinline__ void prompt_pack(const prompt_pairs<_Float16> &v, int t, prompt_op<_Float16> &o)
+{
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_perm(v.x[2 * e + 1], v.x[2 * e], t ? 0x07060302u : 0x05040100u);
+    o.p = __builtin_bit_cast(f16x8, w);
 }
 
 /* Scores in units of log 2; not 0, which would make NaN of the masked ones. */
@@ -353,30 +361,39 @@ __device__ __forceinline__ void prompt_weight_op(const f32x16 &s, int u, prompt_
 /* Whether one of eight values is not finite; such values are then 0: they must not
  * meet the weights 0 of queries that do not see them.  prompt_odd adds them to
  * the queries that do. */
-__device__ __forceinline__ bool prompt_look(const float (&v)[2][8])
+__device__ __forceinline__ bool prompt_look(const prompt_pairs<float> &v)
 {
     float z[2] = {};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        z[0] = fmaf(v[0][e], 0.f, z[0]);
-        z[1] = fmaf(v[1][e], 0.f, z[1]);
+        z[0] = fmaf(v.x[0][e], 0.f, z[0]);
+        z[1] = fmaf(v.x[1][e], 0.f, z[1]);
     }
     return wave_any(z[0] + z[1] != 0.f);
 }
-__device__ __forceinline__ bool prompt_look(const _Float16 (&v)[2][8])
+__device__ __forceinline__ bool prompt_look(const prompt_pairs<_Float16> &v)
 {
-    _Float16 z0 = 0, z1 = 0;
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 zero = { (_Float16)0.f, (_Float16)0.f };
+    f16x2 z = zero;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, v.x[e]), zero, z);
+    return wave_any((__builtin_bit_cast(unsigned, z) & 0x7FFF7FFFu) != 0);
+}
+__device__ __forceinline__ void prompt_clean(prompt_pairs<float> &v)
+{
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v.x[t][e] = __builtin_isfinite(v.x[t][e]) ? v.x[t][e] : 0.f;
+}
+__device__ __forceinline__ void prompt_clean(prompt_pairs<_Float16> &v)
+{
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        z0 = __builtin_fmaf16(v[0][e], (_Float16)0.f, z0);
-        z1 = __builtin_fmaf16(v[1][e], (_Float16)0.f, z1);
+        if ((v.x[e] & 0x7C00u) == 0x7C00u) v.x[e] &= 0xFFFF0000u;
+        if ((v.x[e] & 0x7C000000u) == 0x7C000000u) v.x[e] &= 0xFFFFu;
     }
-    return wave_any(z0 + z1 != (_Float16)0.f);
-}
-template <typename T> __device__ __forceinline__ void prompt_clean(T (&v)[8])
-{
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = __builtin_isfinite((float)v[e]) ? v[e] : (T)0.f;
 }
 template <typename T>
 __device__ __forceinline__ void prompt_odd(prompt_query<T> &y, const T *v, long stride, int j0, int n, int g)
@@ -440,7 +457,8 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
     const float c = prompt_unit(a.scale);
     const long stride = a.kv_stride;
     const T *kp = (const T *)a.k + hk * G2B_DH, *vp = (const T *)a.v + hk * G2B_DH;
-    T k[4][8], v[2][2][8]; /* v: step, dim of the pair, key */
+    T k[4][8];
+    prompt_pairs<T> v[2]; /* of the two steps */
     const unsigned at[2] = { prompt_value_at<T>(0, g, lane & 31, stride), prompt_value_at<T>(1, g, lane & 31, stride) };
     auto load_k = [&](int j0) {
         const T *p = kp + (size_t)j0 * stride + (size_t)min(lane & 31, y.k1 - j0 - 1) * stride + 8 * g;
@@ -468,10 +486,8 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
         prompt_weights(y, s, c);
         const bool odd0 = prompt_look(v[0]), odd1 = prompt_look(v[1]);
         if (odd0 || odd1) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) prompt_clean(v[u][t]);
+            prompt_clean(v[0]);
+            prompt_clean(v[1]);
             prompt_odd(y, vp, stride, j0, min(32, y.k1 - j0), g);
         }
 #pragma unroll
@@ -480,7 +496,7 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
             prompt_weight_op(s, u, p);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                prompt_pack(v[u][t], x);
+                prompt_pack(v[u], t, x);
                 y.o[t] = prompt_mma(x, p, y.o[t]);
             }
         }
@@ -554,7 +570,10 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
     const float c = prompt_unit(a.scale);
     const long stride = a.kv_stride;
     const T *kp = (const T *)a.k + hk * G2B_DH, *vp = (const T *)a.v + hk * G2B_DH;
-    T x[KT][2][8]; /* this lane's share: two chunks of a key's dims, or two dims of eight keys */
+    union share { /* this lane's: two chunks of a key's dims, or two dims of eight keys */
+        T k[2][8];
+        prompt_pairs<T> v;
+    } x[KT];
     const unsigned at = prompt_value_at<T>(w & 1, g, m, stride);
     auto brings_keys = [&](int i) { return ((w >> 1) ^ i) & 1; };
     const int chunk = 4 * (w & 1) + 2 * g;
@@ -564,14 +583,12 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
             const int j = min(j0 + 32 * i, k1 - 1); /* (keys behind the last are masked) */
             if (brings_keys(i)) {
                 const T *p = kp + (size_t)j * stride + (size_t)min(m, k1 - j - 1) * stride + 8 * chunk;
-                prompt_load_k(x[i][0], p);
-                prompt_load_k(x[i][1], p + 8);
-            } else prompt_load_v(x[i], prompt_rows(vp, j, k1, stride), at, stride, a.even);
+                prompt_load_k(x[i].k[0], p);
+                prompt_load_k(x[i].k[1], p + 8);
+            } else prompt_load_v(x[i].v, prompt_rows(vp, j, k1, stride), at, stride, a.even);
         }
     };
-    auto put = [&](u32x4 *p, const T (&v)[8]) {
-        prompt_op<T> z;
-        prompt_pack(v, z);
+    auto put = [&](u32x4 *p, const prompt_op<T> &z) {
         if constexpr (P == 3) {
 #pragma unroll
             for (int i = 0; i < 3; ++i) p[256 * i] = z.p[i];
@@ -580,15 +597,20 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
     auto stage = [&](int b) {
 #pragma unroll
         for (int i = 0; i < KT; ++i) {
+            prompt_op<T> z;
             if (brings_keys(i)) {
-                put(lds[b][i] + chunk * 32 + m, x[i][0]);
-                put(lds[b][i] + chunk * 32 + 32 + m, x[i][1]);
+                prompt_pack(x[i].k[0], z);
+                put(lds[b][i] + chunk * 32 + m, z);
+                prompt_pack(x[i].k[1], z);
+                put(lds[b][i] + chunk * 32 + 32 + m, z);
             } else {
-                const bool any = prompt_look(x[i]);
-                if (any) { prompt_clean(x[i][0]); prompt_clean(x[i][1]); }
+                const bool any = prompt_look(x[i].v);
+                if (any) prompt_clean(x[i].v);
                 if (lane == 0) odd[b][i][w & 1] = any;
-                put(lds[b][i] + UNITS + (w & 1) * 64 + lane, x[i][0]);
-                put(lds[b][i] + UNITS + 128 + (w & 1) * 64 + lane, x[i][1]);
+                prompt_pack(x[i].v, 0, z);
+                put(lds[b][i] + UNITS + (w & 1) * 64 + lane, z);
+                prompt_pack(x[i].v, 1, z);
+                put(lds[b][i] + UNITS + 128 + (w & 1) * 64 + lane, z);
             }
         }
     };
