@@ -451,9 +451,9 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
     long tile;
     g2b_prompt_item(blockIdx.x, a.NKV, a.tiles, &hk, &tile);
     prompt_query<T> y;
-    const prompt_place place = prompt_find(a, 128 / KW, a.tiles - 1 - (int)tile, lane);
+    const prompt_place place = prompt_find(a, 32, a.tiles - 1 - (int)tile, lane);
     if (place.first < 0) return;
-    prompt_start(y, a, hk, place, KW == 1 ? 32 * w : 0, lane);
+    prompt_start(y, a, hk, place, 0, lane);
     const float c = prompt_unit(a.scale);
     const long stride = a.kv_stride;
     const T *kp = (const T *)a.k + hk * G2B_DH, *vp = (const T *)a.v + hk * G2B_DH;
@@ -470,7 +470,7 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
 #pragma unroll
         for (int u = 0; u < 2; ++u) prompt_load_v(v[u], rows, at[u], stride, a.even);
     };
-    int j0 = y.k0 < y.k1 ? y.k0 + (KW == 1 ? 0 : 32 * w) : y.k1;
+    int j0 = y.k0 < y.k1 ? y.k0 + 32 * w : y.k1;
     if (j0 < y.k1) { load_k(j0); load_v(j0); }
     for (; j0 < y.k1; j0 += 32 * KW) {
         const int j1 = j0 + 32 * KW;
@@ -503,11 +503,7 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
         if (j1 < y.k1) load_v(j1);
     }
     y.l = swap_sum(y.l);
-    if constexpr (KW == 1) {
-        if (y.keys.there) prompt_out(y, a, y.l, g);
-        return;
-    }
-    /* the waves' parts meet; wave w writes the dims of its share of the registers */
+    /* the waves' parts meet; the first four waves write a quarter of the dims each */
     red[w][0][lane] = y.m;
     red[w][1][lane] = y.l;
 #pragma unroll
@@ -515,7 +511,7 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
 #pragma unroll
         for (int r = 0; r < 16; ++r) red[w][2 + 16 * t + r][lane] = y.o[t][r];
     __syncthreads();
-    if (!y.keys.there) return;
+    if (!y.keys.there || w >= 4) return;
     float top = -INFINITY, part[KW], l = 0.f;
 #pragma unroll
     for (int i = 0; i < KW; ++i) top = fmaxf(top, red[i][0][lane]);
@@ -537,8 +533,11 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
         }
     prompt_store(out + 16 * w, x[0], x[1]);
 }
-extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g2k_prompt_split_f32(const g2_attn_prompt_args a) { prompt_split_impl<float, 4>(a); }
-extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g2k_prompt_split_f16(const g2_attn_prompt_args a) { prompt_split_impl<_Float16, 4>(a); }
+#define PROMPT_SPLIT(NAME, T, KW)                                                                                      \
+    extern "C" __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(2)))                           \
+    void NAME(const g2_attn_prompt_args a) { prompt_split_impl<T, KW>(a); }
+PROMPT_SPLIT(g2k_prompt_split_f32, float, 4)
+PROMPT_SPLIT(g2k_prompt_split_f16, _Float16, 4)
 
 /* ---- many queries: a work-group takes 128 of them, 32 a wave, and its waves
  * read KT times 32 keys and values together, once, as operands in LDS: unit
@@ -721,7 +720,7 @@ __device__ void kv4_append_impl(const g2_kv4_append_args &a)
         q1 = q0 + a.per;
     }
     const bool there = s >= 0 && s < a.S && row >= q0 && row < q1 && row < a.rows;
-    const long p = there ? (long)(a.pos ? a.pos[s] : a.start) + (row - q0) : -1;
+    const long p = there ? (long)(a.pos ? a.pos[s] : a.start) + ((long)row - q0) : -1;
     float x[8];
     unsigned amax = 0;
 #pragma unroll

@@ -76,6 +76,37 @@ def test_every_form_of_the_selection_is_tested():
     assert len(seen) == 6
 
 
+def prompt_form(f16, q_rows, k_rows, S, NH, NKV):
+    fn = g2hip._lib.g2i_prompt_form
+    fn.argtypes = [C.c_int] * 6 + [C.POINTER(C.c_long)]
+    tiles = C.c_long()
+    return fn(int(f16), q_rows, k_rows, S, NH, NKV, C.byref(tiles)), tiles.value
+
+
+def test_prompt_tiles_cover_the_rows():
+    for f16 in (False, True):
+        for S in (1, 2, 63, 64, 500):
+            for rows in (1, 31, 32, 33, 600, 5000, 100000):
+                for NH, NKV in ((1, 1), (12, 12), (16, 4), (25, 5), (7, 1)):
+                    form, tiles = prompt_form(f16, rows, rows, S, NH, NKV)
+                    size, group = 32 if form == 0 else 128, NH // NKV
+                    assert tiles >= -(-rows * group // size)
+                    if 1 < S < 64:  # (sequences' own tiles: the most is one that is not full for each)
+                        lens = [rows // S + (i < rows % S) for i in range(S)]
+                        assert tiles >= sum(-(-n * group // size) for n in lens)
+
+
+def test_every_form_of_the_prompts_is_tested():
+    cases = [(f16, seqs, NH, NKV) for f16, seqs, NH, NKV in gpu.prompt_forms()]
+    cases += [(f16, s, NH, NKV) for f16 in (False, True) for s in gpu.SEQS.values() for NH, NKV in gpu.HEADS]
+    seen = set()
+    for f16, seqs, NH, NKV in cases:
+        n, m = sum(n for n, _ in seqs), sum(max(0, n + p) for n, p in seqs)
+        seen.add((f16, prompt_form(f16, max(n, 1), m, len(seqs), NH, NKV)[0], min(len(seqs), 64) // 32))
+    for f16, form in ((False, 0), (False, 1), (True, 0), (True, 1), (True, 2)):
+        assert {k for g, f, k in seen if (g, f) == (f16, form)} >= {0, 2}, (f16, form, seen)
+
+
 def kv4_form(S, NH, NKV, T):
     fn = g2hip._lib.g2i_kv4_form
     fn.argtypes = [C.c_int] * 4 + [C.POINTER(C.c_int)] * 4

@@ -108,14 +108,35 @@ def test_prompt(g2, name, f16):
         Prompts(SEQS[name], NH, NKV, f16).check(g2)
 
 
-@pytest.mark.parametrize("f16", [False, True])
-def test_prompt_many_rows(g2, f16):
-    """The other side of the choice of form: many long rows and heads."""
+def prompt_forms():
+    """(f16, sequences, NH, NKV): every form for many rows, with starts that a wave holds and with more of them."""
     r = rng(11)
-    seqs = [(int(n), 0) for n in r.integers(100, 400, 24)]
-    Prompts(seqs, 8, 8, f16).check(g2)
-    Prompts([(n, 5 * i) for i, (n, _) in enumerate(seqs)], 10, 2, f16, gap=3).check(g2)
-    Prompts([(2100, 0), (1, 0), (77, 900)], 12, 4, f16).check(g2)
+
+    def some(n, lo, hi, past=0):
+        return [(int(k), past) for k in r.integers(lo, hi, n)]
+
+    few, more = some(24, 150, 350), some(70, 60, 120)
+    return [(False, few, 12, 12), (False, more, 12, 6), (False, [(400, 0), (1, 7), (3000, 5)], 20, 4), (False, [(2100, 0)], 32, 32),
+            (True, few, 8, 8), (True, more, 10, 2), (True, [(n, 5 * i) for i, (n, _) in enumerate(few)], 25, 25), (True, more, 20, 20),
+            (True, [(2100, 0)], 20, 5), (True, [(2100, 0), (1, 0), (77, 900)], 12, 4), (True, some(80, 60, 90, -3), 25, 25), (True, [(1600, 0)], 12, 12)]
+
+
+@pytest.mark.parametrize("case", range(len(prompt_forms())))
+def test_prompt_many_rows(g2, case):
+    f16, seqs, NH, NKV = prompt_forms()[case]
+    Prompts(seqs, NH, NKV, f16, gap=case % 4).check(g2)
+
+
+@pytest.mark.parametrize("case", range(len(prompt_forms())))
+def test_prompt_many_rows_not_finite(g2, case):
+    """Values that are not finite count for the rows that see them, and for no others, in the forms for many rows."""
+    f16, seqs, NH, NKV = prompt_forms()[case]
+    p = Prompts(seqs, NH, NKV, f16, seed=1)
+    r = rng(case)
+    for bad in (np.inf, np.nan, -np.inf):
+        for j in r.integers(0, p.keys, 3):
+            p.v[j, r.integers(0, NKV * H)] = bad
+    p.check(g2)
 
 
 @pytest.mark.parametrize("f16", [False, True])
