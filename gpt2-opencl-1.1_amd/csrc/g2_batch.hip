@@ -197,38 +197,51 @@ template <typename T> __device__ __forceinline__ unsigned prompt_value_at(int u,
 {
     return ((unsigned)(16 * u + 4 * g) * (unsigned)stride + 2u * (unsigned)pair) * (unsigned)sizeof(T);
 }
-/* (fp16 values stay the pairs that they are in memory) */
+/* They stay the pairs that they are in memory. */
 template <typename T> struct prompt_pairs;
-template <> struct prompt_pairs<float> { float x[2][8]; };
+template <> struct prompt_pairs<float> { unsigned x[16]; };
 template <> struct prompt_pairs<_Float16> { unsigned x[8]; };
-__device__ __forceinline__ void prompt_load_v(prompt_pairs<float> &v, __amdgpu_buffer_rsrc_t rows, unsigned at, long stride, int)
+/* Eight loads of two elements each from a buffer: the first at byte `at`, the others
+ * step0 bytes on from one to the next and step1 more from the fourth to the fifth
+ * (the same in every lane). */
+__device__ __forceinline__ void prompt_load8(unsigned (&x)[16], __amdgpu_buffer_rsrc_t rows, unsigned at, unsigned step0, unsigned step1, int)
 {
     typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
     asm volatile("" : "+v"(at));
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rows, (int)(at + (unsigned)(8 * (e / 4) + e % 4) * (unsigned)stride * 4u), 0, 0));
-        v.x[0][e] = __uint_as_float(w[0]);
-        v.x[1][e] = __uint_as_float(w[1]);
+        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rows, (int)(at + (unsigned)e * step0 + (unsigned)(e / 4) * step1), 0, 0));
+        x[2 * e] = w[0];
+        x[2 * e + 1] = w[1];
     }
 }
-/* (`even` where pairs are at multiples of four bytes, which a load of both asks for) */
-__device__ __forceinline__ void prompt_load_v(prompt_pairs<_Float16> &v, __amdgpu_buffer_rsrc_t rows, unsigned at, long stride, int even)
+/* (`even` where pairs of fp16 are at multiples of four bytes, which a load of both asks for) */
+__device__ __forceinline__ void prompt_load8(unsigned (&x)[8], __amdgpu_buffer_rsrc_t rows, unsigned at, unsigned step0, unsigned step1, int even)
 {
     asm volatile("" : "+v"(at));
     if (even)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            v.x[e] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(rows, (int)(at + (unsigned)(8 * (e / 4) + e % 4) * (unsigned)stride * 2u), 0, 0);
+        for (int e = 0; e < 8; ++e) x[e] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(rows, (int)(at + (unsigned)e * step0 + (unsigned)(e / 4) * step1), 0, 0);
     else
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int p = (int)(at + (unsigned)(8 * (e / 4) + e % 4) * (unsigned)stride * 2u);
-            v.x[e] = (unsigned)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rows, p, 0, 0) | (unsigned)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rows, p + 2, 0, 0) << 16;
+            const int p = (int)(at + (unsigned)e * step0 + (unsigned)(e / 4) * step1);
+            x[e] = (unsigned)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rows, p, 0, 0) | (unsigned)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rows, p + 2, 0, 0) << 16;
         }
 }
+template <typename T> __device__ __forceinline__ void prompt_load_v(prompt_pairs<T> &v, __amdgpu_buffer_rsrc_t rows, unsigned at, long stride, int even)
+{
+    const unsigned sb = (unsigned)stride * (unsigned)sizeof(T);
+    prompt_load8(v.x, rows, at, sb, 4 * sb, even);
+}
 /* The operand of dim t of the pairs. */
-__device__ __forceinline__ void prompt_pack(const prompt_pairs<float> &v, int t, prompt_op<float> &o) { parts3(v.x[t], o.p); }
+__device__ __forceinline__ void prompt_pack(const prompt_pairs<float> &v, int t, prompt_op<float> &o)
+{
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(v.x[2 * e + t]);
+    parts3(x, o.p);
+}
 __device__ __forceinline__ void prompt_pack(const prompt_pairs<_Float16> &v, int t, prompt_op<_Float16> &o)
 {
     u32x4 w;
@@ -237,8 +250,26 @@ __device__ __forceinline__ void prompt_pack(const prompt_pairs<_Float16> &v, int
     o.p = __builtin_bit_cast(f16x8, w);
 }
 
+/* The operand of the first or second eight dims of a key. */
+__device__ __forceinline__ void prompt_key(const prompt_pairs<float> &k, int h, prompt_op<float> &o)
+{
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(k.x[8 * h + e]);
+    parts3(x, o.p);
+}
+__device__ __forceinline__ void prompt_key(const prompt_pairs<_Float16> &k, int h, prompt_op<_Float16> &o)
+{
+    const u32x4 w = { k.x[4 * h], k.x[4 * h + 1], k.x[4 * h + 2], k.x[4 * h + 3] };
+    o.p = __builtin_bit_cast(f16x8, w);
+}
+
 /* Scores in units of log 2; not 0, which would make NaN of the masked ones. */
-__device__ __forceinline__ float prompt_unit(float scale) { return fmaxf(fabsf(scale) * 1.44269504f, 0x1p-126f); }
+__device__ __forceinline__ float prompt_unit(float scale)
+{
+    const float c = fmaxf(fabsf(scale) * 1.44269504f, 0x1p-126f);
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(c)));
+}
 /* The weight of a state of maximum m beside one of maximum top (an empty one's is -infinity). */
 __device__ __forceinline__ float prompt_factor(float m, float top, float c) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * c); }
 
@@ -246,8 +277,8 @@ __device__ __forceinline__ float prompt_factor(float m, float top, float c) { re
  * state, where its output goes. */
 template <typename T> struct prompt_query {
     g2b_row keys;
-    int row, head, k0, k1; /* k0 .. k1 - 1: what the wave's queries see together */
-    bool sees;
+    int row, head; /* (row -1: none) */
+    int k0, k1;    /* k0 .. k1 - 1: what the wave's queries see together */
     prompt_op<T> q[4];
     f32x16 o[2];
     float m, l, base; /* base: added to a score in units of log 2, this time */
@@ -269,9 +300,9 @@ __device__ __forceinline__ void prompt_start(prompt_query<T> &y, const g2_attn_p
         const int i = in ? s : 0;
         y.keys = g2b_row_keys(y.row, in, a.q_start[i], a.q_start[i + 1], a.k_start[i], a.k_start[i + 1], a.q_rows, a.k_rows);
     }
-    y.sees = y.keys.there && y.keys.end > y.keys.lo;
-    y.k0 = __builtin_amdgcn_readfirstlane(lanes_min_int(y.sees ? y.keys.lo : INT_MAX));
-    y.k1 = __builtin_amdgcn_readfirstlane(-lanes_min_int(y.sees ? -y.keys.end : INT_MAX));
+    const bool sees = y.keys.end > y.keys.lo; /* (a row that is none of a sequence's has no keys) */
+    y.k0 = __builtin_amdgcn_readfirstlane(lanes_min_int(sees ? y.keys.lo : INT_MAX));
+    y.k1 = __builtin_amdgcn_readfirstlane(-lanes_min_int(sees ? -y.keys.end : INT_MAX));
     const T *qp = (const T *)a.q + (size_t)min(y.row, a.q_rows - 1) * a.q_stride + y.head * G2B_DH + 8 * g;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
@@ -282,6 +313,7 @@ __device__ __forceinline__ void prompt_start(prompt_query<T> &y, const g2_attn_p
             for (int e = 0; e < 8; ++e) x[e] = -x[e]; /* (the unit is positive: prompt_unit) */
         prompt_pack(x, y.q[s]);
     }
+    if (!y.keys.there) y.row = -1;
     /* (loaded now: a wait for them inside the loop would wait for the keys, too) */
     if constexpr (sizeof(T) == 2)
 #pragma unroll
@@ -366,8 +398,8 @@ __device__ __forceinline__ bool prompt_look(const prompt_pairs<float> &v)
     float z[2] = {};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        z[0] = fmaf(v.x[0][e], 0.f, z[0]);
-        z[1] = fmaf(v.x[1][e], 0.f, z[1]);
+        z[0] = fmaf(__uint_as_float(v.x[2 * e]), 0.f, z[0]);
+        z[1] = fmaf(__uint_as_float(v.x[2 * e + 1]), 0.f, z[1]);
     }
     return wave_any(z[0] + z[1] != 0.f);
 }
@@ -383,9 +415,7 @@ __device__ __forceinline__ bool prompt_look(const prompt_pairs<_Float16> &v)
 __device__ __forceinline__ void prompt_clean(prompt_pairs<float> &v)
 {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v.x[t][e] = __builtin_isfinite(v.x[t][e]) ? v.x[t][e] : 0.f;
+    for (int e = 0; e < 16; ++e) v.x[e] = __builtin_isfinite(__uint_as_float(v.x[e])) ? v.x[e] : 0u;
 }
 __device__ __forceinline__ void prompt_clean(prompt_pairs<_Float16> &v)
 {
@@ -433,7 +463,7 @@ template <typename T> __device__ __forceinline__ void prompt_out(const prompt_qu
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[t][e] = y.sees ? y.o[t][4 * q + e] * one : 0.f;
+            for (int e = 0; e < 4; ++e) v[t][e] = y.keys.end > y.keys.lo ? y.o[t][4 * q + e] * one : 0.f;
         prompt_store(out + 16 * q, v[0], v[1]);
     }
 }
@@ -511,7 +541,7 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
 #pragma unroll
         for (int r = 0; r < 16; ++r) red[w][2 + 16 * t + r][lane] = y.o[t][r];
     __syncthreads();
-    if (!y.keys.there || w >= 4) return;
+    if (y.row < 0 || w >= 4) return;
     float top = -INFINITY, part[KW], l = 0.f;
 #pragma unroll
     for (int i = 0; i < KW; ++i) top = fmaxf(top, red[i][0][lane]);
@@ -529,7 +559,7 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
         for (int e = 0; e < 4; ++e) {
 #pragma unroll
             for (int j = 0; j < KW; ++j) x[t][e] = fmaf(red[j][2 + 16 * t + 4 * w + e][lane], part[j], x[t][e]);
-            x[t][e] = y.sees ? x[t][e] * one : 0.f;
+            x[t][e] = y.keys.end > y.keys.lo ? x[t][e] * one : 0.f;
         }
     prompt_store(out + 16 * w, x[0], x[1]);
 }
@@ -569,22 +599,31 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
     const float c = prompt_unit(a.scale);
     const long stride = a.kv_stride;
     const T *kp = (const T *)a.k + hk * G2B_DH, *vp = (const T *)a.v + hk * G2B_DH;
-    union share { /* this lane's: two chunks of a key's dims, or two dims of eight keys */
-        T k[2][8];
-        prompt_pairs<T> v;
-    } x[KT];
-    const unsigned at = prompt_value_at<T>(w & 1, g, m, stride);
+    /* This lane's share of 32 keys: 16 dims of a key, or two dims of eight keys. */
+    prompt_pairs<T> x[KT];
     auto brings_keys = [&](int i) { return ((w >> 1) ^ i) & 1; };
     const int chunk = 4 * (w & 1) + 2 * g;
+    const unsigned sb = (unsigned)stride * (unsigned)sizeof(T);
+    const unsigned at_key = (unsigned)m * sb + 8 * (unsigned)chunk * (unsigned)sizeof(T), at_value = prompt_value_at<T>(w & 1, g, m, stride);
     auto load = [&](int j0) {
 #pragma unroll
         for (int i = 0; i < KT; ++i) {
             const int j = min(j0 + 32 * i, k1 - 1); /* (keys behind the last are masked) */
-            if (brings_keys(i)) {
+            const bool keys = brings_keys(i);
+            /* fp32: either way eight loads of a pair into the same registers.  Where a
+             * wave's keys were four wide loads and its values eight others, both
+             * meeting in them, 16 texts of 100 to 1023 rows took 163 us, now 153;
+             * fp16 keys in pairs take 274 us instead of 200 for 8001 rows. */
+            if constexpr (P == 3) prompt_load8(x[i].x, prompt_rows(keys ? kp : vp, j, k1, stride), keys ? at_key : at_value, keys ? 8u : sb, keys ? 0u : 4 * sb, 0);
+            else if (keys) {
                 const T *p = kp + (size_t)j * stride + (size_t)min(m, k1 - j - 1) * stride + 8 * chunk;
-                prompt_load_k(x[i].k[0], p);
-                prompt_load_k(x[i].k[1], p + 8);
-            } else prompt_load_v(x[i].v, prompt_rows(vp, j, k1, stride), at, stride, a.even);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const u32x4 z = __builtin_bit_cast(u32x4, *(const f16x8u *)(p + 8 * h));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[i].x[4 * h + e] = z[e];
+                }
+            } else prompt_load_v(x[i], prompt_rows(vp, j, k1, stride), at_value, stride, a.even);
         }
     };
     auto put = [&](u32x4 *p, const prompt_op<T> &z) {
@@ -598,17 +637,17 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
         for (int i = 0; i < KT; ++i) {
             prompt_op<T> z;
             if (brings_keys(i)) {
-                prompt_pack(x[i].k[0], z);
+                prompt_key(x[i], 0, z);
                 put(lds[b][i] + chunk * 32 + m, z);
-                prompt_pack(x[i].k[1], z);
+                prompt_key(x[i], 1, z);
                 put(lds[b][i] + chunk * 32 + 32 + m, z);
             } else {
-                const bool any = prompt_look(x[i].v);
-                if (any) prompt_clean(x[i].v);
+                const bool any = prompt_look(x[i]);
+                if (any) prompt_clean(x[i]);
                 if (lane == 0) odd[b][i][w & 1] = any;
-                prompt_pack(x[i].v, 0, z);
+                prompt_pack(x[i], 0, z);
                 put(lds[b][i] + UNITS + (w & 1) * 64 + lane, z);
-                prompt_pack(x[i].v, 1, z);
+                prompt_pack(x[i], 1, z);
                 put(lds[b][i] + UNITS + 128 + (w & 1) * 64 + lane, z);
             }
         }
@@ -636,12 +675,11 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
             if (j >= y.k1 || j + 32 <= y.k0) continue; /* (none of the wave's queries sees any of them) */
             const u32x4 *kd = lds[b][i] + lane, *vd = kd + UNITS;
             f32x16 s = {};
-            {
-                prompt_op<T> z[4];
 #pragma unroll
-                for (int t = 0; t < 4; ++t) fetch(kd + 64 * t, z[t]);
-#pragma unroll
-                for (int t = 0; t < 4; ++t) s = prompt_mma(z[t], y.q[t], s);
+            for (int t = 0; t < 4; ++t) {
+                prompt_op<T> z;
+                fetch(kd + 64 * t, z);
+                s = prompt_mma(z, y.q[t], s);
             }
             prompt_follow(y, s, j, c, g);
             prompt_weights(y, s, c);
@@ -681,7 +719,7 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
 #pragma unroll
             for (int r = 0; r < 16; ++r) y.o[t][r] = y.o[t][r] * mine + red[256 * (2 + 16 * t + r)] * other;
     }
-    if (y.keys.there) prompt_out(y, a, y.l, g);
+    if (y.row >= 0) prompt_out(y, a, y.l, g);
 }
 #define PROMPT_TILE(NAME, T, KT, KW, WAVES)                                                                            \
     extern "C" __global__ __launch_bounds__(256 * KW) __attribute__((amdgpu_waves_per_eu(WAVES)))                      \
