@@ -152,7 +152,13 @@ __device__ __forceinline__ prompt_place prompt_find(const g2_attn_prompt_args &a
  * keys in the same order, 16 u + 8 (e / 4) + 4 (l / 32) + e % 4.
  *
  * Queries are the rows' heads that share a key head, row by row: 32
- * of them are fewer rows where heads are grouped, so less is masked. */
+ * of them are fewer rows where heads are grouped, so less is masked.
+ *
+ * What bounds it: instructions, not memory.  A matrix instruction of 32 x 32 x 16
+ * keeps the SIMD from its vector instructions for about 25 of its 37 cycles, so
+ * that their times nearly add, and 32 x 32 scores are 8 matrix instructions in
+ * fp16, 48 in fp32 (six products of parts), beside some 100 and 350 others for
+ * exponentials, sums, maxima and parts.  Timed at the forms below. */
 template <typename T> struct prompt_op; /* an operand of one instruction, 8 values a lane */
 template <> struct prompt_op<float> { u32x4 p[3]; };
 template <> struct prompt_op<_Float16> { f16x8 p; };
@@ -471,7 +477,13 @@ template <typename T> __device__ __forceinline__ void prompt_out(const prompt_qu
 /* ---- few queries: a work-group takes 32 of them, its four waves every fourth 32
  * keys each, whose rows they read as the operands that they are (a key's dims
  * 16 bytes at a time, a value's dims side by side, so that eight loads are
- * eight keys of a dim); the waves' states meet at the end. */
+ * eight keys of a dim); the waves' states meet at the end.  Each wave converts its
+ * own keys, for 32 queries only: the price of having four times the waves.
+ * 1001 rows of 12 heads 24 us in fp32 (64 TFLOP/s of useful products; a tile of
+ * 128 queries: 75) and 12 in fp16; 40 turns of 20 to 60 rows behind 700 keys, 16
+ * heads on 4, fp16: 22.6 us; one text of 17 rows 5.5, a launch's own time.
+ * Eight waves to a work-group instead of four: 50 us where this takes 40 (1001
+ * rows, 25 heads). */
 template <typename T, int KW>
 __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
 {
@@ -574,7 +586,18 @@ PROMPT_SPLIT(g2k_prompt_split_f16, _Float16, 4)
  * (part, step, lane) of 16 bytes is what the lane reads of it, so that reads and
  * writes are both rows of units.  Two stages: the next keys are on their way from
  * memory while the products of these run, and one barrier stands between.  Of 32
- * keys two waves bring the keys, two the values (a step each), in turns. */
+ * keys two waves bring the keys, two the values (a step each), in turns.
+ * With KW = 2 two such groups take every other piece of the same queries' keys,
+ * and their states meet at the end.
+ * fp32, 16 texts of 100 to 1023 rows, 25 heads: 153 us, 132 TFLOP/s of useful
+ * products (790 of bf16 ones; a large library product reaches 1223), three
+ * work-groups to a CU by registers and LDS; four waves a group, one piece.
+ * fp16, one text of 8001 rows, 16 heads on 4: 193 us, 680 TFLOP/s, with vector
+ * instructions on 68 % and matrix instructions on 28 % of the cycles; one group of
+ * waves takes 235.  Two groups of fp32 waves: 212 us for 153.
+ * Tried beside it: the next keys' scores among this piece's exponentials (fp32 171,
+ * fp16 up to 1.5 times as long: registers), no LDS, each wave by itself (187),
+ * two waves a SIMD with all operands in registers (175). */
 template <typename T, int KT, int KW>
 __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
 {
@@ -734,7 +757,9 @@ PROMPT_TILE(g2k_prompt_duo_f16, _Float16, 2, 2, 4)
  * ==================================================================== */
 
 /* A wave takes 8 rows of keys or values of a head, eight lanes of 8 dims to a
- * row, neighbouring waves neighbouring heads. */
+ * row, neighbouring waves neighbouring heads.  Bound by memory: 7 bytes read for
+ * one written; 16 texts of 100 to 1023 rows, 25 heads, in 30 us, 4.3 TB/s (a large
+ * copy: 4.8), one token of 8 texts in 3.6. */
 template <typename T>
 __device__ void kv4_append_impl(const g2_kv4_append_args &a)
 {
@@ -780,7 +805,7 @@ G2K void g2k_kv4_append_f32(const g2_kv4_append_args a) { kv4_append_impl<float>
 G2K void g2k_kv4_append_f16(const g2_kv4_append_args a) { kv4_append_impl<_Float16>(a); }
 
 /* One thread per four dims of a position, keys and values, in the order of the
- * output, which does not stay in the L2. */
+ * output, which does not stay in the L2.  30 us for what the above puts down. */
 G2K void g2k_kv4_read(const g2_kv4_read_args a)
 {
     const unsigned quads = (unsigned)a.NKV * (G2B_DH / 4);
@@ -814,7 +839,13 @@ G2K void g2k_kv4_read(const g2_kv4_read_args a)
  * follows the maximum only where it grew by more than 2^8.  The slots meet once,
  * at the end: over the lanes, over the waves in LDS, and over the parts of a long
  * sequence in a second launch.  The next positions' loads go out before the last
- * ones' sums. */
+ * ones' sums.
+ * 72 bytes a position and head hold 128 numbers: reading them at the speed of
+ * memory leaves few instructions for each, so codes become values by one conversion
+ * a pair, scales enter once a position, and the work is spread for its latency
+ * where it is small.  48 texts of 256 to 1024 positions, 25 heads: 15.2 us, 3.7 TB/s;
+ * 8 beams of 901 through their table 6.3; 50001 positions of 4 heads, 16 queries:
+ * 13.4 with the second launch, which is 3.9 of it. */
 template <int W, int U> struct kv4_in {
     unsigned k[U][W], v[U][W];
     unsigned ks[U], vs[U]; /* bf16 */
@@ -1081,7 +1112,11 @@ G2K void g2k_kv4_join(const g2_kv4_attn_args a)
 /* Candidates are few once a bound is known that n of them reach.  One is the
  * least of the greatest of G >= n groups: of values that are spread over the
  * groups, about G (1 + 1/2 + ... + 1/G) reach it (54 for 16).  What reaches it is
- * put down in LDS, in any order, and each candidate counts those above it. */
+ * put down in LDS, in any order, and each candidate counts those above it.
+ * A row is read once, its ids in registers meanwhile.  128 rows of 50257 ids: 13.8 us
+ * (25.7 MB, 1.9 TB/s); 4 rows 9.2, of which the last work-group's pick, one
+ * wait for memory behind another, is about half.  One launch instead of two: the
+ * last of a group's work-groups, by a count that it leaves at 0, picks. */
 
 #define BEAM_THREADS 1024
 #define BEAM_WAVES (BEAM_THREADS / 64)
@@ -1445,7 +1480,8 @@ BEAM_SELECT(g2k_beam_select1, 1)
 BEAM_SELECT(g2k_beam_select4, 4)
 BEAM_SELECT(g2k_beam_select7, 7)
 
-/* Rows of the tables in their parents' order, 256 ints of a row to a work-group. */
+/* Rows of the tables in their parents' order, 256 ints of a row to a work-group.
+ * Beams move by their tables alone (8 bytes a position): 128 rows of 1001 in 4 us. */
 G2K void g2k_beam_copy(const g2_beam_move_args a)
 {
     const int chunks = (a.T + 1 + 255) / 256;

@@ -306,7 +306,8 @@ int g2_apply_logit_rules(const float *logits, float *out, int *pick, int rows,
  * fp32 rows enter whole (products of magnitudes below 2^-102 may lose their
  * last bits), sums are fp32; of fp16 rows the softmax's weights are rounded to
  * fp16 for the second product.  A key with an infinity or NaN makes the rows
- * that see it NaN, a value with one counts where it is seen. */
+ * that see it NaN (an fp16 score of -infinity alone is a weight of 0), a value
+ * with one counts where it is seen. */
 int g2_attn_prompt(const void *q, int q_stride, const void *k, const void *v, int kv_stride,
                    void *out, int out_stride, int dtype, const int *q_start, const int *k_start,
                    int n_seq, int q_rows, int k_rows, int n_head, int n_kv, float scale);
