@@ -187,12 +187,12 @@ template <typename T> __device__ __forceinline__ void prompt_load_k(T (&x)[8], c
 }
 
 /* The rows of keys or values from j0 on, up to 32 and below k1, as a buffer:
- * what is read behind the last of them is 0. */
+ * what is read behind the last of them is 0 (everything, unless any). */
 template <typename T>
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t prompt_rows(const T *p, int j0, int k1, long stride)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t prompt_rows(const T *p, int j0, int k1, long stride, bool any = true)
 {
     const int n = min(32, k1 - j0);
-    const unsigned bytes = ((unsigned)(n - 1) * (unsigned)stride + G2B_DH) * (unsigned)sizeof(T);
+    const unsigned bytes = any ? ((unsigned)(n - 1) * (unsigned)stride + G2B_DH) * (unsigned)sizeof(T) : 0;
     return __builtin_amdgcn_make_buffer_rsrc((void *)(p + (size_t)j0 * stride), (short)0, bytes, 0x00020000);
 }
 /* Two dims' values of the eight keys that a lane of half g takes in step u (in the
@@ -209,16 +209,23 @@ template <> struct prompt_pairs<float> { unsigned x[16]; };
 template <> struct prompt_pairs<_Float16> { unsigned x[8]; };
 /* Eight loads of two elements each from a buffer: the first at byte `at`, the others
  * step0 bytes on from one to the next and step1 more from the fourth to the fifth
- * (the same in every lane). */
+ * (the same in every lane).  Each address comes from the one before: the multiples of
+ * step0 would be held in more scalar registers than there are. */
+__device__ __forceinline__ void prompt_next(unsigned &at, int e, unsigned step0, unsigned step1)
+{
+    at += e == 3 ? step0 + step1 : step0;
+    asm volatile("" : "+v"(at));
+}
 __device__ __forceinline__ void prompt_load8(unsigned (&x)[16], __amdgpu_buffer_rsrc_t rows, unsigned at, unsigned step0, unsigned step1, int)
 {
     typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
     asm volatile("" : "+v"(at));
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rows, (int)(at + (unsigned)e * step0 + (unsigned)(e / 4) * step1), 0, 0));
+        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rows, (int)at, 0, 0));
         x[2 * e] = w[0];
         x[2 * e + 1] = w[1];
+        prompt_next(at, e, step0, step1);
     }
 }
 /* (`even` where pairs of fp16 are at multiples of four bytes, which a load of both asks for) */
@@ -227,12 +234,15 @@ __device__ __forceinline__ void prompt_load8(unsigned (&x)[8], __amdgpu_buffer_r
     asm volatile("" : "+v"(at));
     if (even)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(rows, (int)(at + (unsigned)e * step0 + (unsigned)(e / 4) * step1), 0, 0);
+        for (int e = 0; e < 8; ++e) {
+            x[e] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(rows, (int)at, 0, 0);
+            prompt_next(at, e, step0, step1);
+        }
     else
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int p = (int)(at + (unsigned)e * step0 + (unsigned)(e / 4) * step1);
-            x[e] = (unsigned)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rows, p, 0, 0) | (unsigned)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rows, p + 2, 0, 0) << 16;
+            x[e] = (unsigned)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rows, (int)at, 0, 0) | (unsigned)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rows, (int)at + 2, 0, 0) << 16;
+            prompt_next(at, e, step0, step1);
         }
 }
 template <typename T> __device__ __forceinline__ void prompt_load_v(prompt_pairs<T> &v, __amdgpu_buffer_rsrc_t rows, unsigned at, long stride, int even)
@@ -484,7 +494,7 @@ template <typename T> __device__ __forceinline__ void prompt_out(const prompt_qu
  * heads on 4, fp16: 22.6 us; one text of 17 rows 5.5, a launch's own time.
  * Eight waves to a work-group instead of four: 50 us where this takes 40 (1001
  * rows, 25 heads). */
-template <typename T, int KW>
+template <typename T, int KW, int EVEN>
 __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
 {
     __shared__ float red[KW][34][64];
@@ -508,9 +518,9 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
         for (int s = 0; s < 4; ++s) prompt_load_k(k[s], p + 16 * s);
     };
     auto load_v = [&](int j0) {
-        const __amdgpu_buffer_rsrc_t rows = prompt_rows(vp, j0, y.k1, stride);
+        const __amdgpu_buffer_rsrc_t rows = prompt_rows(vp, min(j0, y.k1 - 1), y.k1, stride, j0 < y.k1);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) prompt_load_v(v[u], rows, at[u], stride, a.even);
+        for (int u = 0; u < 2; ++u) prompt_load_v(v[u], rows, at[u], stride, EVEN);
     };
     int j0 = y.k0 < y.k1 ? y.k0 + 32 * w : y.k1;
     if (j0 < y.k1) { load_k(j0); load_v(j0); }
@@ -523,7 +533,9 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
             prompt_pack(k[i], x);
             s = prompt_mma(x, y.q[i], s);
         }
-        if (j1 < y.k1) load_k(j1);
+        /* (always, behind the last ones a row of them and none of the values: with a branch
+         * around either what waits for the keys waits for the values, too) */
+        load_k(min(j1, y.k1 - 1));
         prompt_follow(y, s, j0, c, g);
         prompt_weights(y, s, c);
         const bool odd0 = prompt_look(v[0]), odd1 = prompt_look(v[1]);
@@ -542,7 +554,7 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
                 y.o[t] = prompt_mma(x, p, y.o[t]);
             }
         }
-        if (j1 < y.k1) load_v(j1);
+        load_v(j1);
     }
     y.l = swap_sum(y.l);
     /* the waves' parts meet; the first four waves write a quarter of the dims each */
@@ -575,11 +587,15 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
         }
     prompt_store(out + 16 * w, x[0], x[1]);
 }
-#define PROMPT_SPLIT(NAME, T, KW)                                                                                      \
+/* (f16_odd: pairs of values at odd multiples of two bytes.  A kernel of its own: beside
+ * a branch between the two kinds of loads the wait for the keys was one for the values,
+ * too.) */
+#define PROMPT_SPLIT(NAME, T, KW, EVEN)                                                                                \
     extern "C" __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(2)))                           \
-    void NAME(const g2_attn_prompt_args a) { prompt_split_impl<T, KW>(a); }
-PROMPT_SPLIT(g2k_prompt_split_f32, float, 4)
-PROMPT_SPLIT(g2k_prompt_split_f16, _Float16, 4)
+    void NAME(const g2_attn_prompt_args a) { prompt_split_impl<T, KW, EVEN>(a); }
+PROMPT_SPLIT(g2k_prompt_split_f32, float, 4, 1)
+PROMPT_SPLIT(g2k_prompt_split_f16, _Float16, 4, 1)
+PROMPT_SPLIT(g2k_prompt_split_f16_odd, _Float16, 4, 0)
 
 /* ---- many queries: a work-group takes 128 of them, 32 a wave, and its waves
  * read KT times 32 keys and values together, once, as operands in LDS: unit

@@ -129,6 +129,7 @@ extern "C" {
     X(LOGITS, "g2k_logits") X(LOGITS_WIDE, "g2k_logits_wide")                 \
     X(PROMPT_SPLIT_F32, "g2k_prompt_split_f32")                               \
     X(PROMPT_SPLIT_F16, "g2k_prompt_split_f16")                               \
+    X(PROMPT_SPLIT_F16_ODD, "g2k_prompt_split_f16_odd")                       \
     X(PROMPT_TILE_F32, "g2k_prompt_tile_f32")                                 \
     X(PROMPT_TILE_F16, "g2k_prompt_tile_f16")                                 \
     X(PROMPT_DUO_F16, "g2k_prompt_duo_f16")                                   \
