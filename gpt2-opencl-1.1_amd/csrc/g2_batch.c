@@ -42,15 +42,15 @@ static int heads_check(const char *fn, int n_head, int n_kv)
 /* Work-groups of 128 queries convert each key once for four times as many of them,
  * those of 32 are four times as many.  Measured, in us (tiles, parts):
  *                                 groups of 128    128     32    two groups of waves
- *   fp32  1001 rows,   12 heads              96     75     24
+ *   fp32  1001 rows,   12 heads              96     75     23
  *         2 x 1000,    16                   256     77     48
  *         4001,        12                   384    300    179
- *         8 x 500,     20                   640     57     71
+ *         8 x 500,     20                   640     49     71
  *         4 x 1000,    25                   800    105    131
  *         16 x 100 to 1023, 25             1700    153    224
  *   fp16  1001,        12                    96     30     12      22
  *         1000,        25                   200     31     16      23
- *         40 x 20 to 60 behind 700, 16/4    200     28     23      26
+ *         40 x 20 to 60 behind 700, 16/4    200     28     22      26
  *         16 x 200,    12                   300     12     15      12
  *         2 x 1000,    25                   400     34     32      27
  *         8001,        16/4                1000    235    287     193

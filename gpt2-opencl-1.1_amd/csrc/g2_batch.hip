@@ -489,9 +489,9 @@ template <typename T> __device__ __forceinline__ void prompt_out(const prompt_qu
  * 16 bytes at a time, a value's dims side by side, so that eight loads are
  * eight keys of a dim); the waves' states meet at the end.  Each wave converts its
  * own keys, for 32 queries only: the price of having four times the waves.
- * 1001 rows of 12 heads 24 us in fp32 (64 TFLOP/s of useful products; a tile of
+ * 1001 rows of 12 heads 23 us in fp32 (68 TFLOP/s of useful products; a tile of
  * 128 queries: 75) and 12 in fp16; 40 turns of 20 to 60 rows behind 700 keys, 16
- * heads on 4, fp16: 22.6 us; one text of 17 rows 5.5, a launch's own time.
+ * heads on 4, fp16: 22.2 us; one text of 17 rows 5.5, a launch's own time.
  * Eight waves to a work-group instead of four: 50 us where this takes 40 (1001
  * rows, 25 heads). */
 template <typename T, int KW, int EVEN>
