@@ -168,6 +168,7 @@ int g2_kv4_read(const void *cache, float *k, float *v, const int *origin, const 
     if (!k || !v) return g2i_err(G2_E_ARG, "%s: NULL buffer", fn);
     if (T_kv < 0 || T_kv > max_seq || start < 0 || T < 1 || start > max_seq - T)
         return g2i_err(G2_E_ARG, "%s: positions %d..%ld, length %d, cache of %d", fn, start, (long)start + T - 1, T_kv, max_seq);
+    if (!aligned(k, 4) || !aligned(v, 4)) return g2i_err(G2_E_ARG, "%s: a buffer is not at an element's address", fn);
     const size_t n = (size_t)n_seq * T * n_kv * 256, nc = g2_kv4_bytes(n_seq, n_kv, max_seq), nl = (size_t)n_seq * 4;
     const size_t nt = (size_t)n_seq * max_seq * 4;
     if (g2i_overlap(k, n, v, n) || g2i_overlap(k, n, cache, nc) || g2i_overlap(v, n, cache, nc) ||
@@ -293,6 +294,7 @@ int g2_beam_select(const float *logits, const float *score, const int *done, int
                        fn, groups, beams, V, n_out, G2B_MAX_BEAMS, 1 << 16, MAX_VOCAB, G2B_MAX_OUT);
     if (eos < -1 || eos >= V || (done && eos < 0)) return g2i_err(G2_E_ARG, "%s: end id %d of %d", fn, eos, V);
     if (!aligned(work, 8)) return g2i_err(G2_E_ARG, "%s: the workspace must be 8-byte aligned", fn);
+    if (!aligned(logits, 4) || !aligned(score, 4) || !aligned(out_score, 4)) return g2i_err(G2_E_ARG, "%s: a buffer is not at an element's address", fn);
     const long rows = (long)groups * beams;
     const size_t n = (size_t)groups * n_out * 4, nr = (size_t)rows * 4, nw = g2_beam_work_bytes(groups, beams, V, n_out);
     const struct { const void *p; size_t n; } in[] = { { logits, nr * V }, { score, nr }, { done, done ? nr : 0 } };

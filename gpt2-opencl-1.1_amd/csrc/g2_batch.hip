@@ -280,10 +280,11 @@ __device__ __forceinline__ void prompt_key(const prompt_pairs<_Float16> &k, int 
     o.p = __builtin_bit_cast(f16x8, w);
 }
 
-/* Scores in units of log 2; not 0, which would make NaN of the masked ones. */
+/* Scores in units of log 2; not 0, which would make NaN of the masked ones, but so small
+ * that no score makes a difference (those below 2^128 then are below 2^-21). */
 __device__ __forceinline__ float prompt_unit(float scale)
 {
-    const float c = fmaxf(fabsf(scale) * 1.44269504f, 0x1p-126f);
+    const float c = fmaxf(fabsf(scale) * 1.44269504f, 0x1p-149f);
     return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(c)));
 }
 /* The weight of a state of maximum m beside one of maximum top (an empty one's is -infinity). */

@@ -304,7 +304,8 @@ int g2_apply_logit_rules(const float *logits, float *out, int *pick, int rows,
  * / n_kv)).  Rows begin strides apart, in elements of dtype (G2_F32 or G2_F16,
  * for q, k, v and out alike): a row of qkv products serves, its queries first.
  * fp32 rows enter whole (products of magnitudes below 2^-102 may lose their
- * last bits), sums are fp32; of fp16 rows the softmax's weights are rounded to
+ * last bits), sums are fp32 and divided last (values whose sum over the keys seen
+ * is above 2^119 may overflow); of fp16 rows the softmax's weights are rounded to
  * fp16 for the second product.  A key with an infinity or NaN makes the rows
  * that see it NaN (an fp16 score of -infinity alone is a weight of 0), a value
  * with one counts where it is seen. */

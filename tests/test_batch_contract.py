@@ -76,7 +76,7 @@ def test_kv4_read():
     refused(g2hip.kv4_read, good, [
         (ARG, dict(cache=None)), (ARG, dict(k=None)), (ARG, dict(v=None)), (ARG, dict(T_kv=-1)), (ARG, dict(T_kv=1025)), (ARG, dict(start=-1)), (ARG, dict(T=0)),
         (ARG, dict(start=25)), (ARG, dict(cache=A[0] + 4)), (LIMIT, dict(n_seq=1 << 21)), (ARG, dict(v=A[1] + n - 4)), (ARG, dict(k=A[0])),
-        (ARG, dict(origin=A[1] + n - 4)), (ARG, dict(lens=A[2])),
+        (ARG, dict(origin=A[1] + n - 4)), (ARG, dict(lens=A[2])), (ARG, dict(k=A[1] + 2)), (ARG, dict(v=A[2] + 1)),
     ])
 
 
@@ -107,6 +107,7 @@ def test_beam_select():
         (LIMIT, dict(V=(1 << 18) + 1)), (LIMIT, dict(groups=(1 << 14) + 1)), (ARG, dict(eos=100)), (ARG, dict(eos=-2)), (ARG, dict(eos=-1)), (ARG, dict(work=A[7] + 4)),
         (ARG, dict(out_score=A[1])), (ARG, dict(out_parent=A[2] + 44)), (ARG, dict(out_id=A[0] + 4 * 1200 - 4)), (ARG, dict(out_done=A[2])), (ARG, dict(out_id=A[4])),
         (ARG, dict(out_done=A[3] + 44)), (ARG, dict(work=A[0])), (ARG, dict(out_parent=A[7] + nw - 4)),
+        (ARG, dict(logits=A[0] + 2)), (ARG, dict(score=A[1] + 1)), (ARG, dict(out_score=A[3] + 2)),
     ])
     assert g2hip.beam_work_bytes(1, 33, 10, 1) == g2hip.beam_work_bytes(1, 1, 10, 65) == g2hip.beam_work_bytes(0, 1, 1, 1) == 0
 

@@ -183,6 +183,16 @@ def test_prompt_scales_and_magnitudes(g2, f16):
     p.check(g2)
 
 
+@pytest.mark.parametrize("seqs,NH", [([(70, 0), (9, 5)], 2), ([(700, 0)], 100)])
+@pytest.mark.parametrize("scale", [0.0, 1e-42, -2.0 ** -140])
+def test_prompt_smallest_scales(g2, seqs, NH, scale):
+    """Scores near fp32's end times scales near 0 are still small: the exponent's factor, scale / log 2, is off by half
+    of fp32's smallest step at most, 2^-150 of scores below 2^125, within the bound's share for the exponent."""
+    p = Prompts(seqs, NH, NH, False, seed=8)
+    p.q, p.k = np.clip(p.q, -4, 4) * np.float32(2.0 ** 60), np.clip(p.k, -4, 4) * np.float32(2.0 ** 54)
+    p.check(g2, scale=scale)
+
+
 @pytest.mark.parametrize("f16", [False, True])
 def test_prompt_not_finite_in_masked_places(g2, f16):
     """Infinities and NaN in keys and values that a row does not see leave it as it is; a value counts where it is
