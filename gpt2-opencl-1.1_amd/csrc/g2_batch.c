@@ -98,7 +98,7 @@ int g2_attn_prompt(const void *q, int q_stride, const void *k, const void *v, in
     if ((rc = ready())) return rc;
     g2_attn_prompt_args a = { q, k, v, out, q_start, k_start, q_rows > 1 ? q_stride : nq, k_rows > 1 ? kv_stride : nk,
                               q_rows > 1 ? out_stride : nq, n_seq, q_rows, k_rows, n_head, n_kv, (int)tiles,
-                              aligned(v, 4) && (k_rows <= 1 || kv_stride % 2 == 0), scale };
+                              aligned(k, 4) && aligned(v, 4) && (k_rows <= 1 || kv_stride % 2 == 0), scale };
     const int fid = form == PF_SPLIT ? (!f16 ? G2F_PROMPT_SPLIT_F32 : a.even ? G2F_PROMPT_SPLIT_F16 : G2F_PROMPT_SPLIT_F16_ODD)
                   : form == PF_DUO ? G2F_PROMPT_DUO_F16 : f16 ? G2F_PROMPT_TILE_F16 : G2F_PROMPT_TILE_F32;
     return g2i_launch(fid, (unsigned)(tiles * n_kv), 1, form == PF_DUO ? 512 : 256, &a);

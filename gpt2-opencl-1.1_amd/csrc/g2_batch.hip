@@ -195,6 +195,18 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t prompt_rows(const T *p, int j0
     const unsigned bytes = any ? ((unsigned)(n - 1) * (unsigned)stride + G2B_DH) * (unsigned)sizeof(T) : 0;
     return __builtin_amdgcn_make_buffer_rsrc((void *)(p + (size_t)j0 * stride), (short)0, bytes, 0x00020000);
 }
+template <typename T> __device__ __forceinline__ void prompt_load_k(T (&x)[8], __amdgpu_buffer_rsrc_t rows, unsigned at)
+{
+    constexpr int W = 4 * (int)sizeof(T) / 2; /* dwords */
+    unsigned w[W];
+#pragma unroll
+    for (int i = 0; i < W; i += 4) {
+        const u32x4 z = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, (int)(at + 4u * (unsigned)i), 0, 0));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[i + e] = z[e];
+    }
+    __builtin_memcpy(x, w, sizeof x);
+}
 /* Two dims' values of the eight keys that a lane of half g takes in step u (in the
  * second product's order): where the first of them is, from the buffer's begin.
  * (Where the others are is added up for each load: eight registers held for it
@@ -455,6 +467,7 @@ __device__ __forceinline__ void prompt_odd(prompt_query<T> &y, const T *v, long 
             for (int r = 0; r < 16; ++r) {
                 const float x = (float)p[16 * (r / 4) + 2 * (r % 4) + t];
                 if (seen && !__builtin_isfinite(x)) y.o[t][r] += x;
+                asm volatile("" : "+v"(y.o[t]) :: "memory");
             }
     }
 }
@@ -513,10 +526,17 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
     T k[4][8];
     prompt_pairs<T> v[2]; /* of the two steps */
     const unsigned at[2] = { prompt_value_at<T>(0, g, lane & 31, stride), prompt_value_at<T>(1, g, lane & 31, stride) };
+    const unsigned at_key = ((unsigned)(lane & 31) * (unsigned)stride + 8u * (unsigned)g) * (unsigned)sizeof(T);
     auto load_k = [&](int j0) {
-        const T *p = kp + (size_t)j0 * stride + (size_t)min(lane & 31, y.k1 - j0 - 1) * stride + 8 * g;
+        if constexpr (EVEN) {
+            const __amdgpu_buffer_rsrc_t rows = prompt_rows(kp, min(j0, y.k1 - 1), y.k1, stride, j0 < y.k1);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) prompt_load_k(k[s], p + 16 * s);
+            for (int s = 0; s < 4; ++s) prompt_load_k(k[s], rows, at_key + 16u * (unsigned)s * (unsigned)sizeof(T));
+        } else {
+            const T *p = kp + (size_t)min(j0 + (lane & 31), y.k1 - 1) * stride + 8 * g;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) prompt_load_k(k[s], p + 16 * s);
+        }
     };
     auto load_v = [&](int j0) {
         const __amdgpu_buffer_rsrc_t rows = prompt_rows(vp, min(j0, y.k1 - 1), y.k1, stride, j0 < y.k1);
@@ -534,9 +554,9 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
             prompt_pack(k[i], x);
             s = prompt_mma(x, y.q[i], s);
         }
-        /* (always, behind the last ones a row of them and none of the values: with a branch
-         * around either what waits for the keys waits for the values, too) */
-        load_k(min(j1, y.k1 - 1));
+        /* (always, behind the last ones of no bytes: with a branch around keys or values
+         * what waits for the ones waits for the others, too) */
+        load_k(j1);
         prompt_follow(y, s, j0, c, g);
         prompt_weights(y, s, c);
         const bool odd0 = prompt_look(v[0]), odd1 = prompt_look(v[1]);
@@ -591,12 +611,12 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
 /* (f16_odd: pairs of values at odd multiples of two bytes.  A kernel of its own: beside
  * a branch between the two kinds of loads the wait for the keys was one for the values,
  * too.) */
-#define PROMPT_SPLIT(NAME, T, KW, EVEN)                                                                                \
-    extern "C" __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(2)))                           \
+#define PROMPT_SPLIT(NAME, T, KW, EVEN, WAVES)                                                                                \
+    extern "C" __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(WAVES)))                       \
     void NAME(const g2_attn_prompt_args a) { prompt_split_impl<T, KW, EVEN>(a); }
-PROMPT_SPLIT(g2k_prompt_split_f32, float, 4, 1)
-PROMPT_SPLIT(g2k_prompt_split_f16, _Float16, 4, 1)
-PROMPT_SPLIT(g2k_prompt_split_f16_odd, _Float16, 4, 0)
+PROMPT_SPLIT(g2k_prompt_split_f32, float, 4, 1, 2)
+PROMPT_SPLIT(g2k_prompt_split_f16, _Float16, 4, 1, 2)
+PROMPT_SPLIT(g2k_prompt_split_f16_odd, _Float16, 4, 0, 3)
 
 /* ---- many queries: a work-group takes 128 of them, 32 a wave, and its waves
  * read KT times 32 keys and values together, once, as operands in LDS: unit

@@ -463,7 +463,7 @@ typedef struct {
     const int *k_start;
     int q_stride, kv_stride, out_stride;
     int S, q_rows, k_rows, NH, NKV, tiles;
-    int even; /* fp16: pairs of values are at multiples of four bytes */
+    int even; /* fp16: pairs of keys and of values are at multiples of four bytes */
     float scale;
 } g2_attn_prompt_args;
 
