@@ -467,7 +467,7 @@ __device__ __forceinline__ void prompt_odd(prompt_query<T> &y, const T *v, long 
             for (int r = 0; r < 16; ++r) {
                 const float x = (float)p[16 * (r / 4) + 2 * (r % 4) + t];
                 if (seen && !__builtin_isfinite(x)) y.o[t][r] += x;
-                asm volatile("" : "+v"(y.o[t]) :: "memory");
+                asm volatile("" : "+v"(y.o[t]) :: "memory"); /* (one at a time: together they were the kernel's registers) */
             }
     }
 }
@@ -611,12 +611,12 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
 /* (f16_odd: pairs of values at odd multiples of two bytes.  A kernel of its own: beside
  * a branch between the two kinds of loads the wait for the keys was one for the values,
  * too.) */
-#define PROMPT_SPLIT(NAME, T, KW, EVEN, WAVES)                                                                                \
-    extern "C" __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(WAVES)))                       \
+#define PROMPT_SPLIT(NAME, T, KW, EVEN)                                                                                \
+    extern "C" __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(2)))                           \
     void NAME(const g2_attn_prompt_args a) { prompt_split_impl<T, KW, EVEN>(a); }
-PROMPT_SPLIT(g2k_prompt_split_f32, float, 4, 1, 2)
-PROMPT_SPLIT(g2k_prompt_split_f16, _Float16, 4, 1, 2)
-PROMPT_SPLIT(g2k_prompt_split_f16_odd, _Float16, 4, 0, 3)
+PROMPT_SPLIT(g2k_prompt_split_f32, float, 4, 1)
+PROMPT_SPLIT(g2k_prompt_split_f16, _Float16, 4, 1)
+PROMPT_SPLIT(g2k_prompt_split_f16_odd, _Float16, 4, 0)
 
 /* ---- many queries: a work-group takes 128 of them, 32 a wave, and its waves
  * read KT times 32 keys and values together, once, as operands in LDS: unit
