@@ -299,8 +299,9 @@ __device__ __forceinline__ float prompt_unit(float scale)
     const float c = fmaxf(fabsf(scale) * 1.44269504f, 0x1p-149f);
     return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(c)));
 }
-/* The weight of a state of maximum m beside one of maximum top (an empty one's is -infinity). */
-__device__ __forceinline__ float prompt_factor(float m, float top, float c) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * c); }
+/* The weight of a state of maximum m beside one of maximum top (an empty one's is
+ * -infinity).  (Halves: their difference does not overflow.) */
+__device__ __forceinline__ float prompt_factor(float m, float top, float c) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(2.f * ((0.5f * m - 0.5f * top) * c)); }
 
 /* A lane's query: its row's keys, its operands of the four steps of 16 dims, its
  * state, where its output goes. */
@@ -355,8 +356,9 @@ __device__ __forceinline__ void prompt_start(prompt_query<T> &y, const g2_attn_p
 /* Scores of the keys j0 .. j0 + 31 to weights, with the state's maximum and sum.
  * The state follows the maximum only where a query's grew by more than 2^8: then
  * the sums are scaled down to it, else weights up to 2^8 are as good (fp16
- * weights are 2^6 times that, so that small ones keep their bits: 2^14 at most,
- * exact down to 2^-20 of the largest). */
+ * weights are 2^6 times that, so that small ones keep their bits: up to 2^14 and
+ * a rounding, exact down to 2^-20 of the largest).  Whether it grew is a matter of the
+ * difference: products with c have steps of their own, 8 and more from 2^26 on. */
 template <typename T>
 __device__ __forceinline__ void prompt_follow(prompt_query<T> &y, f32x16 &s, int j0, float c, int g)
 {
@@ -370,7 +372,7 @@ __device__ __forceinline__ void prompt_follow(prompt_query<T> &y, f32x16 &s, int
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
     top = swap_max(top);
-    const bool grew = top * c > y.m * c + 8.f; /* (an empty state's maximum is -infinity) */
+    const bool grew = (top - y.m) * c > 8.f; /* (an empty state's maximum is -infinity, and two of them are no growth) */
     if (wave_any(grew)) {
         if (!grew) top = y.m; /* (each query by itself: its result does not depend on its neighbours') */
         const float down = prompt_factor(y.m, top, c);
@@ -382,9 +384,11 @@ __device__ __forceinline__ void prompt_follow(prompt_query<T> &y, f32x16 &s, int
         y.m = top;
     }
     /* The exponent will be one operation on the score: what the rounding of m c adds is
-     * the same factor for all weights of a query.  Where it could be a large one, the
-     * scores become differences now. */
-    const bool far = !(fabsf(y.m * c) < 0x1p28f) && y.m != -INFINITY;
+     * one factor for all weights beside the same maximum, 2^(2^-15) at most below 2^10,
+     * about what scores of that size have lost in their own sums; weights beside another
+     * maximum (earlier ones, other waves') have another.  From 2^10 on the scores
+     * become differences now. */
+    const bool far = !(fabsf(y.m * c) < 0x1p10f) && y.m != -INFINITY;
     if (wave_any(far)) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = far ? s[r] - y.m : s[r];
