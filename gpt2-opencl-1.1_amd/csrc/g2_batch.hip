@@ -658,8 +658,9 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
     prompt_start(y, a, hk, place, 32 * w, lane);
     if (lane == 0 && kw == 0) { range[w][0] = y.k0; range[w][1] = y.k1; }
     __syncthreads();
-    const int k0 = __builtin_amdgcn_readfirstlane(min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0])));
-    const int k1 = __builtin_amdgcn_readfirstlane(max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1])));
+    const int low = __builtin_amdgcn_readfirstlane(min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0])));
+    const int high = __builtin_amdgcn_readfirstlane(max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1])));
+    const int k0 = g2b_span_begin(low, high), k1 = g2b_span_end(low, high);
     const float c = prompt_unit(a.scale);
     const long stride = a.kv_stride;
     const T *kp = (const T *)a.k + hk * G2B_DH, *vp = (const T *)a.v + hk * G2B_DH;

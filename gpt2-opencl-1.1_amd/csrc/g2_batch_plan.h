@@ -83,6 +83,12 @@ G2B_FN g2b_row g2b_row_keys(int row, int in, int q0, int q1, int k0, int k1, int
     return r;
 }
 
+/* The keys that a tile's rows see together, from the least and the greatest of its
+ * waves' own: those begin at INT_MAX and end at -INT_MAX where no row sees any, which
+ * is no range to count pieces in.  Such a tile has the keys 0 .. -1. */
+G2B_FN int g2b_span_begin(int low, int high) { return low < high ? low : 0; }
+G2B_FN int g2b_span_end(int low, int high) { return low < high ? high : 0; }
+
 /* Work-group b of tiles * NKV: its key head and tile of queries.  Work-group b
  * runs on XCD b % 8.  The last tiles, whose rows see most keys, come first, all
  * heads of a tile side by side; of the heads, 8 n of them keep to XCD head % 8,

@@ -36,3 +36,12 @@ def test_prompt_scores_far_from_zero(g2, f16, NH, e, unit):
     if f16:
         bound = bound + 2.0 ** -11 * mass * 1.001 + 2.0 ** -11 * np.abs(want) + 2.0 ** -25
     within(got, want, bound)
+
+
+@pytest.mark.parametrize("f16,NH", [(False, 1), (False, 32), (True, 1), (True, 64), (True, 20)])
+@pytest.mark.parametrize("seqs", [[(2100, -2100)], [(2100, -2050)], [(700, -700), (1300, -1290), (100, 0)], [(33, -33)] * 70 + [(5, 200)]])
+def test_prompt_tiles_that_see_no_key(g2, f16, NH, seqs):
+    """Whole tiles whose rows come before the first key, in every form: zeros."""
+    p = Prompts(seqs, NH, NH, f16, seed=23)
+    got, blind = p.check(g2), [r for i, (n, _) in enumerate(seqs) for r in range(p.qs[i], p.qs[i] + n - p.m[i])]
+    assert len(blind) >= 1990 and (got[blind] == 0).all()
