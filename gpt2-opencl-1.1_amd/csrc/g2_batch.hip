@@ -424,8 +424,8 @@ __device__ __forceinline__ void prompt_weight_op(const f32x16 &s, int u, prompt_
 }
 
 /* Whether one of eight values is not finite; such values are then 0: they must not
- * meet the weights 0 of queries that do not see them.  prompt_odd adds them to
- * the queries that do. */
+ * meet the weights 0 of queries that do not see them, nor those that are 0 in 32 bits
+ * alone.  prompt_odd adds them to the outputs of the queries that see them. */
 __device__ __forceinline__ bool prompt_look(const prompt_pairs<float> &v)
 {
     float z[2] = {};
@@ -458,21 +458,28 @@ __device__ __forceinline__ void prompt_clean(prompt_pairs<_Float16> &v)
         if ((v.x[e] & 0x7C000000u) == 0x7C000000u) v.x[e] &= 0xFFFFu;
     }
 }
-template <typename T>
-__device__ __forceinline__ void prompt_odd(prompt_query<T> &y, const T *v, long stride, int j0, int n, int g)
+/* Pieces of 32 keys j0 .. with such values: the first, and what follows the last. */
+struct prompt_span {
+    int lo, end;
+};
+__device__ __forceinline__ void prompt_note(prompt_span &s, bool odd, int j0)
 {
-#pragma unroll 1
-    for (int i = 0; i < n; ++i) {
-        const bool seen = j0 + i >= y.keys.lo && j0 + i < y.keys.end;
-        const T *p = v + (size_t)(j0 + i) * stride + 8 * g;
+    s.lo = odd ? min(s.lo, j0) : s.lo;
+    s.end = odd ? max(s.end, j0 + 32) : s.end;
+}
+/* What is not finite among the eight dims of a query's output from d on, for the keys of
+ * the span that it sees; at the end, because sums that held it would be scaled by 0 where later
+ * scores are far larger. */
+template <typename T>
+__device__ __forceinline__ void prompt_odd(f32x4 (&x)[2], const g2b_row &keys, const T *v, long stride, prompt_span s, int d)
+{
+    const int end = min(s.end, keys.end);
+#pragma unroll 4
+    for (int j = max(s.lo, keys.lo); j < end; ++j) {
+        T z[8];
+        prompt_load_k(z, v + (size_t)j * stride + d);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float x = (float)p[16 * (r / 4) + 2 * (r % 4) + t];
-                if (seen && !__builtin_isfinite(x)) y.o[t][r] += x;
-                asm volatile("" : "+v"(y.o[t]) :: "memory"); /* (one at a time: together they were the kernel's registers) */
-            }
+        for (int e = 0; e < 8; ++e) x[e & 1][e >> 1] += __builtin_isfinite((float)z[e]) ? 0.f : (float)z[e];
     }
 }
 
@@ -487,7 +494,8 @@ template <typename T> __device__ __forceinline__ void prompt_store(T *p, const f
     }
 }
 
-template <typename T> __device__ __forceinline__ void prompt_out(const prompt_query<T> &y, const g2_attn_prompt_args &a, float l, int g)
+template <typename T>
+__device__ __forceinline__ void prompt_out(const prompt_query<T> &y, const g2_attn_prompt_args &a, float l, int g, const T *vp, prompt_span odd)
 {
     const float one = 1.f / l;
     T *out = (T *)a.out + (size_t)y.row * a.out_stride + y.head * G2B_DH + 8 * g;
@@ -498,6 +506,7 @@ template <typename T> __device__ __forceinline__ void prompt_out(const prompt_qu
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[t][e] = y.keys.end > y.keys.lo ? y.o[t][4 * q + e] * one : 0.f;
+        if (odd.lo < odd.end) prompt_odd(v, y.keys, vp, a.kv_stride, odd, 16 * q + 8 * g);
         prompt_store(out + 16 * q, v[0], v[1]);
     }
 }
@@ -516,6 +525,7 @@ template <typename T, int KW, int EVEN>
 __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
 {
     __shared__ float red[KW][34][64];
+    __shared__ prompt_span odds[KW];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     int hk;
     long tile;
@@ -548,6 +558,7 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
         for (int u = 0; u < 2; ++u) prompt_load_v(v[u], rows, at[u], stride, EVEN);
     };
     int j0 = y.k0 < y.k1 ? y.k0 + 32 * w : y.k1;
+    prompt_span odd = { INT_MAX, 0 };
     if (j0 < y.k1) { load_k(j0); load_v(j0); }
     for (; j0 < y.k1; j0 += 32 * KW) {
         const int j1 = j0 + 32 * KW;
@@ -567,7 +578,7 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
         if (odd0 || odd1) {
             prompt_clean(v[0]);
             prompt_clean(v[1]);
-            prompt_odd(y, vp, stride, j0, min(32, y.k1 - j0), g);
+            prompt_note(odd, true, j0);
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -583,6 +594,7 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
     }
     y.l = swap_sum(y.l);
     /* the waves' parts meet; the first four waves write a quarter of the dims each */
+    if (lane == 0) odds[w] = odd;
     red[w][0][lane] = y.m;
     red[w][1][lane] = y.l;
 #pragma unroll
@@ -598,6 +610,8 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
     for (int i = 0; i < KW; ++i) {
         part[i] = prompt_factor(red[i][0][lane], top, c);
         l = fmaf(red[i][1][lane], part[i], l);
+        odd.lo = min(odd.lo, odds[i].lo);
+        odd.end = max(odd.end, odds[i].end);
     }
     const float one = 1.f / l;
     T *out = (T *)a.out + (size_t)y.row * a.out_stride + y.head * G2B_DH + 8 * g;
@@ -610,6 +624,7 @@ __device__ void prompt_split_impl(const g2_attn_prompt_args &a)
             for (int j = 0; j < KW; ++j) x[t][e] = fmaf(red[j][2 + 16 * t + 4 * w + e][lane], part[j], x[t][e]);
             x[t][e] = y.keys.end > y.keys.lo ? x[t][e] * one : 0.f;
         }
+    if (odd.lo < odd.end) prompt_odd(x, y.keys, vp, stride, odd, 16 * w + 8 * g);
     prompt_store(out + 16 * w, x[0], x[1]);
 }
 /* (f16_odd: pairs of values at odd multiples of two bytes.  A kernel of its own: beside
@@ -726,6 +741,7 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
     /* (the groups of four waves take every KW-th piece; all go through as many barriers) */
     constexpr int STEP = 32 * KT * KW;
     int j0 = k0 + 32 * KT * kw, b = 0;
+    prompt_span any = { INT_MAX, 0 };
     if (j0 < k1) {
         load(j0);
         stage(0);
@@ -748,7 +764,7 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
             }
             prompt_follow(y, s, j, c, g);
             prompt_weights(y, s, c);
-            if (__builtin_amdgcn_readfirstlane(odd[b][i][0] | odd[b][i][1])) prompt_odd(y, vp, stride, j, min(32, k1 - j), g);
+            prompt_note(any, __builtin_amdgcn_readfirstlane(odd[b][i][0] | odd[b][i][1]), j);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 prompt_op<T> p, z;
@@ -768,6 +784,7 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
         static_assert(KW == 2 && sizeof(all) >= 34 * 256 * sizeof(float), "one state a query in LDS");
         float *red = (float *)all + w * 64 + lane;
         if (kw) {
+            if (lane == 0) { range[w][0] = any.lo; range[w][1] = any.end; }
             red[0] = y.m;
             red[256] = y.l;
 #pragma unroll
@@ -777,6 +794,8 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
         }
         __syncthreads();
         if (kw) return;
+        any.lo = min(any.lo, __builtin_amdgcn_readfirstlane(range[w][0]));
+        any.end = max(any.end, __builtin_amdgcn_readfirstlane(range[w][1]));
         const float top = fmaxf(y.m, red[0]), mine = prompt_factor(y.m, top, c), other = prompt_factor(red[0], top, c);
         y.l = y.l * mine + red[256] * other;
 #pragma unroll
@@ -784,7 +803,7 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
 #pragma unroll
             for (int r = 0; r < 16; ++r) y.o[t][r] = y.o[t][r] * mine + red[256 * (2 + 16 * t + r)] * other;
     }
-    if (y.row >= 0) prompt_out(y, a, y.l, g);
+    if (y.row >= 0) prompt_out(y, a, y.l, g, vp, any);
 }
 #define PROMPT_TILE(NAME, T, KT, KW, WAVES)                                                                            \
     extern "C" __global__ __launch_bounds__(256 * KW) __attribute__((amdgpu_waves_per_eu(WAVES)))                      \

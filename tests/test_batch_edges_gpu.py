@@ -38,6 +38,19 @@ def test_prompt_scores_far_from_zero(g2, f16, NH, e, unit):
     within(got, want, bound)
 
 
+@pytest.mark.parametrize("f16,NH", FORMS)
+def test_prompt_values_not_finite_before_far_larger_scores(g2, f16, NH):
+    """A value that is not finite counts in the rows that see it also where later keys' scores are so much larger that its
+    weight is 0 in 32 bits: a weight is never 0 by the formula."""
+    for down in (1, -1):
+        p = Prompts([(700, 0)], NH, NH, f16, seed=21)
+        p.q[:], p.k[:] = 0, 0
+        p.q[:, 0::H], p.k[:, 0::H] = 32, (64 * (np.arange(700) // 100))[:, None] * down
+        for j, bad, d in ((5, np.inf, 3), (130, -np.inf, 7), (250, np.nan, 9), (10, np.inf, 11), (420, -np.inf, 11), (333, np.inf, 62), (699, np.inf, 20)):
+            p.v[j, d::H] = bad
+        p.check(g2)
+
+
 @pytest.mark.parametrize("f16,NH", [(False, 1), (False, 32), (True, 1), (True, 64), (True, 20)])
 @pytest.mark.parametrize("seqs", [[(2100, -2100)], [(2100, -2050)], [(700, -700), (1300, -1290), (100, 0)], [(33, -33)] * 70 + [(5, 200)]])
 def test_prompt_tiles_that_see_no_key(g2, f16, NH, seqs):
