@@ -1273,20 +1273,20 @@ __device__ __forceinline__ float beam_bound_of(const float *least, const int *co
     }
     return all >= n ? v : -INFINITY;
 }
-/* How many of LDS's first n keys are above k, and how many are k; the list is a multiple of 8 long, 0 behind the n-th. */
-__device__ __forceinline__ int beam_rank(const unsigned long long *list, int n, unsigned long long k, int &same)
+/* How many of LDS's first n keys are above hi, and how many are lo or above; the list is a multiple of 8 long, 0 behind the n-th. */
+__device__ __forceinline__ int beam_rank(const unsigned long long *list, int n, unsigned long long hi, unsigned long long lo, int &reach)
 {
     typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
     int at = 0;
-    same = 0;
+    reach = 0;
     for (int j = 0; j < n; j += 8) {
         u64x2 v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = *(const u64x2 *)(list + j + 2 * i);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            at += (v[i][0] > k) + (v[i][1] > k);
-            same += (v[i][0] == k) + (v[i][1] == k);
+            at += (v[i][0] > hi) + (v[i][1] > hi);
+            reach += (v[i][0] >= lo) + (v[i][1] >= lo);
         }
     }
     return at;
@@ -1300,6 +1300,9 @@ union beam_lds {
     } slice;
     struct {
         double lse[G2B_MAX_BEAMS]; /* score - log sum exp; NaN: no continuations */
+        float most[G2B_MAX_BEAMS]; /* a row's largest logit */
+        unsigned close;            /* beams whose sums 32 bits do not tell apart */
+        double sum[BEAM_WAVES];
         alignas(16) unsigned long long list[BEAM_LIST + 8];
         unsigned flat[BEAM_LIST];
         alignas(16) float bound[BEAM_WAVES];
@@ -1309,6 +1312,48 @@ union beam_lds {
         unsigned best_flat[BEAM_WAVES];
     } pick;
 };
+
+/* Beams' sums of exponentials come from the slices in 32 bits. What their logarithm is
+ * off by: three maxima (a wave's, a slice's, the row's) below each other scale a term by
+ * three exponentials, each within 2^-23, of exponents off by 2.25 * 2^-24 of the
+ * distance to the row's largest logit, of which the terms' mean is log V at most (28 *
+ * 2^-24 at 2^18 ids); two products and 51 additions: 87 * 2^-24 together, below 2^-17.
+ * So totals of two beams that are further apart than 2^-16 are in order. Beams with
+ * closer ones among the n_out best (with gaps of 0.1 between them, one group in a
+ * thousand) are summed again, in 64 bits, by the group's last work-group: some 20 us a row of
+ * 50257, bound by the exponentials. */
+#define BEAM_CLOSE 0x1p-16
+/* score - log sum exp of the beams whose bit is set, in 64 bits. */
+__device__ void beam_exact(const g2_beam_args &a, unsigned row0, unsigned beams, beam_lds &lds)
+{
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    while (beams) {
+        const unsigned b = (unsigned)__builtin_ctz(beams);
+        beams &= beams - 1;
+        if (!__builtin_isfinite(lds.pick.lse[b])) continue; /* (the same in every thread) */
+        const float *in = a.logits + (size_t)(row0 + b) * (unsigned)a.V;
+        const double most = (double)lds.pick.most[b];
+        double sum = 0;
+#pragma unroll 1
+        for (int i0 = tid; i0 < a.V; i0 += 8 * BEAM_THREADS) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = in[min(i0 + BEAM_THREADS * e, a.V - 1)];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum += i0 + BEAM_THREADS * e < a.V ? exp((double)x[e] - most) : 0.;
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+        if (lane == 0) lds.pick.sum[w] = sum;
+        __syncthreads();
+        if (tid == 0) {
+            sum = 0;
+            for (int i = 0; i < BEAM_WAVES; ++i) sum += lds.pick.sum[i];
+            lds.pick.lse[b] = (double)a.score[row0 + b] - (most + log(sum));
+        }
+        __syncthreads();
+    }
+}
 
 /* The last of a group's work-groups: the n_out best of all its slices' candidates.
  * One work-group, once: what it costs are its waits for memory (one, for sums and
@@ -1334,10 +1379,12 @@ __device__ void beam_pick(const g2_beam_args &a, unsigned g, beam_lds &lds, int 
         double sum = (double)(__uint_as_float((unsigned)(v >> 32)) * (top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((top - most) * 1.44269504f)));
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-        if (lane == 0)
+        if (lane == 0) {
+            lds.pick.most[b] = most;
             lds.pick.lse[b] = a.done && a.done[row0 + (unsigned)b] ? __longlong_as_double(0x7ff8000000000000ll) : (double)a.score[row0 + (unsigned)b] - ((double)most + log(sum));
+        }
     }
-    if (tid == 0) *count = 0;
+    if (tid == 0) { *count = 0; lds.pick.close = 0; }
     __syncthreads();
     auto cand = [&](unsigned beam, unsigned long long k) { /* from its logit's key */
         const double t = (double)key_logit(k) + lds.pick.lse[beam];
@@ -1357,33 +1404,8 @@ __device__ void beam_pick(const g2_beam_args &a, unsigned g, beam_lds &lds, int 
         if (a.done[row0 + beam] && score > -INFINITY) e.k = double_key((double)score);
         return e;
     };
-    beam_cand c0 = { 0, 0 };
-    if ((unsigned)tid < listed) c0 = cand(beam0, key0);
-    else if ((unsigned)tid < all) c0 = get((unsigned)tid);
-    float best = c0.k ? (float)key_double(c0.k) : -INFINITY;
-#pragma unroll 1
-    for (unsigned c = (unsigned)tid + BEAM_THREADS; c < all; c += BEAM_THREADS) {
-        const beam_cand x = get(c);
-        if (x.k) best = fmaxf(best, (float)key_double(x.k));
-    }
     const int full = min((int)(listed / 64), BEAM_WAVES);
-    beam_groups own = { INFINITY, 0 };
-    if (w < full) own = beam_bound(best, beam_groups_log(n, full));
-    if (lane == 0) { lds.pick.bound[w] = own.least; lds.pick.groups[w] = own.count; }
-    __syncthreads();
-    /* (rounded to 32 bits a total keeps its place among the others, but for equal ones) */
-    const float bound = beam_bound_of(lds.pick.bound, lds.pick.groups, n);
-    auto reaches = [&](const beam_cand &c) { return c.k && (float)key_double(c.k) >= bound; };
-    auto add = [&](const beam_cand &c) {
-        if (!reaches(c)) return;
-        const int at = atomicAdd(count, 1);
-        if (at < BEAM_LIST) { lds.pick.list[at] = c.k; lds.pick.flat[at] = c.f; }
-    };
-    add(c0);
-#pragma unroll 1
-    for (unsigned c = (unsigned)tid + BEAM_THREADS; c < all; c += BEAM_THREADS) add(get(c));
-    __syncthreads();
-    const int total = *count;
+    const beam_cand none = { 0, ~0u };
     auto put = [&](int i, const beam_cand &c) {
         const size_t at = (size_t)g * (unsigned)n + (unsigned)i;
         const int parent = c.k ? (int)(c.f >> BEAM_ID_BITS) : -1, id = c.k ? (int)(c.f & ((1u << BEAM_ID_BITS) - 1)) : -1;
@@ -1392,43 +1414,101 @@ __device__ void beam_pick(const g2_beam_args &a, unsigned g, beam_lds &lds, int 
         a.out_id[at] = id;
         if (a.out_done) a.out_done[at] = c.k && (id == a.eos || (a.done && a.done[row0 + (unsigned)parent]));
     };
-    const beam_cand none = { 0, ~0u };
-    if (total <= BEAM_LIST) {
-        if (tid < 8) lds.pick.list[total + tid] = 0;
-        __syncthreads();
-        if (tid < total) {
-            const beam_cand c = { lds.pick.list[tid], lds.pick.flat[tid] };
-            int same, at = beam_rank(lds.pick.list, total, c.k, same);
-            if (same > 1 && at < n)
+    /* Once, or twice where beams come too close for sums in 32 bits. */
 #pragma unroll 1
-                for (int j = 0; j < total; ++j) at += lds.pick.list[j] == c.k && lds.pick.flat[j] < c.f;
-            if (at < n) put(at, c);
-        } else if (tid < n) put(tid, none);
-        return;
-    }
-    beam_cand last = { ~0ull, 0 };
+    for (bool exact = false;; exact = true) {
+        beam_cand c0 = { 0, 0 };
+        if ((unsigned)tid < listed) c0 = cand(beam0, key0);
+        else if ((unsigned)tid < all) c0 = get((unsigned)tid);
+        float best = c0.k ? (float)key_double(c0.k) : -INFINITY;
 #pragma unroll 1
-    for (int i = 0; i < n; ++i) { /* one by one: the best that is below the last one */
-        beam_cand c = none;
-#pragma unroll 1
-        for (unsigned l = (unsigned)tid; l < all; l += BEAM_THREADS) {
-            const beam_cand x = get(l);
-            if (reaches(x) && (i == 0 || beam_above(last, x)) && beam_above(x, c)) c = x;
+        for (unsigned c = (unsigned)tid + BEAM_THREADS; c < all; c += BEAM_THREADS) {
+            const beam_cand x = get(c);
+            if (x.k) best = fmaxf(best, (float)key_double(x.k));
         }
+        beam_groups own = { INFINITY, 0 };
+        if (w < full) own = beam_bound(best, beam_groups_log(n, full));
+        if (lane == 0) { lds.pick.bound[w] = own.least; lds.pick.groups[w] = own.count; }
+        __syncthreads();
+        /* (rounded to 32 bits a total keeps its place among the others, but for equal ones;
+         * those close to the n-th are wanted, too, 2^-22 for the bound's own rounding) */
+        float bound = beam_bound_of(lds.pick.bound, lds.pick.groups, n);
+        if (__builtin_isfinite(bound)) bound -= (float)BEAM_CLOSE + fabsf(bound) * 0x1p-22f;
+        auto reaches = [&](const beam_cand &c) { return c.k && (float)key_double(c.k) >= bound; };
+        auto add = [&](const beam_cand &c) {
+            if (!reaches(c)) return;
+            const int at = atomicAdd(count, 1);
+            if (at < BEAM_LIST) { lds.pick.list[at] = c.k; lds.pick.flat[at] = c.f; }
+        };
+        add(c0);
+#pragma unroll 1
+        for (unsigned c = (unsigned)tid + BEAM_THREADS; c < all; c += BEAM_THREADS) add(get(c));
+        __syncthreads();
+        const int total = *count;
+        int at = tid; /* (whose place is below n is put down) */
+        beam_cand mine = none;
+        if (total <= BEAM_LIST) {
+            if (tid < 8) lds.pick.list[total + tid] = 0;
+            __syncthreads();
+            if (tid < total) {
+                mine = { lds.pick.list[tid], lds.pick.flat[tid] };
+                const double t = key_double(mine.k), near = exact ? 0. : BEAM_CLOSE;
+                const unsigned long long hi = double_key(t + near), lo = double_key(t - near);
+                int reach;
+                at = beam_rank(lds.pick.list, total, hi, lo, reach);
+                if (reach - at > 1 && at < n) {
+                    at = 0;
+                    unsigned close = 0;
+#pragma unroll 1
+                    for (int j = 0; j < total; ++j) {
+                        const beam_cand x = { lds.pick.list[j], lds.pick.flat[j] };
+                        at += beam_above(x, mine);
+                        if (x.k <= hi && x.k >= lo && x.f >> BEAM_ID_BITS != mine.f >> BEAM_ID_BITS) close |= 1u << (x.f >> BEAM_ID_BITS) | 1u << (mine.f >> BEAM_ID_BITS);
+                    }
+                    if (close && !exact) atomicOr(&lds.pick.close, close);
+                }
+            }
+        } else {
+            beam_cand last = { ~0ull, 0 }; /* (the list is free: it takes what is chosen) */
+            unsigned close = 0;
+#pragma unroll 1
+            for (int i = 0; i < n + !exact; ++i) { /* one by one: the best that is below the last one */
+                beam_cand c = none;
+#pragma unroll 1
+                for (unsigned l = (unsigned)tid; l < all; l += BEAM_THREADS) {
+                    const beam_cand x = get(l);
+                    if (reaches(x) && (i == 0 || beam_above(last, x)) && beam_above(x, c)) c = x;
+                }
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const beam_cand x = { __shfl_xor(c.k, o), __shfl_xor(c.f, o) };
-            if (beam_above(x, c)) c = x;
+                for (int o = 32; o > 0; o >>= 1) {
+                    const beam_cand x = { __shfl_xor(c.k, o), __shfl_xor(c.f, o) };
+                    if (beam_above(x, c)) c = x;
+                }
+                __syncthreads();
+                if (lane == 0) { lds.pick.best[w] = c.k; lds.pick.best_flat[w] = c.f; }
+                __syncthreads();
+                for (int t = 0; t < BEAM_WAVES; ++t) {
+                    const beam_cand x = { lds.pick.best[t], lds.pick.best_flat[t] };
+                    if (beam_above(x, c)) c = x;
+                }
+                if (i && c.k && c.f >> BEAM_ID_BITS != last.f >> BEAM_ID_BITS && key_double(last.k) - key_double(c.k) <= BEAM_CLOSE)
+                    close |= 1u << (c.f >> BEAM_ID_BITS) | 1u << (last.f >> BEAM_ID_BITS);
+                if (tid == 0 && i < n) { lds.pick.list[i] = c.k; lds.pick.flat[i] = c.f; }
+                last = c.k ? c : beam_cand{ 1, 0 }; /* (no key is 1: nothing is left) */
+            }
+            if (tid == 0 && !exact) lds.pick.close = close;
+            __syncthreads();
+            if (tid < n) mine = { lds.pick.list[tid], lds.pick.flat[tid] };
         }
+        if (at < n) put(at, mine);
+        if (exact) return;
         __syncthreads();
-        if (lane == 0) { lds.pick.best[w] = c.k; lds.pick.best_flat[w] = c.f; }
+        const unsigned close = lds.pick.close;
+        if (__builtin_expect(!close, 1)) return;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); /* (what was put down is there before another thread's) */
+        if (tid == 0) *count = 0;
+        beam_exact(a, row0, close, lds);
         __syncthreads();
-        for (int t = 0; t < BEAM_WAVES; ++t) {
-            const beam_cand x = { lds.pick.best[t], lds.pick.best_flat[t] };
-            if (beam_above(x, c)) c = x;
-        }
-        if (tid == 0) put(i, c);
-        last = c.k ? c : beam_cand{ 1, 0 }; /* (no key is 1: nothing is left) */
     }
 }
 
@@ -1489,8 +1569,8 @@ __device__ void beam_select_impl(const g2_beam_args &a)
         __syncthreads();
         if (tid < total) {
             const unsigned long long k = lds.slice.list[tid];
-            int same; /* (one: ids differ) */
-            const int at = beam_rank(lds.slice.list, total, k, same);
+            int reach; /* (keys differ: at + 1) */
+            const int at = beam_rank(lds.slice.list, total, k, k, reach);
             if (at < n) st_agent64(cands + at, k);
         } else if (tid < n) st_agent64(cands + tid, 0);
     } else {

@@ -4,8 +4,8 @@ import pytest
 
 from oracle import batch
 from parity import EPS32
-from test_batch_gpu import H, Prompts
-from test_lowbit_gpu import within
+from test_batch_gpu import H, Prompts, select
+from test_lowbit_gpu import rng, same, within
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +58,71 @@ def test_prompt_tiles_that_see_no_key(g2, f16, NH, seqs):
     p = Prompts(seqs, NH, NH, f16, seed=23)
     got, blind = p.check(g2), [r for i, (n, _) in enumerate(seqs) for r in range(p.qs[i], p.qs[i] + n - p.m[i])]
     assert len(blind) >= 1990 and (got[blind] == 0).all()
+
+
+def close_beams(V, G, spread, seed):
+    """Logits of G groups of two beams, and scores that leave the beams' best sums apart by some 1e-8 to 1e-6, far below
+    what an fp32 sum of the exponentials tells apart."""
+    r = rng(V, G, seed)
+    logits = (spread * r.standard_normal((2 * G, V))).astype(np.float32)
+    l = logits.astype(np.float64)
+    top = l.max(1)
+    lse = top + np.log(np.exp(l - top[:, None]).sum(1))
+    best = top - lse
+    gap = r.choice([-1, 1], G) * 10.0 ** r.uniform(-8, -6, G)
+    score = np.zeros(2 * G, np.float32)
+    score[1::2] = (best[0::2] - best[1::2] + gap).astype(np.float32)
+    gap = (score + best).reshape(G, 2)
+    return logits, score, np.abs(gap[:, 0] - gap[:, 1]).min()
+
+
+@pytest.mark.parametrize("V,G,spread,seed", [(50257, 2, 4, 0), (50257, 32, 4, 1), (50257, 64, 4, 2), (5000, 100, 1, 3), (262144, 4, 0.1, 4), (700, 200, 2, 5)])
+def test_select_between_close_beams(g2, V, G, spread, seed):
+    """Continuations of different beams are compared in 64 bits as those of one beam are."""
+    logits, score, gap = close_beams(V, G, spread, seed)
+    assert gap > 1e-11, "the 64-bit oracle's own choice is not certain"
+    want = batch.select(logits, score, None, -1, 2, 4)
+    got = select(g2, logits, score, None, -1, 2, 4)
+    for g, w, name in zip(got[1:3], want[1:3], ("parents", "ids")):
+        same(g, w, name)
+
+
+def chosen(g2, logits, score, done, eos, beams, n_out):
+    want = batch.select(logits, score, done, eos, beams, n_out)
+    for _ in range(2):
+        got = select(g2, logits, score, done, eos, beams, n_out)
+        for g, w, name in zip(got[1:], want[1:], ("parents", "ids", "ended")):
+            same(g, w, name)
+    return want
+
+
+def test_select_close_beams_of_equal_ones(g2):
+    """Close beams where more continuations are equal than the lists hold, and close ended beams."""
+    for V, G in ((5000, 8), (1024, 40)):
+        r = rng(V)
+        logits = np.repeat(r.uniform(-3, 3, 2 * G).astype(np.float32), V).reshape(2 * G, V)
+        score = np.zeros(2 * G, np.float32)
+        score[r.integers(0, 2, G) + 2 * np.arange(G)] = 10.0 ** r.uniform(-8, -6, G)
+        chosen(g2, logits, score, None, -1, 2, 9)
+    logits, score, _ = close_beams(3000, 50, 3, 6)
+    l = logits.astype(np.float64)
+    lse = l.max(1) + np.log(np.exp(l - l.max(1, keepdims=True)).sum(1))
+    score[1::2] = (lse - l.max(1))[1::2].astype(np.float32)  # the beam's best sum: 0 and a rounding
+    score[0::2] = rng(7).uniform(-3e-7, 3e-7, 50).astype(np.float32)
+    total = score[1::2] + (l.max(1) - lse)[1::2]
+    assert np.abs(total - score[0::2]).min() > 1e-10
+    want = chosen(g2, logits, score, np.tile([1, 0], 50), 5, 2, 3)
+    assert 5 < (want[1][:, 0] == 0).sum() < 45
+
+
+@pytest.mark.parametrize("beams,n_out,V", [(32, 64, 1500), (8, 8, 50257), (5, 40, 300)])
+def test_select_chains_of_close_beams(g2, beams, n_out, V):
+    """Every beam close to the next one, in each of the groups."""
+    G, r = 3, rng(beams, n_out)
+    logits = (2 * r.standard_normal((G * beams, V))).astype(np.float32)
+    l = logits.astype(np.float64)
+    best = -np.log(np.exp(l - l.max(1, keepdims=True)).sum(1))
+    score = (-best + 3e-7 * r.permuted(np.tile(np.arange(beams), (G, 1)), axis=1).ravel()).astype(np.float32)
+    total = np.sort((score + best).reshape(G, beams), 1)
+    assert np.diff(total, axis=1).min() > 1e-12
+    chosen(g2, logits, score, None, 7, beams, n_out)
