@@ -19,6 +19,15 @@
 #define MAX_VOCAB (1 << 18)
 
 static int aligned(const void *p, size_t a) { return (uintptr_t)p % a == 0; }
+/* whether the arrays of ints (NULL: not there) are at ints' addresses: a kernel may read
+ * an entry that all lanes want by a scalar load, which drops an address's last two bits */
+static int ints_ok(const char *fn, const int *const *p, int n)
+{
+    for (int i = 0; i < n; ++i)
+        if (!aligned(p[i], sizeof(int))) return g2i_err(G2_E_ARG, "%s: an array of ints is not at an int's address", fn);
+    return G2_OK;
+}
+#define INTS_OK(fn, ...) ints_ok(fn, (const int *const[]){ __VA_ARGS__ }, (int)(sizeof((const int *const[]){ __VA_ARGS__ }) / sizeof(int *)))
 static unsigned cdiv(long a, long b) { return (unsigned)((a + b - 1) / b); }
 static int fits(long groups) { return groups <= (long)UINT32_MAX / 256; }
 static int ready(void) { return g2i_ready() ? G2_OK : g2i_err(G2_E_STATE, "g2_init has not been called"); }
@@ -88,6 +97,7 @@ int g2_attn_prompt(const void *q, int q_stride, const void *k, const void *v, in
     const size_t size = dsize(dtype), no = span_of(q_rows, out_stride, nq, size), ns = ((size_t)n_seq + 1) * sizeof(int);
     if (!aligned(q, size) || !aligned(k, size) || !aligned(v, size) || !aligned(out, size))
         return g2i_err(G2_E_ARG, "%s: a buffer is not at an element's address", fn);
+    if ((rc = INTS_OK(fn, q_start, k_start))) return rc;
     const size_t nkv = span_of(k_rows, kv_stride, nk, size);
     if (g2i_overlap(out, no, q, span_of(q_rows, q_stride, nq, size)) || g2i_overlap(out, no, k, nkv) || g2i_overlap(out, no, v, nkv) ||
         (q_start && g2i_overlap(out, no, q_start, ns)) || (k_start && g2i_overlap(out, no, k_start, ns)))
@@ -148,6 +158,7 @@ int g2_kv4_append(const void *k, const void *v, int stride, int dtype, void *cac
     if (!pos && (start < 0 || start >= max_seq)) return g2i_err(G2_E_ARG, "%s: position %d outside the cache of %d", fn, start, max_seq);
     const size_t size = dsize(dtype), n = span_of(rows, stride, n_kv * G2B_DH, size), nc = g2_kv4_bytes(n_seq, n_kv, max_seq);
     if (!aligned(k, size) || !aligned(v, size)) return g2i_err(G2_E_ARG, "%s: a buffer is not at an element's address", fn);
+    if ((rc = INTS_OK(fn, row_start, pos))) return rc;
     if (g2i_overlap(cache, nc, k, n) || g2i_overlap(cache, nc, v, n) || (row_start && g2i_overlap(cache, nc, row_start, ((size_t)n_seq + 1) * 4)) ||
         (pos && g2i_overlap(cache, nc, pos, (size_t)n_seq * 4)))
         return g2i_err(G2_E_ARG, "%s: overlapping buffers", fn);
@@ -169,6 +180,7 @@ int g2_kv4_read(const void *cache, float *k, float *v, const int *origin, const 
     if (T_kv < 0 || T_kv > max_seq || start < 0 || T < 1 || start > max_seq - T)
         return g2i_err(G2_E_ARG, "%s: positions %d..%ld, length %d, cache of %d", fn, start, (long)start + T - 1, T_kv, max_seq);
     if (!aligned(k, 4) || !aligned(v, 4)) return g2i_err(G2_E_ARG, "%s: a buffer is not at an element's address", fn);
+    if ((rc = INTS_OK(fn, origin, len))) return rc;
     const size_t n = (size_t)n_seq * T * n_kv * 256, nc = g2_kv4_bytes(n_seq, n_kv, max_seq), nl = (size_t)n_seq * 4;
     const size_t nt = (size_t)n_seq * max_seq * 4;
     if (g2i_overlap(k, n, v, n) || g2i_overlap(k, n, cache, nc) || g2i_overlap(v, n, cache, nc) ||
@@ -232,6 +244,7 @@ int g2_attn_kv4(const float *q, int q_stride, const void *cache, float *out, int
         return g2i_err(G2_E_ARG, "%s: length %d of %d, strides %d and %d of rows of %d", fn, T_kv, max_seq, q_stride, out_stride, D);
     if (!isfinite(scale)) return g2i_err(G2_E_ARG, "%s: the scale is not finite", fn);
     if (!aligned(q, 4) || !aligned(out, 4) || !aligned(work, 4)) return g2i_err(G2_E_ARG, "%s: a buffer is not at an element's address", fn);
+    if ((rc = INTS_OK(fn, origin, len))) return rc;
     const size_t nq = span_of(n_seq, q_stride, D, 4), no = span_of(n_seq, out_stride, D, 4), nl = (size_t)n_seq * 4;
     const size_t nc = g2_kv4_bytes(n_seq, n_kv, max_seq), nw = g2_kv4_work_bytes(n_seq, n_head), nt = nl * max_seq;
     if (g2i_overlap(out, no, q, nq) || g2i_overlap(out, no, cache, nc) || g2i_overlap(out, no, work, nw) ||
@@ -295,6 +308,8 @@ int g2_beam_select(const float *logits, const float *score, const int *done, int
     if (eos < -1 || eos >= V || (done && eos < 0)) return g2i_err(G2_E_ARG, "%s: end id %d of %d", fn, eos, V);
     if (!aligned(work, 8)) return g2i_err(G2_E_ARG, "%s: the workspace must be 8-byte aligned", fn);
     if (!aligned(logits, 4) || !aligned(score, 4) || !aligned(out_score, 4)) return g2i_err(G2_E_ARG, "%s: a buffer is not at an element's address", fn);
+    int rc = INTS_OK(fn, done, out_parent, out_id, out_done);
+    if (rc) return rc;
     const long rows = (long)groups * beams;
     const size_t n = (size_t)groups * n_out * 4, nr = (size_t)rows * 4, nw = g2_beam_work_bytes(groups, beams, V, n_out);
     const struct { const void *p; size_t n; } in[] = { { logits, nr * V }, { score, nr }, { done, done ? nr : 0 } };
@@ -305,8 +320,7 @@ int g2_beam_select(const float *logits, const float *score, const int *done, int
         for (int j = 0; j < i; ++j) bad |= outs[i].n && outs[j].n && g2i_overlap(outs[i].p, outs[i].n, outs[j].p, outs[j].n);
         if (bad) return g2i_err(G2_E_ARG, "%s: overlapping buffers", fn);
     }
-    const int rc = ready();
-    if (rc) return rc;
+    if ((rc = ready())) return rc;
     char *p = work;
     g2_beam_args a;
     memset(&a, 0, sizeof a);
@@ -333,6 +347,8 @@ int g2_beam_reorder(const int *ids, int *ids_out, int ids_stride, const int *nex
     if (T < 0 || (has_ids && T >= ids_stride) || (has_origin && T >= origin_stride))
         return g2i_err(G2_E_ARG, "%s: %d ints and one more in rows of %d and %d", fn, T, ids_stride, origin_stride);
     if (T >= MAX_ROWS) return g2i_err(G2_E_LIMIT, "%s: rows of %d: at most %d", fn, T, MAX_ROWS);
+    int rc = INTS_OK(fn, ids, ids_out, next, origin, origin_out, parent, len);
+    if (rc) return rc;
     const long rows = (long)groups * beams;
     const size_t ni = has_ids ? span_of(rows, ids_stride, T + 1, 4) : 0, no = has_origin ? span_of(rows, origin_stride, T + 1, 4) : 0;
     const size_t nr = (size_t)rows * 4;
@@ -345,8 +361,7 @@ int g2_beam_reorder(const int *ids, int *ids_out, int ids_stride, const int *nex
     if (bad) return g2i_err(G2_E_ARG, "%s: overlapping buffers", fn);
     const long chunks = ((long)T + 1 + 255) / 256;
     if (!fits(chunks * rows)) return g2i_err(G2_E_LIMIT, "%s: too many ints for one call", fn);
-    const int rc = ready();
-    if (rc) return rc;
+    if ((rc = ready())) return rc;
     g2_beam_move_args a = { ids, ids_out, next, origin, origin_out, parent, len, ids_stride, origin_stride, T, groups, beams };
     if ((has_ids && ids == ids_out) || (has_origin && origin == origin_out))
         return g2i_launch(G2F_BEAM_MOVE, (unsigned)(chunks * groups), 1, 256, &a);

@@ -290,7 +290,8 @@ int g2_apply_logit_rules(const float *logits, float *out, int *pick, int rows,
  * section before: no buffer of the library, arguments checked also before
  * g2_init, outputs that overlap inputs refused except where a line allows it,
  * device arrays of starts, lengths, positions and rows cut off or left out by
- * the kernels. */
+ * the kernels; every buffer and array at an address of its elements' size, where
+ * a line does not ask for more. */
 
 /* Causal attention of whole prompts that stand one behind the other in q, k
  * and v (the fused g2_attn_1q for every row): sequence s has the query rows
