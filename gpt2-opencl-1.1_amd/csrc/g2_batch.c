@@ -15,6 +15,7 @@
 #define MAX_ROWS (1 << 24)   /* rows of a packed buffer, positions of a cache */
 #define MAX_STRIDE (1 << 24) /* elements from row to row: 31 rows apart is below 2^32 bytes */
 #define MAX_HEADS 1024
+#define MAX_SCALE 0x1p127f    /* times log2 e it is finite, so that a score of 0 stays 0 */
 #define MAX_SEQS (1 << 20)
 #define MAX_VOCAB (1 << 18)
 
@@ -93,7 +94,7 @@ int g2_attn_prompt(const void *q, int q_stride, const void *k, const void *v, in
     if (q_rows > MAX_ROWS || k_rows > MAX_ROWS || n_seq > MAX_SEQS ||
         (q_rows > 1 && (q_stride > MAX_STRIDE || out_stride > MAX_STRIDE)) || (k_rows > 1 && kv_stride > MAX_STRIDE))
         return g2i_err(G2_E_LIMIT, "%s: at most %d rows, %d elements apart, and %d sequences", fn, MAX_ROWS, MAX_STRIDE, MAX_SEQS);
-    if (!isfinite(scale)) return g2i_err(G2_E_ARG, "%s: the scale is not finite", fn);
+    if (!(fabsf(scale) <= MAX_SCALE)) return g2i_err(G2_E_ARG, "%s: the scale is not finite or above 2^127", fn);
     const size_t size = dsize(dtype), no = span_of(q_rows, out_stride, nq, size), ns = ((size_t)n_seq + 1) * sizeof(int);
     if (!aligned(q, size) || !aligned(k, size) || !aligned(v, size) || !aligned(out, size))
         return g2i_err(G2_E_ARG, "%s: a buffer is not at an element's address", fn);
@@ -242,7 +243,7 @@ int g2_attn_kv4(const float *q, int q_stride, const void *cache, float *out, int
     const int D = n_head * G2B_DH;
     if (T_kv < 0 || T_kv > max_seq || (n_seq > 1 && (q_stride < D || out_stride < D)))
         return g2i_err(G2_E_ARG, "%s: length %d of %d, strides %d and %d of rows of %d", fn, T_kv, max_seq, q_stride, out_stride, D);
-    if (!isfinite(scale)) return g2i_err(G2_E_ARG, "%s: the scale is not finite", fn);
+    if (!(fabsf(scale) <= MAX_SCALE)) return g2i_err(G2_E_ARG, "%s: the scale is not finite or above 2^127", fn);
     if (!aligned(q, 4) || !aligned(out, 4) || !aligned(work, 4)) return g2i_err(G2_E_ARG, "%s: a buffer is not at an element's address", fn);
     if ((rc = INTS_OK(fn, origin, len))) return rc;
     const size_t nq = span_of(n_seq, q_stride, D, 4), no = span_of(n_seq, out_stride, D, 4), nl = (size_t)n_seq * 4;

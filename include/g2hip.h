@@ -304,6 +304,7 @@ int g2_apply_logit_rules(const float *logits, float *out, int *pick, int rows,
  * heads of 64 dims, n_kv key heads (a divisor; head h uses key head h / (n_head
  * / n_kv)).  Rows begin strides apart, in elements of dtype (G2_F32 or G2_F16,
  * for q, k, v and out alike): a row of qkv products serves, its queries first.
+ * The scale is finite and at most 2^127.
  * fp32 rows enter whole (products of magnitudes below 2^-102 may lose their
  * last bits), sums are fp32 and divided last (values whose sum over the keys seen
  * is above 2^119 may overflow); of fp16 rows the softmax's weights are rounded to
@@ -348,6 +349,8 @@ size_t g2_kv4_work_bytes(int n_seq, int n_head);
 /* Attention of one query row per sequence over its cached positions
  * (g2_attn_kv8 over this cache, with n_kv key heads as in g2_attn_prompt): rows,
  * strides and lengths as there, origin as in g2_kv4_read.  No position: zeros.
+ * The scale (at most 2^127) times log2 e times an element of q is an fp32 number:
+ * where that or a score overflows, a head's result is NaN or zeros.
  * work: g2_kv4_work_bytes, 4-byte aligned, for this call alone while it runs. */
 int g2_attn_kv4(const float *q, int q_stride, const void *cache, float *out, int out_stride,
                 const int *origin, const int *len, int T_kv, int n_seq, int n_head, int n_kv,

@@ -30,3 +30,14 @@ def test_ints_at_ints_addresses(name):
         for off in (1, 2, 3):
             assert code(fn, {**good, arg: good[arg] + off}.values()) == ARG, (arg, off)
             assert "int's address" in g2hip.last_error()
+
+
+@pytest.mark.parametrize("name", ["attn_prompt", "attn_kv4"])
+def test_scales_whose_unit_overflows(name):
+    """Scores are taken in units of log 2: scale / log 2 has to be finite, or a score of 0 becomes NaN."""
+    good, _ = CALLS[name]
+    fn = getattr(g2hip, name)
+    for scale in (2.0 ** 127, -(2.0 ** 127), 0.0):
+        assert code(fn, {**good, "scale": scale}.values()) == STATE
+    for scale in (1.0001 * 2.0 ** 127, -3e38, float("-inf"), float("nan")):
+        assert code(fn, {**good, "scale": scale}.values()) == ARG
