@@ -5,6 +5,7 @@ import pytest
 from oracle import batch
 from parity import EPS32
 from test_batch_gpu import H, Prompts, select
+from test_batch_parts import NORM16, NORM32, off
 from test_lowbit_gpu import rng, same, within
 
 pytestmark = pytest.mark.gpu
@@ -36,6 +37,17 @@ def test_prompt_scores_far_from_zero(g2, f16, NH, e, unit):
     if f16:
         bound = bound + 2.0 ** -11 * mass * 1.001 + 2.0 ** -11 * np.abs(want) + 2.0 ** -25
     within(got, want, bound)
+
+
+@pytest.mark.parametrize("seqs", [[(17, 0)], [(700, 0)], [(300, 0), (1000, 0), (64, 200), (1, 0)], [(9, 30)] * 80])
+@pytest.mark.parametrize("f16,NH,NKV", [(False, 2, 2), (False, 6, 2), (False, 100, 100), (False, 120, 60), (True, 4, 2), (True, 180, 180), (True, 100, 100)])
+def test_prompt_norms(g2, seqs, f16, NH, NKV):
+    """The error of all outputs together and of each head's: test_batch_parts.py has the limits' reasons."""
+    p = Prompts(seqs, NH, NKV, f16, seed=24)
+    got, want = p.run(g2), p.want()[0]
+    limit = NORM16 if f16 else NORM32
+    assert off(got, want) < limit
+    assert max(off(got[:, h], want[:, h]) for h in range(NH)) < limit
 
 
 @pytest.mark.parametrize("f16,NH", FORMS)
