@@ -63,6 +63,20 @@ def test_prompt_values_not_finite_before_far_larger_scores(g2, f16, NH):
         p.check(g2)
 
 
+def test_prompt_smallest_f16_numbers(g2):
+    """Numbers below 2^-14 (fp16's subnormal ones) as queries, keys and values: products are exact as any others."""
+    for NH in (2, 100, 180):
+        p = Prompts([(700, 0)], NH, NH, True, seed=22)
+        small, large = np.float32(2.0 ** -17), np.float32(2.0 ** 14)
+        q, k = p.q.astype(np.float32).clip(-3.9, 3.9), p.k.astype(np.float32).clip(-3.9, 3.9)
+        p.q, p.k = (q * small).astype(p.t), (k * large).astype(p.t)
+        p.v[:, 0::2] = (p.v[:, 0::2].astype(np.float32) * np.float32(2.0 ** -18)).astype(p.t)
+        assert (p.q != 0).mean() > 0.99
+        p.check(g2, scale=0.5)
+        p.q, p.k = (q * large).astype(p.t), (k * small).astype(p.t)
+        p.check(g2, scale=0.5)
+
+
 @pytest.mark.parametrize("f16,NH", [(False, 1), (False, 32), (True, 1), (True, 64), (True, 20)])
 @pytest.mark.parametrize("seqs", [[(2100, -2100)], [(2100, -2050)], [(700, -700), (1300, -1290), (100, 0)], [(33, -33)] * 70 + [(5, 200)]])
 def test_prompt_tiles_that_see_no_key(g2, f16, NH, seqs):
