@@ -77,6 +77,14 @@ def test_prompt_smallest_f16_numbers(g2):
         p.check(g2, scale=0.5)
 
 
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("S,rows,NH,NKV,past", [(64, 1, 4, 4, 700), (64, 40, 6, 2, 300), (100, 5, 5, 1, 129), (500, 3, 2, 2, 40), (70, 300, 25, 5, 17)])
+def test_prompt_many_sequences_behind_earlier_keys(g2, f16, S, rows, NH, NKV, past):
+    """64 sequences and more, whose tiles are cut from all rows, with keys that were there before."""
+    r = rng(S, rows)
+    Prompts([(int(n), int(m)) for n, m in zip(r.integers(min(rows, 2) - 1, rows + 1, S), r.integers(past - 10, past + 1, S))], NH, NKV, f16, gap=S % 3).check(g2)
+
+
 @pytest.mark.parametrize("f16,NH", [(False, 1), (False, 32), (True, 1), (True, 64), (True, 20)])
 @pytest.mark.parametrize("seqs", [[(2100, -2100)], [(2100, -2050)], [(700, -700), (1300, -1290), (100, 0)], [(33, -33)] * 70 + [(5, 200)]])
 def test_prompt_tiles_that_see_no_key(g2, f16, NH, seqs):
