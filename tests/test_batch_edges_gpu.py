@@ -1,12 +1,12 @@
-"""The operators for several texts at once where their arithmetic or their index ranges end."""
+"""The operators for several texts at once where their arithmetic or their index ranges end, and as they are used with others."""
 import numpy as np
 import pytest
 
 from oracle import batch
 from parity import EPS32
-from test_batch_gpu import H, Prompts, select
+from test_batch_gpu import H, Cache, Prompts, attend_bound, ints, prompt_bound, select
 from test_batch_parts import NORM16, NORM32, off
-from test_lowbit_gpu import rng, same, within
+from test_lowbit_gpu import guarded, rng, same, take, within
 
 pytestmark = pytest.mark.gpu
 
@@ -160,3 +160,32 @@ def test_select_chains_of_close_beams(g2, beams, n_out, V):
     total = np.sort((score + best).reshape(G, beams), 1)
     assert np.diff(total, axis=1).min() > 1e-12
     chosen(g2, logits, score, None, 7, beams, n_out)
+
+
+# ------------------------------------------------------------------ as they are used
+
+@pytest.mark.parametrize("lens,new", [([33, 5, 64], [7, 40, 1]), ([10] * 40, [3] * 40), ([0, 90], [20, 2])])
+def test_second_turn_over_the_cache(g2, lens, new):
+    """Texts of different lengths go on: their new rows are appended to the 4-bit cache, all positions read back, [S][T],
+    and the packed new rows see their own; what lies between a text's last position and the next text's first belongs to
+    sequences without rows."""
+    S, NH, NKV, M = len(lens), 4, 2, 128
+    KD = NKV * H
+    c = Cache(g2, S, NKV, M)
+    c.append(lens, [0] * S)
+    x = c.append(new, lens, seed=1)
+    total = np.add(lens, new)
+    T = int(total.max())
+    k, v = guarded(g2, S * T * KD, 0.0), guarded(g2, S * T * KD, 0.0)
+    g2.kv4_read(c.buf, k, v, None, ints(g2, total), M, 0, T, S, NKV, M)
+    rows = np.concatenate([[0], np.cumsum(new)])
+    qs = np.concatenate([[0], np.repeat(rows[1:], 2)])  # 0, r1, r1, r2, r2, ...: every second one has no rows
+    ks = np.append(np.stack([T * np.arange(S), T * np.arange(S) + total], 1).ravel(), S * T)
+    q = rng(3, S).standard_normal((rows[-1], NH * H)).astype(np.float32)
+    out = guarded(g2, q.size)
+    g2.attn_prompt(g2.to_device(q), NH * H, k, v, KD, out, NH * H, g2.F32, ints(g2, qs), ints(g2, ks), 2 * S, int(rows[-1]), S * T, NH, NKV, 0.125)
+    got, vals = take(out, q.size).reshape(-1, NH, H), c.values()
+    for s in range(S):
+        a = slice(rows[s], rows[s + 1])
+        want, mass, top = batch.attend(q[a].reshape(-1, NH, H), vals[0, s, :total[s]], vals[1, s, :total[s]], 0.125, batch.causal(new[s], total[s]))
+        within(got[a], want, prompt_bound(mass, top, T, False, want), f"text {s}")
