@@ -189,3 +189,130 @@ def test_second_turn_over_the_cache(g2, lens, new):
         a = slice(rows[s], rows[s + 1])
         want, mass, top = batch.attend(q[a].reshape(-1, NH, H), vals[0, s, :total[s]], vals[1, s, :total[s]], 0.125, batch.causal(new[s], total[s]))
         within(got[a], want, prompt_bound(mass, top, T, False, want), f"text {s}")
+
+
+class Layer:
+    """A model of one layer whose embedding, norms, products and sums are the framework's own operators."""
+
+    NH, NKV, E, V = 4, 2, 256, 500
+    W = (NH + 2 * NKV) * H
+
+    def __init__(self, g2, max_seq):
+        r = rng(77, max_seq)
+        self.g2 = g2
+        self.h = {n: (s * r.standard_normal(shape)).astype(np.float32) for n, s, shape in (
+            ("wte", 1, (self.V, self.E)), ("wpe", 0.3, (max_seq, self.E)), ("g1", 1, self.E), ("b1", 0.1, self.E), ("g2", 1, self.E), ("b2", 0.1, self.E),
+            ("wqkv", 0.1, (self.E, self.W)), ("bqkv", 0.1, self.W), ("wo", 0.1, (self.E, self.E)), ("bo", 0.1, self.E), ("head", 0.2, (self.E, self.V)))}
+        self.d = {n: g2.to_device(x) for n, x in self.h.items()}
+
+    def qkv(self, ids, runs):
+        """(x, qkv) of tokens on the device: runs of (first row, rows, first position)."""
+        g2, d = self.g2, self.d
+        n = sum(r[1] for r in runs)
+        x, y, rows = (guarded(g2, n * w) for w in (self.E, self.E, self.W))
+        for row, count, pos in runs:
+            g2.embed(d["wte"], d["wpe"], x.offset(4 * row * self.E), self.E, count, pos, ids.offset(4 * row))
+        g2.layernorm(x, y, d["g1"], d["b1"], self.E, n)
+        g2.matmul(y, d["wqkv"], d["bqkv"], rows, n, self.W, self.E)
+        return x, rows, n
+
+    def logits(self, x, att, n, at):
+        """Logits [len(at), V] of the rows `at`, on the device."""
+        g2, d = self.g2, self.d
+        y, z, out = guarded(g2, n * self.E), guarded(g2, n * self.E), guarded(g2, len(at) * self.V)
+        g2.matmul(att, d["wo"], d["bo"], y, n, self.E, self.E)
+        g2.add(y, x, n * self.E)
+        g2.layernorm(y, z, d["g2"], d["b2"], self.E, n)
+        for i, row in enumerate(at):
+            g2.matmul(z.offset(4 * int(row) * self.E), d["head"], None, out.offset(4 * i * self.V), 1, self.V, self.E)
+        return out
+
+    def check(self, ids, pos, x, rows, att, l, at):
+        """Each product's and norm's rows against 64 bits, from the tokens and the attention's rows: sums of 256 in fp32, 2^-16
+        of the sum of magnitudes each, and three of them, one behind the other, through norms that keep the size."""
+        h, n = {k: v.astype(np.float64) for k, v in self.h.items()}, len(ids)
+
+        def norm(y, g, b):
+            y = y - y.mean(1, keepdims=True)
+            return y / np.sqrt((y * y).mean(1, keepdims=True) + 1e-5) * h[g] + h[b]
+
+        e = h["wte"][ids] + h["wpe"][pos]
+        within(take(x, n * self.E).reshape(n, -1), e, 2.0 ** -23 * (1 + np.abs(e)))
+        y = norm(e, "g1", "b1")
+        within(take(rows, n * self.W).reshape(n, -1), y @ h["wqkv"] + h["bqkv"], 2.0 ** -14 * (1 + np.abs(y) @ np.abs(h["wqkv"])), "qkv")
+        z = norm(e + att.reshape(n, -1) @ h["wo"] + h["bo"], "g2", "b2")[at]
+        within(take(l, len(at) * self.V).reshape(len(at), -1), z @ h["head"], 2.0 ** -13 * (1 + np.abs(z) @ np.abs(h["head"])), "logits")
+
+
+@pytest.mark.parametrize("lens,B,steps", [([5, 40, 1], 4, 6), ([70], 8, 5), ([12] * 9, 2, 4)])
+def test_beams_between_the_frameworks_own_operators(g2, lens, B, steps):
+    """Prompts packed, then steps of all beams: embedding, norms and products by the framework's operators, keys and values
+    to the 4-bit cache, attention through the beams' table, selection, tables moved; every call against the oracle on what
+    the device had before it, and the tables at the end against the choices followed by hand."""
+    G, M = len(lens), max(lens) + steps
+    R, m = G * B, Layer(g2, M)
+    r = rng(5, G, B)
+    prompts = [r.integers(0, m.V, n) for n in lens]
+    flat, start = np.concatenate(prompts), np.concatenate([[0], np.cumsum(lens)])
+    pos = np.concatenate([np.arange(n) for n in lens])
+    ND, KD, W = m.NH * H, m.NKV * H, m.W
+    x, rows, n = m.qkv(ints(g2, flat), [(int(start[g]), lens[g], 0) for g in range(G)])
+    att = guarded(g2, n * ND)
+    ds = ints(g2, start)
+    g2.attn_prompt(rows, W, rows.offset(4 * ND), rows.offset(4 * (ND + KD)), W, att, ND, g2.F32, ds, ds, G, n, n, m.NH, m.NKV, 0.125)
+    got, qkv = take(att, n * ND).reshape(n, m.NH, H), take(rows, n * W).reshape(n, W)
+    q, k, v = qkv[:, :ND].reshape(n, m.NH, H), qkv[:, ND:ND + KD].reshape(n, m.NKV, H), qkv[:, ND + KD:].reshape(n, m.NKV, H)
+    for g in range(G):
+        a = slice(start[g], start[g + 1])
+        want, mass, top = batch.attend(q[a], k[a], v[a], 0.125, batch.causal(lens[g], lens[g]))
+        within(got[a], want, prompt_bound(mass, top, lens[g], False, want), f"prompt {g}")
+    cache = g2.to_device(np.full(g2.kv4_bytes(R, m.NKV, M), 0xCD, np.uint8))
+    held = np.zeros((2, R, M, m.NKV, H), np.float32)  # what the cache was given
+    for g in range(G):
+        held[:, g * B, :lens[g]] = k[start[g]:start[g + 1]], v[start[g]:start[g + 1]]
+    of_beam = np.repeat(start[:-1], B) + np.repeat(lens, B) * (np.arange(R) % B > 0)
+    g2.kv4_append(rows.offset(4 * ND), rows.offset(4 * (ND + KD)), W, g2.F32, cache, ints(g2, np.append(of_beam, n)), None, 0, R, n, m.NKV, M)
+    at = start[1:] - 1
+    l = m.logits(x, att, n, at)
+    m.check(flat, pos, x, rows, got, l, at)
+    ids, origin = np.zeros((R, M), np.int32), np.repeat(np.arange(G) * B, B)[:, None].astype(np.int32) * np.ones((1, M), np.int32)
+    for g in range(G):
+        ids[g * B:(g + 1) * B, :lens[g]] = prompts[g]
+    dids, dorigin = g2.to_device(ids), g2.to_device(origin)
+    score, done, eos = np.zeros(R, np.float32), np.zeros(R, np.int32), m.V - 1
+    dscore, ddone, dnew, dended, parent, nxt = (g2.to_device(np.zeros(R, t)) for t in (np.float32, np.int32, np.float32, np.int32, np.int32, np.int32))
+    works = g2.beam_work(G, 1, m.V, B), g2.beam_work(G, B, m.V, B)
+    awork, length = g2.to_device(np.zeros(g2.kv4_work_bytes(R, m.NH) // 4, np.float32)), np.array(lens)
+    for step in range(steps):
+        beams = B if step else 1
+        old = (np.zeros(G, np.float32), None) if not step else (score, done)
+        want = batch.select(take(l, G * beams * m.V).reshape(-1, m.V), old[0], old[1], eos, beams, B)
+        g2.beam_select(l, dscore if step else g2.to_device(old[0]), ddone if step else None, eos, dnew, parent, nxt, dended, G, beams, m.V, B, works[step > 0])
+        score, done = dnew.download(np.float32), dended.download(np.int32)
+        hp, hn = parent.download(np.int32), nxt.download(np.int32)
+        for name, a, b in (("parents", hp, want[1]), ("ids", hn, want[2]), ("ended", done, want[3])):
+            same(a.reshape(G, B), b, f"{name} of step {step}")
+        within(score.reshape(G, B), want[0], 2.0 ** -20 + 2.0 ** -23 * np.abs(want[0]))
+        g2.beam_reorder(dids, dids, M, nxt, dorigin, dorigin, M, parent, ints(g2, length), int(length.max()), G, B)
+        ids, origin = batch.reorder(ids, hp, hn, length, B), batch.reorder(origin, hp, np.arange(R), length, B)
+        same(dids.download(np.int32).reshape(R, M), ids)
+        same(dorigin.download(np.int32).reshape(R, M), origin)
+        dscore, dnew, ddone, dended = dnew, dscore, dended, ddone
+        if step == steps - 1:
+            break
+        p = np.repeat(length, B)
+        x, rows, _ = m.qkv(nxt, [(b, 1, int(p[b])) for b in range(R)])
+        g2.kv4_append(rows.offset(4 * ND), rows.offset(4 * (ND + KD)), W, g2.F32, cache, None, ints(g2, p), 0, R, R, m.NKV, M)
+        qkv = take(rows, R * W).reshape(R, W)
+        held[:, np.arange(R), p] = qkv[:, ND:ND + KD].reshape(R, m.NKV, H), qkv[:, ND + KD:].reshape(R, m.NKV, H)
+        length = length + 1
+        att = guarded(g2, R * ND)
+        g2.attn_kv4(rows, W, cache, att, ND, dorigin, ints(g2, np.repeat(length, B)), M, R, m.NH, m.NKV, M, 0.125, awork)
+        got, vals = take(att, R * ND).reshape(R, m.NH, H), batch.to4(held)[0]
+        for b in range(R):
+            t = np.arange(length[b // B])
+            kv = vals[:, origin[b, t], t]
+            want, mass, top = batch.attend(qkv[b:b + 1, :ND].reshape(1, m.NH, H), kv[0], kv[1], 0.125, np.ones((1, len(t)), bool))
+            within(got[b:b + 1], want, attend_bound(mass, top, len(t)), f"beam {b}, step {step}")
+        l = m.logits(x, att, R, np.arange(R))
+        m.check(hn, p, x, rows, got, l, np.arange(R))
