@@ -72,7 +72,8 @@ int g2i_prompt_form(int f16, int q_rows, int k_rows, int n_seq, int n_head, int 
 {
     const long queries = (long)q_rows * (n_head / n_kv);
     const int many = (queries + 127) / 128 * n_kv >= (f16 ? 300 : 512), size = many ? 128 : 32;
-    /* (tiles of up to 63 sequences are their own, the last of each may not be full) */
+    /* (tiles of up to 63 sequences are their own, the last of each may not be full; of more
+     * sequences they are of all rows: prompt_find has both sides) */
     *tiles = n_seq > 1 && n_seq < 64 ? queries / size + n_seq : (queries + size - 1) / size;
     return !many ? PF_SPLIT : f16 && (k_rows / n_seq >= 1500 || *tiles * n_kv < 1024) ? PF_DUO : PF_TILE;
 }
@@ -278,10 +279,15 @@ static int beam_sizes(int groups, int beams, int V, int n_out)
            groups <= (1 << 16) / beams;
 }
 
-/* Slices of 4096 ids while that makes at most 256 work-groups (one for each CU), else
- * of 16384, else of 28672 (us: 4 rows of 50257 8.9 with 4096; 16 rows 14.8 with
- * 28672, 10.1 with 16384; 64 rows 12.7, 10.4; 128 rows 11.4 with 28672, 13.5 with
- * 16384; 512 rows 40, 39). */
+/* Slices of 4096 ids while that makes at most 256 work-groups (one for each CU, which
+ * it has to itself), else of 16384, else of 28672.  us, rows of 50257, eight chosen in
+ * groups of one beam (of eight):
+ *                 4096         16384        28672
+ *    16 rows   9.3 (10.8)   10.1 (12.1)  10.6 (11.8)
+ *    32       13.6 (15.0)   10.1 (12.7)  10.8 (12.1)
+ *    64       22.9 (22.2)   10.6 (12.4)  11.2 (11.9)
+ *   128       42.5 (36.3)   20.4 (22.2)  11.7 (12.8)
+ *   512        172  (129)    74  (68)    43.9 (41.9) */
 int g2i_beam_form(int rows, int V, int *slices)
 {
     const int times = (long)rows * cdiv(V, G2B_SLICE) <= 256 ? 1 : (long)rows * cdiv(V, 4 * G2B_SLICE) <= 256 ? 4 : 7;

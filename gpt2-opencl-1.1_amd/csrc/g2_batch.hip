@@ -105,8 +105,11 @@ __device__ __forceinline__ int lanes_min_int(int v)
 /* Where a work-group's tile of queries is.  With up to 63 sequences the tiles are the
  * sequences' own, deepest first: a tile's depth, its place in its sequence, is what
  * its rows see, so long work begins first, and the starts are read once, an entry
- * to a lane.  With more sequences, which are short ones, tiles are cut from all
- * rows in their order, and each row's sequence is searched. */
+ * to a lane.  With more sequences tiles are cut from all rows in their order, and each
+ * row's sequence is searched: full tiles of short texts (64 of 20 rows, 12 heads: 9.3
+ * us, 63 in tiles of their own 11.8), but a wave goes through the keys of all its rows'
+ * sequences, which is slow where each has many of them (one row behind 700 keys: 63
+ * sequences 47 us, 64 of them 332). */
 struct prompt_place {
     int first;          /* the tile's first query: in its sequence, or of all */
     int q0, q1, k0, k1; /* the sequence's rows and keys */
@@ -154,10 +157,10 @@ __device__ __forceinline__ prompt_place prompt_find(const g2_attn_prompt_args &a
  * Queries are the rows' heads that share a key head, row by row: 32
  * of them are fewer rows where heads are grouped, so less is masked.
  *
- * What bounds it: instructions, not memory.  A matrix instruction of 32 x 32 x 16
- * keeps the SIMD from its vector instructions for about 25 of its 37 cycles, so
- * that their times nearly add, and 32 x 32 scores are 8 matrix instructions in
- * fp16, 48 in fp32 (six products of parts), beside some 100 and 350 others for
+ * What bounds it: instructions, not memory.  Vector and matrix instructions are under
+ * way on 48 % and 41 % of the SIMDs' cycles in the fp32 tiles, 68 % and 28 % in the fp16
+ * ones: their times nearly add.  32 x 32 scores are 8 matrix instructions in fp16,
+ * 48 in fp32 (six products of parts), beside some 135 and 430 others for
  * exponentials, sums, maxima and parts.  Timed at the forms below. */
 template <typename T> struct prompt_op; /* an operand of one instruction, 8 values a lane */
 template <> struct prompt_op<float> { u32x4 p[3]; };
@@ -409,7 +412,11 @@ __device__ __forceinline__ void prompt_weights(prompt_query<T> &y, f32x16 &s, fl
     y.l += sum[0] + sum[1];
 }
 
-/* The operand of the weights of step u. */
+/* The operand of the weights of step u.  fp16: rounded to fp16, which adds 1.6e-4 to the
+ * 2.0e-4 of the outputs' own rounding (2-norms; 2.6e-4 together).  Two parts of a weight,
+ * four more matrix instructions and 24 others to a piece, leave the outputs' alone, and
+ * take 262 us for 8001 rows instead of 201, 61 for 51 (16 texts of 25 heads), 22.3 for
+ * 21.1 (40 turns). */
 __device__ __forceinline__ void prompt_weight_op(const f32x16 &s, int u, prompt_op<float> &p)
 {
     float x[8];
@@ -693,7 +700,7 @@ __device__ void prompt_tile_impl(const g2_attn_prompt_args &a)
             /* fp32: either way eight loads of a pair into the same registers.  Where a
              * wave's keys were four wide loads and its values eight others, both
              * meeting in them, 16 texts of 100 to 1023 rows took 163 us, now 153;
-             * fp16 keys in pairs take 274 us instead of 200 for 8001 rows. */
+             * fp16 keys in pairs take 274 us for 8001 rows, which take 193. */
             if constexpr (P == 3) prompt_load8(x[i].x, prompt_rows(keys ? kp : vp, j, k1, stride), keys ? at_key : at_value, keys ? 8u : sb, keys ? 0u : 4 * sb, 0);
             else if (keys) {
                 const T *p = kp + (size_t)j * stride + (size_t)min(m, k1 - j - 1) * stride + 8 * chunk;
@@ -1174,10 +1181,12 @@ G2K void g2k_kv4_join(const g2_kv4_attn_args a)
  * least of the greatest of G >= n groups: of values that are spread over the
  * groups, about G (1 + 1/2 + ... + 1/G) reach it (54 for 16).  What reaches it is
  * put down in LDS, in any order, and each candidate counts those above it.
- * A row is read once, its ids in registers meanwhile.  128 rows of 50257 ids: 13.8 us
- * (25.7 MB, 1.9 TB/s); 4 rows 9.2, of which the last work-group's pick, one
- * wait for memory behind another, is about half.  One launch instead of two: the
- * last of a group's work-groups, by a count that it leaves at 0, picks. */
+ * A row is read once, its ids in registers meanwhile.  128 rows of 50257 ids: 12.8 us
+ * (25.7 MB, 2.0 TB/s: a work-group's sixteen waves of 101 registers have a CU to
+ * themselves, so nothing is loaded while it ranks and picks); 4 rows 9.1, of which the
+ * last work-group's pick, one wait for memory behind another, is about half.  One
+ * launch instead of two: the last of a group's work-groups, by a count that it leaves
+ * at 0, picks. */
 
 #define BEAM_THREADS 1024
 #define BEAM_WAVES (BEAM_THREADS / 64)

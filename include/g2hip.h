@@ -364,7 +364,8 @@ size_t g2_beam_work_bytes(int groups, int beams, int V, int n_out);
  * with the greatest sums of log-probabilities, greatest first; of equal ones
  * the lower beam's, then the lower id's first.  logits [groups * beams][V], score
  * [groups * beams] the beams' sums so far; a continuation's is score + logit -
- * log sum exp(logits), compared in 64 bits.  done (NULL: none) marks beams that
+ * log sum exp(logits), compared in 64 bits (where beams' are within 2^-16 of each
+ * other, their rows are read a second time, some 20 us a row of 50257).  done (NULL: none) marks beams that
  * have ended: such a beam goes on as it is, with id eos and its own score.
  * out_score, out_parent (a beam of the group), out_id and out_done (NULL: not
  * wanted; 1 where the beam had ended or the id is eos) are [groups * n_out].
