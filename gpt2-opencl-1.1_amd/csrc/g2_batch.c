@@ -67,7 +67,9 @@ static int heads_check(const char *fn, int n_head, int n_kv)
  *         16 x 100 to 1023, 25             1700     55     98      68
  *         2 x 2900,    16/4                 728     89    129      74
  * fp32: 128 from two work-groups a CU on.  fp16: from 300 on, with two groups of
- * waves where keys are long or tiles too few for four to a CU. */
+ * waves where keys are long or tiles too few for four to a CU.  Long by their mean, all
+ * that the host knows: one text of 4000 before 60 of 70 (16/4) counts as short and takes
+ * 91, with two groups 75; one of 8000 before ten of 10 212, and 218. */
 int g2i_prompt_form(int f16, int q_rows, int k_rows, int n_seq, int n_head, int n_kv, long *tiles)
 {
     const long queries = (long)q_rows * (n_head / n_kv);
@@ -210,7 +212,12 @@ int g2_kv4_read(const void *cache, float *k, float *v, const int *origin, const 
  *    to 128 positions, for many heads up to 256 (3600 heads x 200 15.6, four 20.1;
  *    360 x 128 4.2, 4.9), eight from 800 for few heads (96 x 901 6.3, four 6.5; 256
  *    passes of two heads x 2000 12.1, 14.6), four else (12 x 700 5.0, eight 5.3;
- *    1200 x 640 14.4, eight 17.5, one 15.3). */
+ *    1200 x 640 14.4, eight 17.5, one 15.3).
+ * Positions are T_kv, all that the host knows: where it is a bound far above the lengths, as
+ * in a recorded step, a call takes the bound's form (1024 for lengths of 60, 250 and 700:
+ * 48 x 25 heads 6.9 for 4.7, 8.3 for 7.6, 13.3 for 13.2; 8 x 12 heads 4.5 for 3.6, 4.3 for
+ * 3.9, 5.3 for 5.1; 50000 for 5000, 16 heads on 4: 12.9 for 7.2, the parts beyond being
+ * empty). */
 int g2i_kv4_form(int n_seq, int n_head, int n_kv, int T_kv, int *heads, int *chunks, int *span, int *waves)
 {
     const int group = n_head / n_kv;
